@@ -199,6 +199,71 @@ class DecodeRowsArgs(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "dtype", "batch", "total_q", "max_seqlen_q", "heads", "heads_kv", "heads_graph",
+        "head_dim", "rank", "num_pages", "page_size", "table_width")] + [
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("seqlens_k", ctypes.c_void_p),
+        ("cu_seqlens_q", ctypes.c_void_p),
+        ("k_pages", Tensor),
+        ("v_pages", Tensor),
+        ("rk_pages", Tensor),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("c", PagedCache),
+        ("causal", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("q", Tensor),
+        ("r_q", Tensor),
+        ("graph_scale", ctypes.c_void_p),
+        ("out", Tensor),
+        ("lse", Tensor),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class PagedWeightsArgs(ctypes.Structure):
+    _fields_ = [
+        ("attn", PagedAttnArgs),
+        ("key_weights", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("stride_h", ctypes.c_int64),
+        ("capacity", ctypes.c_int32),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [("c", PagedCache)] + [(n, Tensor) for n in ("q", "k", "v", "r_k", "q_out")] + [
+        ("positions", ctypes.c_void_p),
+        ("inv_freq", ctypes.c_void_p),
+        ("norm_q", ctypes.c_void_p),
+        ("norm_k", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("c", PagedCache),
+        ("budget", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+        ("first", ctypes.c_int32),
+        ("key_weights", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("stride_h", ctypes.c_int64),
+        ("capacity", ctypes.c_int32),
+        ("weights_out", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+    ]
+
+
 # Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
     "fna2_version": (ctypes.c_int, []),
@@ -225,6 +290,15 @@ SIGNATURES = {
     "fna2_decode": (ctypes.c_int, [ctypes.POINTER(DecodeArgs), ctypes.c_void_p]),
     "fna2_check_decode_rows": (ctypes.c_int, [ctypes.POINTER(DecodeRowsArgs)]),
     "fna2_decode_rows": (ctypes.c_int, [ctypes.POINTER(DecodeRowsArgs), ctypes.c_void_p]),
+    "fna2_check_paged_attn": (ctypes.c_int, [ctypes.POINTER(PagedAttnArgs)]),
+    "fna2_paged_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
+    "fna2_paged_attn": (ctypes.c_int, [ctypes.POINTER(PagedAttnArgs), ctypes.c_void_p]),
+    "fna2_check_paged_weights": (ctypes.c_int, [ctypes.POINTER(PagedWeightsArgs)]),
+    "fna2_paged_weights": (ctypes.c_int, [ctypes.POINTER(PagedWeightsArgs), ctypes.c_void_p]),
+    "fna2_check_paged_append": (ctypes.c_int, [ctypes.POINTER(PagedAppendArgs)]),
+    "fna2_paged_append": (ctypes.c_int, [ctypes.POINTER(PagedAppendArgs), ctypes.c_void_p]),
+    "fna2_check_paged_evict": (ctypes.c_int, [ctypes.POINTER(PagedEvictArgs)]),
+    "fna2_paged_evict": (ctypes.c_int, [ctypes.POINTER(PagedEvictArgs), ctypes.c_void_p]),
 }
 
 _lib = None

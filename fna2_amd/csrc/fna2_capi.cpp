@@ -10,6 +10,7 @@
 
 #include "fna2.h"
 #include "fna2_kernels.h"
+#include "fna2_paged.h"
 #include "fna2_sched.h"
 
 namespace {
@@ -1304,6 +1305,275 @@ int fna2_decode_rows(const fna2_decode_rows_args* a, void* stream) {
   K.cos = (const uint16_t*)a->cos;
   K.sin = (const uint16_t*)a->sin;
   if (fna2::launch_decode_rows(K, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
+  return FNA2_OK;
+}
+
+}  // extern "C"
+
+// ── Paged cache ──────────────────────────────────────────────────────────────
+
+namespace {
+
+constexpr int64_t kMaxCached = (int64_t)1 << 30;  // rows of a sequence (int arithmetic on them)
+
+int64_t cached_rows(const fna2_paged_cache& c) { return (int64_t)c.table_width * c.page_size; }
+
+// A pool of rows of `feat` elements.
+int check_pool(const fna2_tensor& t, int64_t feat) {
+  FNA2_TRY(check_bf16_rows(t));
+  if (t.stride_s < feat) return FNA2_E_STRIDE;
+  if (16 * t.stride_s * 2 > kOff31) return FNA2_E_SHAPE;
+  return FNA2_OK;
+}
+
+int check_paged_cache(const fna2_paged_cache& c, bool chunk) {
+  if (c.dtype != FNA2_BF16 && c.dtype != FNA2_F16) return FNA2_E_DTYPE;
+  if (c.head_dim != 64 && c.head_dim != 128) return FNA2_E_HEAD_DIM;
+  if (c.heads <= 0 || c.heads_kv <= 0 || c.heads % c.heads_kv != 0) return FNA2_E_HEADS;
+  if (c.heads_graph < 0 || c.heads_graph > c.heads || c.heads > 65536) return FNA2_E_HEADS;
+  if (c.heads_graph > 0 && (c.rank < 8 || c.rank > 64 || c.rank % 8 != 0)) return FNA2_E_RANK;
+  if (c.batch < 0 || c.total_q < 0 || c.max_seqlen_q < 0 || c.num_pages < 0) return FNA2_E_SHAPE;
+  if (c.page_size <= 0 || c.page_size % 16 != 0) return FNA2_E_SHAPE;
+  if (c.table_width < 0 || c.table_stride < 0 || cached_rows(c) > kMaxCached) return FNA2_E_SHAPE;
+  if (c.total_q > kMaxCached || c.batch > (1 << 20)) return FNA2_E_SHAPE;
+  if (c.batch > 1 && c.table_stride < c.table_width) return FNA2_E_STRIDE;
+  if (chunk && c.total_q > 0 && !c.cu_seqlens_q) return FNA2_E_SEQLENS;
+  if (c.batch == 0) return FNA2_OK;
+  if (!c.seqlens_k) return FNA2_E_SEQLENS;
+  if (c.table_width == 0) return FNA2_OK;  // no row is ever touched
+  if (!c.block_table) return FNA2_E_NULL;
+  if (c.num_pages == 0) return FNA2_OK;  // no page is ever there
+  FNA2_TRY(check_pool(c.k_pages, c.head_dim));
+  FNA2_TRY(check_pool(c.v_pages, c.head_dim));
+  if (c.heads_graph > 0) FNA2_TRY(check_pool(c.rk_pages, c.rank));
+  return FNA2_OK;
+}
+
+void fill_cache(fna2::PagedParams& K, const fna2_paged_cache& c) {
+  K.N = c.batch;
+  K.T = c.total_q;
+  K.H = c.heads;
+  K.H_KV = c.heads_kv;
+  K.H_G = c.heads_graph;
+  K.D = c.head_dim;
+  K.R = c.heads_graph > 0 ? c.rank : 0;
+  K.group = c.heads / c.heads_kv;
+  K.ps = c.page_size;
+  K.npages = c.num_pages;
+  K.width = c.table_width;
+  K.tstride = c.table_stride;
+  K.table = c.block_table;
+  K.lens = c.seqlens_k;
+  K.cu = c.cu_seqlens_q;
+  K.k = view(c.k_pages);
+  K.v = view(c.v_pages);
+  K.rk = view(c.rk_pages);
+  K.f16 = c.dtype == FNA2_F16;
+}
+
+// Column tiles of the packed kernel: as many of a KV head's query heads as
+// have their ranks in one tile, and as many tokens as the columns then hold.
+struct Packed {
+  int gsub, nsub, tpt, rc, waves;
+  size_t part, bytes;  // offset of the (max, sum) pairs; workspace
+};
+constexpr int kPagedMinSteps = 4;
+Packed packed_of(const fna2_paged_cache& c) {
+  Packed k{};
+  const int group = c.heads / c.heads_kv;
+  for (k.nsub = 1;; ++k.nsub) {
+    k.gsub = (group + k.nsub - 1) / k.nsub;
+    const int rch = c.heads_graph > 0 ? std::min(k.gsub, c.heads_graph) * (c.rank / 8) : 0;
+    k.rc = fna2::paged_rank_chunks(rch);
+    if (k.gsub <= 32 && k.rc >= 0) break;
+  }
+  k.tpt = std::max(1, std::min(32 / k.gsub, c.max_seqlen_q));
+  const int64_t tiles = ((int64_t)c.total_q / k.tpt + c.batch) * c.heads_kv * k.nsub;
+  const double units = (double)tiles * (double)std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);
+  k.waves = (int)std::min(256. * fna2::paged_waves_per_cu(c.head_dim, k.rc),
+                          std::max(std::ceil(units / kPagedMinSteps), 1.));
+  const size_t rows = 2 * (size_t)k.waves * (size_t)(k.gsub * k.tpt);
+  k.part = align_up(rows * (size_t)c.head_dim * 4u);
+  k.bytes = k.part + align_up(rows * 8u);
+  return k;
+}
+
+int check_paged_attn_common(const fna2_paged_attn_args& a) {
+  FNA2_TRY(check_paged_cache(a.c, true));
+  if (!std::isfinite(a.softmax_scale)) return FNA2_E_SCALE;
+  if (a.c.total_q == 0) return FNA2_OK;
+  FNA2_TRY(check_bf16_rows(a.q));
+  if (a.c.heads_graph > 0) {
+    FNA2_TRY(check_bf16_rows(a.r_q));
+    if (!a.graph_scale) return FNA2_E_NULL;
+    const fna2_tensor& r = a.c.rk_pages;
+    if (r.ptr && (int64_t)(a.c.heads / a.c.heads_kv - 1) * r.stride_h * 2 + 16 * r.stride_s * 2 +
+                         a.c.rank * 2 > kOff31)
+      return FNA2_E_SHAPE;
+  }
+  if (a.lse.ptr && (!aligned(a.lse.ptr, 4) || a.lse.stride_s < 0 || a.lse.stride_h < 0))
+    return FNA2_E_STRIDE;
+  return FNA2_OK;
+}
+
+void fill_attn(fna2::PagedParams& K, const fna2_paged_attn_args& a) {
+  std::memset(&K, 0, sizeof(K));
+  fill_cache(K, a.c);
+  K.q = view(a.q);
+  K.rq = view(a.r_q);
+  K.o = view(a.out);
+  K.lse = view(a.lse);
+  K.gs = a.graph_scale;
+  K.causal = a.causal != 0;
+  const float sc = a.softmax_scale;
+  K.c = sc > 0.f ? sc : sc < 0.f ? -sc : 1.f;
+  K.qa = sc > 0.f ? 1.f : sc < 0.f ? -1.f : 0.f;
+  K.c2 = K.c * fna2::kLog2e;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fna2_check_paged_attn(const fna2_paged_attn_args* a) {
+  if (!a) return FNA2_E_NULL;
+  FNA2_TRY(check_paged_attn_common(*a));
+  if (a->c.total_q == 0) return FNA2_OK;
+  FNA2_TRY(check_bf16_rows(a->out));
+  return FNA2_OK;
+}
+
+size_t fna2_paged_attn_workspace_bytes(const fna2_paged_attn_args* a) {
+  if (fna2_check_paged_attn(a) != FNA2_OK || a->c.total_q == 0) return 0;
+  return packed_of(a->c).bytes;
+}
+
+int fna2_paged_attn(const fna2_paged_attn_args* a, void* stream_ptr) {
+  FNA2_TRY(fna2_check_paged_attn(a));
+  if (a->c.total_q == 0) return FNA2_OK;
+  FNA2_TRY(check_device());
+  const Packed k = packed_of(a->c);
+  if (!a->workspace || a->workspace_bytes < k.bytes || !aligned(a->workspace, 16))
+    return FNA2_E_WORKSPACE;
+  hipStream_t stream = (hipStream_t)stream_ptr;
+  fna2::PagedParams K;
+  fill_attn(K, *a);
+  K.gsub = k.gsub;
+  K.nsub = k.nsub;
+  K.tpt = k.tpt;
+  K.waves = k.waves;
+  K.min_steps = kPagedMinSteps;
+  K.part = (float*)a->workspace;
+  K.ml = (float*)((char*)a->workspace + k.part);
+  if (fna2::launch_paged_packed(K, k.rc, stream) != hipSuccess) return FNA2_E_LAUNCH;
+  if (fna2::launch_paged_merge(K, stream) != hipSuccess) return FNA2_E_LAUNCH;
+  return FNA2_OK;
+}
+
+int fna2_check_paged_weights(const fna2_paged_weights_args* w) {
+  if (!w) return FNA2_E_NULL;
+  FNA2_TRY(check_paged_attn_common(w->attn));
+  if (w->capacity < 0 || w->stride_b < 0 || w->stride_h < 0) return FNA2_E_SHAPE;
+  if (w->attn.c.total_q == 0 || w->attn.c.batch == 0 || w->capacity == 0) return FNA2_OK;
+  if (!w->attn.lse.ptr || !w->key_weights) return FNA2_E_NULL;
+  if (!aligned(w->key_weights, 4)) return FNA2_E_STRIDE;
+  if ((w->attn.c.heads_kv > 1 && w->stride_h < w->capacity) ||
+      (w->attn.c.batch > 1 && w->stride_b < w->capacity))
+    return FNA2_E_STRIDE;
+  return FNA2_OK;
+}
+
+int fna2_paged_weights(const fna2_paged_weights_args* w, void* stream) {
+  FNA2_TRY(fna2_check_paged_weights(w));
+  const fna2_paged_cache& c = w->attn.c;
+  if (c.total_q == 0 || c.batch == 0 || w->capacity == 0) return FNA2_OK;
+  FNA2_TRY(check_device());
+  fna2::PagedWeightsParams K;
+  std::memset(&K, 0, sizeof(K));
+  fill_attn(K.p, w->attn);
+  K.w = w->key_weights;
+  K.w_sb = w->stride_b;
+  K.w_sh = w->stride_h;
+  K.cap = w->capacity;
+  const int64_t blocks = (int64_t)c.batch * c.heads_kv * std::max<int64_t>(cdiv64(cached_rows(c), 128), 1);
+  K.grid = (int)std::min<int64_t>(blocks, 2048);
+  if (fna2::launch_paged_weights(K, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
+  return FNA2_OK;
+}
+
+int fna2_check_paged_append(const fna2_paged_append_args* a) {
+  if (!a) return FNA2_E_NULL;
+  FNA2_TRY(check_paged_cache(a->c, true));
+  if ((a->norm_q || a->norm_k) && !std::isfinite(a->eps)) return FNA2_E_SCALE;
+  for (const void* p : {(const void*)a->norm_q, (const void*)a->norm_k, (const void*)a->inv_freq,
+                        (const void*)a->positions})
+    if (!aligned(p, 4)) return FNA2_E_STRIDE;
+  if (a->c.total_q == 0) return FNA2_OK;
+  for (const fna2_tensor* t : {&a->q, &a->k, &a->v, &a->q_out}) FNA2_TRY(check_bf16_rows(*t));
+  if (a->c.heads_graph > 0) FNA2_TRY(check_bf16_rows(a->r_k));
+  return FNA2_OK;
+}
+
+int fna2_paged_append(const fna2_paged_append_args* a, void* stream) {
+  FNA2_TRY(fna2_check_paged_append(a));
+  if (a->c.total_q == 0) return FNA2_OK;
+  FNA2_TRY(check_device());
+  fna2::PagedAppendParams K;
+  std::memset(&K, 0, sizeof(K));
+  fill_cache(K.p, a->c);
+  K.p.q = view(a->q);
+  K.p.o = view(a->q_out);
+  K.kn = view(a->k);
+  K.vn = view(a->v);
+  K.rkn = view(a->r_k);
+  K.pos = a->positions;
+  K.inv_freq = a->inv_freq;
+  K.wq = a->norm_q;
+  K.wk = a->norm_k;
+  K.eps = a->eps;
+  if (fna2::launch_paged_append(K, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
+  return FNA2_OK;
+}
+
+int fna2_check_paged_evict(const fna2_paged_evict_args* a) {
+  if (!a) return FNA2_E_NULL;
+  FNA2_TRY(check_paged_cache(a->c, false));
+  if (a->budget < 0 || a->recent < 0 || a->first < 0 || a->capacity < 0) return FNA2_E_SHAPE;
+  if ((int64_t)a->recent + a->first > a->budget || a->budget > kMaxCached) return FNA2_E_SHAPE;
+  if (a->stride_b < 0 || a->stride_h < 0) return FNA2_E_STRIDE;
+  const int64_t per = 2 * (int64_t)a->c.heads_kv * (a->c.head_dim / 32) + 2 * (int64_t)a->c.heads_graph;
+  if (per * a->c.batch > 4 * kMaxGrid || (int64_t)a->c.batch * a->c.heads_kv > kMaxGrid)
+    return FNA2_E_SHAPE;
+  if (a->c.batch == 0) return FNA2_OK;
+  if (!a->new_lens || (a->budget > 0 && !a->kept)) return FNA2_E_NULL;
+  if (a->capacity > 0 && (!a->key_weights || !a->weights_out)) return FNA2_E_NULL;
+  for (const void* p : {(const void*)a->key_weights, (const void*)a->weights_out,
+                        (const void*)a->kept, (const void*)a->new_lens})
+    if (!aligned(p, 4)) return FNA2_E_STRIDE;
+  if (a->capacity > 0 && a->key_weights == a->weights_out) return FNA2_E_ALIAS;
+  return FNA2_OK;
+}
+
+int fna2_paged_evict(const fna2_paged_evict_args* a, void* stream) {
+  FNA2_TRY(fna2_check_paged_evict(a));
+  if (a->c.batch == 0) return FNA2_OK;
+  FNA2_TRY(check_device());
+  fna2::PagedEvictParams K;
+  std::memset(&K, 0, sizeof(K));
+  fill_cache(K.p, a->c);
+  K.budget = a->budget;
+  K.recent = a->recent;
+  K.first = a->first;
+  K.w = a->key_weights;
+  K.w_sb = a->stride_b;
+  K.w_sh = a->stride_h;
+  K.cap = a->capacity;
+  K.w_out = a->weights_out;
+  K.kept = a->kept;
+  K.new_lens = a->new_lens;
+  if (fna2::launch_paged_select(K, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
+  if (K.budget > 0 && K.p.width > 0)
+    if (fna2::launch_paged_compact(K, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
   return FNA2_OK;
 }
 

@@ -1,0 +1,667 @@
+// fna2_paged_attn.hip — attention of chunks of new tokens over a paged cache.
+//
+// Token i of a sequence's chunk of lq tokens sits at row off + i of the cache,
+// off = lk - lq, and sees the rows up to its own (all lk, not causal):
+//     S_j = softmax_scale <q, K_j> + [h < H_G] graph_scale[h] <rq, Rk_j>,
+//     O = sum_j e^{S_j - m} V_j / (l + 1e-6),  LSE = m + log(l + 1e-6).
+//
+// Packed kernel.  The columns of a 32-wide MFMA tile are (token, query head)
+// pairs: the gsub query heads that share a KV head (and whose ranks fit one
+// tile) times as many tokens as fit.  One token and a few drafted ones so
+// read K and V once per KV head.  A wave works alone: per 32-row step it
+// forms S^T = Ka Qa^T by one MFMA chain over the head dim and the
+// concatenated ranks of its heads (Rq block diagonal), the online softmax by
+// column, and O^T += V^T P^T with V^T read transposed from LDS.
+//
+// Work.  The column tiles' key steps are laid end to end over all sequences
+// and every wave takes an equal run of them, so that the chip is evenly busy
+// however ragged the lengths are; the lengths stay on the device, where every
+// wave finds its run from them.  A run that covers a tile writes its output;
+// a tile cut by runs leaves unnormalised parts that the merge kernel joins in
+// the order of the runs.
+//
+// Pages.  A step's rows come as two groups of 16, each within one page
+// (page_size is a multiple of 16), DMA'd to LDS through descriptors of their
+// own that end with the sequence: what lies behind its last row, or in a
+// page that is not there, is never read and comes as zeros.  The page ids
+// are read a step ahead.
+#include <algorithm>
+
+#include "fna2_kernels.h"
+#include "fna2_paged.h"
+#include "fna2_tile.h"
+
+namespace fna2 {
+
+namespace {
+
+constexpr int kPagBN = 32;  // keys per step
+
+template <int N>
+__device__ __forceinline__ void paged_wait() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));  // lgkmcnt(0)
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// Whether an element-type word holds an infinity or a NaN.
+template <bool F16>
+__device__ __forceinline__ bool word_odd(uint32_t w) {
+  constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+  return (w & E) == E || (w & (E << 16)) == (E << 16);
+}
+
+// Zeroes the keys at or past `limit` (relative to the tile's first key) of a
+// V^T operand of keys k0 .. k0 + 15 (element e of lane half hl: key k0 + 8
+// (e / 4) + 4 hl + e % 4).
+__device__ __forceinline__ bf16x8 cut_keys(bf16x8 x, int k0, int hl, int limit) {
+  u32x4 w = as_u32x4(x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = k0 + 8 * (i >> 1) + 4 * hl + 2 * (i & 1);
+    w[i] &= (key < limit ? 0xffffu : 0u) | (key + 1 < limit ? 0xffff0000u : 0u);
+  }
+  return as_bf16x8(w);
+}
+
+template <int D, int RC>
+struct PackCfg {
+  static constexpr int CD = D / 8;
+  static constexpr int KSD = D / 16;
+  static constexpr int KSR = RC / 2;
+  static constexpr int KBYTES = kPagBN * D * 2;
+  static constexpr int RBYTES = kPagBN * RC * 16;
+  static constexpr int STAGE = 2 * KBYTES + RBYTES;
+  static constexpr int NG = CD / 4;      // column groups of a K / V tile
+  static constexpr int NR = RC / 4;      // ... of an Rk tile
+  static constexpr int OPS = 4 * NG + 2 * NR;  // VMEM instructions per step
+};
+
+template <int D, int RC, bool F16>
+__device__ __forceinline__ void packed_body(const PagedParams& P) {
+  using C = PackCfg<D, RC>;
+  __shared__ __attribute__((aligned(1024))) uint8_t st0[C::STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t st1[C::STAGE];
+  const int lane = threadIdx.x;
+  const int col = lane & 31, hl = lane >> 5;
+  const int tk = col / P.gsub, hc = col - tk * P.gsub;  // token of the tile, head of the group
+  const int cols = P.gsub * P.tpt;
+  const int HB = P.H_KV * P.nsub;
+  const PackedPlan plan(P, lane);
+
+  // Tokens of no sequence: zeros.
+  {
+    const int t0 = min(max(uni(*const_space(P.cu)), 0), P.T);
+    const int t1 = min(max(uni(*const_space(P.cu + P.N)), t0), P.T);
+    const int64_t rows = (int64_t)(t0 + P.T - t1) * P.H;
+    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+      const int h = (int)(i % P.H);
+      int t = (int)(i / P.H);
+      if (t >= t0) t += t1 - t0;
+      uint16_t* o = (uint16_t*)P.o.ptr + (int64_t)t * P.o.ss + (int64_t)h * P.o.sh;
+      if (lane < D / 8) st16(o + 8 * lane, u32x4{0, 0, 0, 0});
+      if (lane == 0 && P.lse.ptr)
+        ((float*)P.lse.ptr)[(int64_t)t * P.lse.ss + (int64_t)h * P.lse.sh] = kNegInf;
+    }
+  }
+
+  int64_t u = (int64_t)blockIdx.x * plan.per;
+  const int64_t u_end = min(plan.total, u + plan.per);
+  if (u >= u_end) return;
+  const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return PackedPlan::units(P, s); });
+  int b = at.b;
+  PagedSeq e = paged_seq_uniform(P, b);
+  int steps = PackedPlan::steps(e);
+  int ct, sg, s0;
+  {
+    const int64_t tile = at.rem / steps;
+    s0 = (int)(at.rem - tile * steps);
+    ct = (int)(tile / HB);
+    sg = (int)(tile - (int64_t)ct * HB);
+  }
+
+  const TrLane tl(lane);
+  const RowLane rdl(lane);
+  const int crr = P.R / 8;
+  const uint32_t krb = (uint32_t)P.k.ss * 2u, vrb = (uint32_t)P.v.ss * 2u;
+  // lane offsets within a 16-row group: row lane / 4, chunk 4 g + (lane % 4)
+  // swizzled (row bits 1..3 only, so both groups of a tile agree)
+  const int lrow = lane >> 2, lch = (lane & 3) ^ swz4(lane >> 2);
+  const uint32_t kvo = (uint32_t)lrow * krb + 16u * lch, vvo = (uint32_t)lrow * vrb + 16u * lch;
+
+  while (u < u_end) {
+    const int s1 = (int)min((int64_t)steps, (int64_t)s0 + (u_end - u));
+    const int kvh = sg / P.nsub, h_in = (sg - kvh * P.nsub) * P.gsub;
+    const int nh = min(P.gsub, P.group - h_in);  // heads of this group
+    const int h0 = kvh * P.group + h_in;
+    const int gg = RC > 0 ? min(max(P.H_G - h0, 0), nh) : 0;  // graph heads
+    const int rch = gg * crr, nrs = cdiv(rch, 2);
+    const int tok = ct * P.tpt + tk;
+    const bool live = tk < P.tpt && tok < e.lq && hc < nh;
+    const int off = e.lk - e.lq;
+    // last key that this column, and that every column, sees
+    const int lim = P.causal ? off + tok : e.lk - 1;
+    const int lim_all = P.causal ? min(off + ct * P.tpt, e.lk - 1) : e.lk - 1;
+    const int lim_any = P.causal ? off + ct * P.tpt + P.tpt - 1 : e.lk - 1;  // ... that any sees
+    const int* trow = P.table + (int64_t)b * P.tstride;
+
+    uint32_t roff[RC > 0 ? C::NR : 1];
+    if constexpr (RC > 0) {
+      const uint32_t hs = (uint32_t)P.rk.sh * 2u, rs = (uint32_t)P.rk.ss * 2u;
+#pragma unroll
+      for (int i = 0; i < C::NR; ++i) {
+        const int c = 4 * i + lch;
+        roff[i] = c < rch ? (uint32_t)(c / crr) * hs + (uint32_t)lrow * rs + (uint32_t)(c % crr) * 16u
+                          : kOOB;
+      }
+    }
+    PageCursor cur;
+    cur.at(P, 32 * s0);
+    auto page_id = [&](int row) {  // of the cursor's row group; -1 past the run or the pool
+      if (row >= e.lk) return -1;
+      const int id = uni(*const_space(trow + cur.page));
+      return (uint32_t)id < (uint32_t)P.npages ? id : -1;
+    };
+    // ids and places of the next tile's two row groups
+    int pid[2], poff[2];
+    auto look = [&](int t) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        pid[g] = t < s1 ? page_id(32 * t + 16 * g) : -1;
+        poff[g] = cur.off;
+        cur.next(P);
+      }
+    };
+    // Tile t (looked up before) into `base`; returns the row groups that are
+    // not there although below lk (bit g).  Then looks up tile t + 1.
+    auto issue = [&](int t, uint8_t* base) {
+      int gone = 0;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int row = 32 * t + 16 * g;
+        const bool here = pid[g] >= 0;
+        const int rows = here ? clamp_rows(e.lk - row, 16) : 0;
+        if (!here && row < e.lk) gone |= 1 << g;
+        const int64_t id = here ? pid[g] : 0;
+        const int r = here ? poff[g] : 0;
+        const auto rk_ = make_rsrc((const uint16_t*)P.k.ptr + id * P.k.sb + (int64_t)kvh * P.k.sh +
+                                       (int64_t)r * P.k.ss, (uint32_t)rows * krb);
+        const auto rv_ = make_rsrc((const uint16_t*)P.v.ptr + id * P.v.sb + (int64_t)kvh * P.v.sh +
+                                       (int64_t)r * P.v.ss, (uint32_t)rows * vrb);
+#pragma unroll
+        for (int i = 0; i < C::NG; ++i) {
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rk_, (lds_void*)(base + (2 * i + g) * 1024), 16,
+                                                   kvo + 64u * i, 0, 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              rv_, (lds_void*)(base + C::KBYTES + C::RBYTES + (2 * i + g) * 1024), 16,
+              vvo + 64u * i, 0, 0, 0);
+        }
+        if constexpr (RC > 0) {
+          const auto rr = make_rsrc(gg > 0 ? (const uint16_t*)P.rk.ptr + id * P.rk.sb +
+                                                 (int64_t)h0 * P.rk.sh + (int64_t)r * P.rk.ss
+                                           : (const uint16_t*)P.k.ptr,
+                                    rows > 0 && gg > 0 ? 0x7ffffff0u : 0u);
+#pragma unroll
+          for (int i = 0; i < C::NR; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rr, (lds_void*)(base + C::KBYTES + (2 * i + g) * 1024), 16,
+                lrow < rows ? roff[i] : kOOB, 0, 0, 0);
+        }
+      }
+      look(t + 1);
+      return gone;
+    };
+
+    look(s0);
+    int gone = issue(s0, st0);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // Query operand (B of S^T): lane holds Qa[col][16 s + 8 hl .. +7].
+    bf16x8 qreg[C::KSD + (RC > 0 ? C::KSR : 0)];
+    float bh = 0.f;
+    {
+      const int64_t t = (int64_t)(e.q0 + (live ? tok : 0));
+      const uint16_t* qrow = (const uint16_t*)P.q.ptr + t * P.q.ss + (int64_t)(h0 + hc) * P.q.sh;
+      const uint32_t qxor = P.qa < 0.f ? 0x80008000u : 0u;
+      const uint32_t qand = P.qa == 0.f ? 0u : 0xffffffffu;
+#pragma unroll
+      for (int s = 0; s < C::KSD; ++s) {
+        u32x4 w = {0, 0, 0, 0};
+        if (live) w = ld16(qrow + 16 * s + 8 * hl);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (w[i] & qand) ^ qxor;
+        qreg[s] = as_bf16x8(w);
+      }
+      if constexpr (RC > 0) {
+        const bool g = live && hc < gg;
+        const uint16_t* rrow = (const uint16_t*)P.rq.ptr + t * P.rq.ss + (int64_t)(h0 + hc) * P.rq.sh;
+        bh = g ? P.gs[h0 + hc] / P.c : 0.f;
+#pragma unroll
+        for (int s = 0; s < C::KSR; ++s) {
+          const int c = 2 * s + hl;  // concatenated chunk of this lane
+          u32x4 w = {0, 0, 0, 0};
+          if (g && c < rch && c / crr == hc) w = ld16(rrow + 8 * (c - hc * crr));
+          qreg[C::KSD + s] = as_bf16x8(w);
+        }
+      }
+    }
+
+    f32x16 oacc[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) oacc[d] = f32x16{};
+    float m_i = kNegInf, l_i = 0.f;
+
+    auto step = [&](int t, const uint8_t* cur_st, uint8_t* nxt_st) {
+      paged_wait<0>();
+      const int gone_now = gone;
+      gone = issue(t + 1, nxt_st);  // (past the run: zeros, from no memory)
+      __builtin_amdgcn_sched_barrier(0);
+      if (32 * t > lim_any) return;  // no column sees these rows
+      const uint8_t* kl = cur_st;
+      const uint8_t* rl = kl + C::KBYTES;
+      const uint8_t* vl = rl + C::RBYTES;
+      f32x16 acc = f32x16{};
+      if constexpr (RC > 0) {
+#pragma unroll
+        for (int s = 0; s < C::KSR; ++s)
+          if (s < nrs) acc = mfma32(row_read<kPagBN>(rl, rdl, 0, s), qreg[C::KSD + s], acc);
+        acc *= bh;
+      }
+#pragma unroll
+      for (int s = 0; s < C::KSD; ++s)
+        acc = mfma_e<F16>(row_read<kPagBN>(kl, rdl, 0, s), qreg[s], acc);
+      const int kbase = 32 * t;
+      const bool masked = kbase + 31 > lim_all || gone_now;
+      if (masked) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int key = kbase + 8 * (v >> 2) + 4 * hl + (v & 3);
+          const bool dead = key > lim || key >= e.lk || ((gone_now >> (v >> 3)) & 1);
+          acc[v] = dead ? kNegInf : acc[v];
+        }
+      }
+      float mx = kNegInf;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) mx = fmaxf(mx, acc[v]);
+      mx = wave_pair_max(mx);
+      const float m_new = fmaxf(m_i, mx);
+      const float m_use = (m_new == kNegInf) ? 0.f : m_new;
+      const float nm = -m_use * P.c2;
+      float ls = 0.f;
+      // P in two parts (as the decode kernel): the first cut to the element
+      // type, the second what that cut off, so that the result does not
+      // depend on where a tile is split.  A part of a visible key is never
+      // zero (an infinite V stays infinite), a hidden key's both are.
+      bf16x8 pb[2], pe[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        u32x4 pk, ek;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int v0 = 8 * half + 2 * i;
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v0], P.c2, nm));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v0 + 1], P.c2, nm));
+          ls += p0 + p1;
+          if constexpr (F16) {
+            pk[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+            ek[i] = pack_e<true>(p0 - elt_lo<true>(pk[i]), p1 - elt_hi<true>(pk[i]));
+          } else {
+            const uint32_t u0 = __builtin_bit_cast(uint32_t, p0);
+            const uint32_t u1 = __builtin_bit_cast(uint32_t, p1);
+            pk[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // their upper halves
+            ek[i] = pack_bf16(p0 - __builtin_bit_cast(float, u0 & 0xffff0000u),
+                              p1 - __builtin_bit_cast(float, u1 & 0xffff0000u));
+          }
+          ek[i] |= (p0 > 0.f ? 1u : 0u) | (p1 > 0.f ? 0x10000u : 0u);
+        }
+        pb[half] = as_bf16x8(pk);
+        pe[half] = as_bf16x8(ek);
+      }
+      if (__builtin_amdgcn_ballot_w64(m_new != m_i) != 0) {
+        const float alpha = __builtin_amdgcn_exp2f((m_i - m_use) * P.c2);
+        l_i *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) oacc[d] *= alpha;
+      }
+      l_i += ls;
+      m_i = m_new;
+      // Rows that some columns see and others do not may hold infinities or
+      // NaN (a later token's V): 0 times those is NaN, so then each token's
+      // columns take their product with the rows past its own zeroed.
+      bool odd = false;
+      if (masked && P.causal) {
+        for (int i = 0; i < C::KBYTES / 1024; ++i) {
+          const u32x4 w = *(const u32x4*)(vl + 1024 * i + 16 * lane);
+          odd |= word_odd<F16>(w[0]) || word_odd<F16>(w[1]) || word_odd<F16>(w[2]) ||
+                 word_odd<F16>(w[3]);
+        }
+        odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+      }
+      if (!odd) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) {
+            const bf16x8 vt = tr_operand<kPagBN>(vl, tl, 16 * s, 32 * d);
+            oacc[d] = mfma_e<F16>(vt, pb[s], oacc[d]);
+            oacc[d] = mfma_e<F16>(vt, pe[s], oacc[d]);
+          }
+      } else {
+        for (int j = 0; j < P.tpt; ++j) {
+          const int cut = off + ct * P.tpt + j + 1 - kbase;  // keys the token sees
+          const uint32_t mine = tk == j ? 0xffffffffu : 0u;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            u32x4 a = as_u32x4(pb[s]), c = as_u32x4(pe[s]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] &= mine, c[i] &= mine;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+              const bf16x8 vt = cut_keys(tr_operand<kPagBN>(vl, tl, 16 * s, 32 * d), 16 * s, hl, cut);
+              // (the other columns' accumulators must not see this V at all)
+              const f32x16 y = mfma_e<F16>(vt, as_bf16x8(c), mfma_e<F16>(vt, as_bf16x8(a), oacc[d]));
+#pragma unroll
+              for (int v = 0; v < 16; ++v) oacc[d][v] = mine ? y[v] : oacc[d][v];
+            }
+          }
+        }
+      }
+    };
+
+    for (int t = s0; t < s1; t += 2) {
+      step(t, st0, st1);
+      if (t + 1 < s1) step(t + 1, st1, st0);
+    }
+    paged_wait<0>();  // no DMA may still write when the ring is used again, or the wave ends
+
+    const float l_tot = wave_pair_sum(l_i);
+    if (s0 == 0 && s1 == steps) {
+      if (live) {
+        const float inv = 1.f / (l_tot + 1e-6f);
+        uint16_t* orow = (uint16_t*)P.o.ptr + (int64_t)(e.q0 + tok) * P.o.ss + (int64_t)(h0 + hc) * P.o.sh;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            u32x2 val;
+            val[0] = pack_e<F16>(oacc[d][4 * g] * inv, oacc[d][4 * g + 1] * inv);
+            val[1] = pack_e<F16>(oacc[d][4 * g + 2] * inv, oacc[d][4 * g + 3] * inv);
+            *(u32x2*)(orow + d * 32 + 8 * g + 4 * hl) = val;
+          }
+        if (hl == 0 && P.lse.ptr)
+          ((float*)P.lse.ptr)[(int64_t)(e.q0 + tok) * P.lse.ss + (int64_t)(h0 + hc) * P.lse.sh] =
+              m_i == kNegInf ? kNegInf : m_i * P.c + __builtin_amdgcn_logf(l_tot + 1e-6f) * kLn2;
+      }
+    } else if (col < cols) {
+      // slot 2 w: wave w's run ends or lies in a tile begun before it; 2 w + 1:
+      // it begins the tile
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (s0 == 0 ? 1 : 0);
+      float* arow = P.part + (slot * cols + col) * D;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4_t val = {oacc[d][4 * g], oacc[d][4 * g + 1], oacc[d][4 * g + 2], oacc[d][4 * g + 3]};
+          *(f32x4_t*)(arow + d * 32 + 8 * g + 4 * hl) = val;
+        }
+      if (hl == 0) *(f32x2*)(P.ml + 2 * (slot * cols + col)) = f32x2{m_i, l_tot};
+    }
+
+    u += s1 - s0;
+    s0 = 0;
+    if (u < u_end && ++sg == HB) {
+      sg = 0;
+      if ((++ct) * P.tpt >= e.lq) {
+        ct = 0;
+        do e = paged_seq_uniform(P, ++b); while (e.lq == 0 && b + 1 < P.N);
+        steps = PackedPlan::steps(e);
+      }
+    }
+  }
+}
+
+// Joins the parts of the tiles that runs cut: workgroup (i, y) takes the tile
+// that the boundary between runs i and i + 1 cuts, if it is the tile's first.
+// LPR lanes hold a row of D values; `WAYS` groups of lanes share a row's parts.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams P) {
+  constexpr int LPR = D / 4, NG = 256 / LPR;
+  __shared__ float part[NG][D];
+  __shared__ float stat[NG][2];
+  const int lane = threadIdx.x & 63;
+  const PackedPlan plan(P, lane);
+  const int64_t i0 = blockIdx.x;  // the run before the boundary
+  const int64_t u = (i0 + 1) * plan.per;
+  if (u >= plan.total) return;
+  const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return PackedPlan::units(P, s); });
+  const PagedSeq e = paged_seq_uniform(P, at.b);
+  const int steps = PackedPlan::steps(e), HB = P.H_KV * P.nsub;
+  const int64_t tile = at.rem / steps;
+  const int s0 = (int)(at.rem - tile * steps);
+  if (s0 == 0 || s0 > plan.per) return;  // not cut here; or an earlier boundary cuts it too
+  const int64_t tile_end = u - s0 + steps;
+  const int n = (int)((tile_end - 1) / plan.per - i0) + 1;  // runs that hold a part
+  const int ct = (int)(tile / HB), sg = (int)(tile - (int64_t)ct * HB);
+  const int kvh = sg / P.nsub, h_in = (sg - kvh * P.nsub) * P.gsub;
+  const int nh = min(P.gsub, P.group - h_in), h0 = kvh * P.group + h_in;
+  const int cols = P.gsub * P.tpt;
+  const int grp = threadIdx.x / LPR, f = 4 * (threadIdx.x % LPR);
+  for (int c = blockIdx.y; c < cols; c += gridDim.y) {
+    const int tk = c / P.gsub, hc = c - tk * P.gsub, tok = ct * P.tpt + tk;
+    if (tok >= e.lq || hc >= nh) continue;  // (uniform)
+    float M = kNegInf, L = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int j = grp; j < n; j += NG) {
+      const int64_t slot = j == 0 ? 2 * i0 + 1 : 2 * (i0 + j);
+      const f32x2 ml = *(const f32x2*)(P.ml + 2 * (slot * cols + c));
+      const f32x4_t x = *(const f32x4_t*)(P.part + (slot * cols + c) * D + f);
+      const float m = fmaxf(M, ml[0]);
+      const float ref = m == kNegInf ? 0.f : m;
+      const float wa = __builtin_amdgcn_exp2f((M - ref) * P.c2);
+      const float wb = __builtin_amdgcn_exp2f((ml[0] - ref) * P.c2);
+      L = L * wa + ml[1] * wb;
+      o = o * wa + x * wb;
+      M = m;
+    }
+    *(f32x4_t*)(&part[grp][f]) = o;
+    if (f == 0) stat[grp][0] = M, stat[grp][1] = L;
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+      const int d = 2 * threadIdx.x;
+      float m = kNegInf, l = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) m = fmaxf(m, stat[g][0]);
+      const float ref = m == kNegInf ? 0.f : m;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float w = __builtin_amdgcn_exp2f((stat[g][0] - ref) * P.c2);
+        l += stat[g][1] * w;
+        y0 += part[g][d] * w;
+        y1 += part[g][d + 1] * w;
+      }
+      const float inv = 1.f / (l + 1e-6f);
+      uint16_t* orow = (uint16_t*)P.o.ptr + (int64_t)(e.q0 + tok) * P.o.ss + (int64_t)(h0 + hc) * P.o.sh;
+      *(uint32_t*)(orow + d) = pack_e<F16>(y0 * inv, y1 * inv);
+      if (d == 0 && P.lse.ptr)
+        ((float*)P.lse.ptr)[(int64_t)(e.q0 + tok) * P.lse.ss + (int64_t)(h0 + hc) * P.lse.sh] =
+            m == kNegInf ? kNegInf : m * P.c + __builtin_amdgcn_logf(l + 1e-6f) * kLn2;
+    }
+    __syncthreads();
+  }
+}
+
+// Attention weights of the cached rows: W_j += sum over tokens and heads of
+// e^{S_j - LSE}.  A wave holds 32 keys (the columns of S = Q K^T, so a lane
+// sums its key's weights over the rows in registers) and walks the chunk's
+// tokens, 32 at a time, of each query head of the KV head.  One workgroup's
+// four waves take 128 keys; blocks of keys go round over the workgroups.
+template <int D, int RPL, bool F16>
+__global__ __launch_bounds__(256) void paged_weights_kernel(const PagedWeightsParams W) {
+  constexpr int KSD = D / 16, KSR = RPL / 16;
+  const PagedParams& P = W.p;
+  const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
+  const int col = lane & 31, hl = lane >> 5;
+  auto units = [&](const PagedSeq& s) { return s.lq > 0 ? (int64_t)P.H_KV * cdiv(s.lk, 128) : 0; };
+  const int64_t total = uni64(wave_total(P, lane, units));
+  const uint32_t qxor = P.qa < 0.f ? 0x80008000u : 0u;
+  const uint32_t qand = P.qa == 0.f ? 0u : 0xffffffffu;
+  for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
+    const PagedAt at = wave_locate(P, lane, id, units);
+    const PagedSeq e = paged_seq_uniform(P, at.b);
+    const int nkb = cdiv(e.lk, 128);
+    const int kvh = (int)(at.rem / nkb);
+    const int k0 = 128 * (int)(at.rem - (int64_t)kvh * nkb) + 32 * wv;
+    const int key = k0 + col, off = e.lk - e.lq;
+    int page = -1, r = 0;
+    if (key < e.lk) {
+      page = P.table[(int64_t)at.b * P.tstride + key / P.ps];
+      r = key % P.ps;
+      if ((uint32_t)page >= (uint32_t)P.npages) page = -1;
+    }
+    const bool here = page >= 0 && key < W.cap;
+    if (__builtin_amdgcn_ballot_w64(here) == 0) continue;
+    bf16x8 kreg[KSD];
+    const int64_t id64 = page < 0 ? 0 : page;
+    {
+      const uint16_t* krow = (const uint16_t*)P.k.ptr + id64 * P.k.sb + (int64_t)kvh * P.k.sh + (int64_t)r * P.k.ss;
+#pragma unroll
+      for (int s = 0; s < KSD; ++s) {
+        u32x4 w = {0, 0, 0, 0};
+        if (here) w = ld16(krow + 16 * s + 8 * hl);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (w[i] & qand) ^ qxor;
+        kreg[s] = as_bf16x8(w);
+      }
+    }
+    float sum = 0.f;
+    const int i_first = P.causal ? max(k0 - off, 0) & ~31 : 0;  // earlier tokens see no key here
+    for (int h = kvh * P.group; h < (kvh + 1) * P.group; ++h) {
+      const bool graph = RPL > 0 && h < P.H_G;
+      bf16x8 rkreg[KSR > 0 ? KSR : 1];
+      float bh = 0.f;
+      if constexpr (KSR > 0) {
+        const uint16_t* rrow = (const uint16_t*)P.rk.ptr + id64 * P.rk.sb + (int64_t)h * P.rk.sh + (int64_t)r * P.rk.ss;
+        bh = graph ? *const_space(P.gs + h) / P.c : 0.f;
+#pragma unroll
+        for (int s = 0; s < KSR; ++s) {
+          u32x4 w = {0, 0, 0, 0};
+          if (here && graph && 16 * s + 8 * hl < P.R) w = ld16(rrow + 16 * s + 8 * hl);
+          rkreg[s] = as_bf16x8(w);
+        }
+      }
+      for (int i0 = i_first; i0 < e.lq; i0 += 32) {
+        const int tok = i0 + col;  // the row this lane loads
+        const bool have = tok < e.lq;
+        const int64_t t = e.q0 + (have ? tok : 0);
+        f32x16 acc = f32x16{};
+        if constexpr (KSR > 0) {
+          const uint16_t* rrow = (const uint16_t*)P.rq.ptr + t * P.rq.ss + (int64_t)h * P.rq.sh;
+#pragma unroll
+          for (int s = 0; s < KSR; ++s) {
+            u32x4 w = {0, 0, 0, 0};
+            if (have && graph && 16 * s + 8 * hl < P.R) w = ld16(rrow + 16 * s + 8 * hl);
+            acc = mfma32(as_bf16x8(w), rkreg[s], acc);
+          }
+          acc *= bh;
+        }
+        const uint16_t* qrow = (const uint16_t*)P.q.ptr + t * P.q.ss + (int64_t)h * P.q.sh;
+#pragma unroll
+        for (int s = 0; s < KSD; ++s) {
+          u32x4 w = {0, 0, 0, 0};
+          if (have) w = ld16(qrow + 16 * s + 8 * hl);
+          acc = mfma_e<F16>(as_bf16x8(w), kreg[s], acc);
+        }
+        float part = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int row = i0 + 8 * (v >> 2) + 4 * hl + (v & 3);
+          const bool see = row < e.lq && (!P.causal || key <= off + row);
+          float nl = kNegInf;
+          if (row < e.lq) {
+            const float l = ((const float*)P.lse.ptr)[(int64_t)(e.q0 + row) * P.lse.ss + (int64_t)h * P.lse.sh];
+            nl = l == kNegInf ? kNegInf : -l * kLog2e;
+          }
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], P.c2, nl));
+          part += see && nl != kNegInf ? p : 0.f;
+        }
+        sum += part;
+      }
+    }
+    sum = wave_pair_sum(sum);
+    if (here && hl == 0) {
+      float* w = W.w + (int64_t)at.b * W.w_sb + (int64_t)kvh * W.w_sh + key;
+      *w += sum;
+    }
+  }
+}
+
+#define FNA2_PACKED(D, RC)                                                                     \
+  __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC(const PagedParams P) {    \
+    packed_body<D, RC, false>(P);                                                              \
+  }                                                                                            \
+  __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC##_f16(const PagedParams P) { \
+    packed_body<D, RC, true>(P);                                                               \
+  }
+FNA2_PACKED(64, 0)
+FNA2_PACKED(64, 4)
+FNA2_PACKED(64, 8)
+FNA2_PACKED(64, 16)
+FNA2_PACKED(64, 32)
+FNA2_PACKED(128, 0)
+FNA2_PACKED(128, 4)
+FNA2_PACKED(128, 8)
+FNA2_PACKED(128, 16)
+FNA2_PACKED(128, 32)
+#undef FNA2_PACKED
+
+}  // namespace
+
+int paged_rank_chunks(int rch) {
+  return rch <= 0 ? 0 : rch <= 4 ? 4 : rch <= 8 ? 8 : rch <= 16 ? 16 : rch <= 32 ? 32 : -1;
+}
+
+int paged_waves_per_cu(int D, int rc) {
+  const int ring = 2 * kPagBN * (2 * D * 2 + rc * 16);
+  return std::max(1, std::min(8, (160 * 1024 - 1) / ring));
+}
+
+hipError_t launch_paged_packed(const PagedParams& P, int rc, hipStream_t s) {
+  void (*k)(const PagedParams) = nullptr;
+#define FNA2_PACKED_OF(D, RC) (P.f16 ? paged_packed_d##D##_c##RC##_f16 : paged_packed_d##D##_c##RC)
+  if (P.D == 64)
+    k = rc == 0 ? FNA2_PACKED_OF(64, 0) : rc == 4 ? FNA2_PACKED_OF(64, 4) : rc == 8 ? FNA2_PACKED_OF(64, 8)
+      : rc == 16 ? FNA2_PACKED_OF(64, 16) : rc == 32 ? FNA2_PACKED_OF(64, 32) : nullptr;
+  if (P.D == 128)
+    k = rc == 0 ? FNA2_PACKED_OF(128, 0) : rc == 4 ? FNA2_PACKED_OF(128, 4) : rc == 8 ? FNA2_PACKED_OF(128, 8)
+      : rc == 16 ? FNA2_PACKED_OF(128, 16) : rc == 32 ? FNA2_PACKED_OF(128, 32) : nullptr;
+#undef FNA2_PACKED_OF
+  if (!k) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(k, dim3((uint32_t)P.waves), dim3(64), 0, s, P);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_merge(const PagedParams& P, hipStream_t s) {
+  if (P.waves <= 1) return hipSuccess;
+  const dim3 grid((uint32_t)(P.waves - 1), (uint32_t)std::min(P.gsub * P.tpt, 8));
+  if (P.D == 64)
+    hipLaunchKernelGGL(P.f16 ? (paged_merge_kernel<64, true>) : (paged_merge_kernel<64, false>), grid, dim3(256), 0, s, P);
+  else
+    hipLaunchKernelGGL(P.f16 ? (paged_merge_kernel<128, true>) : (paged_merge_kernel<128, false>), grid, dim3(256), 0, s, P);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_weights(const PagedWeightsParams& W, hipStream_t s) {
+  const PagedParams& P = W.p;
+  const int rpl = padded_rank32(P.H_G, P.R);
+  void (*k)(const PagedWeightsParams) = nullptr;
+#define FNA2_W(D, RPL) (P.f16 ? paged_weights_kernel<D, RPL, true> : paged_weights_kernel<D, RPL, false>)
+  if (P.D == 64) k = rpl == 0 ? FNA2_W(64, 0) : rpl == 32 ? FNA2_W(64, 32) : FNA2_W(64, 64);
+  if (P.D == 128) k = rpl == 0 ? FNA2_W(128, 0) : rpl == 32 ? FNA2_W(128, 32) : FNA2_W(128, 64);
+#undef FNA2_W
+  if (!k) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(k, dim3((uint32_t)W.grid), dim3(256), 0, s, W);
+  return hipGetLastError();
+}
+
+}  // namespace fna2

@@ -311,6 +311,122 @@ int fna2_check_decode_rows(const fna2_decode_rows_args* args);
 
 int fna2_decode_rows(const fna2_decode_rows_args* args, void* hip_stream);
 
+/* ── Paged cache ──────────────────────────────────────────────────────────
+ * The cached rows of a sequence lie in pages of page_size rows, anywhere in a
+ * pool, in the order its row of the block table names them: row j of
+ * sequence b is row j % page_size of page block_table[b][j / page_size].
+ * Element (page, head, row, f) of a pool lies at
+ *     ptr + page*stride_b + head*stride_h + row*stride_s + f
+ * (element strides, feature stride 1, rows 16-byte aligned).  A row whose
+ * page id is outside [0, num_pages) is not there: it is neither read nor
+ * written.  Pages may be shared by sequences for reading.
+ *
+ * The new tokens of a call are packed: tokens [cu_seqlens_q[b],
+ * cu_seqlens_q[b+1]) of [T, heads, f] belong to sequence b (any number, none
+ * included) and are the last of the seqlens_k[b] rows that its cache holds,
+ * theirs included: token i of lq sits at row seqlens_k[b] - lq + i.
+ * seqlens_k is clamped to [0, table_width * page_size]. */
+typedef struct fna2_paged_cache {
+  int32_t dtype;        /* FNA2_BF16 or FNA2_F16: q, k, v, out; R_q, R_k bf16   */
+  int32_t batch;        /* N sequences                                          */
+  int32_t total_q;      /* T: new tokens (bounds every access to them)          */
+  int32_t max_seqlen_q; /* a hint of the longest chunk: picks the kernels       */
+  int32_t heads, heads_kv, heads_graph, head_dim, rank; /* as in fna2_problem   */
+  int32_t num_pages;    /* pages of every pool                                  */
+  int32_t page_size;    /* rows of a page: a multiple of 16                     */
+  int32_t table_width;  /* entries of a block table row                         */
+  const int32_t* block_table;  /* [N][table_stride] device                      */
+  int64_t table_stride;        /* entries between rows                          */
+  const int32_t* seqlens_k;    /* [N] device                                    */
+  const int32_t* cu_seqlens_q; /* [N+1] device                                  */
+  fna2_tensor k_pages, v_pages; /* [pages, H_KV, page_size, D]                  */
+  fna2_tensor rk_pages;         /* [pages, H_G, page_size, R]                   */
+} fna2_paged_cache;
+
+/* Attention of the new tokens over the cache:
+ *     S_ij = softmax_scale <q_i, K_j> + [h < H_G] graph_scale[h] <rq_i, Rk_j>
+ * over rows j < seqlens_k[b], with causal those up to the token's own,
+ * normalised as in fna2_fwd.  One token for each sequence is a decode step, a
+ * piece of a prompt a prefill; a call may mix them.  A token that sees no row
+ * gets out = 0, lse = -inf; so do tokens of no sequence.  No counterpart in the
+ * reference, whose multi-token step against a cache fails with the bias
+ * (FNA2/attention_fna2.py:412-429, :445-473). */
+typedef struct fna2_paged_attn_args {
+  fna2_paged_cache c;
+  int32_t causal;
+  float softmax_scale;
+  fna2_tensor q, r_q;  /* [T, H, D], [T, H_G, R]: stride_s, stride_h           */
+  const float* graph_scale; /* [H_G] fp32                                       */
+  fna2_tensor out;     /* [T, H, D], written                                   */
+  fna2_tensor lse;     /* fp32 [T, H], written; ptr NULL: not computed         */
+  void* workspace;     /* fna2_paged_attn_workspace_bytes, 16-byte aligned     */
+  size_t workspace_bytes;
+} fna2_paged_attn_args;
+
+/* Host-only validation; no GPU call. */
+int fna2_check_paged_attn(const fna2_paged_attn_args* args);
+size_t fna2_paged_attn_workspace_bytes(const fna2_paged_attn_args* args);
+/* One launch, and a second that joins the parts of split rows. */
+int fna2_paged_attn(const fna2_paged_attn_args* args, void* hip_stream);
+
+/* The cached rows' attention weights of a fna2_paged_attn call:
+ *     key_weights[b][kvh][j] += sum over b's tokens i and the query heads h of
+ *                               KV head kvh of exp(S_hij - lse[i][h])
+ * in fp32, in a fixed order (no atomics).  attn: the call's arguments, its
+ * lse written (out and workspace unused).  Rows at or past `capacity` have no
+ * weight. */
+typedef struct fna2_paged_weights_args {
+  fna2_paged_attn_args attn;
+  float* key_weights;          /* [N][H_KV][capacity], added to               */
+  int64_t stride_b, stride_h;  /* of key_weights; rows are contiguous         */
+  int32_t capacity;
+} fna2_paged_weights_args;
+
+int fna2_check_paged_weights(const fna2_paged_weights_args* args);
+int fna2_paged_weights(const fna2_paged_weights_args* args, void* hip_stream);
+
+/* The new tokens' rows into the cache, in one launch: q and k rows
+ * RMS-normalised (optional: x rsqrt(mean(x^2) + eps) w) and rotated (optional:
+ * by positions[t] * inv_freq[i], the position being the cache row unless
+ * given; y as in fna2_rope_args), in fp32 (the angle in fp64) with one
+ * rounding; q to q_out [T, H, D], k, v and r_k to their pages.  Tokens of no
+ * sequence: q copied, nothing stored.  Rows before 0 or past the table: not
+ * stored. */
+typedef struct fna2_paged_append_args {
+  fna2_paged_cache c;          /* (max_seqlen_q unused)                         */
+  fna2_tensor q, k, v, r_k;    /* [T, H, D], [T, H_KV, D] x 2, [T, H_G, R]     */
+  fna2_tensor q_out;           /* written; disjoint from every input           */
+  const int32_t* positions;    /* [T] device, or NULL                          */
+  const float* inv_freq;       /* [D/2] device, or NULL: no rotation           */
+  const float* norm_q;         /* [D] fp32, or NULL                            */
+  const float* norm_k;
+  float eps;
+} fna2_paged_append_args;
+
+int fna2_check_paged_append(const fna2_paged_append_args* args);
+int fna2_paged_append(const fna2_paged_append_args* args, void* hip_stream);
+
+/* Eviction: of every sequence with more than `budget` rows each KV head keeps
+ * the first `first`, the last `recent` and, between them, the budget - first
+ * - recent of largest key weight (NaN above all others, equal weights: the
+ * lower row), in their order, as rows 0 .. budget - 1; the others keep all.
+ * Rows are moved within the sequence's own pages (which no other sequence of
+ * the call may share), R_k rows with their KV head's.  c.cu_seqlens_q,
+ * total_q and max_seqlen_q are unused. */
+typedef struct fna2_paged_evict_args {
+  fna2_paged_cache c;
+  int32_t budget, recent, first;   /* first + recent <= budget                 */
+  const float* key_weights;        /* [N][H_KV][capacity]                      */
+  int64_t stride_b, stride_h;
+  int32_t capacity;                /* rows at or past it weigh 0               */
+  float* weights_out;              /* [N][H_KV][capacity] contiguous: the kept rows' weights, then 0 */
+  int32_t* kept;                   /* [N][H_KV][budget]: the rows kept, then -1 */
+  int32_t* new_lens;               /* [N]: min(seqlens_k, budget)              */
+} fna2_paged_evict_args;
+
+int fna2_check_paged_evict(const fna2_paged_evict_args* args);
+int fna2_paged_evict(const fna2_paged_evict_args* args, void* hip_stream);
+
 /* ABI version (FNA2_ABI_VERSION). */
 int fna2_version(void);
 
