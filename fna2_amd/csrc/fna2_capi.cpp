@@ -1371,15 +1371,22 @@ void fill_cache(fna2::PagedParams& K, const fna2_paged_cache& c) {
   K.f16 = c.dtype == FNA2_F16;
 }
 
-// Column tiles of the packed kernel: as many of a KV head's query heads as
-// have their ranks in one tile, and as many tokens as the columns then hold.
-struct Packed {
-  int gsub, nsub, tpt, rc, waves;
+// How a call runs: the kernel, its tiles, the runs that share the work, and
+// the workspace for the parts of cut tiles.
+//
+// Packed kernel: column tiles of as many of a KV head's query heads as have
+// their ranks in one tile, and as many tokens as the 32 columns then hold; where
+// the longest chunk fits one tile.  Tile kernel (`tile`) for longer ones: hw
+// heads of a KV head (up to 4) times 128 / hw tokens, so that short chunks of
+// grouped heads still read K and V once; with ranks each head brings its own
+// R_k tile, so chunks that fill 64 or 128 tokens anyway take 2 heads or one.
+struct PagedPlan {
+  bool tile;
+  int gsub, nsub, tpt, rc, hw, waves, min_steps;
   size_t part, bytes;  // offset of the (max, sum) pairs; workspace
 };
-constexpr int kPagedMinSteps = 4;
-Packed packed_of(const fna2_paged_cache& c) {
-  Packed k{};
+PagedPlan paged_plan(const fna2_paged_cache& c) {
+  PagedPlan k{};
   const int group = c.heads / c.heads_kv;
   for (k.nsub = 1;; ++k.nsub) {
     k.gsub = (group + k.nsub - 1) / k.nsub;
@@ -1388,10 +1395,26 @@ Packed packed_of(const fna2_paged_cache& c) {
     if (k.gsub <= 32 && k.rc >= 0) break;
   }
   k.tpt = std::max(1, std::min(32 / k.gsub, c.max_seqlen_q));
+  const int64_t steps = std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);
+  k.tile = c.max_seqlen_q > k.tpt;
+  if (k.tile) {
+    const int rpl = fna2::padded_rank32(c.heads_graph, c.rank);
+    const int64_t mean = cdiv64(c.total_q, std::max(c.batch, 1));
+    k.hw = group >= 3 ? 4 : group;
+    if (rpl > 0 && mean >= 64) k.hw = std::min(k.hw, mean >= 128 ? 1 : 2);
+    k.min_steps = 8;
+    const int64_t tiles = ((int64_t)c.total_q / (128 / k.hw) + c.batch) * c.heads_kv * ((group + k.hw - 1) / k.hw);
+    k.waves = (int)std::min(256. * fna2::paged_tile_per_cu(c.head_dim, rpl, k.hw),
+                            std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
+    k.waves = (int)cdiv64(k.waves, 8) * 8;  // (whole turns of the XCDs)
+    k.part = align_up(2 * (size_t)k.waves * fna2::paged_tile_slot(c.head_dim));
+    k.bytes = k.part + align_up(2 * (size_t)k.waves * 128 * 8u);
+    return k;
+  }
+  k.min_steps = 4;
   const int64_t tiles = ((int64_t)c.total_q / k.tpt + c.batch) * c.heads_kv * k.nsub;
-  const double units = (double)tiles * (double)std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);
   k.waves = (int)std::min(256. * fna2::paged_waves_per_cu(c.head_dim, k.rc),
-                          std::max(std::ceil(units / kPagedMinSteps), 1.));
+                          std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
   const size_t rows = 2 * (size_t)k.waves * (size_t)(k.gsub * k.tpt);
   k.part = align_up(rows * (size_t)c.head_dim * 4u);
   k.bytes = k.part + align_up(rows * 8u);
@@ -1445,14 +1468,14 @@ int fna2_check_paged_attn(const fna2_paged_attn_args* a) {
 
 size_t fna2_paged_attn_workspace_bytes(const fna2_paged_attn_args* a) {
   if (fna2_check_paged_attn(a) != FNA2_OK || a->c.total_q == 0) return 0;
-  return packed_of(a->c).bytes;
+  return paged_plan(a->c).bytes;
 }
 
 int fna2_paged_attn(const fna2_paged_attn_args* a, void* stream_ptr) {
   FNA2_TRY(fna2_check_paged_attn(a));
   if (a->c.total_q == 0) return FNA2_OK;
   FNA2_TRY(check_device());
-  const Packed k = packed_of(a->c);
+  const PagedPlan k = paged_plan(a->c);
   if (!a->workspace || a->workspace_bytes < k.bytes || !aligned(a->workspace, 16))
     return FNA2_E_WORKSPACE;
   hipStream_t stream = (hipStream_t)stream_ptr;
@@ -1462,9 +1485,14 @@ int fna2_paged_attn(const fna2_paged_attn_args* a, void* stream_ptr) {
   K.nsub = k.nsub;
   K.tpt = k.tpt;
   K.waves = k.waves;
-  K.min_steps = kPagedMinSteps;
+  K.min_steps = k.min_steps;
+  K.hw = k.hw;
   K.part = (float*)a->workspace;
   K.ml = (float*)((char*)a->workspace + k.part);
+  if (k.tile) {
+    const int rpl = fna2::padded_rank32(K.H_G, K.R);
+    return fna2::launch_paged_tile(K, rpl, stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
+  }
   if (fna2::launch_paged_packed(K, k.rc, stream) != hipSuccess) return FNA2_E_LAUNCH;
   if (fna2::launch_paged_merge(K, stream) != hipSuccess) return FNA2_E_LAUNCH;
   return FNA2_OK;

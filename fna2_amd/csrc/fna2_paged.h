@@ -25,42 +25,55 @@ struct PagedParams {
   // Column tiles (the packed kernel): gsub query heads of a KV head times
   // tpt tokens are the columns of a tile; nsub such groups a KV head.
   int gsub, nsub, tpt;
-  int waves;      // resident waves that share the work
+  int waves;      // resident waves (workgroups of the tile kernel) that share the work
   int min_steps;  // key steps a wave takes at least
-  float* part;    // [2 * waves][cols][D] unnormalised numerators of split tiles
-  float* ml;      // [2 * waves][cols] (max, sum)
+  int hw;         // tile kernel: query heads of a KV head that a workgroup's waves take
+  float* part;    // [2 * waves] slots of unnormalised numerators of split tiles
+  float* ml;      // [2 * waves][columns of a tile] (max, sum)
 };
+
+// The kernels read their parameters where the launch put them, through a
+// pointer that the compiler cannot see through (kargs()): it then loads a field
+// where that is used.  Read as an ordinary argument, all of the block stays in
+// scalar registers through the key loop and pushes the loop's own out (100
+// spilled).  PagedParams is the first member of every parameter block here.
+typedef const __attribute__((address_space(4))) PagedParams* KArg;
+__device__ __forceinline__ KArg kargs() {
+  KArg p = (KArg)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 // A sequence's tokens and rows, clamped so that no access leaves [0, T) or
 // its row of the table.
 struct PagedSeq {
   int q0, lq, lk;
 };
-__device__ __forceinline__ PagedSeq paged_clamp(const PagedParams& P, int qs, int qe, int lk) {
+__device__ __forceinline__ PagedSeq paged_clamp(KArg P, int qs, int qe, int lk) {
   PagedSeq s;
-  qs = min(max(qs, 0), P.T);
-  qe = min(max(qe, qs), P.T);
+  qs = min(max(qs, 0), P->T);
+  qe = min(max(qe, qs), P->T);
   s.q0 = qs;
   s.lq = qe - qs;
-  s.lk = min(max(lk, 0), P.width * P.ps);
+  s.lk = min(max(lk, 0), P->width * P->ps);
   return s;
 }
-__device__ __forceinline__ PagedSeq paged_seq(const PagedParams& P, int b) {
-  return paged_clamp(P, P.cu[b], P.cu[b + 1], P.lens[b]);
+__device__ __forceinline__ PagedSeq paged_seq(KArg P, int b) {
+  return paged_clamp(P, P->cu[b], P->cu[b + 1], P->lens[b]);
 }
-__device__ __forceinline__ PagedSeq paged_seq_uniform(const PagedParams& P, int b) {
+__device__ __forceinline__ PagedSeq paged_seq_uniform(KArg P, int b) {
   b = uni(b);
-  const auto cu = const_space(P.cu);
-  return paged_clamp(P, uni(cu[b]), uni(cu[b + 1]), uni(*const_space(P.lens + b)));
+  const auto cu = const_space(P->cu);
+  return paged_clamp(P, uni(cu[b]), uni(cu[b + 1]), uni(*const_space(P->lens + b)));
 }
 
 // Work that the host cannot count (the lengths are on the device): the
 // sequences' units, laid end to end, are found again by every wave from the
 // lengths alone.  `units(s)` is a sequence's count.
 template <typename F>
-__device__ __forceinline__ int64_t wave_total(const PagedParams& P, int lane, F&& units) {
+__device__ __forceinline__ int64_t wave_total(KArg P, int lane, F&& units) {
   int64_t sum = 0;
-  for (int b = lane; b < P.N; b += 64) sum += units(paged_seq(P, b));
+  for (int b = lane; b < P->N; b += 64) sum += units(paged_seq(P, b));
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
   return sum;
@@ -72,12 +85,12 @@ struct PagedAt {
   int64_t rem;
 };
 template <typename F>
-__device__ __forceinline__ PagedAt wave_locate(const PagedParams& P, int lane, int64_t u,
+__device__ __forceinline__ PagedAt wave_locate(KArg P, int lane, int64_t u,
                                                F&& units) {
   int64_t base = 0;
-  for (int b0 = 0; b0 < P.N; b0 += 64) {
+  for (int b0 = 0; b0 < P->N; b0 += 64) {
     const int b = b0 + lane;
-    const int64_t mine = b < P.N ? units(paged_seq(P, b)) : 0;
+    const int64_t mine = b < P->N ? units(paged_seq(P, b)) : 0;
     int64_t end = mine;  // inclusive sum over the lanes
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -96,20 +109,20 @@ __device__ __forceinline__ PagedAt wave_locate(const PagedParams& P, int lane, i
     }
     base += __shfl(end, 63);
   }
-  return PagedAt{P.N, 0};
+  return PagedAt{P->N, 0};
 }
 
 // The page of row group `row` (a multiple of 16, below lk) and the row's
 // place in it, stepped 16 rows at a time.
 struct PageCursor {
   int page, off;
-  __device__ __forceinline__ void at(const PagedParams& P, int row) {
-    page = row / P.ps;
-    off = row - page * P.ps;
+  __device__ __forceinline__ void at(int ps, int row) {
+    page = row / ps;
+    off = row - page * ps;
   }
-  __device__ __forceinline__ void next(const PagedParams& P) {
+  __device__ __forceinline__ void next(int ps) {
     off += 16;
-    if (off >= P.ps) {
+    if (off >= ps) {
       off = 0;
       ++page;
     }
@@ -125,16 +138,67 @@ __device__ __forceinline__ int64_t uni64(int64_t x) {
 struct PackedPlan {
   int64_t total, per;
   __device__ __forceinline__ static int steps(const PagedSeq& s) { return max(cdiv(s.lk, 32), 1); }
-  __device__ __forceinline__ static int64_t units(const PagedParams& P, const PagedSeq& s) {
-    return (int64_t)cdiv(s.lq, P.tpt) * (P.H_KV * P.nsub) * steps(s);
+  __device__ __forceinline__ static int64_t units(KArg P, const PagedSeq& s) {
+    return (int64_t)cdiv(s.lq, P->tpt) * (P->H_KV * P->nsub) * steps(s);
   }
-  __device__ __forceinline__ PackedPlan(const PagedParams& P, int lane) {
+  __device__ __forceinline__ PackedPlan(KArg P, int lane) {
     total = uni64(wave_total(P, lane, [&](const PagedSeq& s) { return units(P, s); }));
-    per = max((total + P.waves - 1) / P.waves, (int64_t)P.min_steps);
+    per = max((total + P->waves - 1) / P->waves, (int64_t)P->min_steps);
   }
 };
 
-// Kernel launches (fna2_paged_attn.hip, fna2_paged_rows.hip).
+// The tile kernel's units: key steps of 32 rows of a tile of 32 * (4 / hw)
+// tokens and hw query heads of a KV head (a block; the last one of a KV head
+// may be short of heads).  Tile i of a sequence sees, causal, the rows up to
+// its last token's: ceil((off + min((i + 1) TB, lq)) / 32) units, one at least.
+struct TilePlan {
+  int64_t total, per;
+  __device__ __forceinline__ static int tokens(KArg P) { return 128 / P->hw; }
+  __device__ __forceinline__ static int blocks(KArg P) {
+    return P->H_KV * cdiv(P->group, P->hw);
+  }
+  // Units of tiles 0 .. m - 1, none of them the sequence's last.
+  __device__ __forceinline__ static int64_t before(KArg P, const PagedSeq& s, int m) {
+    if (!P->causal) return (int64_t)m * max(cdiv(s.lk, 32), 1);
+    const int t = 4 / P->hw, off = s.lk - s.lq;
+    const int64_t a = off >= 0 ? (off + 31) / 32 : -(-off / 32);  // ceil(off / 32)
+    const int64_t n0 = a > 0 ? 0 : min((int64_t)m, -a / t);       // tiles that see no row
+    return n0 + a * (m - n0) + t * ((int64_t)m * (m + 1) - n0 * (n0 + 1)) / 2;
+  }
+  __device__ __forceinline__ static int steps(KArg P, const PagedSeq& s, int i) {
+    int vis = s.lk;
+    if (P->causal) vis = min(vis, s.lk - s.lq + (i + 1) * tokens(P));
+    return max(cdiv(max(vis, 0), 32), 1);
+  }
+  __device__ __forceinline__ static int64_t head_units(KArg P, const PagedSeq& s) {
+    if (s.lq <= 0) return 0;
+    const int n = cdiv(s.lq, tokens(P));
+    return before(P, s, n - 1) + steps(P, s, n - 1);
+  }
+  __device__ __forceinline__ static int64_t units(KArg P, const PagedSeq& s) {
+    return head_units(P, s) * blocks(P);
+  }
+  // The tile of unit r (of one block of heads) and the unit's place in it.
+  __device__ __forceinline__ static int find(KArg P, const PagedSeq& s, int64_t& r) {
+    int lo = 0, hi = cdiv(s.lq, tokens(P)) - 1;  // before(lo) <= r
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before(P, s, mid) <= r) lo = mid;
+      else hi = mid - 1;
+    }
+    r -= before(P, s, lo);
+    return lo;
+  }
+  __device__ __forceinline__ TilePlan(KArg P, int lane) {
+    total = uni64(wave_total(P, lane, [&](const PagedSeq& s) { return units(P, s); }));
+    per = max((total + P->waves - 1) / P->waves, (int64_t)P->min_steps);
+  }
+};
+
+// Kernel launches (fna2_paged_attn.hip, fna2_paged_tile.hip, fna2_paged_rows.hip).
+int paged_tile_per_cu(int D, int rpl, int hw);  // resident workgroups of the tile kernel
+size_t paged_tile_slot(int D);                  // bytes of a split tile's part
+hipError_t launch_paged_tile(const PagedParams& P, int rpl, hipStream_t s);
 int paged_rank_chunks(int rch);      // as decode_rank_chunks
 int paged_waves_per_cu(int D, int rc);  // resident waves of the packed kernel
 hipError_t launch_paged_packed(const PagedParams& P, int rc, hipStream_t s);

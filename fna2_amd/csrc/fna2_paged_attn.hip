@@ -28,8 +28,7 @@
 #include <algorithm>
 
 #include "fna2_kernels.h"
-#include "fna2_paged.h"
-#include "fna2_tile.h"
+#include "fna2_paged_dev.h"
 
 namespace fna2 {
 
@@ -43,26 +42,6 @@ __device__ __forceinline__ void paged_wait() {
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));  // lgkmcnt(0)
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
-}
-
-// Whether an element-type word holds an infinity or a NaN.
-template <bool F16>
-__device__ __forceinline__ bool word_odd(uint32_t w) {
-  constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
-  return (w & E) == E || (w & (E << 16)) == (E << 16);
-}
-
-// Zeroes the keys at or past `limit` (relative to the tile's first key) of a
-// V^T operand of keys k0 .. k0 + 15 (element e of lane half hl: key k0 + 8
-// (e / 4) + 4 hl + e % 4).
-__device__ __forceinline__ bf16x8 cut_keys(bf16x8 x, int k0, int hl, int limit) {
-  u32x4 w = as_u32x4(x);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int key = k0 + 8 * (i >> 1) + 4 * hl + 2 * (i & 1);
-    w[i] &= (key < limit ? 0xffffu : 0u) | (key + 1 < limit ? 0xffff0000u : 0u);
-  }
-  return as_bf16x8(w);
 }
 
 template <int D, int RC>
@@ -79,30 +58,31 @@ struct PackCfg {
 };
 
 template <int D, int RC, bool F16>
-__device__ __forceinline__ void packed_body(const PagedParams& P) {
+__device__ __forceinline__ void packed_body() {
+  KArg P = kargs();
   using C = PackCfg<D, RC>;
   __shared__ __attribute__((aligned(1024))) uint8_t st0[C::STAGE];
   __shared__ __attribute__((aligned(1024))) uint8_t st1[C::STAGE];
   const int lane = threadIdx.x;
   const int col = lane & 31, hl = lane >> 5;
-  const int tk = col / P.gsub, hc = col - tk * P.gsub;  // token of the tile, head of the group
-  const int cols = P.gsub * P.tpt;
-  const int HB = P.H_KV * P.nsub;
+  const int tk = col / P->gsub, hc = col - tk * P->gsub;  // token of the tile, head of the group
+  const int cols = P->gsub * P->tpt;
+  const int HB = P->H_KV * P->nsub;
   const PackedPlan plan(P, lane);
 
   // Tokens of no sequence: zeros.
   {
-    const int t0 = min(max(uni(*const_space(P.cu)), 0), P.T);
-    const int t1 = min(max(uni(*const_space(P.cu + P.N)), t0), P.T);
-    const int64_t rows = (int64_t)(t0 + P.T - t1) * P.H;
+    const int t0 = min(max(uni(*const_space(P->cu)), 0), P->T);
+    const int t1 = min(max(uni(*const_space(P->cu + P->N)), t0), P->T);
+    const int64_t rows = (int64_t)(t0 + P->T - t1) * P->H;
     for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-      const int h = (int)(i % P.H);
-      int t = (int)(i / P.H);
+      const int h = (int)(i % P->H);
+      int t = (int)(i / P->H);
       if (t >= t0) t += t1 - t0;
-      uint16_t* o = (uint16_t*)P.o.ptr + (int64_t)t * P.o.ss + (int64_t)h * P.o.sh;
+      uint16_t* o = (uint16_t*)P->o.ptr + (int64_t)t * P->o.ss + (int64_t)h * P->o.sh;
       if (lane < D / 8) st16(o + 8 * lane, u32x4{0, 0, 0, 0});
-      if (lane == 0 && P.lse.ptr)
-        ((float*)P.lse.ptr)[(int64_t)t * P.lse.ss + (int64_t)h * P.lse.sh] = kNegInf;
+      if (lane == 0 && P->lse.ptr)
+        ((float*)P->lse.ptr)[(int64_t)t * P->lse.ss + (int64_t)h * P->lse.sh] = kNegInf;
     }
   }
 
@@ -123,32 +103,41 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
 
   const TrLane tl(lane);
   const RowLane rdl(lane);
-  const int crr = P.R / 8;
-  const uint32_t krb = (uint32_t)P.k.ss * 2u, vrb = (uint32_t)P.v.ss * 2u;
+  const int crr = P->R / 8;
+  const uint32_t krb = (uint32_t)P->k.ss * 2u, vrb = (uint32_t)P->v.ss * 2u;
   // lane offsets within a 16-row group: row lane / 4, chunk 4 g + (lane % 4)
   // swizzled (row bits 1..3 only, so both groups of a tile agree)
   const int lrow = lane >> 2, lch = (lane & 3) ^ swz4(lane >> 2);
   const uint32_t kvo = (uint32_t)lrow * krb + 16u * lch, vvo = (uint32_t)lrow * vrb + 16u * lch;
 
   while (u < u_end) {
+    P = kargs();
+    const bool causal = P->causal != 0;
+    const int ps = P->ps, npages = P->npages;
+    const float c2 = P->c2;
     const int s1 = (int)min((int64_t)steps, (int64_t)s0 + (u_end - u));
-    const int kvh = sg / P.nsub, h_in = (sg - kvh * P.nsub) * P.gsub;
-    const int nh = min(P.gsub, P.group - h_in);  // heads of this group
-    const int h0 = kvh * P.group + h_in;
-    const int gg = RC > 0 ? min(max(P.H_G - h0, 0), nh) : 0;  // graph heads
+    const int kvh = sg / P->nsub, h_in = (sg - kvh * P->nsub) * P->gsub;
+    const int nh = min(P->gsub, P->group - h_in);  // heads of this group
+    const int h0 = kvh * P->group + h_in;
+    const int gg = RC > 0 ? min(max(P->H_G - h0, 0), nh) : 0;  // graph heads
     const int rch = gg * crr, nrs = cdiv(rch, 2);
-    const int tok = ct * P.tpt + tk;
-    const bool live = tk < P.tpt && tok < e.lq && hc < nh;
+    const int tok = ct * P->tpt + tk;
+    const bool live = tk < P->tpt && tok < e.lq && hc < nh;
     const int off = e.lk - e.lq;
     // last key that this column, and that every column, sees
-    const int lim = P.causal ? off + tok : e.lk - 1;
-    const int lim_all = P.causal ? min(off + ct * P.tpt, e.lk - 1) : e.lk - 1;
-    const int lim_any = P.causal ? off + ct * P.tpt + P.tpt - 1 : e.lk - 1;  // ... that any sees
-    const int* trow = P.table + (int64_t)b * P.tstride;
+    const int lim = causal ? off + tok : e.lk - 1;
+    const int lim_all = causal ? min(off + ct * P->tpt, e.lk - 1) : e.lk - 1;
+    const int lim_any = causal ? off + ct * P->tpt + P->tpt - 1 : e.lk - 1;  // ... that any sees
+    const int* trow = P->table + (int64_t)b * P->tstride;
+    const uint16_t* const kpool = (const uint16_t*)P->k.ptr + (int64_t)kvh * P->k.sh;
+    const uint16_t* const vpool = (const uint16_t*)P->v.ptr + (int64_t)kvh * P->v.sh;
+    const uint16_t* const rpool = RC > 0 ? (const uint16_t*)P->rk.ptr + (int64_t)h0 * P->rk.sh : nullptr;
+    const int64_t ksb = P->k.sb, vsb = P->v.sb, rsb = P->rk.sb;
+    const uint32_t rrb = (uint32_t)P->rk.ss * 2u;
 
     uint32_t roff[RC > 0 ? C::NR : 1];
     if constexpr (RC > 0) {
-      const uint32_t hs = (uint32_t)P.rk.sh * 2u, rs = (uint32_t)P.rk.ss * 2u;
+      const uint32_t hs = (uint32_t)P->rk.sh * 2u, rs = (uint32_t)P->rk.ss * 2u;
 #pragma unroll
       for (int i = 0; i < C::NR; ++i) {
         const int c = 4 * i + lch;
@@ -157,11 +146,11 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
       }
     }
     PageCursor cur;
-    cur.at(P, 32 * s0);
+    cur.at(ps, 32 * s0);
     auto page_id = [&](int row) {  // of the cursor's row group; -1 past the run or the pool
       if (row >= e.lk) return -1;
       const int id = uni(*const_space(trow + cur.page));
-      return (uint32_t)id < (uint32_t)P.npages ? id : -1;
+      return (uint32_t)id < (uint32_t)npages ? id : -1;
     };
     // ids and places of the next tile's two row groups
     int pid[2], poff[2];
@@ -170,7 +159,7 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
       for (int g = 0; g < 2; ++g) {
         pid[g] = t < s1 ? page_id(32 * t + 16 * g) : -1;
         poff[g] = cur.off;
-        cur.next(P);
+        cur.next(ps);
       }
     };
     // Tile t (looked up before) into `base`; returns the row groups that are
@@ -185,10 +174,10 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
         if (!here && row < e.lk) gone |= 1 << g;
         const int64_t id = here ? pid[g] : 0;
         const int r = here ? poff[g] : 0;
-        const auto rk_ = make_rsrc((const uint16_t*)P.k.ptr + id * P.k.sb + (int64_t)kvh * P.k.sh +
-                                       (int64_t)r * P.k.ss, (uint32_t)rows * krb);
-        const auto rv_ = make_rsrc((const uint16_t*)P.v.ptr + id * P.v.sb + (int64_t)kvh * P.v.sh +
-                                       (int64_t)r * P.v.ss, (uint32_t)rows * vrb);
+        const auto rk_ = make_rsrc((const uint8_t*)(kpool + id * ksb) + (uint64_t)(uint32_t)r * krb,
+                                   (uint32_t)rows * krb);
+        const auto rv_ = make_rsrc((const uint8_t*)(vpool + id * vsb) + (uint64_t)(uint32_t)r * vrb,
+                                   (uint32_t)rows * vrb);
 #pragma unroll
         for (int i = 0; i < C::NG; ++i) {
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rk_, (lds_void*)(base + (2 * i + g) * 1024), 16,
@@ -198,9 +187,7 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
               vvo + 64u * i, 0, 0, 0);
         }
         if constexpr (RC > 0) {
-          const auto rr = make_rsrc(gg > 0 ? (const uint16_t*)P.rk.ptr + id * P.rk.sb +
-                                                 (int64_t)h0 * P.rk.sh + (int64_t)r * P.rk.ss
-                                           : (const uint16_t*)P.k.ptr,
+          const auto rr = make_rsrc((const uint8_t*)(rpool + id * rsb) + (uint64_t)(uint32_t)r * rrb,
                                     rows > 0 && gg > 0 ? 0x7ffffff0u : 0u);
 #pragma unroll
           for (int i = 0; i < C::NR; ++i)
@@ -222,9 +209,9 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
     float bh = 0.f;
     {
       const int64_t t = (int64_t)(e.q0 + (live ? tok : 0));
-      const uint16_t* qrow = (const uint16_t*)P.q.ptr + t * P.q.ss + (int64_t)(h0 + hc) * P.q.sh;
-      const uint32_t qxor = P.qa < 0.f ? 0x80008000u : 0u;
-      const uint32_t qand = P.qa == 0.f ? 0u : 0xffffffffu;
+      const uint16_t* qrow = (const uint16_t*)P->q.ptr + t * P->q.ss + (int64_t)(h0 + hc) * P->q.sh;
+      const uint32_t qxor = P->qa < 0.f ? 0x80008000u : 0u;
+      const uint32_t qand = P->qa == 0.f ? 0u : 0xffffffffu;
 #pragma unroll
       for (int s = 0; s < C::KSD; ++s) {
         u32x4 w = {0, 0, 0, 0};
@@ -235,8 +222,8 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
       }
       if constexpr (RC > 0) {
         const bool g = live && hc < gg;
-        const uint16_t* rrow = (const uint16_t*)P.rq.ptr + t * P.rq.ss + (int64_t)(h0 + hc) * P.rq.sh;
-        bh = g ? P.gs[h0 + hc] / P.c : 0.f;
+        const uint16_t* rrow = (const uint16_t*)P->rq.ptr + t * P->rq.ss + (int64_t)(h0 + hc) * P->rq.sh;
+        bh = g ? P->gs[h0 + hc] / P->c : 0.f;
 #pragma unroll
         for (int s = 0; s < C::KSR; ++s) {
           const int c = 2 * s + hl;  // concatenated chunk of this lane
@@ -252,12 +239,19 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
     for (int d = 0; d < D / 32; ++d) oacc[d] = f32x16{};
     float m_i = kNegInf, l_i = 0.f;
 
-    auto step = [&](int t, const uint8_t* cur_st, uint8_t* nxt_st) {
+    auto step = [&](int t, uint8_t* cur_st, uint8_t* nxt_st) {
       paged_wait<0>();
       const int gone_now = gone;
       gone = issue(t + 1, nxt_st);  // (past the run: zeros, from no memory)
       __builtin_amdgcn_sched_barrier(0);
       if (32 * t > lim_any) return;  // no column sees these rows
+      if (causal && 32 * t + 31 > lim_all) {
+        uint8_t* v = cur_st + C::KBYTES + C::RBYTES;
+        if (__builtin_expect(tile_odd<C::KBYTES / 1024, F16>(v, lane), 0)) {
+          add_odd<D, kPagBN, F16>(v, 32 * t, lim, hl, oacc);
+          tile_clean<C::KBYTES / 1024, F16>(v, lane);
+        }
+      }
       const uint8_t* kl = cur_st;
       const uint8_t* rl = kl + C::KBYTES;
       const uint8_t* vl = rl + C::RBYTES;
@@ -287,7 +281,7 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
       mx = wave_pair_max(mx);
       const float m_new = fmaxf(m_i, mx);
       const float m_use = (m_new == kNegInf) ? 0.f : m_new;
-      const float nm = -m_use * P.c2;
+      const float nm = -m_use * c2;
       float ls = 0.f;
       // P in two parts (as the decode kernel): the first cut to the element
       // type, the second what that cut off, so that the result does not
@@ -300,8 +294,8 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int v0 = 8 * half + 2 * i;
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v0], P.c2, nm));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v0 + 1], P.c2, nm));
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v0], c2, nm));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v0 + 1], c2, nm));
           ls += p0 + p1;
           if constexpr (F16) {
             pk[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
@@ -319,54 +313,21 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
         pe[half] = as_bf16x8(ek);
       }
       if (__builtin_amdgcn_ballot_w64(m_new != m_i) != 0) {
-        const float alpha = __builtin_amdgcn_exp2f((m_i - m_use) * P.c2);
+        const float alpha = weight2((m_i - m_use) * c2);
         l_i *= alpha;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) oacc[d] *= alpha;
       }
       l_i += ls;
       m_i = m_new;
-      // Rows that some columns see and others do not may hold infinities or
-      // NaN (a later token's V): 0 times those is NaN, so then each token's
-      // columns take their product with the rows past its own zeroed.
-      bool odd = false;
-      if (masked && P.causal) {
-        for (int i = 0; i < C::KBYTES / 1024; ++i) {
-          const u32x4 w = *(const u32x4*)(vl + 1024 * i + 16 * lane);
-          odd |= word_odd<F16>(w[0]) || word_odd<F16>(w[1]) || word_odd<F16>(w[2]) ||
-                 word_odd<F16>(w[3]);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+          const bf16x8 vt = tr_operand<kPagBN>(vl, tl, 16 * s, 32 * d);
+          oacc[d] = mfma_e<F16>(vt, pb[s], oacc[d]);
+          oacc[d] = mfma_e<F16>(vt, pe[s], oacc[d]);
         }
-        odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-      }
-      if (!odd) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d) {
-            const bf16x8 vt = tr_operand<kPagBN>(vl, tl, 16 * s, 32 * d);
-            oacc[d] = mfma_e<F16>(vt, pb[s], oacc[d]);
-            oacc[d] = mfma_e<F16>(vt, pe[s], oacc[d]);
-          }
-      } else {
-        for (int j = 0; j < P.tpt; ++j) {
-          const int cut = off + ct * P.tpt + j + 1 - kbase;  // keys the token sees
-          const uint32_t mine = tk == j ? 0xffffffffu : 0u;
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            u32x4 a = as_u32x4(pb[s]), c = as_u32x4(pe[s]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] &= mine, c[i] &= mine;
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-              const bf16x8 vt = cut_keys(tr_operand<kPagBN>(vl, tl, 16 * s, 32 * d), 16 * s, hl, cut);
-              // (the other columns' accumulators must not see this V at all)
-              const f32x16 y = mfma_e<F16>(vt, as_bf16x8(c), mfma_e<F16>(vt, as_bf16x8(a), oacc[d]));
-#pragma unroll
-              for (int v = 0; v < 16; ++v) oacc[d][v] = mine ? y[v] : oacc[d][v];
-            }
-          }
-        }
-      }
     };
 
     for (int t = s0; t < s1; t += 2) {
@@ -375,11 +336,12 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
     }
     paged_wait<0>();  // no DMA may still write when the ring is used again, or the wave ends
 
+    P = kargs();
     const float l_tot = wave_pair_sum(l_i);
     if (s0 == 0 && s1 == steps) {
       if (live) {
         const float inv = 1.f / (l_tot + 1e-6f);
-        uint16_t* orow = (uint16_t*)P.o.ptr + (int64_t)(e.q0 + tok) * P.o.ss + (int64_t)(h0 + hc) * P.o.sh;
+        uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)(h0 + hc) * P->o.sh;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -389,15 +351,15 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
             val[1] = pack_e<F16>(oacc[d][4 * g + 2] * inv, oacc[d][4 * g + 3] * inv);
             *(u32x2*)(orow + d * 32 + 8 * g + 4 * hl) = val;
           }
-        if (hl == 0 && P.lse.ptr)
-          ((float*)P.lse.ptr)[(int64_t)(e.q0 + tok) * P.lse.ss + (int64_t)(h0 + hc) * P.lse.sh] =
-              m_i == kNegInf ? kNegInf : m_i * P.c + __builtin_amdgcn_logf(l_tot + 1e-6f) * kLn2;
+        if (hl == 0 && P->lse.ptr)
+          ((float*)P->lse.ptr)[(int64_t)(e.q0 + tok) * P->lse.ss + (int64_t)(h0 + hc) * P->lse.sh] =
+              m_i == kNegInf ? kNegInf : m_i * P->c + __builtin_amdgcn_logf(l_tot + 1e-6f) * kLn2;
       }
     } else if (col < cols) {
       // slot 2 w: wave w's run ends or lies in a tile begun before it; 2 w + 1:
       // it begins the tile
       const int64_t slot = 2 * (int64_t)blockIdx.x + (s0 == 0 ? 1 : 0);
-      float* arow = P.part + (slot * cols + col) * D;
+      float* arow = P->part + (slot * cols + col) * D;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -405,16 +367,16 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
           f32x4_t val = {oacc[d][4 * g], oacc[d][4 * g + 1], oacc[d][4 * g + 2], oacc[d][4 * g + 3]};
           *(f32x4_t*)(arow + d * 32 + 8 * g + 4 * hl) = val;
         }
-      if (hl == 0) *(f32x2*)(P.ml + 2 * (slot * cols + col)) = f32x2{m_i, l_tot};
+      if (hl == 0) *(f32x2*)(P->ml + 2 * (slot * cols + col)) = f32x2{m_i, l_tot};
     }
 
     u += s1 - s0;
     s0 = 0;
     if (u < u_end && ++sg == HB) {
       sg = 0;
-      if ((++ct) * P.tpt >= e.lq) {
+      if ((++ct) * P->tpt >= e.lq) {
         ct = 0;
-        do e = paged_seq_uniform(P, ++b); while (e.lq == 0 && b + 1 < P.N);
+        do e = paged_seq_uniform(P, ++b); while (e.lq == 0 && b + 1 < P->N);
         steps = PackedPlan::steps(e);
       }
     }
@@ -425,7 +387,8 @@ __device__ __forceinline__ void packed_body(const PagedParams& P) {
 // that the boundary between runs i and i + 1 cuts, if it is the tile's first.
 // LPR lanes hold a row of D values; `WAYS` groups of lanes share a row's parts.
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams P) {
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
+  KArg P = kargs();
   constexpr int LPR = D / 4, NG = 256 / LPR;
   __shared__ float part[NG][D];
   __shared__ float stat[NG][2];
@@ -436,30 +399,30 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams P) {
   if (u >= plan.total) return;
   const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return PackedPlan::units(P, s); });
   const PagedSeq e = paged_seq_uniform(P, at.b);
-  const int steps = PackedPlan::steps(e), HB = P.H_KV * P.nsub;
+  const int steps = PackedPlan::steps(e), HB = P->H_KV * P->nsub;
   const int64_t tile = at.rem / steps;
   const int s0 = (int)(at.rem - tile * steps);
   if (s0 == 0 || s0 > plan.per) return;  // not cut here; or an earlier boundary cuts it too
   const int64_t tile_end = u - s0 + steps;
   const int n = (int)((tile_end - 1) / plan.per - i0) + 1;  // runs that hold a part
   const int ct = (int)(tile / HB), sg = (int)(tile - (int64_t)ct * HB);
-  const int kvh = sg / P.nsub, h_in = (sg - kvh * P.nsub) * P.gsub;
-  const int nh = min(P.gsub, P.group - h_in), h0 = kvh * P.group + h_in;
-  const int cols = P.gsub * P.tpt;
+  const int kvh = sg / P->nsub, h_in = (sg - kvh * P->nsub) * P->gsub;
+  const int nh = min(P->gsub, P->group - h_in), h0 = kvh * P->group + h_in;
+  const int cols = P->gsub * P->tpt;
   const int grp = threadIdx.x / LPR, f = 4 * (threadIdx.x % LPR);
   for (int c = blockIdx.y; c < cols; c += gridDim.y) {
-    const int tk = c / P.gsub, hc = c - tk * P.gsub, tok = ct * P.tpt + tk;
+    const int tk = c / P->gsub, hc = c - tk * P->gsub, tok = ct * P->tpt + tk;
     if (tok >= e.lq || hc >= nh) continue;  // (uniform)
     float M = kNegInf, L = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
     for (int j = grp; j < n; j += NG) {
       const int64_t slot = j == 0 ? 2 * i0 + 1 : 2 * (i0 + j);
-      const f32x2 ml = *(const f32x2*)(P.ml + 2 * (slot * cols + c));
-      const f32x4_t x = *(const f32x4_t*)(P.part + (slot * cols + c) * D + f);
+      const f32x2 ml = *(const f32x2*)(P->ml + 2 * (slot * cols + c));
+      const f32x4_t x = *(const f32x4_t*)(P->part + (slot * cols + c) * D + f);
       const float m = fmaxf(M, ml[0]);
       const float ref = m == kNegInf ? 0.f : m;
-      const float wa = __builtin_amdgcn_exp2f((M - ref) * P.c2);
-      const float wb = __builtin_amdgcn_exp2f((ml[0] - ref) * P.c2);
+      const float wa = weight2((M - ref) * P->c2);
+      const float wb = weight2((ml[0] - ref) * P->c2);
       L = L * wa + ml[1] * wb;
       o = o * wa + x * wb;
       M = m;
@@ -475,17 +438,17 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams P) {
       const float ref = m == kNegInf ? 0.f : m;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        const float w = __builtin_amdgcn_exp2f((stat[g][0] - ref) * P.c2);
+        const float w = weight2((stat[g][0] - ref) * P->c2);
         l += stat[g][1] * w;
         y0 += part[g][d] * w;
         y1 += part[g][d + 1] * w;
       }
       const float inv = 1.f / (l + 1e-6f);
-      uint16_t* orow = (uint16_t*)P.o.ptr + (int64_t)(e.q0 + tok) * P.o.ss + (int64_t)(h0 + hc) * P.o.sh;
+      uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)(h0 + hc) * P->o.sh;
       *(uint32_t*)(orow + d) = pack_e<F16>(y0 * inv, y1 * inv);
-      if (d == 0 && P.lse.ptr)
-        ((float*)P.lse.ptr)[(int64_t)(e.q0 + tok) * P.lse.ss + (int64_t)(h0 + hc) * P.lse.sh] =
-            m == kNegInf ? kNegInf : m * P.c + __builtin_amdgcn_logf(l + 1e-6f) * kLn2;
+      if (d == 0 && P->lse.ptr)
+        ((float*)P->lse.ptr)[(int64_t)(e.q0 + tok) * P->lse.ss + (int64_t)(h0 + hc) * P->lse.sh] =
+            m == kNegInf ? kNegInf : m * P->c + __builtin_amdgcn_logf(l + 1e-6f) * kLn2;
     }
     __syncthreads();
   }
@@ -499,13 +462,13 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams P) {
 template <int D, int RPL, bool F16>
 __global__ __launch_bounds__(256) void paged_weights_kernel(const PagedWeightsParams W) {
   constexpr int KSD = D / 16, KSR = RPL / 16;
-  const PagedParams& P = W.p;
+  KArg P = kargs();
   const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
   const int col = lane & 31, hl = lane >> 5;
-  auto units = [&](const PagedSeq& s) { return s.lq > 0 ? (int64_t)P.H_KV * cdiv(s.lk, 128) : 0; };
+  auto units = [&](const PagedSeq& s) { return s.lq > 0 ? (int64_t)P->H_KV * cdiv(s.lk, 128) : 0; };
   const int64_t total = uni64(wave_total(P, lane, units));
-  const uint32_t qxor = P.qa < 0.f ? 0x80008000u : 0u;
-  const uint32_t qand = P.qa == 0.f ? 0u : 0xffffffffu;
+  const uint32_t qxor = P->qa < 0.f ? 0x80008000u : 0u;
+  const uint32_t qand = P->qa == 0.f ? 0u : 0xffffffffu;
   for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
     const PagedAt at = wave_locate(P, lane, id, units);
     const PagedSeq e = paged_seq_uniform(P, at.b);
@@ -515,16 +478,16 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const PagedWeightsPa
     const int key = k0 + col, off = e.lk - e.lq;
     int page = -1, r = 0;
     if (key < e.lk) {
-      page = P.table[(int64_t)at.b * P.tstride + key / P.ps];
-      r = key % P.ps;
-      if ((uint32_t)page >= (uint32_t)P.npages) page = -1;
+      page = P->table[(int64_t)at.b * P->tstride + key / P->ps];
+      r = key % P->ps;
+      if ((uint32_t)page >= (uint32_t)P->npages) page = -1;
     }
     const bool here = page >= 0 && key < W.cap;
     if (__builtin_amdgcn_ballot_w64(here) == 0) continue;
     bf16x8 kreg[KSD];
     const int64_t id64 = page < 0 ? 0 : page;
     {
-      const uint16_t* krow = (const uint16_t*)P.k.ptr + id64 * P.k.sb + (int64_t)kvh * P.k.sh + (int64_t)r * P.k.ss;
+      const uint16_t* krow = (const uint16_t*)P->k.ptr + id64 * P->k.sb + (int64_t)kvh * P->k.sh + (int64_t)r * P->k.ss;
 #pragma unroll
       for (int s = 0; s < KSD; ++s) {
         u32x4 w = {0, 0, 0, 0};
@@ -535,18 +498,18 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const PagedWeightsPa
       }
     }
     float sum = 0.f;
-    const int i_first = P.causal ? max(k0 - off, 0) & ~31 : 0;  // earlier tokens see no key here
-    for (int h = kvh * P.group; h < (kvh + 1) * P.group; ++h) {
-      const bool graph = RPL > 0 && h < P.H_G;
+    const int i_first = P->causal ? max(k0 - off, 0) & ~31 : 0;  // earlier tokens see no key here
+    for (int h = kvh * P->group; h < (kvh + 1) * P->group; ++h) {
+      const bool graph = RPL > 0 && h < P->H_G;
       bf16x8 rkreg[KSR > 0 ? KSR : 1];
       float bh = 0.f;
       if constexpr (KSR > 0) {
-        const uint16_t* rrow = (const uint16_t*)P.rk.ptr + id64 * P.rk.sb + (int64_t)h * P.rk.sh + (int64_t)r * P.rk.ss;
-        bh = graph ? *const_space(P.gs + h) / P.c : 0.f;
+        const uint16_t* rrow = (const uint16_t*)P->rk.ptr + id64 * P->rk.sb + (int64_t)h * P->rk.sh + (int64_t)r * P->rk.ss;
+        bh = graph ? *const_space(P->gs + h) / P->c : 0.f;
 #pragma unroll
         for (int s = 0; s < KSR; ++s) {
           u32x4 w = {0, 0, 0, 0};
-          if (here && graph && 16 * s + 8 * hl < P.R) w = ld16(rrow + 16 * s + 8 * hl);
+          if (here && graph && 16 * s + 8 * hl < P->R) w = ld16(rrow + 16 * s + 8 * hl);
           rkreg[s] = as_bf16x8(w);
         }
       }
@@ -556,16 +519,16 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const PagedWeightsPa
         const int64_t t = e.q0 + (have ? tok : 0);
         f32x16 acc = f32x16{};
         if constexpr (KSR > 0) {
-          const uint16_t* rrow = (const uint16_t*)P.rq.ptr + t * P.rq.ss + (int64_t)h * P.rq.sh;
+          const uint16_t* rrow = (const uint16_t*)P->rq.ptr + t * P->rq.ss + (int64_t)h * P->rq.sh;
 #pragma unroll
           for (int s = 0; s < KSR; ++s) {
             u32x4 w = {0, 0, 0, 0};
-            if (have && graph && 16 * s + 8 * hl < P.R) w = ld16(rrow + 16 * s + 8 * hl);
+            if (have && graph && 16 * s + 8 * hl < P->R) w = ld16(rrow + 16 * s + 8 * hl);
             acc = mfma32(as_bf16x8(w), rkreg[s], acc);
           }
           acc *= bh;
         }
-        const uint16_t* qrow = (const uint16_t*)P.q.ptr + t * P.q.ss + (int64_t)h * P.q.sh;
+        const uint16_t* qrow = (const uint16_t*)P->q.ptr + t * P->q.ss + (int64_t)h * P->q.sh;
 #pragma unroll
         for (int s = 0; s < KSD; ++s) {
           u32x4 w = {0, 0, 0, 0};
@@ -576,13 +539,13 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const PagedWeightsPa
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const int row = i0 + 8 * (v >> 2) + 4 * hl + (v & 3);
-          const bool see = row < e.lq && (!P.causal || key <= off + row);
+          const bool see = row < e.lq && (!P->causal || key <= off + row);
           float nl = kNegInf;
           if (row < e.lq) {
-            const float l = ((const float*)P.lse.ptr)[(int64_t)(e.q0 + row) * P.lse.ss + (int64_t)h * P.lse.sh];
+            const float l = ((const float*)P->lse.ptr)[(int64_t)(e.q0 + row) * P->lse.ss + (int64_t)h * P->lse.sh];
             nl = l == kNegInf ? kNegInf : -l * kLog2e;
           }
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], P.c2, nl));
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], P->c2, nl));
           part += see && nl != kNegInf ? p : 0.f;
         }
         sum += part;
@@ -597,11 +560,11 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(const PagedWeightsPa
 }
 
 #define FNA2_PACKED(D, RC)                                                                     \
-  __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC(const PagedParams P) {    \
-    packed_body<D, RC, false>(P);                                                              \
+  __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC(const PagedParams) {    \
+    packed_body<D, RC, false>();                                                               \
   }                                                                                            \
-  __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC##_f16(const PagedParams P) { \
-    packed_body<D, RC, true>(P);                                                               \
+  __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC##_f16(const PagedParams) { \
+    packed_body<D, RC, true>();                                                                \
   }
 FNA2_PACKED(64, 0)
 FNA2_PACKED(64, 4)

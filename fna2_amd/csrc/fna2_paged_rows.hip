@@ -56,7 +56,7 @@ __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const Page
     int64_t page = -1;
     int pr = 0;
     if (inside) {
-      const PagedSeq e = paged_seq_uniform(P, lo);
+      const PagedSeq e = paged_seq_uniform(kargs(), lo);
       row = e.lk - e.lq + (t - e.q0);
       if (row >= 0 && row < e.lk) {
         const int pg = row / P.ps;
