@@ -1383,7 +1383,7 @@ void fill_cache(fna2::PagedParams& K, const fna2_paged_cache& c) {
 struct PagedPlan {
   bool tile;
   int gsub, nsub, tpt, rc, hw, waves, min_steps;
-  size_t part, bytes;  // offset of the (max, sum) pairs; workspace
+  size_t ml, cuts, bytes;  // offsets of the (max, sum) pairs and the cuts; workspace
 };
 PagedPlan paged_plan(const fna2_paged_cache& c) {
   PagedPlan k{};
@@ -1407,8 +1407,9 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
     k.waves = (int)std::min(256. * fna2::paged_tile_per_cu(c.head_dim, rpl, k.hw),
                             std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
     k.waves = (int)cdiv64(k.waves, 8) * 8;  // (whole turns of the XCDs)
-    k.part = align_up(2 * (size_t)k.waves * fna2::paged_tile_slot(c.head_dim));
-    k.bytes = k.part + align_up(2 * (size_t)k.waves * 128 * 8u);
+    k.ml = align_up(2 * (size_t)k.waves * fna2::paged_tile_slot(c.head_dim));
+    k.cuts = k.ml + align_up(2 * (size_t)k.waves * 128 * 8u);
+    k.bytes = k.cuts + align_up((size_t)k.waves * sizeof(fna2::PagedCut));
     return k;
   }
   k.min_steps = 4;
@@ -1416,8 +1417,9 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
   k.waves = (int)std::min(256. * fna2::paged_waves_per_cu(c.head_dim, k.rc),
                           std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
   const size_t rows = 2 * (size_t)k.waves * (size_t)(k.gsub * k.tpt);
-  k.part = align_up(rows * (size_t)c.head_dim * 4u);
-  k.bytes = k.part + align_up(rows * 8u);
+  k.ml = align_up(rows * (size_t)c.head_dim * 4u);
+  k.cuts = k.ml + align_up(rows * 8u);
+  k.bytes = k.cuts + align_up((size_t)k.waves * sizeof(fna2::PagedCut));
   return k;
 }
 
@@ -1488,7 +1490,8 @@ int fna2_paged_attn(const fna2_paged_attn_args* a, void* stream_ptr) {
   K.min_steps = k.min_steps;
   K.hw = k.hw;
   K.part = (float*)a->workspace;
-  K.ml = (float*)((char*)a->workspace + k.part);
+  K.ml = (float*)((char*)a->workspace + k.ml);
+  K.cuts = (fna2::PagedCut*)((char*)a->workspace + k.cuts);
   if (k.tile) {
     const int rpl = fna2::padded_rank32(K.H_G, K.R);
     return fna2::launch_paged_tile(K, rpl, stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;

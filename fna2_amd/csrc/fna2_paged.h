@@ -6,6 +6,12 @@
 
 namespace fna2 {
 
+// A tile that the end of run i cuts (parts > 0), if no earlier run's end does:
+// what the merge needs to join its parts, which lie with runs i .. i + parts - 1.
+struct __attribute__((aligned(16))) PagedCut {
+  int b, head, tile, parts;  // sequence; block of heads; tile of tokens
+};
+
 // A paged cache and the chunk of new tokens that belongs to it.  Row j of
 // sequence b: row j % ps of page table[b * tstride + j / ps]; page p, head
 // h, row r of a pool at ptr + p * sb + h * sh + r * ss.
@@ -28,6 +34,7 @@ struct PagedParams {
   int waves;      // resident waves (workgroups of the tile kernel) that share the work
   int min_steps;  // key steps a wave takes at least
   int hw;         // tile kernel: query heads of a KV head that a workgroup's waves take
+  struct PagedCut* cuts;  // [waves]
   float* part;    // [2 * waves] slots of unnormalised numerators of split tiles
   float* ml;      // [2 * waves][columns of a tile] (max, sum)
 };

@@ -88,7 +88,13 @@ __device__ __forceinline__ void packed_body() {
 
   int64_t u = (int64_t)blockIdx.x * plan.per;
   const int64_t u_end = min(plan.total, u + plan.per);
-  if (u >= u_end) return;
+  auto cut = [&](int b, int head, int tile, int parts) {
+    if (lane == 0) P->cuts[blockIdx.x] = PagedCut{b, head, tile, parts};
+  };
+  if (u >= u_end) {
+    cut(0, 0, 0, 0);
+    return;
+  }
   const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return PackedPlan::units(P, s); });
   int b = at.b;
   PagedSeq e = paged_seq_uniform(P, b);
@@ -110,7 +116,7 @@ __device__ __forceinline__ void packed_body() {
   const int lrow = lane >> 2, lch = (lane & 3) ^ swz4(lane >> 2);
   const uint32_t kvo = (uint32_t)lrow * krb + 16u * lch, vvo = (uint32_t)lrow * vrb + 16u * lch;
 
-  while (u < u_end) {
+  while (true) {
     P = kargs();
     const bool causal = P->causal != 0;
     const int ps = P->ps, npages = P->npages;
@@ -371,8 +377,13 @@ __device__ __forceinline__ void packed_body() {
     }
 
     u += s1 - s0;
+    if (u >= u_end) {
+      const int rest = steps - s1;
+      cut(b, sg, ct, s0 == 0 && rest > 0 ? 1 + (int)((rest + plan.per - 1) / plan.per) : 0);
+      return;
+    }
     s0 = 0;
-    if (u < u_end && ++sg == HB) {
+    if (++sg == HB) {
       sg = 0;
       if ((++ct) * P->tpt >= e.lq) {
         ct = 0;
@@ -383,67 +394,82 @@ __device__ __forceinline__ void packed_body() {
   }
 }
 
-// Joins the parts of the tiles that runs cut: workgroup (i, y) takes the tile
-// that the boundary between runs i and i + 1 cuts, if it is the tile's first.
-// LPR lanes hold a row of D values; `WAYS` groups of lanes share a row's parts.
+// Joins the parts of a tile that runs cut: workgroup (i, y) columns y, y +
+// gridDim.y, ... of the tile that run i's end cuts.  The parts' weights first
+// (their maxima and sums), then D / 4 lanes a row and as many parts at once as
+// the workgroup then holds, four deep.  The parts' order is that of the runs.
+constexpr int kMergeParts = 2048;  // at most one part for each resident wave
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
   KArg P = kargs();
   constexpr int LPR = D / 4, NG = 256 / LPR;
+  __shared__ float wt[kMergeParts];
   __shared__ float part[NG][D];
-  __shared__ float stat[NG][2];
-  const int lane = threadIdx.x & 63;
-  const PackedPlan plan(P, lane);
-  const int64_t i0 = blockIdx.x;  // the run before the boundary
-  const int64_t u = (i0 + 1) * plan.per;
-  if (u >= plan.total) return;
-  const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return PackedPlan::units(P, s); });
-  const PagedSeq e = paged_seq_uniform(P, at.b);
-  const int steps = PackedPlan::steps(e), HB = P->H_KV * P->nsub;
-  const int64_t tile = at.rem / steps;
-  const int s0 = (int)(at.rem - tile * steps);
-  if (s0 == 0 || s0 > plan.per) return;  // not cut here; or an earlier boundary cuts it too
-  const int64_t tile_end = u - s0 + steps;
-  const int n = (int)((tile_end - 1) / plan.per - i0) + 1;  // runs that hold a part
-  const int ct = (int)(tile / HB), sg = (int)(tile - (int64_t)ct * HB);
+  __shared__ float red[4], red2[4];
+  const int i0 = blockIdx.x;
+  const auto rec = const_space(P->cuts + i0);
+  const int n = uni(rec->parts);
+  if (n <= 0) return;
+  const int ct = uni(rec->tile), sg = uni(rec->head);
+  const PagedSeq e = paged_seq_uniform(P, rec->b);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int kvh = sg / P->nsub, h_in = (sg - kvh * P->nsub) * P->gsub;
   const int nh = min(P->gsub, P->group - h_in), h0 = kvh * P->group + h_in;
   const int cols = P->gsub * P->tpt;
   const int grp = threadIdx.x / LPR, f = 4 * (threadIdx.x % LPR);
+  const float c2 = P->c2;
+  auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * i0 + 1 : 2 * (i0 + j)); };
   for (int c = blockIdx.y; c < cols; c += gridDim.y) {
     const int tk = c / P->gsub, hc = c - tk * P->gsub, tok = ct * P->tpt + tk;
     if (tok >= e.lq || hc >= nh) continue;  // (uniform)
-    float M = kNegInf, L = 0.f;
+    const float* src = P->part + (int64_t)c * D + f;
+    f32x4_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = grp + k * NG;
+      if (j < n) x[k] = *(const f32x4_t*)(src + slot(j) * cols * D);
+    }
+    float m = kNegInf;
+    for (int j = threadIdx.x; j < n; j += 256) m = fmaxf(m, P->ml[2 * (slot(j) * cols + c)]);
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    if (lane == 0) red[wv] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float ref = m == kNegInf ? 0.f : m;
+    float l = 0.f;
+    for (int j = threadIdx.x; j < n; j += 256) {
+      const f32x2 ml = *(const f32x2*)(P->ml + 2 * (slot(j) * cols + c));
+      const float w = weight2((ml[0] - ref) * c2);
+      wt[j] = w;
+      l += ml[1] * w;
+    }
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) l += __shfl_xor(l, k);
+    if (lane == 0) red2[wv] = l;
+    __syncthreads();
+    l = (red2[0] + red2[1]) + (red2[2] + red2[3]);
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int j = grp; j < n; j += NG) {
-      const int64_t slot = j == 0 ? 2 * i0 + 1 : 2 * (i0 + j);
-      const f32x2 ml = *(const f32x2*)(P->ml + 2 * (slot * cols + c));
-      const f32x4_t x = *(const f32x4_t*)(P->part + (slot * cols + c) * D + f);
-      const float m = fmaxf(M, ml[0]);
-      const float ref = m == kNegInf ? 0.f : m;
-      const float wa = weight2((M - ref) * P->c2);
-      const float wb = weight2((ml[0] - ref) * P->c2);
-      L = L * wa + ml[1] * wb;
-      o = o * wa + x * wb;
-      M = m;
+    for (int base = 0; base < n; base += 4 * NG) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = base + grp + k * NG;
+        if (j < n) o += wt[j] * x[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = base + grp + (4 + k) * NG;
+        if (j < n) x[k] = *(const f32x4_t*)(src + slot(j) * cols * D);
+      }
     }
     *(f32x4_t*)(&part[grp][f]) = o;
-    if (f == 0) stat[grp][0] = M, stat[grp][1] = L;
     __syncthreads();
+    const float inv = 1.f / (l + 1e-6f);
     if (threadIdx.x < D / 2) {
       const int d = 2 * threadIdx.x;
-      float m = kNegInf, l = 0.f, y0 = 0.f, y1 = 0.f;
+      float y0 = 0.f, y1 = 0.f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) m = fmaxf(m, stat[g][0]);
-      const float ref = m == kNegInf ? 0.f : m;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const float w = weight2((stat[g][0] - ref) * P->c2);
-        l += stat[g][1] * w;
-        y0 += part[g][d] * w;
-        y1 += part[g][d + 1] * w;
-      }
-      const float inv = 1.f / (l + 1e-6f);
+      for (int g = 0; g < NG; ++g) y0 += part[g][d], y1 += part[g][d + 1];
       uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)(h0 + hc) * P->o.sh;
       *(uint32_t*)(orow + d) = pack_e<F16>(y0 * inv, y1 * inv);
       if (d == 0 && P->lse.ptr)
@@ -606,7 +632,7 @@ hipError_t launch_paged_packed(const PagedParams& P, int rc, hipStream_t s) {
 
 hipError_t launch_paged_merge(const PagedParams& P, hipStream_t s) {
   if (P.waves <= 1) return hipSuccess;
-  const dim3 grid((uint32_t)(P.waves - 1), (uint32_t)std::min(P.gsub * P.tpt, 8));
+  const dim3 grid((uint32_t)(P.waves - 1), (uint32_t)(P.gsub * P.tpt));
   if (P.D == 64)
     hipLaunchKernelGGL(P.f16 ? (paged_merge_kernel<64, true>) : (paged_merge_kernel<64, false>), grid, dim3(256), 0, s, P);
   else

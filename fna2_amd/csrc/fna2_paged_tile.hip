@@ -78,14 +78,21 @@ __device__ __forceinline__ void tile_body() {
   }
 
   const int run = run_of(blockIdx.x, gridDim.x);
-  int64_t left;  // units of this run still to do
+  int64_t left, per;  // units of this run still to do, and of a run
   int b, hb, qt, s0;
   PagedSeq e;
+  auto cut = [&](int seq, int head, int tile, int parts) {
+    if (threadIdx.x == 0) P->cuts[run] = PagedCut{seq, head, tile, parts};
+  };
   {
     const TilePlan plan(P, lane);
-    const int64_t u = (int64_t)run * plan.per;
-    left = min(plan.total - u, plan.per);
-    if (left <= 0) return;
+    per = plan.per;
+    const int64_t u = (int64_t)run * per;
+    left = min(plan.total - u, per);
+    if (left <= 0) {
+      cut(0, 0, 0, 0);
+      return;
+    }
     const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return TilePlan::units(P, s); });
     b = at.b;
     e = paged_seq_uniform(P, b);
@@ -385,7 +392,7 @@ __device__ __forceinline__ void tile_body() {
           ((float*)P->lse.ptr)[(int64_t)(e.q0 + tok) * P->lse.ss + (int64_t)h * P->lse.sh] =
               m_i == kNegInf ? kNegInf : m_i * P->c + __builtin_amdgcn_logf(l_tot + 1e-6f) * kLn2;
       }
-    } else if (!idle) {
+    } else if (live) {
       // As the registers lie: [slot][wave][d][4][lane] of 16 bytes.
       const int64_t slot = (2 * (int64_t)run + (s0 == 0 ? 1 : 0)) * 4 + wv;
       float* arow = P->part + slot * 32 * D + 4 * lane;
@@ -400,7 +407,11 @@ __device__ __forceinline__ void tile_body() {
     }
 
     left -= s1 - s0;
-    if (left <= 0) return;
+    if (left <= 0) {
+      const int rest = steps - s1;
+      cut(b, hb, qt, s0 == 0 && rest > 0 ? 1 + (int)((rest + per - 1) / per) : 0);
+      return;
+    }
     s0 = 0;
     if (++qt * TB >= e.lq) {
       qt = 0;
@@ -412,53 +423,60 @@ __device__ __forceinline__ void tile_body() {
   }
 }
 
-// Joins the parts of cut tiles: workgroup (i, d) takes 32 features of the
-// tile that the boundary behind run i cuts, if no earlier one does; a wave the
-// tokens of one wave of the tile.  Parts come in the order of the runs.
+// Joins the parts of a tile that runs cut: workgroup (i, d) takes 32 features
+// of the tile that run i's end cuts; a wave the tokens of one wave of the tile, four
+// parts at a time.  Parts come in the order of the runs.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedParams) {
   KArg P = kargs();
   const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6), d = blockIdx.y;
   const int l32 = lane & 31, hl = lane >> 5;
-  const TilePlan plan(P, lane);
-  const int64_t i0 = blockIdx.x, u = (i0 + 1) * plan.per;
-  if (u >= plan.total) return;
-  const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return TilePlan::units(P, s); });
-  const PagedSeq e = paged_seq_uniform(P, at.b);
-  const int64_t hu = TilePlan::head_units(P, e);
-  const int hb = uni((int)(at.rem / hu));
-  int64_t r = at.rem - hb * hu;
-  const int qt = uni(TilePlan::find(P, e, r));
-  if (r == 0 || r > plan.per) return;
-  const int64_t tile_end = u - r + TilePlan::steps(P, e, qt);
-  const int n = uni((int)((tile_end - 1) / plan.per - i0) + 1);
+  const int i0 = blockIdx.x;
+  const auto rec = const_space(P->cuts + i0);
+  const int n = uni(rec->parts);
+  if (n <= 0) return;
+  const int hb = uni(rec->head), qt = uni(rec->tile);
+  const PagedSeq e = paged_seq_uniform(P, rec->b);
   const int hblk = cdiv(P->group, P->hw), kvh = hb / hblk, h_in = (hb - kvh * hblk) * P->hw + wv % P->hw;
-  const int tok0 = qt * TilePlan::tokens(P) + 32 * (wv / P->hw), tok = tok0 + l32;
-  if (tok0 >= e.lq || h_in >= P->group) return;
+  const int tok = qt * TilePlan::tokens(P) + 32 * (wv / P->hw) + l32;
+  if (tok >= e.lq || h_in >= P->group) return;
   const int h = kvh * P->group + h_in;
+  const float c2 = P->c2;
   float M = kNegInf, L = 0.f;
   f32x4_t o[4];
 #pragma unroll
   for (int g = 0; g < 4; ++g) o[g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < n; ++j) {
-    const int64_t slot = (j == 0 ? 2 * i0 + 1 : 2 * (i0 + j)) * 4 + wv;
-    const float* src = P->part + slot * 32 * D + d * 1024 + 4 * lane;
-    f32x4_t x[4];
+  constexpr int U = 4;  // parts in flight
+  for (int j0 = 0; j0 < n; j0 += U) {
+    f32x4_t x[U][4];
+    f32x2 ml[U];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) x[g] = *(const f32x4_t*)(src + g * 256);
-    const f32x2 ml = *(const f32x2*)(P->ml + 2 * (slot * 32 + l32));
-    const float m = fmaxf(M, ml[0]);
+    for (int k = 0; k < U; ++k) {
+      const int j = min(j0 + k, n - 1);  // (past the last: weighed 0 below)
+      const int64_t slot = (int64_t)(j == 0 ? 2 * i0 + 1 : 2 * (i0 + j)) * 4 + wv;
+      const float* src = P->part + slot * 32 * D + d * 1024 + 4 * lane;
+      ml[k] = *(const f32x2*)(P->ml + 2 * (slot * 32 + l32));
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x[k][g] = *(const f32x4_t*)(src + g * 256);
+    }
+    float m = M;
+#pragma unroll
+    for (int k = 0; k < U; ++k) m = fmaxf(m, ml[k][0]);
     const float ref = m == kNegInf ? 0.f : m;
-    const float wa = weight2((M - ref) * P->c2);
-    const float wb = weight2((ml[0] - ref) * P->c2);
-    L = L * wa + ml[1] * wb;
+    const float wa = weight2((M - ref) * c2);
+    L *= wa;
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < 4; ++g) o[g] *= wa;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[g][k] = o[g][k] * wa + x[g][k] * wb;
+    for (int k = 0; k < U; ++k) {
+      if (j0 + k >= n) break;  // (uniform)
+      const float wb = weight2((ml[k][0] - ref) * c2);
+      L += ml[k][1] * wb;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) o[g] += x[k][g] * wb;
+    }
     M = m;
   }
-  if (tok >= e.lq) return;
   const float inv = 1.f / (L + 1e-6f);
   uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)h * P->o.sh;
 #pragma unroll
