@@ -1573,7 +1573,7 @@ int fna2_check_paged_evict(const fna2_paged_evict_args* a) {
   if ((int64_t)a->recent + a->first > a->budget || a->budget > kMaxCached) return FNA2_E_SHAPE;
   if (a->stride_b < 0 || a->stride_h < 0) return FNA2_E_STRIDE;
   const int64_t per = 2 * (int64_t)a->c.heads_kv * (a->c.head_dim / 32) + 2 * (int64_t)a->c.heads_graph;
-  if (per * a->c.batch > 4 * kMaxGrid || (int64_t)a->c.batch * a->c.heads_kv > kMaxGrid)
+  if (per * a->c.batch > kMaxGrid || (int64_t)a->c.batch * a->c.heads_kv > kMaxGrid)
     return FNA2_E_SHAPE;
   if (a->c.batch == 0) return FNA2_OK;
   if (!a->new_lens || (a->budget > 0 && !a->kept)) return FNA2_E_NULL;

@@ -163,59 +163,52 @@ __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const Page
 // ── Eviction ───────────────────────────────────────────────────────────────
 // Selection, one workgroup per (sequence, KV head): the `top` = budget - first
 // - recent rows of largest weight among rows [first, lk - recent).  Weights
-// become unsigned keys in their order; four passes of 8 bits find the top-th
-// largest key K, and the rows kept are those above K and, of those equal
-// to K, the lowest (top minus the rows above).  A last pass writes the kept
-// rows in their order.
-constexpr int kSelThreads = 1024;
+// become unsigned keys in their order; three passes of 11, 11 and 10 bits find the
+// top-th largest key K, and the rows kept are those above K and, of those equal
+// to K, the lowest (top minus the rows above).  Two last passes write
+// the kept rows in their order: every wave counts, then writes, a range of its
+// own.  Bound by its passes over the weights, from L2, not by memory: eight
+// loads of a lane in flight.  (8 bits a pass: the first digit of positive
+// weights is their exponent's, a few bins that all lanes count in.)
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelAhead = 8;
+constexpr int kSelBins = 2048;
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (w != w) return 0xffffffffu;
   const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.f);  // (-0 as 0)
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Sum over the workgroup's threads up to and including this one (exclusive
-// of it: minus x); `total` the sum of all.  sh: one int per wave.
-__device__ __forceinline__ int block_scan(int x, int* sh, int& total) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  int s = x;
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int wave_scan(int x, int lane) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
-    const int o = __shfl_up(s, m);
-    if (lane >= m) s += o;
+    const int o = __shfl_up(x, m);
+    if (lane >= m) x += o;
   }
-  __syncthreads();
-  if (lane == 63) sh[wv] = s;
-  __syncthreads();
-  int base = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kSelThreads / 64; ++i) {
-    if (i < wv) base += sh[i];
-    total += sh[i];
-  }
-  return base + s;
+  return x;
 }
 
 __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEvictParams E) {
   const PagedParams& P = E.p;
-  __shared__ int hist[256];
-  __shared__ int sh[kSelThreads / 64];
+  __shared__ int hist[kSelBins];
+  __shared__ int wsum[kSelWaves];
+  __shared__ int gt_of[kSelWaves], eq_of[kSelWaves];
   __shared__ int pick[2];
   const int b = blockIdx.x / P.H_KV, kvh = blockIdx.x % P.H_KV, tid = threadIdx.x;
+  const int lane = tid & 63, wv = uni(tid >> 6);
   const int lk = min(max(uni(*const_space(P.lens + b)), 0), P.width * P.ps);
   const int keep = min(lk, E.budget);
   if (kvh == 0 && tid == 0) E.new_lens[b] = keep;
   const float* w = E.w + (int64_t)b * E.w_sb + (int64_t)kvh * E.w_sh;
   float* wo = E.w_out + ((int64_t)b * P.H_KV + kvh) * E.cap;
   int* kept = E.kept + ((int64_t)b * P.H_KV + kvh) * E.budget;
-  auto weight = [&](int j) { return j < E.cap ? w[j] : 0.f; };
+  const int cap = E.cap;
   for (int j = keep + tid; j < E.budget; j += kSelThreads) kept[j] = -1;
-  for (int j = keep + tid; j < E.cap; j += kSelThreads) wo[j] = 0.f;
+  for (int j = keep + tid; j < cap; j += kSelThreads) wo[j] = 0.f;
   if (lk <= E.budget) {
     for (int j = tid; j < keep; j += kSelThreads) {
       kept[j] = j;
-      if (j < E.cap) wo[j] = w[j];
+      if (j < cap) wo[j] = w[j];
     }
     return;
   }
@@ -223,119 +216,184 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEv
   uint32_t prefix = 0, mask = 0;
   int need = top;  // rows still to find among those that match the prefix
   if (top > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digit = pass == 2 ? 1023u : 2047u;
+      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int j = lo + tid; j < hi; j += kSelThreads) {
-        const uint32_t k = weight_key(weight(j));
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      for (int j0 = lo + tid; j0 < hi; j0 += kSelAhead * kSelThreads) {
+        float x[kSelAhead];
+#pragma unroll
+        for (int i = 0; i < kSelAhead; ++i) {
+          const int j = j0 + i * kSelThreads;
+          x[i] = j < hi && j < cap ? w[j] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kSelAhead; ++i) {
+          const uint32_t k = weight_key(x[i]);
+          if (j0 + i * kSelThreads < hi && (k & mask) == prefix)
+            atomicAdd(&hist[(k >> shift) & digit], 1);
+        }
       }
       __syncthreads();
-      // the digit d whose rows, with those of larger digits, reach `need`
-      int total;
-      const int mine = tid < 256 ? hist[255 - tid] : 0;
-      const int s = block_scan(mine, sh, total);
-      if (tid < 256 && s >= need && s - mine < need) {
-        pick[0] = 255 - tid;
-        pick[1] = s - mine;
-      }
+      // The digit d whose rows, with those of larger digits, reach `need`: a
+      // thread has the two bins 2047 - 2 tid and the one below.
+      const int h0 = hist[2047 - 2 * tid], h1 = hist[2046 - 2 * tid];
+      int s = wave_scan(h0 + h1, lane);
+      if (lane == 63) wsum[wv] = s;
+      __syncthreads();
+      for (int i = 0; i < wv; ++i) s += wsum[i];
+      const int before = s - h0 - h1;
+      if (before < need && before + h0 >= need) pick[0] = 2047 - 2 * tid, pick[1] = before;
+      if (before + h0 < need && s >= need) pick[0] = 2046 - 2 * tid, pick[1] = before + h0;
       __syncthreads();
       prefix |= (uint32_t)pick[0] << shift;
-      mask |= 255u << shift;
+      mask |= digit << shift;
       need -= pick[1];
       __syncthreads();
     }
   }
-  // kept rows in order; of the rows equal to the key, the first `need`
-  int out = 0, equal = 0;  // rows written, equal rows passed
-  for (int j0 = 0; j0 < lk; j0 += kSelThreads) {
-    const int j = j0 + tid;
-    const bool fixed = j < lk && (j < lo || j >= hi);
-    const uint32_t k = j >= lo && j < hi && top > 0 ? weight_key(weight(j)) : 0u;
-    const bool cand = j >= lo && j < hi && top > 0;
-    const bool eq = cand && k == prefix;
-    int eq_all;
-    const int eq_at = equal + block_scan(eq ? 1 : 0, sh, eq_all) - 1;
-    const bool yes = fixed || (cand && k > prefix) || (eq && eq_at < need);
-    int all;
-    const int at = out + block_scan(yes ? 1 : 0, sh, all) - 1;
-    if (yes) {
-      kept[at] = j;
-      if (at < E.cap) wo[at] = weight(j);
+  // This wave's rows [j_lo, j_hi): above the key (or always kept), and equal.
+  const int span = cdiv(cdiv(lk, kSelWaves), 64) * 64;
+  const int j_lo = wv * span, j_hi = min(lk, j_lo + span);
+  auto sort_of = [&](int j, float x) {  // 2 kept, 1 equal to the key, 0 below it
+    if (j < lo || j >= hi) return 2;
+    if (top <= 0) return 0;
+    const uint32_t k = weight_key(x);
+    return k > prefix ? 2 : k == prefix ? 1 : 0;
+  };
+  int n_gt = 0, n_eq = 0;
+  for (int j0 = j_lo; j0 < j_hi; j0 += kSelAhead * 64) {
+    float x[kSelAhead];
+#pragma unroll
+    for (int i = 0; i < kSelAhead; ++i) {
+      const int j = j0 + i * 64 + lane;
+      x[i] = j < j_hi && j < cap ? w[j] : 0.f;
     }
-    out += all;
-    equal += eq_all;
+#pragma unroll
+    for (int i = 0; i < kSelAhead; ++i) {
+      const int j = j0 + i * 64 + lane, k = j < j_hi ? sort_of(j, x[i]) : 0;
+      n_gt += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k == 2));
+      n_eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k == 1));
+    }
+  }
+  if (lane == 0) gt_of[wv] = n_gt, eq_of[wv] = n_eq;
+  __syncthreads();
+  int out = 0, left = need;  // where this wave writes; equal rows still to keep
+  for (int i = 0; i < wv; ++i) {
+    const int q = min(eq_of[i], left);
+    out += gt_of[i] + q;
+    left -= q;
+  }
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  for (int j0 = j_lo; j0 < j_hi; j0 += kSelAhead * 64) {
+    float x[kSelAhead];
+#pragma unroll
+    for (int i = 0; i < kSelAhead; ++i) {
+      const int j = j0 + i * 64 + lane;
+      x[i] = j < j_hi && j < cap ? w[j] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kSelAhead; ++i) {
+      const int j = j0 + i * 64 + lane, k = j < j_hi ? sort_of(j, x[i]) : 0;
+      const uint64_t eq = __builtin_amdgcn_ballot_w64(k == 1);
+      const bool yes = k == 2 || (k == 1 && __builtin_popcountll(eq & below) < left);
+      const uint64_t all = __builtin_amdgcn_ballot_w64(yes);
+      if (yes) {
+        const int at = out + __builtin_popcountll(all & below);
+        kept[at] = j;
+        if (at < cap) wo[at] = x[i];
+      }
+      out += __builtin_popcountll(all);
+      left -= min(left, (int)__builtin_popcountll(eq));
+    }
   }
 }
 
 // Compaction in place: row kept[r] becomes row r (kept[r] >= r, increasing).
-// A unit is a wave: a strip of 64 bytes of every row of one (sequence, head)
-// of K, V or R_k, walked in order, kAhead x 16 rows at a time: all of their
-// loads, then all of their stores.  Rows stored so lie before every row that
-// is still to be loaded, so a strip needs no other copy and no barrier.
-// Bound by reading and writing the rows that move; the strips of a row are
-// neighbouring waves, so that its lines are fetched together.
-constexpr int kCompactAhead = 8;
-__global__ __launch_bounds__(256) void paged_compact_kernel(const PagedEvictParams E) {
+// A workgroup takes one strip of 64 bytes of the rows of one (sequence, head) of
+// K, V or R_k, in rounds of kRoundRows rows: all of a round's loads, a barrier,
+// all of its stores.  Rows stored so lie before every row that is still to be
+// loaded, so no other copy is needed.  A round's chain (kept row, its page, the row)
+// is as long as for a few rows, so rounds are as large as the registers
+// allow: 16 waves of 8 loads of 16 rows, 128 KB in flight, and the next
+// round's rows and pages are looked up while this one's are under way.
+constexpr int kCompactThreads = 1024, kCompactAhead = 8;
+constexpr int kRoundRows = kCompactThreads / 4 * kCompactAhead;
+__global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const PagedEvictParams E) {
   const PagedParams& P = E.p;
-  const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
   const int kstrips = P.D / 32, rstrips = P.H_G > 0 ? cdiv(P.R, 32) : 0;
-  const int per = 2 * P.H_KV * kstrips + P.H_G * rstrips;  // units of a sequence
-  const int64_t unit = (int64_t)blockIdx.x * 4 + wv;
-  const int b = uni((int)(unit / per));
-  if (b >= P.N) return;
-  int x = (int)(unit - (int64_t)b * per);
+  const int per = 2 * P.H_KV * kstrips + P.H_G * rstrips;  // strips of a sequence
+  const int b = blockIdx.x / per;
+  int x = blockIdx.x - b * per;
   const int lk = min(max(uni(*const_space(P.lens + b)), 0), P.width * P.ps);
-  if (lk <= E.budget) return;
-  TView t;
+  const int budget = E.budget;
+  if (lk <= budget) return;
   int h, kvh, strip, chunks;  // head, its KV head, 64-byte strip, 16-byte chunks of it
-  if (x < 2 * P.H_KV * kstrips) {
-    t = x < P.H_KV * kstrips ? P.k : P.v;
-    x %= P.H_KV * kstrips;
+  const int nk = P.H_KV * kstrips;
+  const int which = x < nk ? 0 : x < 2 * nk ? 1 : 2;
+  if (which < 2) {
+    x -= which * nk;
     h = kvh = x / kstrips;
-    strip = x % kstrips;
+    strip = x - h * kstrips;
     chunks = 4;
   } else {
-    x -= 2 * P.H_KV * kstrips;
-    t = P.rk;
+    x -= 2 * nk;
     h = x / rstrips;
     kvh = h / P.group;
-    strip = x % rstrips;
+    strip = x - h * rstrips;
     chunks = min(P.R / 8 - 4 * strip, 4);
   }
-  const int* kept = E.kept + ((int64_t)b * P.H_KV + kvh) * E.budget;
+  const TView& t = which == 0 ? P.k : which == 1 ? P.v : P.rk;
+  const int64_t sb = t.sb, ss = t.ss;
+  const int ps = P.ps, npages = P.npages;
+  const int* kept = E.kept + ((int64_t)b * P.H_KV + kvh) * budget;
   const int* trow = P.table + (int64_t)b * P.tstride;
-  uint16_t* base = (uint16_t*)t.ptr + (int64_t)h * t.sh + 32 * strip + 8 * (lane & 3);
-  const bool on = (lane & 3) < chunks;
+  const int c = threadIdx.x & 3, row0 = threadIdx.x >> 2;
+  uint16_t* base = (uint16_t*)t.ptr + (int64_t)h * t.sh + 32 * strip + 8 * c;
   auto place = [&](int j) -> uint16_t* {
-    const int pg = j / P.ps;
+    const int pg = j / ps;
     const int id = trow[pg];
-    if ((uint32_t)id >= (uint32_t)P.npages) return nullptr;
-    return base + (int64_t)id * t.sb + (int64_t)(j - pg * P.ps) * t.ss;
+    return (uint32_t)id < (uint32_t)npages ? base + (int64_t)id * sb + (int64_t)(j - pg * ps) * ss
+                                           : nullptr;
   };
-  for (int r0 = 0; r0 < E.budget; r0 += 16 * kCompactAhead) {
-    u32x4 v[kCompactAhead];
-    uint16_t* dst[kCompactAhead];
+  const uint16_t* src[kCompactAhead];
+  uint16_t* dst[kCompactAhead];
+  auto look = [&](int r0) {
+    int j[kCompactAhead];
 #pragma unroll
     for (int i = 0; i < kCompactAhead; ++i) {
-      const int r = r0 + 16 * i + (lane >> 2);
-      dst[i] = nullptr;
-      if (r < E.budget && on) {
-        const int j = kept[r];
-        if (j != r) {
-          const uint16_t* src = place(j);
-          if (src) {
-            dst[i] = place(r);
-            v[i] = ld16(src);
-          }
-        }
+      const int r = r0 + row0 + i * (kCompactThreads / 4);
+      j[i] = r < budget && c < chunks ? kept[r] : r;
+    }
+#pragma unroll
+    for (int i = 0; i < kCompactAhead; ++i) {
+      const int r = r0 + row0 + i * (kCompactThreads / 4);
+      src[i] = nullptr;
+      if (j[i] != r) {
+        src[i] = place(j[i]);
+        dst[i] = place(r);
+        if (!dst[i]) src[i] = nullptr;
       }
     }
-    __builtin_amdgcn_s_waitcnt(0);  // every load of the group has its data
-    __builtin_amdgcn_sched_barrier(0);
+  };
+  look(0);
+  for (int r0 = 0; r0 < budget; r0 += kRoundRows) {
+    u32x4 v[kCompactAhead];
+    uint16_t* to[kCompactAhead];
+#pragma unroll
+    for (int i = 0; i < kCompactAhead; ++i) {
+      to[i] = src[i] ? dst[i] : nullptr;
+      if (src[i]) v[i] = ld16(src[i]);
+    }
+    if (r0 + kRoundRows < budget) look(r0 + kRoundRows);
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's loads have their data ...
+    __syncthreads();                // ... and every wave's
 #pragma unroll
     for (int i = 0; i < kCompactAhead; ++i)
-      if (dst[i]) st16(dst[i], v[i]);
+      if (to[i]) st16(to[i], v[i]);
+    // (the next round's loads are of rows past every row stored so far)
   }
 }
 
@@ -360,8 +418,7 @@ hipError_t launch_paged_select(const PagedEvictParams& E, hipStream_t s) {
 hipError_t launch_paged_compact(const PagedEvictParams& E, hipStream_t s) {
   const PagedParams& P = E.p;
   const int64_t per = 2 * (int64_t)P.H_KV * (P.D / 32) + (P.H_G > 0 ? (int64_t)P.H_G * ((P.R + 31) / 32) : 0);
-  const int64_t units = per * P.N;
-  hipLaunchKernelGGL(paged_compact_kernel, dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, s, E);
+  hipLaunchKernelGGL(paged_compact_kernel, dim3((uint32_t)(per * P.N)), dim3(kCompactThreads), 0, s, E);
   return hipGetLastError();
 }
 

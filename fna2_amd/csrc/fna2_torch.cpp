@@ -2,7 +2,8 @@
 //
 // Fills the argument structs of include/fna2.h from torch tensors, allocates
 // outputs and workspace and calls the C ABI on torch's current HIP stream:
-// what the Python launchers (flash_naylis_attn.py, decode.py, rope.py) do
+// what the Python launchers (flash_naylis_attn.py, decode.py, rope.py,
+// paged.py) do
 // through ctypes.  What it saves is host time: a training pass of one small
 // layer spends most of its time in these launchers, the backward's share of
 // it on autograd's own thread, where every Python object the launcher
@@ -48,6 +49,13 @@ struct Lib {
   decltype(&fna2_rope_varlen) rope_varlen;
   decltype(&fna2_rope_bwd) rope_bwd;
   decltype(&fna2_rope_bwd_workspace_bytes) rope_bwd_workspace_bytes;
+  decltype(&fna2_check_paged_attn) check_paged_attn;
+  decltype(&fna2_paged_attn_workspace_bytes) paged_attn_workspace_bytes;
+  decltype(&fna2_paged_attn) paged_attn;
+  decltype(&fna2_check_paged_weights) check_paged_weights;
+  decltype(&fna2_paged_weights) paged_weights;
+  decltype(&fna2_paged_append) paged_append;
+  decltype(&fna2_paged_evict) paged_evict;
 };
 Lib L{};
 
@@ -78,6 +86,13 @@ void bind(const std::map<std::string, uintptr_t>& f, py::object error) {
   FNA2_BIND(rope_varlen);
   FNA2_BIND(rope_bwd);
   FNA2_BIND(rope_bwd_workspace_bytes);
+  FNA2_BIND(check_paged_attn);
+  FNA2_BIND(paged_attn_workspace_bytes);
+  FNA2_BIND(paged_attn);
+  FNA2_BIND(check_paged_weights);
+  FNA2_BIND(paged_weights);
+  FNA2_BIND(paged_append);
+  FNA2_BIND(paged_evict);
 #undef FNA2_BIND
 }
 
@@ -564,6 +579,225 @@ std::optional<std::tuple<Tensor, Tensor, OptTensor, OptTensor>> rope_bwd(
   return std::make_tuple(dq, dk, dn[0], dn[1]);
 }
 
+// The paged cache of a call, and the chunk's cu_seqlens where it has one.
+bool paged_cache(fna2_paged_cache& c, const Tensor& kp, const Tensor& vp, const OptTensor& rkp_,
+                 const Tensor& table, const Tensor& lens, const Tensor* cu, int64_t heads) {
+  const Tensor& rkp = opt(rkp_);
+  if (!kp.defined() || !kp.is_cuda()) return false;
+  const c10::Device dev = kp.device();
+  const auto dt = kp.scalar_type();
+  if (dt != at::kBFloat16 && dt != at::kHalf) return false;
+  auto pool = [&](const Tensor& t, at::ScalarType type) {
+    return plain(t, dev) && t.scalar_type() == type && t.dim() == 4 && rows16(t) &&
+           !t.requires_grad() && (!t.is_inference() || c10::InferenceMode::is_enabled());
+  };
+  if (!pool(kp, dt) || !pool(vp, dt) || kp.sizes() != vp.sizes()) return false;
+  if (!plain(table, dev) || table.scalar_type() != at::kInt || table.dim() != 2 ||
+      table.stride(1) != 1 || table.stride(0) < table.size(1))
+    return false;
+  const int64_t N = table.size(0);
+  if (!int32_on(lens, dev) || lens.dim() != 1 || lens.numel() != N) return false;
+  if (cu && (!int32_on(*cu, dev) || cu->dim() != 1 || cu->numel() != N + 1)) return false;
+  if (N > INT32_MAX || kp.size(0) > INT32_MAX || kp.size(2) > INT32_MAX || heads > INT32_MAX ||
+      table.size(1) > INT32_MAX)
+    return false;
+  auto pages = [](const Tensor& t) {
+    fna2_tensor v{};
+    v.ptr = t.data_ptr();
+    v.stride_b = t.stride(0);
+    v.stride_h = t.stride(1);
+    v.stride_s = t.stride(2);
+    return v;
+  };
+  c.dtype = dt == at::kHalf ? FNA2_F16 : FNA2_BF16;
+  c.batch = (int32_t)N;
+  c.heads = (int32_t)heads;
+  c.heads_kv = (int32_t)kp.size(1);
+  c.head_dim = (int32_t)kp.size(3);
+  c.num_pages = (int32_t)kp.size(0);
+  c.page_size = (int32_t)kp.size(2);
+  c.table_width = (int32_t)table.size(1);
+  c.block_table = table.data_ptr<int32_t>();
+  c.table_stride = table.stride(0);
+  c.seqlens_k = lens.data_ptr<int32_t>();
+  if (cu) c.cu_seqlens_q = cu->data_ptr<int32_t>();
+  c.k_pages = pages(kp);
+  c.v_pages = pages(vp);
+  if (rkp.defined()) {
+    if (!pool(rkp, at::kBFloat16) || rkp.size(0) != kp.size(0) || rkp.size(2) != kp.size(2))
+      return false;
+    c.heads_graph = (int32_t)rkp.size(1);
+    c.rank = (int32_t)rkp.size(3);
+    c.rk_pages = pages(rkp);
+  }
+  return true;
+}
+
+// New rows [T, heads, feat] of a type on the pools' device.
+bool new_rows(const Tensor& t, const c10::Device& dev, at::ScalarType dt, int64_t T, int64_t heads,
+              int64_t feat) {
+  return plain(t, dev) && t.scalar_type() == dt && t.dim() == 3 && t.size(0) == T &&
+         t.size(1) == heads && t.size(2) == feat && rows16(t);
+}
+
+// Tensors that a call has written in place, as torch's copy_ counts them.
+void written(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t && t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+// flash_naylis_paged: (out, LSE or None).
+std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
+    const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lens,
+    const Tensor& cu, int64_t max_q, const OptTensor& rq_, const OptTensor& rkp_,
+    const OptTensor& gs_, double scale, bool causal, const OptTensor& w_, bool want_lse) {
+  const Tensor &rq = opt(rq_), &w = opt(w_);
+  Tensor gs = opt(gs_);
+  if (!L.paged_attn || !q.defined() || !q.is_cuda() || q.dim() != 3) return std::nullopt;
+  const c10::Device dev = q.device();
+  const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+  fna2_paged_attn_args a{};
+  static const OptTensor none;
+  if (!kp.defined() || kp.device() != dev || T > INT32_MAX || max_q < 0 ||
+      !paged_cache(a.c, kp, vp, rq.defined() ? rkp_ : none, table, lens, &cu, H))
+    return std::nullopt;
+  if (kp.size(3) != D || !new_rows(q, dev, kp.scalar_type(), T, H, D)) return std::nullopt;
+  if (rq.defined()) {
+    if (a.c.heads_graph <= 0 || !new_rows(rq, dev, at::kBFloat16, T, a.c.heads_graph, a.c.rank) ||
+        !plain(gs, dev) || !gs.is_floating_point())
+      return std::nullopt;
+    gs = gs.detach().to(at::kFloat).contiguous();
+    if (gs.numel() != a.c.heads_graph) return std::nullopt;
+    a.r_q = view(rq, true);
+    a.graph_scale = gs.data_ptr<float>();
+  }
+  a.c.total_q = (int32_t)T;
+  a.c.max_seqlen_q = (int32_t)std::min(max_q, T);
+  a.causal = causal;
+  a.softmax_scale = (float)scale;
+  fna2_paged_weights_args wa{};
+  if (w.defined()) {
+    if (!plain(w, dev) || w.scalar_type() != at::kFloat || w.dim() != 3 ||
+        w.size(0) != a.c.batch || w.size(1) != a.c.heads_kv || w.stride(2) != 1 ||
+        w.requires_grad() || w.size(2) > INT32_MAX ||
+        (w.is_inference() && !c10::InferenceMode::is_enabled()))
+      return std::nullopt;
+    wa.key_weights = w.data_ptr<float>();
+    wa.stride_b = w.stride(0);
+    wa.stride_h = w.stride(1);
+    wa.capacity = (int32_t)w.size(2);
+  }
+  const c10::DeviceGuard guard(dev);
+  const Tensor out = at::empty({T, H, D}, q.options());
+  OptTensor lse;
+  if (want_lse || w.defined()) {
+    lse = at::empty({H, T}, q.options().dtype(at::kFloat)).t();
+    a.lse = view(*lse, true);
+  }
+  a.q = view(q, true);
+  a.out = view(out, true);
+  wa.attn = a;
+  if (L.check_paged_attn(&a) != FNA2_OK ||
+      (w.defined() && L.check_paged_weights(&wa) != FNA2_OK))
+    return std::nullopt;
+  const size_t need = L.paged_attn_workspace_bytes(&a);
+  const Tensor ws = bytes_on(need, q);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = need;
+  if (!launched(L.paged_attn(&a, stream_of(dev)), "flash_naylis_paged")) return std::nullopt;
+  if (w.defined()) {
+    // (checked above: what is left to fail is a launch)
+    if (!launched(L.paged_weights(&wa, stream_of(dev)), "flash_naylis_paged"))
+      launched(FNA2_E_LAUNCH, "flash_naylis_paged");
+    written({&w});
+  }
+  if (!want_lse) lse.reset();
+  return std::make_tuple(out, lse);
+}
+
+// paged_append: the new q.
+OptTensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kp,
+                       const Tensor& vp, const Tensor& table, const Tensor& lens, const Tensor& cu,
+                       const OptTensor& rk_, const OptTensor& rkp_, const OptTensor& inv_,
+                       const OptTensor& pos_, const OptTensor& nq, const OptTensor& nk,
+                       double eps) {
+  const Tensor &rk = opt(rk_), &pos = opt(pos_);
+  if (!L.paged_append || !q.defined() || !q.is_cuda() || q.dim() != 3) return std::nullopt;
+  const c10::Device dev = q.device();
+  const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+  fna2_paged_append_args a{};
+  if (!kp.defined() || kp.device() != dev || T > INT32_MAX ||
+      rk_.has_value() != rkp_.has_value() || !paged_cache(a.c, kp, vp, rkp_, table, lens, &cu, H))
+    return std::nullopt;
+  const auto dt = kp.scalar_type();
+  if (kp.size(3) != D || !new_rows(q, dev, dt, T, H, D) ||
+      !new_rows(k, dev, dt, T, a.c.heads_kv, D) || !new_rows(v, dev, dt, T, a.c.heads_kv, D))
+    return std::nullopt;
+  if (rk.defined()) {
+    if (a.c.heads_graph <= 0 || !new_rows(rk, dev, at::kBFloat16, T, a.c.heads_graph, a.c.rank))
+      return std::nullopt;
+    a.r_k = view(rk, true);
+  }
+  if (pos.defined()) {
+    if (!inv_.has_value() || !int32_on(pos, dev) || pos.dim() != 1 || pos.numel() != T)
+      return std::nullopt;
+    a.positions = pos.data_ptr<int32_t>();
+  }
+  Tensor vec[3];
+  auto fp32 = [&](const OptTensor& t, int64_t n, Tensor& keep, const float*& p) {
+    if (!t.has_value()) return true;
+    if (!plain(*t, dev) || !t->is_floating_point() || t->numel() != n) return false;
+    keep = t->detach().to(at::kFloat).contiguous();
+    p = keep.data_ptr<float>();
+    return true;
+  };
+  const c10::DeviceGuard guard(dev);
+  if (!fp32(inv_, D / 2, vec[0], a.inv_freq) || !fp32(nq, D, vec[1], a.norm_q) ||
+      !fp32(nk, D, vec[2], a.norm_k))
+    return std::nullopt;
+  a.c.total_q = (int32_t)T;
+  a.eps = (float)eps;
+  const Tensor out = at::empty({T, H, D}, q.options());
+  a.q = view(q, true);
+  a.k = view(k, true);
+  a.v = view(v, true);
+  a.q_out = view(out, true);
+  if (!launched(L.paged_append(&a, stream_of(dev)), "paged_append")) return std::nullopt;
+  written({&kp, &vp, &opt(rkp_)});
+  return out;
+}
+
+// paged_evict: (kept, new lengths, the kept rows' weights).
+std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(
+    const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lens, const Tensor& w,
+    int64_t budget, int64_t recent, int64_t first, const OptTensor& rkp_, int64_t heads) {
+  fna2_paged_evict_args a{};
+  if (!L.paged_evict || budget < 0 || recent < 0 || first < 0 || budget > INT32_MAX ||
+      recent + first > budget || !paged_cache(a.c, kp, vp, rkp_, table, lens, nullptr, heads))
+    return std::nullopt;
+  const c10::Device dev = kp.device();
+  if (!plain(w, dev) || w.scalar_type() != at::kFloat || w.dim() != 3 || w.size(0) != a.c.batch ||
+      w.size(1) != a.c.heads_kv || w.stride(2) != 1 || w.size(2) > INT32_MAX)
+    return std::nullopt;
+  const c10::DeviceGuard guard(dev);
+  const Tensor kept = at::empty({w.size(0), w.size(1), budget}, lens.options());
+  const Tensor new_lens = at::empty({w.size(0)}, lens.options());
+  const Tensor w_out = at::empty(w.sizes(), w.options());
+  a.budget = (int32_t)budget;
+  a.recent = (int32_t)recent;
+  a.first = (int32_t)first;
+  a.key_weights = w.data_ptr<float>();
+  a.stride_b = w.stride(0);
+  a.stride_h = w.stride(1);
+  a.capacity = (int32_t)w.size(2);
+  a.weights_out = w_out.data_ptr<float>();
+  a.kept = (int32_t*)kept.data_ptr();
+  a.new_lens = new_lens.data_ptr<int32_t>();
+  if (!launched(L.paged_evict(&a, stream_of(dev)), "paged_evict")) return std::nullopt;
+  written({&kp, &vp, &opt(rkp_)});
+  return std::make_tuple(kept, new_lens, w_out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_binding, m) {
@@ -576,4 +810,7 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("decode_rows", &decode_rows, Free());
   m.def("rope_fwd", &rope_fwd, Free());
   m.def("rope_bwd", &rope_bwd, Free());
+  m.def("paged_attn", &paged_attn, Free());
+  m.def("paged_append", &paged_append, Free());
+  m.def("paged_evict", &paged_evict, Free());
 }

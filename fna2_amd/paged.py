@@ -172,6 +172,15 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
 
     Returns out ``[T, H, D]`` (and the fp32 LSE ``[T, H]``)."""
     what = "flash_naylis_paged"
+    nat = _capi.native_or_none() if q.is_cuda else None
+    if nat is not None:  # the native launch path (None: a call it leaves to the code below)
+        done = nat.paged_attn(
+            q, k_pages, v_pages, block_table, seqlens_k, cu_seqlens_q, int(max_seqlen_q), r_q,
+            rk_pages, graph_scale,
+            float(q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale),
+            bool(is_causal), key_weights, return_lse)
+        if done is not None:
+            return done if return_lse else done[0]
     assert q.dim() == 3, f"{what}: q must be [T, H, D]"
     dev = k_pages.device
     T, H, D = q.shape
@@ -253,6 +262,12 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     stored; tokens of no sequence keep their q and store nothing.  Pages that
     are written may belong to one sequence only."""
     what = "paged_append"
+    nat = _capi.native_or_none() if q.is_cuda else None
+    if nat is not None:
+        done = nat.paged_append(q, k, v, k_pages, v_pages, block_table, seqlens_k, cu_seqlens_q,
+                                r_k, rk_pages, inv_freq, positions, norm_q, norm_k, float(eps))
+        if done is not None:
+            return done
     assert q.dim() == 3 and k.dim() == 3, f"{what}: q [T, H, D] and k [T, H_KV, D] expected"
     dev = k_pages.device
     T, H, D = q.shape
@@ -325,6 +340,13 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     H_G = 0 if rk_pages is None else rk_pages.shape[1]
     if H_G:
         assert heads is not None, f"{what}: rk_pages needs heads, the number of query heads"
+    nat = _capi.native_or_none() if k_pages.is_cuda else None
+    if nat is not None:
+        done = nat.paged_evict(k_pages, v_pages, block_table, seqlens_k, key_weights, int(budget),
+                               int(recent), int(first), rk_pages,
+                               int(heads if heads is not None else k_pages.shape[1]))
+        if done is not None:
+            return done
     c, keep = _cache(what, k_pages, v_pages, block_table, seqlens_k,
                      heads if heads is not None else k_pages.shape[1], rk_pages if H_G else None,
                      H_G)

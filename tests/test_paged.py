@@ -749,6 +749,65 @@ def test_evict_refusals(gpu):
     bad(w, 10, rk_pages=c.rk.half(), heads=4)
 
 
+# ── GPU: the two launch paths ────────────────────────────────────────────────
+
+@pytest.mark.gpu
+def test_native_and_python_launchers_agree(gpu, monkeypatch):
+    nat = _capi.native()
+    c = Case([3, 40, 0], [70, 80, 9], 4, 2, 3, 64, 16, 16, device=gpu, tail=1)
+    w = torch.rand(3, 2, c.width * 16, device=gpu)
+    inv = torch.rand(32, device=gpu)
+    pos = torch.arange(c.T, dtype=torch.int32, device=gpu)
+    pools = [c.k.clone(), c.v.clone(), c.rk.clone()]
+
+    def calls():
+        for a, b in zip((c.k, c.v, c.rk), pools):
+            a.copy_(b)
+        acc = w.clone()
+        q = paged.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, c.rkn, c.rk,
+                               inv.double(), pos, inv.repeat(2), None)
+        out, lse = c.attend(return_lse=True, key_weights=acc)
+        ev = paged.paged_evict(c.k, c.v, c.table, c.lens, acc, 35, 5, 1, c.rk, 4)
+        return (q, out, lse, acc, *ev, c.k.clone(), c.v.clone(), c.rk.clone())
+
+    assert nat.paged_attn(c.q, c.k, c.v, c.table, c.lens, c.cu, 40, c.rq, c.rk, c.gs, 0.1, True,
+                          w.clone(), True) is not None
+    assert nat.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, c.rkn, c.rk, inv,
+                            pos, None, None, 0.0) is not None
+    assert nat.paged_evict(c.k, c.v, c.table, c.lens, w, 35, 5, 1, c.rk, 4) is not None
+    # left to the Python launchers: lengths on the CPU or in 64 bits, strided features
+    assert nat.paged_attn(c.q, c.k, c.v, c.table, c.lens.cpu(), c.cu, 40, c.rq, c.rk, c.gs, 0.1,
+                          True, None, True) is None
+    assert nat.paged_attn(c.q, c.k, c.v, c.table, c.lens, c.cu.long(), 40, c.rq, c.rk, c.gs, 0.1,
+                          True, None, True) is None
+    assert nat.paged_evict(c.k, c.v, c.table, c.lens, w, 3, 5, 1, c.rk, 4) is None
+    a = calls()
+    odd = c.attend()
+    c.lens, c.cu = c.lens.cpu(), c.cu.long()
+    assert torch.equal(odd, c.attend())
+    c.lens, c.cu = c.lens.to(gpu), c.cu.int()
+    monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+    for x, y in zip(a, calls()):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_inference_tensors(gpu):
+    """As torch's own in-place calls: written in inference mode only."""
+    c = Case([3, 1], [70, 80], 4, 2, 4, 64, 16, 16, device=gpu)
+    with torch.inference_mode():
+        k, v, rk = c.k.clone(), c.v.clone(), c.rk.clone()
+        paged.paged_append(c.q, c.kn, c.vn, k, v, c.table, c.lens, c.cu, c.rkn, rk)
+        w = torch.zeros(2, 2, 96, device=gpu)
+        c.attend(key_weights=w)
+    with pytest.raises(RuntimeError):
+        paged.paged_append(c.q, c.kn, c.vn, k, v, c.table, c.lens, c.cu, c.rkn, rk)
+    with pytest.raises(RuntimeError):
+        c.attend(key_weights=w)
+    with pytest.raises(RuntimeError):
+        paged.paged_evict(k, v, c.table, c.lens, w, 10)
+
+
 # ── GPU: as they are used ────────────────────────────────────────────────────
 
 def _serve(c, steps, gpu, budget=None):
