@@ -302,6 +302,6 @@ __device__ __forceinline__ float wave_pair_sum(float x) {
   return p[0] + p[1];
 }
 
-__device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 }  // namespace fna2

@@ -167,8 +167,8 @@ __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const Page
 // top-th largest key K, and the rows kept are those above K and, of those equal
 // to K, the lowest (top minus the rows above).  Two last passes write
 // the kept rows in their order: every wave counts, then writes, a range of its
-// own.  Bound by its passes over the weights, from L2, not by memory: eight
-// loads of a lane in flight.  (8 bits a pass: the first digit of positive
+// own.  Bound by the latency of its passes, not by memory: a wave keeps up to
+// 512 weights in registers over all of them.  (8 bits a pass: the first digit of positive
 // weights is their exponent's, a few bins that all lanes count in.)
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelAhead = 8;
 constexpr int kSelBins = 2048;
@@ -213,6 +213,21 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEv
     return;
   }
   const int lo = E.first, hi = lk - E.recent, top = E.budget - E.first - E.recent;
+  // This wave's rows [j_lo, j_hi), kSelAhead x 64 at a time; up to 8192 rows
+  // in all a wave's are one such chunk, loaded once.
+  const int span = cdiv(cdiv(lk, kSelWaves), 64) * 64;
+  const int j_lo = wv * span, j_hi = min(lk, j_lo + span);
+  float x[kSelAhead];
+  int loaded = -1;
+  auto load = [&](int j0) {
+    if (j0 == loaded) return;
+    loaded = j0;
+#pragma unroll
+    for (int i = 0; i < kSelAhead; ++i) {
+      const int j = j0 + i * 64 + lane;
+      x[i] = j < j_hi && j < cap ? w[j] : 0.f;
+    }
+  };
   uint32_t prefix = 0, mask = 0;
   int need = top;  // rows still to find among those that match the prefix
   if (top > 0) {
@@ -222,17 +237,13 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEv
       const uint32_t digit = pass == 2 ? 1023u : 2047u;
       for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int j0 = lo + tid; j0 < hi; j0 += kSelAhead * kSelThreads) {
-        float x[kSelAhead];
+      for (int j0 = j_lo; j0 < j_hi; j0 += kSelAhead * 64) {
+        load(j0);
 #pragma unroll
         for (int i = 0; i < kSelAhead; ++i) {
-          const int j = j0 + i * kSelThreads;
-          x[i] = j < hi && j < cap ? w[j] : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < kSelAhead; ++i) {
+          const int j = j0 + i * 64 + lane;
           const uint32_t k = weight_key(x[i]);
-          if (j0 + i * kSelThreads < hi && (k & mask) == prefix)
+          if (j >= lo && j < hi && j < j_hi && (k & mask) == prefix)
             atomicAdd(&hist[(k >> shift) & digit], 1);
         }
       }
@@ -254,26 +265,19 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEv
       __syncthreads();
     }
   }
-  // This wave's rows [j_lo, j_hi): above the key (or always kept), and equal.
-  const int span = cdiv(cdiv(lk, kSelWaves), 64) * 64;
-  const int j_lo = wv * span, j_hi = min(lk, j_lo + span);
-  auto sort_of = [&](int j, float x) {  // 2 kept, 1 equal to the key, 0 below it
+  auto sort_of = [&](int j, float v) {  // 2 kept, 1 equal to the key, 0 not
+    if (j >= j_hi) return 0;
     if (j < lo || j >= hi) return 2;
     if (top <= 0) return 0;
-    const uint32_t k = weight_key(x);
+    const uint32_t k = weight_key(v);
     return k > prefix ? 2 : k == prefix ? 1 : 0;
   };
   int n_gt = 0, n_eq = 0;
   for (int j0 = j_lo; j0 < j_hi; j0 += kSelAhead * 64) {
-    float x[kSelAhead];
+    load(j0);
 #pragma unroll
     for (int i = 0; i < kSelAhead; ++i) {
-      const int j = j0 + i * 64 + lane;
-      x[i] = j < j_hi && j < cap ? w[j] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kSelAhead; ++i) {
-      const int j = j0 + i * 64 + lane, k = j < j_hi ? sort_of(j, x[i]) : 0;
+      const int k = sort_of(j0 + i * 64 + lane, x[i]);
       n_gt += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k == 2));
       n_eq += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k == 1));
     }
@@ -288,15 +292,10 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEv
   }
   const uint64_t below = ((uint64_t)1 << lane) - 1;
   for (int j0 = j_lo; j0 < j_hi; j0 += kSelAhead * 64) {
-    float x[kSelAhead];
+    load(j0);
 #pragma unroll
     for (int i = 0; i < kSelAhead; ++i) {
-      const int j = j0 + i * 64 + lane;
-      x[i] = j < j_hi && j < cap ? w[j] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kSelAhead; ++i) {
-      const int j = j0 + i * 64 + lane, k = j < j_hi ? sort_of(j, x[i]) : 0;
+      const int j = j0 + i * 64 + lane, k = sort_of(j, x[i]);
       const uint64_t eq = __builtin_amdgcn_ballot_w64(k == 1);
       const bool yes = k == 2 || (k == 1 && __builtin_popcountll(eq & below) < left);
       const uint64_t all = __builtin_amdgcn_ballot_w64(yes);
@@ -313,17 +312,17 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEv
 
 // Compaction in place: row kept[r] becomes row r (kept[r] >= r, increasing).
 // A workgroup takes one strip of 64 bytes of the rows of one (sequence, head) of
-// K, V or R_k, in rounds of kRoundRows rows: all of a round's loads, a barrier,
+// K, V or R_k, in rounds of some hundred rows: all of a round's loads, a barrier,
 // all of its stores.  Rows stored so lie before every row that is still to be
 // loaded, so no other copy is needed.  A round's chain (kept row, its page, the row)
 // is as long as for a few rows, so rounds are as large as the registers
 // allow: 16 waves of 8 loads of 16 rows, 128 KB in flight, and the next
 // round's rows and pages are looked up while this one's are under way.
-constexpr int kCompactThreads = 1024, kCompactAhead = 8;
-constexpr int kRoundRows = kCompactThreads / 4 * kCompactAhead;
+constexpr int kCompactThreads = 1024, kCompactAhead = 4;
+constexpr int kStrip = 8;  // 16-byte chunks of a strip, at most
 __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const PagedEvictParams E) {
   const PagedParams& P = E.p;
-  const int kstrips = P.D / 32, rstrips = P.H_G > 0 ? cdiv(P.R, 32) : 0;
+  const int kstrips = P.D / (8 * kStrip), rstrips = P.H_G > 0 ? cdiv(P.R, 8 * kStrip) : 0;
   const int per = 2 * P.H_KV * kstrips + P.H_G * rstrips;  // strips of a sequence
   const int b = blockIdx.x / per;
   int x = blockIdx.x - b * per;
@@ -337,21 +336,24 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
     x -= which * nk;
     h = kvh = x / kstrips;
     strip = x - h * kstrips;
-    chunks = 4;
+    chunks = kStrip;
   } else {
     x -= 2 * nk;
     h = x / rstrips;
     kvh = h / P.group;
     strip = x - h * rstrips;
-    chunks = min(P.R / 8 - 4 * strip, 4);
+    chunks = min(P.R / 8 - kStrip * strip, kStrip);
   }
   const TView& t = which == 0 ? P.k : which == 1 ? P.v : P.rk;
   const int64_t sb = t.sb, ss = t.ss;
   const int ps = P.ps, npages = P.npages;
   const int* kept = E.kept + ((int64_t)b * P.H_KV + kvh) * budget;
   const int* trow = P.table + (int64_t)b * P.tstride;
-  const int c = threadIdx.x & 3, row0 = threadIdx.x >> 2;
-  uint16_t* base = (uint16_t*)t.ptr + (int64_t)h * t.sh + 32 * strip + 8 * c;
+  // lanes a row: the chunks, rounded up to a power of two
+  const int lanes = chunks > 8 ? 16 : chunks > 4 ? 8 : chunks > 2 ? 4 : chunks;
+  const int c = threadIdx.x & (lanes - 1), row0 = threadIdx.x / lanes, stride = kCompactThreads / lanes;
+  const int round = stride * kCompactAhead;
+  uint16_t* base = (uint16_t*)t.ptr + (int64_t)h * t.sh + 8 * (kStrip * strip + c);
   auto place = [&](int j) -> uint16_t* {
     const int pg = j / ps;
     const int id = trow[pg];
@@ -364,12 +366,12 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
     int j[kCompactAhead];
 #pragma unroll
     for (int i = 0; i < kCompactAhead; ++i) {
-      const int r = r0 + row0 + i * (kCompactThreads / 4);
+      const int r = r0 + row0 + i * stride;
       j[i] = r < budget && c < chunks ? kept[r] : r;
     }
 #pragma unroll
     for (int i = 0; i < kCompactAhead; ++i) {
-      const int r = r0 + row0 + i * (kCompactThreads / 4);
+      const int r = r0 + row0 + i * stride;
       src[i] = nullptr;
       if (j[i] != r) {
         src[i] = place(j[i]);
@@ -379,7 +381,7 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
     }
   };
   look(0);
-  for (int r0 = 0; r0 < budget; r0 += kRoundRows) {
+  for (int r0 = 0; r0 < budget; r0 += round) {
     u32x4 v[kCompactAhead];
     uint16_t* to[kCompactAhead];
 #pragma unroll
@@ -387,7 +389,8 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
       to[i] = src[i] ? dst[i] : nullptr;
       if (src[i]) v[i] = ld16(src[i]);
     }
-    if (r0 + kRoundRows < budget) look(r0 + kRoundRows);
+    if (r0 + round < budget) look(r0 + round);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __builtin_amdgcn_s_waitcnt(0);  // this wave's loads have their data ...
     __syncthreads();                // ... and every wave's
 #pragma unroll
@@ -417,7 +420,8 @@ hipError_t launch_paged_select(const PagedEvictParams& E, hipStream_t s) {
 
 hipError_t launch_paged_compact(const PagedEvictParams& E, hipStream_t s) {
   const PagedParams& P = E.p;
-  const int64_t per = 2 * (int64_t)P.H_KV * (P.D / 32) + (P.H_G > 0 ? (int64_t)P.H_G * ((P.R + 31) / 32) : 0);
+  const int64_t per = 2 * (int64_t)P.H_KV * (P.D / (8 * kStrip)) +
+                      (P.H_G > 0 ? (int64_t)P.H_G * cdiv(P.R, 8 * kStrip) : 0);
   hipLaunchKernelGGL(paged_compact_kernel, dim3((uint32_t)(per * P.N)), dim3(kCompactThreads), 0, s, E);
   return hipGetLastError();
 }
