@@ -1506,6 +1506,10 @@ int fna2_check_paged_weights(const fna2_paged_weights_args* w) {
   FNA2_TRY(check_paged_attn_common(w->attn));
   if (w->capacity < 0 || w->stride_b < 0 || w->stride_h < 0) return FNA2_E_SHAPE;
   if (w->attn.c.total_q == 0 || w->attn.c.batch == 0 || w->capacity == 0) return FNA2_OK;
+  // (offsets of a row tile's rows, up to 32 tokens by the KV head's heads)
+  const int64_t g = w->attn.c.heads / w->attn.c.heads_kv;
+  for (const fna2_tensor* t : {&w->attn.q, &w->attn.r_q})
+    if (t->ptr && (32 * t->stride_s + g * t->stride_h) * 2 > kOff31) return FNA2_E_SHAPE;
   if (!w->attn.lse.ptr || !w->key_weights) return FNA2_E_NULL;
   if (!aligned(w->key_weights, 4)) return FNA2_E_STRIDE;
   if ((w->attn.c.heads_kv > 1 && w->stride_h < w->capacity) ||
@@ -1526,9 +1530,15 @@ int fna2_paged_weights(const fna2_paged_weights_args* w, void* stream) {
   K.w_sb = w->stride_b;
   K.w_sh = w->stride_h;
   K.cap = w->capacity;
+  // Row tiles: the packed kernel's columns where it runs, else 32 tokens of a head.
+  const PagedPlan k = paged_plan(c);
+  K.p.gsub = k.tile ? 1 : k.gsub;
+  K.p.nsub = k.tile ? K.p.group : k.nsub;
+  K.p.tpt = k.tile ? 32 : k.tpt;
+  const int rc = k.tile ? fna2::paged_rank_chunks(K.p.R / 8) : k.rc;
   const int64_t blocks = (int64_t)c.batch * c.heads_kv * std::max<int64_t>(cdiv64(cached_rows(c), 128), 1);
-  K.grid = (int)std::min<int64_t>(blocks, 2048);
-  if (fna2::launch_paged_weights(K, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
+  K.grid = (int)std::min<int64_t>(blocks, 256 * fna2::paged_weigh_per_cu(rc));
+  if (fna2::launch_paged_weights(K, rc, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
   return FNA2_OK;
 }
 

@@ -218,7 +218,8 @@ struct PagedWeightsParams {
   int cap;
   int grid;
 };
-hipError_t launch_paged_weights(const PagedWeightsParams& P, hipStream_t s);
+int paged_weigh_per_cu(int rc);  // resident workgroups
+hipError_t launch_paged_weights(const PagedWeightsParams& P, int rc, hipStream_t s);
 
 struct PagedAppendParams {
   PagedParams p;  // q, k, v pools and the chunk; o is q_out

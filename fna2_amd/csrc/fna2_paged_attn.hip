@@ -480,111 +480,6 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
   }
 }
 
-// Attention weights of the cached rows: W_j += sum over tokens and heads of
-// e^{S_j - LSE}.  A wave holds 32 keys (the columns of S = Q K^T, so a lane
-// sums its key's weights over the rows in registers) and walks the chunk's
-// tokens, 32 at a time, of each query head of the KV head.  One workgroup's
-// four waves take 128 keys; blocks of keys go round over the workgroups.
-template <int D, int RPL, bool F16>
-__global__ __launch_bounds__(256) void paged_weights_kernel(const PagedWeightsParams W) {
-  constexpr int KSD = D / 16, KSR = RPL / 16;
-  KArg P = kargs();
-  const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
-  const int col = lane & 31, hl = lane >> 5;
-  auto units = [&](const PagedSeq& s) { return s.lq > 0 ? (int64_t)P->H_KV * cdiv(s.lk, 128) : 0; };
-  const int64_t total = uni64(wave_total(P, lane, units));
-  const uint32_t qxor = P->qa < 0.f ? 0x80008000u : 0u;
-  const uint32_t qand = P->qa == 0.f ? 0u : 0xffffffffu;
-  for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
-    const PagedAt at = wave_locate(P, lane, id, units);
-    const PagedSeq e = paged_seq_uniform(P, at.b);
-    const int nkb = cdiv(e.lk, 128);
-    const int kvh = (int)(at.rem / nkb);
-    const int k0 = 128 * (int)(at.rem - (int64_t)kvh * nkb) + 32 * wv;
-    const int key = k0 + col, off = e.lk - e.lq;
-    int page = -1, r = 0;
-    if (key < e.lk) {
-      page = P->table[(int64_t)at.b * P->tstride + key / P->ps];
-      r = key % P->ps;
-      if ((uint32_t)page >= (uint32_t)P->npages) page = -1;
-    }
-    const bool here = page >= 0 && key < W.cap;
-    if (__builtin_amdgcn_ballot_w64(here) == 0) continue;
-    bf16x8 kreg[KSD];
-    const int64_t id64 = page < 0 ? 0 : page;
-    {
-      const uint16_t* krow = (const uint16_t*)P->k.ptr + id64 * P->k.sb + (int64_t)kvh * P->k.sh + (int64_t)r * P->k.ss;
-#pragma unroll
-      for (int s = 0; s < KSD; ++s) {
-        u32x4 w = {0, 0, 0, 0};
-        if (here) w = ld16(krow + 16 * s + 8 * hl);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (w[i] & qand) ^ qxor;
-        kreg[s] = as_bf16x8(w);
-      }
-    }
-    float sum = 0.f;
-    const int i_first = P->causal ? max(k0 - off, 0) & ~31 : 0;  // earlier tokens see no key here
-    for (int h = kvh * P->group; h < (kvh + 1) * P->group; ++h) {
-      const bool graph = RPL > 0 && h < P->H_G;
-      bf16x8 rkreg[KSR > 0 ? KSR : 1];
-      float bh = 0.f;
-      if constexpr (KSR > 0) {
-        const uint16_t* rrow = (const uint16_t*)P->rk.ptr + id64 * P->rk.sb + (int64_t)h * P->rk.sh + (int64_t)r * P->rk.ss;
-        bh = graph ? *const_space(P->gs + h) / P->c : 0.f;
-#pragma unroll
-        for (int s = 0; s < KSR; ++s) {
-          u32x4 w = {0, 0, 0, 0};
-          if (here && graph && 16 * s + 8 * hl < P->R) w = ld16(rrow + 16 * s + 8 * hl);
-          rkreg[s] = as_bf16x8(w);
-        }
-      }
-      for (int i0 = i_first; i0 < e.lq; i0 += 32) {
-        const int tok = i0 + col;  // the row this lane loads
-        const bool have = tok < e.lq;
-        const int64_t t = e.q0 + (have ? tok : 0);
-        f32x16 acc = f32x16{};
-        if constexpr (KSR > 0) {
-          const uint16_t* rrow = (const uint16_t*)P->rq.ptr + t * P->rq.ss + (int64_t)h * P->rq.sh;
-#pragma unroll
-          for (int s = 0; s < KSR; ++s) {
-            u32x4 w = {0, 0, 0, 0};
-            if (have && graph && 16 * s + 8 * hl < P->R) w = ld16(rrow + 16 * s + 8 * hl);
-            acc = mfma32(as_bf16x8(w), rkreg[s], acc);
-          }
-          acc *= bh;
-        }
-        const uint16_t* qrow = (const uint16_t*)P->q.ptr + t * P->q.ss + (int64_t)h * P->q.sh;
-#pragma unroll
-        for (int s = 0; s < KSD; ++s) {
-          u32x4 w = {0, 0, 0, 0};
-          if (have) w = ld16(qrow + 16 * s + 8 * hl);
-          acc = mfma_e<F16>(as_bf16x8(w), kreg[s], acc);
-        }
-        float part = 0.f;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int row = i0 + 8 * (v >> 2) + 4 * hl + (v & 3);
-          const bool see = row < e.lq && (!P->causal || key <= off + row);
-          float nl = kNegInf;
-          if (row < e.lq) {
-            const float l = ((const float*)P->lse.ptr)[(int64_t)(e.q0 + row) * P->lse.ss + (int64_t)h * P->lse.sh];
-            nl = l == kNegInf ? kNegInf : -l * kLog2e;
-          }
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], P->c2, nl));
-          part += see && nl != kNegInf ? p : 0.f;
-        }
-        sum += part;
-      }
-    }
-    sum = wave_pair_sum(sum);
-    if (here && hl == 0) {
-      float* w = W.w + (int64_t)at.b * W.w_sb + (int64_t)kvh * W.w_sh + key;
-      *w += sum;
-    }
-  }
-}
-
 #define FNA2_PACKED(D, RC)                                                                     \
   __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC(const PagedParams) {    \
     packed_body<D, RC, false>();                                                               \
@@ -637,19 +532,6 @@ hipError_t launch_paged_merge(const PagedParams& P, hipStream_t s) {
     hipLaunchKernelGGL(P.f16 ? (paged_merge_kernel<64, true>) : (paged_merge_kernel<64, false>), grid, dim3(256), 0, s, P);
   else
     hipLaunchKernelGGL(P.f16 ? (paged_merge_kernel<128, true>) : (paged_merge_kernel<128, false>), grid, dim3(256), 0, s, P);
-  return hipGetLastError();
-}
-
-hipError_t launch_paged_weights(const PagedWeightsParams& W, hipStream_t s) {
-  const PagedParams& P = W.p;
-  const int rpl = padded_rank32(P.H_G, P.R);
-  void (*k)(const PagedWeightsParams) = nullptr;
-#define FNA2_W(D, RPL) (P.f16 ? paged_weights_kernel<D, RPL, true> : paged_weights_kernel<D, RPL, false>)
-  if (P.D == 64) k = rpl == 0 ? FNA2_W(64, 0) : rpl == 32 ? FNA2_W(64, 32) : FNA2_W(64, 64);
-  if (P.D == 128) k = rpl == 0 ? FNA2_W(128, 0) : rpl == 32 ? FNA2_W(128, 32) : FNA2_W(128, 64);
-#undef FNA2_W
-  if (!k) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(k, dim3((uint32_t)W.grid), dim3(256), 0, s, W);
   return hipGetLastError();
 }
 

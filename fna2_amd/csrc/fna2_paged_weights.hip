@@ -1,0 +1,280 @@
+// fna2_paged_weights.hip — the cached rows' attention weights.
+//
+//     W_j += sum over the chunk's tokens i and the KV head's query heads h of
+//            e^{S_hij - LSE_hi},
+// S as in fna2_paged_attn.hip, whose LSE this takes.
+//
+// The transpose of the attention's loop: a wave keeps 32 keys (K, and R_k of the
+// heads at hand, in registers) as the columns of S = Q K^T and walks the
+// chunk's rows, so that a lane sums its key's weights in registers, in fp32 and
+// in a fixed order.  A row tile is 32 (token, head) pairs: tpt tokens of gsub
+// heads, as the packed kernel's columns for short chunks, 32 tokens of one
+// head for longer ones.  The four waves of a workgroup share the row
+// tiles, which come through a two-stage LDS ring by DMA (rows past the chunk as
+// zeros), with each row's -LSE log2(e) (-inf: it sees nothing, or is none) and last
+// visible key beside them.  Blocks of 128 keys go round over the workgroups.
+//
+// Short chunks are bound by reading K (and R_k) once; long ones by the
+// matrix cores and the exponentials.
+#include <algorithm>
+
+#include "fna2_kernels.h"
+#include "fna2_paged_dev.h"
+
+namespace fna2 {
+
+namespace {
+
+template <int D, int RC>
+struct WeighCfg {
+  static constexpr int KSD = D / 16, KSR = RC / 2;
+  static constexpr int QBYTES = 32 * D * 2, RBYTES = 32 * RC * 16;
+  static constexpr int NQ = QBYTES / 4096;            // DMA instructions per wave and tile
+  static constexpr int NR = (RBYTES / 1024 + 3) / 4;
+};
+
+template <int D, int RC, bool F16>
+__device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
+  using C = WeighCfg<D, RC>;
+  __shared__ __attribute__((aligned(1024))) uint8_t st0[C::QBYTES + C::RBYTES];
+  __shared__ __attribute__((aligned(1024))) uint8_t st1[C::QBYTES + C::RBYTES];
+  // a row tile's -LSE log2(e), and the last keys that its rows see
+  __shared__ __attribute__((aligned(16))) float nl0[32], nl1[32];
+  __shared__ __attribute__((aligned(16))) int lim0[32], lim1[32];
+  KArg P = kargs();
+  const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
+  const int col = lane & 31, hl = lane >> 5;
+  auto units = [&](const PagedSeq& s) { return s.lq > 0 ? (int64_t)P->H_KV * cdiv(s.lk, 128) : 0; };
+  const int64_t total = uni64(wave_total(P, lane, units));
+  const RowLane rdl(lane);
+  const int gsub = P->gsub, tpt = P->tpt;
+  const int lrow = lane >> 2, lch = (lane & 3) ^ swz4(lane >> 2);
+  // DMA slot wv + 4 j of a tile: column group (wv + 4 j) / 2, rows 16 (wv % 2) ..
+  const int drow = 16 * (wv & 1) + lrow;       // the row this lane fetches
+  const int dtk = drow / gsub, dhc = drow - dtk * gsub;
+  const int ltk = col / gsub, lhc = col - ltk * gsub;  // the row whose LSE this lane fetches
+  const uint32_t qxor = P->qa < 0.f ? 0x80008000u : 0u;
+  const uint32_t qand = P->qa == 0.f ? 0u : 0xffffffffu;
+  const float c2 = P->c2;
+
+  for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
+    P = kargs();
+    const PagedAt at = wave_locate(P, lane, id, units);
+    const PagedSeq e = paged_seq_uniform(P, at.b);
+    const int nkb = cdiv(e.lk, 128);
+    const int kvh = uni((int)(at.rem / nkb));
+    const int kb = 128 * (int)(at.rem - (int64_t)kvh * nkb);
+    const int k0 = kb + 32 * wv, key = k0 + col, off = e.lk - e.lq;
+    const bool causal = P->causal != 0;
+    int page = -1, r = 0;
+    if (key < e.lk && key < W.cap) {
+      const int pg = key / P->ps;
+      page = P->table[(int64_t)at.b * P->tstride + pg];
+      r = key - pg * P->ps;
+      if ((uint32_t)page >= (uint32_t)P->npages) page = -1;
+    }
+    const bool here = page >= 0;
+    const bool any = __builtin_amdgcn_ballot_w64(here) != 0;
+    float* wp = W.w + (int64_t)at.b * W.w_sb + (int64_t)kvh * W.w_sh + key;
+    const int64_t id64 = here ? page : 0;
+
+    // row tiles: token tile tt0 + n % ntt of subgroup n / ntt
+    const int tt0 = causal ? max(kb - off, 0) / tpt : 0;  // earlier tokens see none of the keys
+    const int ntt = cdiv(e.lq, tpt) - tt0, n = P->nsub * ntt;
+    const int hkv0 = kvh * P->group, group = P->group, HG = P->H_G;
+    const int crr = P->R / 8;
+    const uint32_t qss = (uint32_t)P->q.ss * 2u, qsh = (uint32_t)P->q.sh * 2u;
+    const uint32_t rss = (uint32_t)P->rq.ss * 2u, rsh = (uint32_t)P->rq.sh * 2u;
+    const uint8_t* const qbase = (const uint8_t*)P->q.ptr + (int64_t)e.q0 * P->q.ss * 2 + (int64_t)hkv0 * P->q.sh * 2;
+    const uint8_t* const rbase = (const uint8_t*)P->rq.ptr + (int64_t)e.q0 * P->rq.ss * 2 + (int64_t)hkv0 * P->rq.sh * 2;
+    const float* const lse = (const float*)P->lse.ptr + (int64_t)e.q0 * P->lse.ss + (int64_t)hkv0 * P->lse.sh;
+    const int64_t lss = P->lse.ss, lsh = P->lse.sh;
+    auto issue = [&](int sub, int tt, uint8_t* base) {
+      const int h0 = sub * gsub, t0 = tt * tpt;
+      const bool on = dtk < tpt && t0 + dtk < e.lq && h0 + dhc < group;
+      const uint32_t vo = on ? (uint32_t)dtk * qss + (uint32_t)dhc * qsh + 16u * lch : kOOB;
+      const auto rs = make_rsrc(qbase + (int64_t)t0 * qss + (int64_t)h0 * qsh, 0x7ffffff0u);
+#pragma unroll
+      for (int j = 0; j < C::NQ; ++j) {
+        const int slot = wv + 4 * j;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(base + slot * 1024), 16,
+                                                 vo + 64u * (slot >> 1), 0, 0, 0);
+      }
+      if constexpr (RC > 0) {
+        // (the row's own head's chunks only: R_q block diagonal)
+        const bool g = on && hkv0 + h0 + dhc < HG;
+        const auto rr = make_rsrc(HG > 0 ? rbase + (int64_t)t0 * rss + (int64_t)h0 * rsh : qbase, 0x7ffffff0u);
+#pragma unroll
+        for (int j = 0; j < C::NR; ++j) {
+          const int slot = wv + 4 * j;
+          if (C::RBYTES / 1024 % 4 == 0 || slot < C::RBYTES / 1024) {
+            const int c = 4 * (slot >> 1) + lch - dhc * crr;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rr, (lds_void*)(base + C::QBYTES + slot * 1024), 16,
+                g && c >= 0 && c < crr ? (uint32_t)dtk * rss + (uint32_t)dhc * rsh + 16u * c : kOOB, 0, 0, 0);
+          }
+        }
+      }
+    };
+    // a tile's LSE (of row `col`), by wave 0
+    auto fetch = [&](int sub, int tt) {
+      const int tok = tt * tpt + ltk, h = sub * gsub + lhc;
+      return ltk < tpt && tok < e.lq && h < group ? lse[(int64_t)tok * lss + (int64_t)h * lsh] : kNegInf;
+    };
+    auto put = [&](int tt, float l, float* nl, int* lim) {
+      if (hl == 0) {
+        nl[col] = l == kNegInf ? kNegInf : -l * kLog2e;
+        lim[col] = causal ? off + tt * tpt + ltk : e.lk;
+      }
+    };
+
+    ring_barrier<0>();  // the ring's last tiles are read
+    issue(0, tt0, st0);
+    float lnext = 0.f;
+    if (wv == 0) lnext = fetch(0, tt0);
+    // K (B of S = Q K^T): lane holds K[key][16 s + 8 hl .. +7]
+    bf16x8 kreg[C::KSD];
+    {
+      const uint16_t* krow = (const uint16_t*)P->k.ptr + id64 * P->k.sb + (int64_t)kvh * P->k.sh + (int64_t)r * P->k.ss;
+#pragma unroll
+      for (int s = 0; s < C::KSD; ++s) {
+        u32x4 w = {0, 0, 0, 0};
+        if (here) w = ld16(krow + 16 * s + 8 * hl);
+        kreg[s] = as_bf16x8(w);
+      }
+    }
+    float old = 0.f;
+    if (here && hl == 0) old = *wp;
+    if (wv == 0) put(tt0, lnext, nl0, lim0);
+#pragma unroll
+    for (int s = 0; s < C::KSD; ++s) {
+      u32x4 w = as_u32x4(kreg[s]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (w[i] & qand) ^ qxor;
+      kreg[s] = as_bf16x8(w);
+    }
+
+    bf16x8 rkreg[C::KSR > 0 ? C::KSR : 1];
+    float bh[16];
+    float sum = 0.f;
+    int sub = 0, tt = tt0;  // of the tile at hand
+    auto step = [&](int t, const uint8_t* cur, const float* nl, const int* lim, uint8_t* nxt,
+                    float* nl_nxt, int* lim_nxt) {
+      ring_barrier<0>();
+      const bool more = t + 1 < n;
+      const int sub1 = tt + 1 < tt0 + ntt ? sub : sub + 1, tt1 = sub1 == sub ? tt + 1 : tt0;
+      if (more) {
+        issue(sub1, tt1, nxt);
+        if (wv == 0) lnext = fetch(sub1, tt1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (RC > 0) {
+        if (tt == tt0) {  // a new subgroup: its R_k, and each row's graph scale
+          const int h0 = hkv0 + sub * gsub;
+          const uint16_t* rrow = (const uint16_t*)P->rk.ptr + id64 * P->rk.sb + (int64_t)h0 * P->rk.sh + (int64_t)r * P->rk.ss;
+          const int gg = min(max(min(HG - h0, group - sub * gsub), 0), gsub);
+#pragma unroll
+          for (int s = 0; s < C::KSR; ++s) {
+            const int c = 2 * s + hl, hh = gsub == 1 ? 0 : c / crr;
+            u32x4 w = {0, 0, 0, 0};
+            if (here && c < gg * crr) w = ld16(rrow + (int64_t)hh * P->rk.sh + 8 * (c - hh * crr));
+            rkreg[s] = as_bf16x8(w);
+          }
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int row = 8 * (v >> 2) + 4 * hl + (v & 3), hc = gsub == 1 ? 0 : row % gsub;
+            bh[v] = hc < gg ? P->gs[h0 + hc] / P->c : 0.f;
+          }
+        }
+      }
+      if (any && (!causal || k0 <= off + tt * tpt + tpt - 1)) {
+        f32x16 acc = f32x16{};
+        if constexpr (RC > 0) {
+#pragma unroll
+          for (int s = 0; s < C::KSR; ++s)
+            acc = mfma32(row_read<32>(cur + C::QBYTES, rdl, 0, s), rkreg[s], acc);
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[v] *= bh[v];
+        }
+#pragma unroll
+        for (int s = 0; s < C::KSD; ++s)
+          acc = mfma_e<F16>(row_read<32>(cur, rdl, 0, s), kreg[s], acc);
+        float part = 0.f;
+        if (causal && k0 + 31 > off + tt * tpt) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4_t a = *(const f32x4_t*)(nl + 8 * q + 4 * hl);
+            const u32x4 m = *(const u32x4*)(lim + 8 * q + 4 * hl);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * q + i], c2, a[i]));
+              part += key <= (int)m[i] && a[i] != kNegInf ? p : 0.f;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4_t a = *(const f32x4_t*)(nl + 8 * q + 4 * hl);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              part += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * q + i], c2, a[i]));
+          }
+        }
+        sum += part;
+      }
+      if (more && wv == 0) put(tt1, lnext, nl_nxt, lim_nxt);
+      sub = sub1;
+      tt = tt1;
+    };
+    for (int t = 0; t < n; t += 2) {
+      step(t, st0, nl0, lim0, st1, nl1, lim1);
+      if (t + 1 < n) step(t + 1, st1, nl1, lim1, st0, nl0, lim0);
+    }
+    sum = wave_pair_sum(sum);
+    if (here && hl == 0) *wp = old + sum;
+  }
+}
+
+// Workgroups of a CU, by the registers that R_k takes.
+constexpr int weigh_occ(int rc) { return rc == 0 ? 4 : rc <= 16 ? 3 : 2; }
+
+#define FNA2_WEIGH(D, RC)                                                                           \
+  __global__ __launch_bounds__(256, weigh_occ(RC)) void paged_weigh_d##D##_c##RC(const PagedWeightsParams W) {  \
+    weigh_body<D, RC, false>(W);                                                                    \
+  }                                                                                                 \
+  __global__ __launch_bounds__(256, weigh_occ(RC)) void paged_weigh_d##D##_c##RC##_f16(const PagedWeightsParams W) { \
+    weigh_body<D, RC, true>(W);                                                                     \
+  }
+FNA2_WEIGH(64, 0)
+FNA2_WEIGH(64, 4)
+FNA2_WEIGH(64, 8)
+FNA2_WEIGH(64, 16)
+FNA2_WEIGH(64, 32)
+FNA2_WEIGH(128, 0)
+FNA2_WEIGH(128, 4)
+FNA2_WEIGH(128, 8)
+FNA2_WEIGH(128, 16)
+FNA2_WEIGH(128, 32)
+#undef FNA2_WEIGH
+
+}  // namespace
+
+int paged_weigh_per_cu(int rc) { return weigh_occ(rc); }
+
+hipError_t launch_paged_weights(const PagedWeightsParams& W, int rc, hipStream_t s) {
+  const PagedParams& P = W.p;
+  void (*k)(const PagedWeightsParams) = nullptr;
+#define FNA2_WEIGH_OF(D, RC) (P.f16 ? paged_weigh_d##D##_c##RC##_f16 : paged_weigh_d##D##_c##RC)
+  if (P.D == 64)
+    k = rc == 0 ? FNA2_WEIGH_OF(64, 0) : rc == 4 ? FNA2_WEIGH_OF(64, 4) : rc == 8 ? FNA2_WEIGH_OF(64, 8)
+      : rc == 16 ? FNA2_WEIGH_OF(64, 16) : rc == 32 ? FNA2_WEIGH_OF(64, 32) : nullptr;
+  if (P.D == 128)
+    k = rc == 0 ? FNA2_WEIGH_OF(128, 0) : rc == 4 ? FNA2_WEIGH_OF(128, 4) : rc == 8 ? FNA2_WEIGH_OF(128, 8)
+      : rc == 16 ? FNA2_WEIGH_OF(128, 16) : rc == 32 ? FNA2_WEIGH_OF(128, 32) : nullptr;
+#undef FNA2_WEIGH_OF
+  if (!k) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(k, dim3((uint32_t)W.grid), dim3(256), 0, s, W);
+  return hipGetLastError();
+}
+
+}  // namespace fna2
