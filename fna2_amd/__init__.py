@@ -20,10 +20,16 @@ from .flash_naylis_attn import (  # noqa: F401
     FlashNaylisAttnFunc,
     flash_naylis_attn,
 )
-from .paged import flash_naylis_paged, paged_append, paged_evict  # noqa: F401
+from .paged import (  # noqa: F401
+    PagedKVCache,
+    PageTable,
+    flash_naylis_paged,
+    paged_append,
+    paged_evict,
+)
 from .rope import rope_varlen  # noqa: F401
 from . import ops  # noqa: F401,E402  (registers the fna2::fwd / fna2::bwd custom ops)
 
 __all__ = ["BLOCK_M", "BLOCK_N", "BLOCK_R", "FlashNaylisAttnFunc", "flash_naylis_attn",
-           "flash_naylis_decode", "flash_naylis_paged", "paged_append", "paged_evict",
+           "flash_naylis_decode", "flash_naylis_paged", "PagedKVCache", "PageTable", "paged_append", "paged_evict",
            "rope_varlen"]

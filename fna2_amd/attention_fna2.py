@@ -16,6 +16,9 @@ The module keeps the reference's constructor and ``forward`` signatures
   that a decode step equals the last row of the full causal forward.
   ``past_kv`` may also be a ``StaticKVCache`` (preallocated, written in
   place: no per-step copy of the cache);
+* with a ``PagedKVCache`` as ``past_kv`` a call serves the new tokens of many
+  sequences, prompts in pieces and single tokens together, on the paged kernels
+  (``paged_append``, ``flash_naylis_paged``), always with the graph bias;
 * the other paths the reference sends elsewhere keep going elsewhere:
   ``soft_cap`` and modules built with ``use_fna2=False`` use PyTorch's SDPA
   with a materialised bias, or the explicit softmax when a ``soft_cap`` or
@@ -46,6 +49,7 @@ from .flash_naylis_attn import BLOCK_R, flash_naylis_attn, rank_supported
 from .flash_naylis_attn import FlashNaylisAttnFunc as _FNA2Func
 from .flash_naylis_attn import _plain_eager as _fna2_plain_eager
 from .decode import decode_supported, flash_naylis_decode
+from .paged import PagedKVCache, PageTable, flash_naylis_paged, paged_append  # noqa: F401
 from .rope import rope_varlen
 
 
@@ -585,6 +589,8 @@ class NaylisAttention(nn.Module):
         max_seqlen_q: Optional[int] = None,
         max_seqlen_k: Optional[int] = None,
     ) -> Tuple[torch.Tensor, Optional[KVCache]]:
+        if isinstance(past_kv, PagedKVCache):
+            return self._forward_paged(x, mask, past_kv, use_kv_cache, cu_seqlens_q, max_seqlen_q)
         if cu_seqlens_q is not None:
             return self._forward_varlen(x, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
                                         max_seqlen_k)
@@ -719,6 +725,53 @@ class NaylisAttention(nn.Module):
             out = self._attend_eager(x, q, kc, vc, mask, rows, scale, False, False, bias)
         out = out.transpose(1, 2).contiguous().view(B, S, self.embed_dim)
         return self._finish(out, orig_dtype), (cache if use_kv_cache else None)
+
+    def _forward_paged(self, x, mask, cache: PagedKVCache, use_kv_cache: bool, cu_seqlens_q,
+                       max_seqlen_q):
+        """The new tokens of the step that ``cache.table`` describes (its last
+        ``extend``), packed as ``[T, E]`` or ``[N, S, E]``: their rows go into
+        the cache, and each attends to its sequence's rows up to its own.  Keys
+        are rotated for their position and stay so.  Forward only."""
+        t = cache.table
+        if not self._use_fna2 or self.soft_cap is not None or mask is not None:
+            raise RuntimeError("a PagedKVCache needs the FNA2 HIP kernels (gfx950, "
+                               "libfna2_hip.so, no soft_cap, no mask)")
+        if (cache.r_k is not None) != (self.graph_heads > 0):
+            raise ValueError("a PagedKVCache holds r_k exactly where the layer has graph heads")
+        lead = x.shape[:-1]
+        x2 = x.reshape(-1, x.shape[-1])
+        cu = t.cu_seqlens_q if cu_seqlens_q is None else cu_seqlens_q
+        max_q = t.max_seqlen_q if max_seqlen_q is None else max_seqlen_q
+        if cu_seqlens_q is None and x2.shape[0] != t.total_q:
+            raise ValueError(f"{x2.shape[0]} tokens, but the PageTable was extended by {t.total_q}")
+        q, k, v, r_q, r_k = self._project(x2)
+        orig_dtype = q.dtype
+        if q.dtype != cache.k.dtype:
+            q, k, v = (y.to(cache.k.dtype) for y in (q, k, v))
+        wq = wk = inv = None
+        eps = 1e-6
+        if self.use_qk_norm:  # with the rotation in the append's launch, in fp32
+            assert self.q_norm.eps == self.k_norm.eps
+            wq, wk, eps = self.q_norm.weight, self.k_norm.weight, self.q_norm.eps
+            inv = None if self.rope is None else self.rope.inv_freq
+        elif self.rope is not None:  # rounded as rope_varlen rounds without a norm
+            pos = t.positions
+            if pos is None:
+                rows = torch.arange(x2.shape[0], device=x.device)
+                b = torch.searchsorted(cu[1:].contiguous(), rows.to(cu.dtype), right=True)
+                b = b.clamp(max=t.seqlens.shape[0] - 1)
+                pos = rows - cu[b + 1] + t.seqlens[b]
+            cos, sin = self.rope._table(max(t.next_position, default=0), q.device, q.dtype)
+            pos = pos.long().clamp(0, cos.shape[0] - 1)
+            cos, sin = cos[pos][:, None], sin[pos][:, None]
+            q, k = self.rope.rotate(q, cos, sin), self.rope.rotate(k, cos, sin)
+        q = paged_append(q, k, v, cache.k, cache.v, t.block_table, t.seqlens, cu, r_k, cache.r_k,
+                         inv, t.positions if inv is not None else None, wq, wk, eps)
+        out = flash_naylis_paged(q, cache.k, cache.v, t.block_table, t.seqlens, cu, max_q, r_q,
+                                 cache.r_k, self.graph_scale, softmax_scale=self._attn_scale(),
+                                 key_weights=cache.key_weights)
+        y = self._finish(out.view(x2.shape[0], self.embed_dim), orig_dtype)
+        return y.view(*lead, self.embed_dim), (cache if use_kv_cache else None)
 
     def _decode_rows(self, q, k, v, r_k, cache: StaticKVCache) -> Optional[torch.Tensor]:
         """The step's QK-RMSNorm, rotation and cache append in one launch:

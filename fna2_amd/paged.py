@@ -30,7 +30,7 @@ fallback: without the HIP library, or off the GPU, the calls raise.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -381,3 +381,142 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     _bump(k_pages, v_pages, rk_pages if H_G else None)
     del keep
     return kept, lens, w_out
+
+
+class PageTable:
+    """Which pages hold the rows of which sequence: one for all the layers of
+    a model, whose pools (``PagedKVCache``) all have its pages.
+
+    ``block_table`` ``[sequences, max_pages]`` and ``seqlens`` ``[sequences]``
+    (int32) are on the device and written in place, so that captured graphs
+    read the step at hand.  ``extend(counts)`` takes in the new tokens of a step;
+    ``cu_seqlens_q``, ``max_seqlen_q``, ``total_q`` and ``positions`` then
+    describe them for every layer.  The bookkeeping is the host's: nothing is
+    read back from the device."""
+
+    def __init__(self, sequences: int, num_pages: int, page_size: int = 64,
+                 max_pages: Optional[int] = None, device=None):
+        assert page_size > 0 and page_size % 16 == 0, "page_size must be a multiple of 16"
+        assert sequences >= 0 and num_pages >= 0
+        self.page_size, self.num_pages = int(page_size), int(num_pages)
+        self.width = int(num_pages if max_pages is None else max_pages)
+        self.rows = [0] * sequences       # rows in use
+        self.next_position = [0] * sequences
+        self.pages = [[] for _ in range(sequences)]
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._host = torch.full((sequences, self.width), -1, dtype=torch.int32)
+        self.block_table = self._host.to(device)
+        self.seqlens = torch.zeros(sequences, dtype=torch.int32, device=device)
+        self.cu_seqlens_q = torch.zeros(sequences + 1, dtype=torch.int32, device=device)
+        self.max_seqlen_q = self.total_q = 0
+        self.positions: Optional[torch.Tensor] = None  # [total_q]; None: a token's row
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _upload(self, table: bool) -> None:
+        self.seqlens.copy_(torch.tensor(self.rows, dtype=torch.int32))
+        if table:
+            self.block_table.copy_(self._host)
+
+    def _give_back(self, b: int, keep: int) -> bool:
+        if len(self.pages[b]) <= keep:
+            return False
+        self._free += reversed(self.pages[b][keep:])
+        del self.pages[b][keep:]
+        self._host[b, keep:] = -1
+        return True
+
+    def extend(self, counts: Sequence[int]) -> None:
+        """counts[b] new tokens for sequence b (0: none this step).  Raises
+        ValueError, with nothing changed, where the pages do not suffice."""
+        counts = [int(c) for c in counts]
+        assert len(counts) == len(self.rows) and all(c >= 0 for c in counts), \
+            "one count for each sequence"
+        ps = self.page_size
+        need = [-(-(r + c) // ps) for r, c in zip(self.rows, counts)]
+        more = [max(n - len(p), 0) for n, p in zip(need, self.pages)]
+        if max(need, default=0) > self.width:
+            raise ValueError(f"PageTable full: a sequence needs {max(need)} pages, "
+                             f"its table holds {self.width}")
+        if sum(more) > len(self._free):
+            raise ValueError(f"PageTable full: {sum(more)} pages needed, {len(self._free)} free")
+        for b, m in enumerate(more):
+            for _ in range(m):
+                self._host[b, len(self.pages[b])] = self._free[-1]
+                self.pages[b].append(self._free.pop())
+        cu, pos = [0], []
+        moved = self.rows != self.next_position
+        for b, c in enumerate(counts):
+            cu.append(cu[-1] + c)
+            if moved:
+                pos += range(self.next_position[b], self.next_position[b] + c)
+            self.rows[b] += c
+            self.next_position[b] += c
+        self.cu_seqlens_q.copy_(torch.tensor(cu, dtype=torch.int32))
+        self.total_q, self.max_seqlen_q = cu[-1], max(counts, default=0)
+        self.positions = torch.tensor(pos, dtype=torch.int32, device=self.seqlens.device) \
+            if moved else None
+        self._upload(any(more))
+
+    def truncate(self, budget: int) -> None:
+        """After every layer's ``PagedKVCache.evict(budget)``: no sequence has
+        more than ``budget`` rows, and the pages behind them are free.  The
+        positions of the tokens to come go on counting."""
+        self.rows = [min(r, int(budget)) for r in self.rows]
+        freed = [self._give_back(b, -(-r // self.page_size)) for b, r in enumerate(self.rows)]
+        self._upload(any(freed))
+
+    def release(self, b: int) -> None:
+        """Sequence b is done: its pages are free, and its place for another."""
+        self.rows[b] = self.next_position[b] = 0
+        self._give_back(b, 0)
+        self._upload(True)
+
+
+class PagedKVCache:
+    """One layer's pools on the pages of a ``PageTable``: a ``past_kv`` of
+    ``NaylisAttention`` that serves many sequences of differing lengths, prompts
+    in pieces and single tokens in one call.
+
+    ``k``, ``v`` ``[pages, H_KV, page_size, D]``, ``r_k`` ``[pages, H_G,
+    page_size, R]`` (bf16) for a layer with graph heads.  With ``weigh`` the
+    layer's calls add up each cached row's attention weight (``key_weights``
+    ``[sequences, H_KV, max_pages * page_size]``), by which ``evict`` goes."""
+
+    def __init__(self, table: PageTable, k: torch.Tensor, v: torch.Tensor,
+                 r_k: Optional[torch.Tensor] = None, key_weights: Optional[torch.Tensor] = None):
+        assert k.shape == v.shape and k.dim() == 4 and k.shape[0] == table.num_pages and \
+            k.shape[2] == table.page_size, "k and v must be [pages, H_KV, page_size, D]"
+        assert r_k is None or (r_k.dim() == 4 and r_k.shape[0] == k.shape[0]
+                               and r_k.shape[2] == k.shape[2]), \
+            "r_k must be [pages, H_G, page_size, R]"
+        self.table, self.k, self.v, self.r_k, self.key_weights = table, k, v, r_k, key_weights
+
+    @classmethod
+    def empty(cls, table: PageTable, n_kv_heads: int, head_dim: int, graph_heads: int = 0,
+              rank: int = 0, dtype=torch.bfloat16, weigh: bool = False) -> "PagedKVCache":
+        dev, ps = table.block_table.device, table.page_size
+        mk = lambda h, f, dt: torch.zeros(table.num_pages, h, ps, f, dtype=dt, device=dev)
+        w = torch.zeros(len(table.rows), n_kv_heads, table.width * ps, device=dev) if weigh else None
+        return cls(table, mk(n_kv_heads, head_dim, dtype), mk(n_kv_heads, head_dim, dtype),
+                   mk(graph_heads, rank, torch.bfloat16) if graph_heads > 0 else None, w)
+
+    def evict(self, budget: int, recent: int = 0, first: int = 0,
+              heads: Optional[int] = None) -> torch.Tensor:
+        """``paged_evict`` of this layer by its ``key_weights`` (``heads``: the
+        layer's query heads, needed with ``r_k``); returns the rows kept.  When
+        every layer has done so, ``PageTable.truncate(budget)``."""
+        assert self.key_weights is not None, "evict: this cache does not weigh its rows"
+        t = self.table
+        kept, _, w = paged_evict(self.k, self.v, t.block_table, t.seqlens, self.key_weights,
+                                 budget, recent, first, self.r_k, heads)
+        self.key_weights.copy_(w)
+        return kept
+
+    def forget(self, b: int) -> None:
+        """Sequence b's place is for another: its weights start at 0 (after
+        ``PageTable.release(b)``, in every layer)."""
+        if self.key_weights is not None:
+            self.key_weights[b].zero_()

@@ -1,0 +1,216 @@
+"""PageTable, PagedKVCache and NaylisAttention on them.
+
+CPU: the page table's bookkeeping.  GPU: a layer that serves prompts in pieces
+and single tokens from pages against its own forward over whole sequences, with
+the page table's steps captured into a graph, and with eviction.
+
+Tolerance of the layer comparison: both sides compute the same products of bf16
+values and may round five things between to other neighbours (the rotated q
+and k, P, the attention's output and the layer's), each by at most 2^-8 of the
+value: 5 * 2^-8 of the output's norm.
+"""
+import pytest
+import torch
+
+from fna2_amd import _capi
+from fna2_amd.paged import PagedKVCache, PageTable
+
+from tests.helpers import rel_norm
+
+
+def test_page_table_counts_rows_and_pages():
+    t = PageTable(3, 10, page_size=16, max_pages=5)
+    t.extend([20, 0, 16])
+    assert t.rows == [20, 0, 16] and [len(p) for p in t.pages] == [2, 0, 1]
+    assert t.cu_seqlens_q.tolist() == [0, 20, 20, 36] and t.max_seqlen_q == 20 and t.total_q == 36
+    assert t.seqlens.tolist() == [20, 0, 16] and t.positions is None and t.free_pages == 7
+    named = [p for row in t.block_table.tolist() for p in row if p >= 0]
+    assert len(set(named)) == 3 and sorted(named) == sorted(sum(t.pages, []))
+    t.extend([1, 1, 1])
+    assert [len(p) for p in t.pages] == [2, 1, 2] and t.free_pages == 5
+    before = (list(t.rows), [list(p) for p in t.pages], t.block_table.tolist())
+    with pytest.raises(ValueError, match="table holds 5"):
+        t.extend([80, 0, 0])
+    with pytest.raises(ValueError, match="5 free"):
+        t.extend([50, 40, 30])
+    assert before == (list(t.rows), [list(p) for p in t.pages], t.block_table.tolist())
+    with pytest.raises(AssertionError):
+        t.extend([1, 1])
+    with pytest.raises(AssertionError):
+        t.extend([1, -1, 0])
+
+
+def test_page_table_truncate_and_release():
+    t = PageTable(2, 6, page_size=16)
+    t.extend([50, 10])
+    data = t.block_table.data_ptr()
+    t.truncate(20)
+    assert t.rows == [20, 10] and [len(p) for p in t.pages] == [2, 1] and t.free_pages == 3
+    assert (t.block_table[0, 2:] == -1).all() and t.seqlens.tolist() == [20, 10]
+    t.extend([2, 1])
+    # rows and positions differ from now on
+    assert t.positions.tolist() == [50, 51, 10] and t.seqlens.tolist() == [22, 11]
+    t.release(0)
+    assert t.rows == [0, 11] and t.free_pages == 5 and (t.block_table[0] == -1).all()
+    t.extend([3, 1])
+    assert t.positions is None or t.positions.tolist() == [0, 1, 2, 11]
+    assert t.block_table.data_ptr() == data  # written in place
+    with pytest.raises(AssertionError):
+        PageTable(1, 4, page_size=24)
+
+
+def test_cache_shapes_are_checked():
+    t = PageTable(2, 6, page_size=16)
+    c = PagedKVCache.empty(t, 2, 64, graph_heads=3, rank=8, weigh=True)
+    assert c.k.shape == (6, 2, 16, 64) and c.r_k.shape == (6, 3, 16, 8)
+    assert c.key_weights.shape == (2, 2, 96)
+    with pytest.raises(AssertionError):
+        PagedKVCache(t, c.k[:5], c.v[:5])
+    with pytest.raises(AssertionError):
+        PagedKVCache(t, c.k, c.v, c.r_k[:, :, :8])
+    with pytest.raises(AssertionError):
+        PagedKVCache.empty(t, 2, 64).evict(10)
+
+
+def test_module_without_the_kernels_raises():
+    from fna2_amd.attention_fna2 import NaylisAttention
+    m = NaylisAttention(128, 2, rel_rank=8, use_fna2=False)
+    t = PageTable(1, 4, page_size=16)
+    t.extend([3])
+    with pytest.raises(RuntimeError):
+        m(torch.zeros(3, 128), past_kv=PagedKVCache.empty(t, 2, 64, 2, 8))
+
+
+# ── GPU ──────────────────────────────────────────────────────────────────────
+
+def _layer(gpu, dtype=torch.bfloat16, **kw):
+    from fna2_amd.attention_fna2 import NaylisAttention
+    torch.manual_seed(0)
+    m = NaylisAttention(512, 8, n_kv_heads=2, max_seq_len=256, **{**dict(rel_rank=16), **kw})
+    if m.graph_scale is not None:
+        with torch.no_grad():
+            m.graph_scale.normal_(1.0, 0.5)
+            m.rel_q_proj.weight.normal_(std=0.05)
+            m.rel_k_proj.weight.normal_(std=0.05)
+    return m.to(gpu).to(dtype).eval()
+
+
+def _cache(m, t, **kw):
+    return PagedKVCache.empty(t, m.n_kv_heads, m.head_dim, m.graph_heads, m.rel_rank, **kw)
+
+
+STEPS = [[37, 0, 5], [40, 70, 1], [1, 1, 1], [1, 0, 1], [0, 3, 33], [1, 1, 1]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(vanilla_heads=3), dict(vanilla_heads=7),
+                                dict(use_qk_norm=False), dict(use_rope=False)])
+def test_pieces_and_tokens_equal_the_whole_sequences(gpu, kw):
+    m = _layer(gpu, **kw)
+    t = PageTable(3, 40, page_size=16, device=gpu)
+    c = _cache(m, t)
+    total = [sum(s[b] for s in STEPS) for b in range(3)]
+    xs = [torch.randn(n, 512, device=gpu).bfloat16() for n in total]
+    got, at = [[] for _ in total], [0, 0, 0]
+    with torch.no_grad():
+        for s in STEPS:
+            t.extend(s)
+            x = torch.cat([xs[b][at[b]:at[b] + s[b]] for b in range(3)])
+            y, back = m(x, past_kv=c, use_kv_cache=True)
+            assert back is c
+            for b, part in enumerate(torch.split(y, s)):
+                got[b].append(part)
+                at[b] += s[b]
+        cu = torch.tensor([0, total[0], total[0] + total[1], sum(total)], dtype=torch.int32, device=gpu)
+        ref, _ = m(torch.cat(xs), cu_seqlens_q=cu, max_seqlen_q=max(total))
+    out = torch.cat([torch.cat(g) for g in got])
+    assert rel_norm(out, ref.double().cpu().numpy()) < 5 * 2.0 ** -8
+    assert t.seqlens.tolist() == total
+
+
+@pytest.mark.gpu
+def test_tokens_as_a_batch_and_wrong_calls(gpu):
+    m = _layer(gpu)
+    t = PageTable(2, 20, page_size=16, device=gpu)
+    c, d = _cache(m, t), _cache(m, t)
+    x = torch.randn(2, 3, 512, device=gpu).bfloat16()
+    t.extend([3, 3])
+    with torch.no_grad():
+        y, none = m(x, past_kv=c)
+        z, _ = m(x.view(6, 512), past_kv=d)
+    assert none is None and y.shape == (2, 3, 512) and torch.equal(y.view(6, 512), z)
+    with pytest.raises(ValueError):
+        m(x[:, :2], past_kv=c)
+    with pytest.raises(ValueError):
+        m(x, past_kv=PagedKVCache.empty(t, 2, 64))
+    with pytest.raises(RuntimeError):
+        m(x, mask=torch.ones(3, 3, dtype=torch.bool, device=gpu), past_kv=c)
+
+
+@pytest.mark.gpu
+def test_a_decode_step_as_a_graph(gpu):
+    """One captured step, replayed while the page table moves on under it, with
+    eager steps of a second cache between."""
+    m = _layer(gpu)
+    t = PageTable(2, 40, page_size=16, device=gpu)
+    a, b = _cache(m, t, weigh=True), _cache(m, t, weigh=True)
+    x0 = torch.randn(2, 12, 512, device=gpu).bfloat16()
+    with torch.no_grad():
+        t.extend([12, 12])
+        for c in (a, b):
+            m(x0, past_kv=c)
+        t.extend([1, 1])
+        x = torch.randn(2, 1, 512, device=gpu).bfloat16()
+        for _ in range(2):  # (the same rows again: nothing changes but the weights)
+            m(x, past_kv=a)
+        m(x, past_kv=b)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, _ = m(x, past_kv=a)
+        for i in range(20):  # over a page's end
+            t.extend([1, 1])
+            x.copy_(torch.randn(2, 1, 512, device=gpu).bfloat16())
+            want, _ = m(x, past_kv=b)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), i
+    assert torch.equal(a.k, b.k) and torch.equal(a.r_k, b.r_k)
+
+
+@pytest.mark.gpu
+def test_two_layers_with_eviction(gpu):
+    """Decoding with a budget: every layer evicts by its own weights, the table
+    is cut once, positions go on counting; what is evicted last is what the
+    weights say, and the outputs stay those of the rows that were kept."""
+    layers = [_layer(gpu), _layer(gpu, vanilla_heads=4)]
+    t = PageTable(2, 12, page_size=16, device=gpu)
+    cs = [_cache(m, t, weigh=True) for m in layers]
+    g = torch.Generator().manual_seed(3)
+    with torch.no_grad():
+        t.extend([60, 41])
+        x = torch.randn(101, 512, generator=g).bfloat16().to(gpu)
+        for m, c in zip(layers, cs):
+            x = x + m(x, past_kv=c)[0]
+        for m, c in zip(layers, cs):
+            # every token's weights sum to one for each query head
+            assert torch.allclose(c.key_weights.sum(-1).sum(-1),
+                                  torch.tensor([60. * 8, 41. * 8], device=gpu), rtol=1e-4)
+            kept = c.evict(48, recent=8, first=2, heads=8)
+            assert kept.shape == (2, 2, 48) and (kept[1, :, 41:] == -1).all()
+            assert (kept[0, :, :2] == torch.tensor([0, 1], device=gpu)).all()
+            assert (kept[0, :, -8:] == torch.arange(52, 60, device=gpu)).all()
+            assert (c.key_weights[0, :, 48:] == 0).all()
+        t.truncate(48)
+        assert t.rows == [48, 41] and t.free_pages == 12 - 3 - 3
+        for _ in range(9):
+            t.extend([1, 1])
+            x = torch.randn(2, 512, generator=g).bfloat16().to(gpu)
+            for m, c in zip(layers, cs):
+                x = x + m(x, past_kv=c)[0]
+                assert torch.isfinite(x).all()
+        assert t.next_position == [69, 50] and t.rows == [57, 50]
+        t.release(1)
+        for c in cs:
+            c.forget(1)
+            assert (c.key_weights[1] == 0).all()
