@@ -131,7 +131,7 @@ __device__ __forceinline__ void packed_body() {
     const bool live = tk < P->tpt && tok < e.lq && hc < nh;
     const int off = e.lk - e.lq;
     // last key that this column, and that every column, sees
-    const int lim = causal ? off + tok : e.lk - 1;
+    const int lim = min(causal ? off + tok : e.lk, e.lk - 1);
     const int lim_all = causal ? min(off + ct * P->tpt, e.lk - 1) : e.lk - 1;
     const int lim_any = causal ? off + ct * P->tpt + P->tpt - 1 : e.lk - 1;  // ... that any sees
     const int* trow = P->table + (int64_t)b * P->tstride;
@@ -153,17 +153,14 @@ __device__ __forceinline__ void packed_body() {
     }
     PageCursor cur;
     cur.at(ps, 32 * s0);
-    auto page_id = [&](int row) {  // of the cursor's row group; -1 past the run or the pool
-      if (row >= e.lk) return -1;
-      const int id = uni(*const_space(trow + cur.page));
-      return (uint32_t)id < (uint32_t)npages ? id : -1;
-    };
-    // ids and places of the next tile's two row groups
-    int pid[2], poff[2];
+    const int page_last = e.lk > 0 ? (e.lk - 1) / ps : -1;
+    // Ids (as loaded, looked at when the tile is issued: no step waits for
+    // them) and places of the next tile's two row groups.
+    int pid[2] = {-1, -1}, poff[2];
     auto look = [&](int t) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        pid[g] = t < s1 ? page_id(32 * t + 16 * g) : -1;
+        if (page_last >= 0) pid[g] = *const_space(trow + min(cur.page, page_last));
         poff[g] = cur.off;
         cur.next(ps);
       }
@@ -175,10 +172,11 @@ __device__ __forceinline__ void packed_body() {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const int row = 32 * t + 16 * g;
-        const bool here = pid[g] >= 0;
+        const bool known = (uint32_t)uni(pid[g]) < (uint32_t)npages;
+        const bool here = known && t < s1;
         const int rows = here ? clamp_rows(e.lk - row, 16) : 0;
-        if (!here && row < e.lk) gone |= 1 << g;
-        const int64_t id = here ? pid[g] : 0;
+        if (!known && row < e.lk) gone |= 1 << g;
+        const int64_t id = here ? uni(pid[g]) : 0;
         const int r = here ? poff[g] : 0;
         const auto rk_ = make_rsrc((const uint8_t*)(kpool + id * ksb) + (uint64_t)(uint32_t)r * krb,
                                    (uint32_t)rows * krb);
@@ -277,7 +275,7 @@ __device__ __forceinline__ void packed_body() {
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const int key = kbase + 8 * (v >> 2) + 4 * hl + (v & 3);
-          const bool dead = key > lim || key >= e.lk || ((gone_now >> (v >> 3)) & 1);
+          const bool dead = key > lim || ((gone_now >> (v >> 3)) & 1);
           acc[v] = dead ? kNegInf : acc[v];
         }
       }

@@ -129,8 +129,7 @@ __device__ __forceinline__ void tile_body() {
     const bool graph = RPL > 0 && h < P->H_G;
     const float bh = uni_f(graph ? *const_space(P->gs + h) / P->c : 0.f);
     const int k_end = min(32 * s1, e.lk);  // rows of this run's part
-    const int lim = causal ? off + tok : e.lk - 1;
-    const int lim_all = causal ? off + tok0 : e.lk - 1;      // all of the wave's tokens see
+    const int lim = min(causal ? off + tok : e.lk - 1, k_end - 1);  // last row this column sees
     const int lim_any = causal ? off + tok_last : e.lk - 1;  // some of them see
     const int* trow = P->table + (int64_t)b * P->tstride;
     const int ps = P->ps, npages = P->npages;
@@ -152,20 +151,20 @@ __device__ __forceinline__ void tile_body() {
       gone = __builtin_amdgcn_ballot_w64(gone) != 0;
     }
 
-    // Page of this wave's row group of the next tile.
+    // Page of this wave's row group of the next tile.  Its id is loaded a step
+    // ahead and looked at only when the tile is issued, so that no step waits
+    // for it.
     int row = 32 * s0 + 16 * rg;
     int page = row / ps, poff = row - page * ps;
+    const int page_last = k_end > 0 ? (k_end - 1) / ps : -1;
     int pid = -1;
     auto look = [&]() {
-      pid = -1;
-      if (row < k_end) {
-        const int id = uni(*const_space(trow + page));
-        pid = (uint32_t)id < (uint32_t)npages ? id : -1;
-      }
+      if (page_last >= 0) pid = *const_space(trow + min(page, page_last));
     };
     auto issue = [&](uint8_t* base) {
-      const int rows = pid >= 0 ? clamp_rows(k_end - row, 16) : 0;
-      const int64_t id = max(pid, 0);
+      const bool in = (uint32_t)uni(pid) < (uint32_t)npages;
+      const int rows = in ? clamp_rows(k_end - row, 16) : 0;
+      const int64_t id = in ? uni(pid) : 0;
       const auto rk_ = make_rsrc((const uint8_t*)(kpool + id * ksb) + (uint64_t)(uint32_t)poff * krb,
                                  (uint32_t)rows * krb);
       const auto rv_ = make_rsrc((const uint8_t*)(vpool + id * vsb) + (uint64_t)(uint32_t)poff * vrb,
@@ -244,11 +243,12 @@ __device__ __forceinline__ void tile_body() {
     for (int d = 0; d < D / 32; ++d) oacc[d] = f32x16{};
     float m_i = kNegInf, l_i = 0.f;
 
-    auto step = [&](int kbase, uint8_t* cur, uint8_t* nxt) {
+    auto step = [&](auto masks, int kbase, uint8_t* cur, uint8_t* nxt) {
+      constexpr bool MASK = decltype(masks)::value;
       ring_barrier<0>();
       if (kbase + BN < k_end) issue(nxt);
       __builtin_amdgcn_sched_barrier(0);
-      if (causal && kbase + BN - 1 > off + qt * TB) {  // (the same for all four waves)
+      if (MASK && causal && kbase + BN - 1 > off + qt * TB) {  // (the same for all four waves)
         uint8_t* v = cur + C::KBYTES + C::RBYTES;
         if (tile_odd<C::KBYTES / 4096, F16>(v + wv * (C::KBYTES / 4), lane)) odd_flag = 1;
         ring_barrier<63>();
@@ -260,7 +260,7 @@ __device__ __forceinline__ void tile_body() {
           ring_barrier<63>();
         }
       }
-      if (idle || kbase > lim_any) return;
+      if (idle || (MASK && kbase > lim_any)) return;
       const uint8_t* kl = cur;
       const uint8_t* rl = kl + C::KBYTES + (HW > 1 ? (wv % HW) * C::RHEAD : 0);
       const uint8_t* vl = kl + C::KBYTES + C::RBYTES;
@@ -294,14 +294,13 @@ __device__ __forceinline__ void tile_body() {
         }
         sacc[kb2] = acc;
       }
-      const bool masked = kbase + BN - 1 > lim_all || kbase + BN > k_end || gone;
-      if (masked) {
+      if constexpr (MASK) {
 #pragma unroll
         for (int kb2 = 0; kb2 < BN / 32; ++kb2)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
             const int key = kbase + kb2 * 32 + 8 * (v >> 2) + 4 * hl + (v & 3);
-            sacc[kb2][v] = key > lim || key >= k_end ? kNegInf : sacc[kb2][v];
+            sacc[kb2][v] = key > lim ? kNegInf : sacc[kb2][v];
           }
         if (gone) {
           for (int g = 0; g < C::G; ++g) {
@@ -365,9 +364,19 @@ __device__ __forceinline__ void tile_body() {
       l_i += ls;
     };
 
-    for (int k = 32 * s0; k < k_end; k += 2 * BN) {
-      step(k, stage0, stage1);
-      if (k + BN < k_end) step(k + BN, stage1, stage0);
+    // The steps whose rows all tokens see, in pairs (the ring's two stages),
+    // without the masks and their registers; then the others.
+    int k = 32 * s0;
+    if (!gone) {
+      const int k_fast = min(causal ? off + qt * TB + 1 : k_end, k_end);
+      for (; k + 2 * BN <= k_fast; k += 2 * BN) {
+        step(std::false_type{}, k, stage0, stage1);
+        step(std::false_type{}, k + BN, stage1, stage0);
+      }
+    }
+    for (; k < k_end; k += 2 * BN) {
+      step(std::true_type{}, k, stage0, stage1);
+      if (k + BN < k_end) step(std::true_type{}, k + BN, stage1, stage0);
     }
     // (every wave has left the ring, and no DMA is under way, before the next
     // part's goes out)
