@@ -500,11 +500,14 @@ __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedParams
         M == kNegInf ? kNegInf : M * P->c + __builtin_amdgcn_logf(L + 1e-6f) * kLn2;
 }
 
-// Waves per SIMD the register budget is cut for, which is also the workgroups
-// that a CU holds (LDS: two stages of at most 32 KB at rank 64 with four heads).
-constexpr int tile_occ(int D, int RPL, int HW) {
-  return D == 128 && RPL == 64 && HW == 4 ? 2 : 3;
-}
+// Waves per SIMD that the register budget is cut for, and workgroups of a CU.
+// Three where one head's ranks or none come with d = 128: such tiles are long,
+// bound by the matrix cores, and a third workgroup fills the others' waits
+// (1024-token piece, rank 64: 346 us, two 351).  Two for the others: the third
+// costs spilled registers (mixed step, 4 heads of rank 32: 146 us, two 133; d =
+// 64, rank 16, 509-token pieces with their weights: 103, 97).  A third ring
+// stage in the room that leaves: 136 and 99.
+constexpr int tile_occ(int D, int RPL, int HW) { return D == 128 && (RPL == 0 || HW == 1) ? 3 : 2; }
 
 #define FNA2_TILE(D, RPL, HW)                                                               \
   __global__ __launch_bounds__(256, tile_occ(D, RPL, HW)) void paged_tile_d##D##_r##RPL##_h##HW( \
