@@ -1359,6 +1359,15 @@ void fill_cache(fna2::PagedParams& K, const fna2_paged_cache& c) {
   K.R = c.heads_graph > 0 ? c.rank : 0;
   K.group = c.heads / c.heads_kv;
   K.ps = c.page_size;
+  // page of row group n = row / 16 < 2^26: n / d, d = page_size / 16, as n m >> (26 + s) with
+  // 2^s >= d and m = ceil(2^(26+s) / d): off by n (m d - 2^(26+s)) / (d 2^(26+s)) < 1 / d
+  {
+    const int64_t d = c.page_size / 16;
+    int s = 0;
+    while (((int64_t)1 << s) < d) ++s;
+    K.ps_shift = 26 + s;
+    K.ps_mul = (uint32_t)cdiv64((int64_t)1 << K.ps_shift, d);
+  }
   K.npages = c.num_pages;
   K.width = c.table_width;
   K.tstride = c.table_stride;

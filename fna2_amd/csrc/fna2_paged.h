@@ -19,6 +19,8 @@ struct PagedParams {
   int N, T;
   int H, H_KV, H_G, D, R, group;
   int ps, npages, width;
+  uint32_t ps_mul;  // row / ps = (row / 16) ps_mul >> ps_shift
+  int ps_shift;
   int64_t tstride;
   const int* table;
   const int* lens;
@@ -74,83 +76,121 @@ __device__ __forceinline__ PagedSeq paged_seq_uniform(KArg P, int b) {
   return paged_clamp(P, uni(cu[b]), uni(cu[b + 1]), uni(*const_space(P->lens + b)));
 }
 
-// Work that the host cannot count (the lengths are on the device): the
-// sequences' units, laid end to end, are found again by every wave from the
-// lengths alone.  `units(s)` is a sequence's count.
-template <typename F>
-__device__ __forceinline__ int64_t wave_total(KArg P, int lane, F&& units) {
-  int64_t sum = 0;
-  for (int b = lane; b < P->N; b += 64) sum += units(paged_seq(P, b));
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
-  return sum;
+__device__ __forceinline__ int64_t lane64(int64_t x, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)x, l);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(x >> 32), l);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t uni64(int64_t x) { return lane64(x, 0); }
+
+// Sum over the lanes up to and including this one, in moves between lanes'
+// registers (shuffles go through LDS: 1 us for the six).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp_add64(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+  return x + (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t lane_scan64(int64_t x) {
+  x = dpp_add64<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within 16 lanes
+  x = dpp_add64<0x112, 0xf>(x);
+  x = dpp_add64<0x114, 0xf>(x);
+  x = dpp_add64<0x118, 0xf>(x);
+  x = dpp_add64<0x142, 0xa>(x);  // row_bcast 15: rows 1 and 3 take the row before
+  return dpp_add64<0x143, 0xc>(x);  // row_bcast 31: rows 2 and 3 the first two
 }
 
-// The sequence that holds unit u (0 <= u < total), and u's place in it.
+// Quotient of nonnegative numbers, by 32-bit division where they fit.
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+  if (((uint64_t)(a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
+// Work that the host cannot count (the lengths are on the device): the
+// sequences' units, laid end to end, are found again by every wave from the
+// lengths alone.  `units(s)` is a sequence's count.  seek(u): the sequence that holds
+// unit u (0 <= u < total) and u's place in it.
 struct PagedAt {
   int b;
   int64_t rem;
+  PagedSeq s;
 };
 template <typename F>
-__device__ __forceinline__ PagedAt wave_locate(KArg P, int lane, int64_t u,
-                                               F&& units) {
-  int64_t base = 0;
-  for (int b0 = 0; b0 < P->N; b0 += 64) {
+struct SeqWork {
+  F units;
+  int64_t total, base, mine, end;  // of the block of 64 sequences scanned last
+  PagedSeq s;
+  __device__ __forceinline__ void scan(KArg P, int lane, int b0, int64_t before) {
     const int b = b0 + lane;
-    const int64_t mine = b < P->N ? units(paged_seq(P, b)) : 0;
-    int64_t end = mine;  // inclusive sum over the lanes
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int64_t o = __shfl_up(end, m);
-      if (lane >= m) end += o;
-    }
-    const uint64_t past = __builtin_amdgcn_ballot_w64(base + end > u);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      const int64_t start = __shfl(end - mine, l) + base;
-      PagedAt at;
-      at.b = uni(b0 + l);
-      const int64_t rem = u - start;
-      at.rem = (int64_t)(((uint64_t)(uint32_t)uni((int)(rem >> 32)) << 32) | (uint32_t)uni((int)rem));
-      return at;
-    }
-    base += __shfl(end, 63);
+    s = PagedSeq{0, 0, 0};
+    if (b < P->N) s = paged_seq(P, b);
+    base = before;
+    mine = b < P->N ? units(s) : 0;
+    end = before + lane_scan64(mine);
   }
-  return PagedAt{P->N, 0};
-}
-
-// The page of row group `row` (a multiple of 16, below lk) and the row's
-// place in it, stepped 16 rows at a time.
-struct PageCursor {
-  int page, off;
-  __device__ __forceinline__ void at(int ps, int row) {
-    page = row / ps;
-    off = row - page * ps;
-  }
-  __device__ __forceinline__ void next(int ps) {
-    off += 16;
-    if (off >= ps) {
-      off = 0;
-      ++page;
+  __device__ __forceinline__ SeqWork(KArg P, int lane, F f) : units(f), total(0) {
+    for (int b0 = 0; b0 < P->N; b0 += 64) {
+      scan(P, lane, b0, total);
+      total = lane64(end, 63);
     }
+  }
+  __device__ __forceinline__ PagedAt seek(KArg P, int lane, int64_t u) {
+    int b0 = 0;
+    if (P->N > 64) {
+      int64_t sum = 0;
+      while (true) {
+        scan(P, lane, b0, sum);
+        sum = lane64(end, 63);
+        if (sum > u || b0 + 64 >= P->N) break;
+        b0 += 64;
+      }
+    }
+    const int l = uni(__builtin_ctzll(__builtin_amdgcn_ballot_w64(end > u) | ((uint64_t)1 << 63)));
+    PagedAt at;
+    at.b = b0 + l;
+    at.rem = u - lane64(end - mine, l);
+    at.s = PagedSeq{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.lq, l),
+                    __builtin_amdgcn_readlane(s.lk, l)};
+    return at;
   }
 };
 
-__device__ __forceinline__ int64_t uni64(int64_t x) {
-  return (int64_t)(((uint64_t)(uint32_t)uni((int)(x >> 32)) << 32) | (uint32_t)uni((int)x));
+// Zeros, and LSE -inf, for the tokens of no sequence: workgroup `i` of `n`.
+__device__ __forceinline__ void clear_loose_tokens(KArg P, int i, int n) {
+  const int t0 = min(max(uni(*const_space(P->cu)), 0), P->T);
+  const int t1 = min(max(uni(*const_space(P->cu + P->N)), t0), P->T);
+  const int64_t rows = (int64_t)(t0 + P->T - t1) * P->H;
+  for (int64_t r = i; r < rows; r += n) {
+    const int h = (int)(r % P->H);
+    int t = (int)(r / P->H);
+    if (t >= t0) t += t1 - t0;
+    uint16_t* o = (uint16_t*)P->o.ptr + (int64_t)t * P->o.ss + (int64_t)h * P->o.sh;
+    if (threadIdx.x < P->D / 8) *(u32x4*)(o + 8 * threadIdx.x) = u32x4{0, 0, 0, 0};
+    if (threadIdx.x == 0 && P->lse.ptr)
+      ((float*)P->lse.ptr)[(int64_t)t * P->lse.ss + (int64_t)h * P->lse.sh] = kNegInf;
+  }
 }
 
-// The packed kernel's units (key steps of 32 rows of a column tile) and the
-// share of each wave: shared with the kernel that joins split tiles.
+// The page of row `row` (below 2^30).
+__device__ __forceinline__ int page_of(uint32_t mul, int shift, int row) {
+  return (int)(((uint64_t)(uint32_t)(row >> 4) * mul) >> shift);
+}
+
+// x / d and x % d for lane numbers (x < 64) and d <= 64.
+__device__ __forceinline__ int small_div(int x, int d) {
+  return (x * (65536 / d + 1)) >> 16;
+}
+
+// The units of a run: an equal share for each of the resident waves (workgroups).
+__device__ __forceinline__ int64_t run_units(KArg P, int64_t total) {
+  return max(div64(total + P->waves - 1, P->waves), (int64_t)P->min_steps);
+}
+
+// The packed kernel's units: key steps of 32 rows of a column tile.
 struct PackedPlan {
-  int64_t total, per;
   __device__ __forceinline__ static int steps(const PagedSeq& s) { return max(cdiv(s.lk, 32), 1); }
   __device__ __forceinline__ static int64_t units(KArg P, const PagedSeq& s) {
     return (int64_t)cdiv(s.lq, P->tpt) * (P->H_KV * P->nsub) * steps(s);
-  }
-  __device__ __forceinline__ PackedPlan(KArg P, int lane) {
-    total = uni64(wave_total(P, lane, [&](const PagedSeq& s) { return units(P, s); }));
-    per = max((total + P->waves - 1) / P->waves, (int64_t)P->min_steps);
   }
 };
 
@@ -159,7 +199,6 @@ struct PackedPlan {
 // may be short of heads).  Tile i of a sequence sees, causal, the rows up to
 // its last token's: ceil((off + min((i + 1) TB, lq)) / 32) units, one at least.
 struct TilePlan {
-  int64_t total, per;
   __device__ __forceinline__ static int tokens(KArg P) { return 128 / P->hw; }
   __device__ __forceinline__ static int blocks(KArg P) {
     return P->H_KV * cdiv(P->group, P->hw);
@@ -195,10 +234,6 @@ struct TilePlan {
     }
     r -= before(P, s, lo);
     return lo;
-  }
-  __device__ __forceinline__ TilePlan(KArg P, int lane) {
-    total = uni64(wave_total(P, lane, [&](const PagedSeq& s) { return units(P, s); }));
-    per = max((total + P->waves - 1) / P->waves, (int64_t)P->min_steps);
   }
 };
 

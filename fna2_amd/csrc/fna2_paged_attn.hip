@@ -65,46 +65,33 @@ __device__ __forceinline__ void packed_body() {
   __shared__ __attribute__((aligned(1024))) uint8_t st1[C::STAGE];
   const int lane = threadIdx.x;
   const int col = lane & 31, hl = lane >> 5;
-  const int tk = col / P->gsub, hc = col - tk * P->gsub;  // token of the tile, head of the group
+  const int tk = small_div(col, P->gsub), hc = col - tk * P->gsub;  // token of the tile, head of the group
   const int cols = P->gsub * P->tpt;
   const int HB = P->H_KV * P->nsub;
-  const PackedPlan plan(P, lane);
-
-  // Tokens of no sequence: zeros.
-  {
-    const int t0 = min(max(uni(*const_space(P->cu)), 0), P->T);
-    const int t1 = min(max(uni(*const_space(P->cu + P->N)), t0), P->T);
-    const int64_t rows = (int64_t)(t0 + P->T - t1) * P->H;
-    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
-      const int h = (int)(i % P->H);
-      int t = (int)(i / P->H);
-      if (t >= t0) t += t1 - t0;
-      uint16_t* o = (uint16_t*)P->o.ptr + (int64_t)t * P->o.ss + (int64_t)h * P->o.sh;
-      if (lane < D / 8) st16(o + 8 * lane, u32x4{0, 0, 0, 0});
-      if (lane == 0 && P->lse.ptr)
-        ((float*)P->lse.ptr)[(int64_t)t * P->lse.ss + (int64_t)h * P->lse.sh] = kNegInf;
-    }
-  }
-
-  int64_t u = (int64_t)blockIdx.x * plan.per;
-  const int64_t u_end = min(plan.total, u + plan.per);
   auto cut = [&](int b, int head, int tile, int parts) {
     if (lane == 0) P->cuts[blockIdx.x] = PagedCut{b, head, tile, parts};
   };
-  if (u >= u_end) {
-    cut(0, 0, 0, 0);
-    return;
-  }
-  const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return PackedPlan::units(P, s); });
-  int b = at.b;
-  PagedSeq e = paged_seq_uniform(P, b);
-  int steps = PackedPlan::steps(e);
-  int ct, sg, s0;
+  int64_t left, per;  // units of this run still to do, and of a run
+  int b, ct, sg, s0, steps;
+  PagedSeq e;
   {
-    const int64_t tile = at.rem / steps;
-    s0 = (int)(at.rem - tile * steps);
-    ct = (int)(tile / HB);
-    sg = (int)(tile - (int64_t)ct * HB);
+    auto units = [&](const PagedSeq& s) { return PackedPlan::units(P, s); };
+    SeqWork<decltype(units)> work(P, lane, units);
+    per = run_units(P, work.total);
+    const int64_t u = (int64_t)blockIdx.x * per;
+    left = min(work.total - u, per);
+    if (left <= 0) {
+      cut(0, 0, 0, 0);
+      return;
+    }
+    const PagedAt at = work.seek(P, lane, u);
+    b = at.b;
+    e = at.s;
+    steps = PackedPlan::steps(e);
+    const int64_t tile = div64(at.rem, steps);
+    s0 = uni((int)(at.rem - tile * steps));
+    ct = uni((int)div64(tile, HB));
+    sg = uni((int)(tile - (int64_t)ct * HB));
   }
 
   const TrLane tl(lane);
@@ -121,8 +108,8 @@ __device__ __forceinline__ void packed_body() {
     const bool causal = P->causal != 0;
     const int ps = P->ps, npages = P->npages;
     const float c2 = P->c2;
-    const int s1 = (int)min((int64_t)steps, (int64_t)s0 + (u_end - u));
-    const int kvh = sg / P->nsub, h_in = (sg - kvh * P->nsub) * P->gsub;
+    const int s1 = (int)min((int64_t)steps, s0 + left);
+    const int kvh = P->nsub == 1 ? sg : sg / P->nsub, h_in = (sg - kvh * P->nsub) * P->gsub;
     const int nh = min(P->gsub, P->group - h_in);  // heads of this group
     const int h0 = kvh * P->group + h_in;
     const int gg = RC > 0 ? min(max(P->H_G - h0, 0), nh) : 0;  // graph heads
@@ -146,41 +133,38 @@ __device__ __forceinline__ void packed_body() {
       const uint32_t hs = (uint32_t)P->rk.sh * 2u, rs = (uint32_t)P->rk.ss * 2u;
 #pragma unroll
       for (int i = 0; i < C::NR; ++i) {
-        const int c = 4 * i + lch;
-        roff[i] = c < rch ? (uint32_t)(c / crr) * hs + (uint32_t)lrow * rs + (uint32_t)(c % crr) * 16u
+        const int c = 4 * i + lch, hh = small_div(c, max(crr, 1));
+        roff[i] = c < rch ? (uint32_t)hh * hs + (uint32_t)lrow * rs + (uint32_t)(c - hh * crr) * 16u
                           : kOOB;
       }
     }
-    PageCursor cur;
-    cur.at(ps, 32 * s0);
-    const int page_last = e.lk > 0 ? (e.lk - 1) / ps : -1;
-    // Ids (as loaded, looked at when the tile is issued: no step waits for
-    // them) and places of the next tile's two row groups.
-    int pid[2] = {-1, -1}, poff[2];
-    auto look = [&](int t) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (page_last >= 0) pid[g] = *const_space(trow + min(cur.page, page_last));
-        poff[g] = cur.off;
-        cur.next(ps);
-      }
-    };
-    // Tile t (looked up before) into `base`; returns the row groups that are
-    // not there although below lk (bit g).  Then looks up tile t + 1.
+    // Page and row within it of the next row group to be issued.
+    PageIds ids;
+    ids.row = trow;
+    ids.last = e.lk > 0 ? page_of(P->ps_mul, P->ps_shift, e.lk - 1) : -1;
+    int page = page_of(P->ps_mul, P->ps_shift, 32 * s0), poff = 32 * s0 - page * ps;
+    ids.load(lane, page);
+    // Tile t into `base`; returns the row groups that are not there although
+    // below lk (bit g).
     auto issue = [&](int t, uint8_t* base) {
       int gone = 0;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const int row = 32 * t + 16 * g;
-        const bool known = (uint32_t)uni(pid[g]) < (uint32_t)npages;
-        const bool here = known && t < s1;
-        const int rows = here ? clamp_rows(e.lk - row, 16) : 0;
-        if (!known && row < e.lk) gone |= 1 << g;
-        const int64_t id = here ? uni(pid[g]) : 0;
-        const int r = here ? poff[g] : 0;
-        const auto rk_ = make_rsrc((const uint8_t*)(kpool + id * ksb) + (uint64_t)(uint32_t)r * krb,
+        const bool in = row < e.lk && t < s1;
+        int id = in ? ids.at(lane, page) : 0;
+        const int r = poff;
+        poff += 16;
+        if (poff >= ps) poff = 0, ++page;
+        if ((uint32_t)id >= (uint32_t)npages) {
+          id = -1;
+          if (in) gone |= 1 << g;
+        }
+        const int rows = in && id >= 0 ? clamp_rows(e.lk - row, 16) : 0;
+        id = max(id, 0);
+        const auto rk_ = make_rsrc((const uint8_t*)(kpool + (int64_t)id * ksb) + (uint64_t)(uint32_t)r * krb,
                                    (uint32_t)rows * krb);
-        const auto rv_ = make_rsrc((const uint8_t*)(vpool + id * vsb) + (uint64_t)(uint32_t)r * vrb,
+        const auto rv_ = make_rsrc((const uint8_t*)(vpool + (int64_t)id * vsb) + (uint64_t)(uint32_t)r * vrb,
                                    (uint32_t)rows * vrb);
 #pragma unroll
         for (int i = 0; i < C::NG; ++i) {
@@ -191,7 +175,7 @@ __device__ __forceinline__ void packed_body() {
               vvo + 64u * i, 0, 0, 0);
         }
         if constexpr (RC > 0) {
-          const auto rr = make_rsrc((const uint8_t*)(rpool + id * rsb) + (uint64_t)(uint32_t)r * rrb,
+          const auto rr = make_rsrc((const uint8_t*)(rpool + (int64_t)id * rsb) + (uint64_t)(uint32_t)r * rrb,
                                     rows > 0 && gg > 0 ? 0x7ffffff0u : 0u);
 #pragma unroll
           for (int i = 0; i < C::NR; ++i)
@@ -200,28 +184,20 @@ __device__ __forceinline__ void packed_body() {
                 lrow < rows ? roff[i] : kOOB, 0, 0, 0);
         }
       }
-      look(t + 1);
       return gone;
     };
 
-    look(s0);
-    int gone = issue(s0, st0);
-    __builtin_amdgcn_sched_barrier(0);
-
-    // Query operand (B of S^T): lane holds Qa[col][16 s + 8 hl .. +7].
+    // Query operand (B of S^T): lane holds Qa[col][16 s + 8 hl .. +7].  Loaded
+    // behind the page ids and ahead of the first tile, whose waits it shares.
     bf16x8 qreg[C::KSD + (RC > 0 ? C::KSR : 0)];
     float bh = 0.f;
     {
       const int64_t t = (int64_t)(e.q0 + (live ? tok : 0));
       const uint16_t* qrow = (const uint16_t*)P->q.ptr + t * P->q.ss + (int64_t)(h0 + hc) * P->q.sh;
-      const uint32_t qxor = P->qa < 0.f ? 0x80008000u : 0u;
-      const uint32_t qand = P->qa == 0.f ? 0u : 0xffffffffu;
 #pragma unroll
       for (int s = 0; s < C::KSD; ++s) {
         u32x4 w = {0, 0, 0, 0};
         if (live) w = ld16(qrow + 16 * s + 8 * hl);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (w[i] & qand) ^ qxor;
         qreg[s] = as_bf16x8(w);
       }
       if constexpr (RC > 0) {
@@ -230,11 +206,24 @@ __device__ __forceinline__ void packed_body() {
         bh = g ? P->gs[h0 + hc] / P->c : 0.f;
 #pragma unroll
         for (int s = 0; s < C::KSR; ++s) {
-          const int c = 2 * s + hl;  // concatenated chunk of this lane
+          const int c = 2 * s + hl - hc * crr;  // this head's chunk of the lane
           u32x4 w = {0, 0, 0, 0};
-          if (g && c < rch && c / crr == hc) w = ld16(rrow + 8 * (c - hc * crr));
+          if (g && c >= 0 && c < crr) w = ld16(rrow + 8 * c);
           qreg[C::KSD + s] = as_bf16x8(w);
         }
+      }
+    }
+    int gone = issue(s0, st0);
+    __builtin_amdgcn_sched_barrier(0);
+    {
+      const uint32_t qxor = P->qa < 0.f ? 0x80008000u : 0u;
+      const uint32_t qand = P->qa == 0.f ? 0u : 0xffffffffu;
+#pragma unroll
+      for (int s = 0; s < C::KSD; ++s) {
+        u32x4 w = as_u32x4(qreg[s]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (w[i] & qand) ^ qxor;
+        qreg[s] = as_bf16x8(w);
       }
     }
 
@@ -374,10 +363,10 @@ __device__ __forceinline__ void packed_body() {
       if (hl == 0) *(f32x2*)(P->ml + 2 * (slot * cols + col)) = f32x2{m_i, l_tot};
     }
 
-    u += s1 - s0;
-    if (u >= u_end) {
+    left -= s1 - s0;
+    if (left <= 0) {
       const int rest = steps - s1;
-      cut(b, sg, ct, s0 == 0 && rest > 0 ? 1 + (int)((rest + plan.per - 1) / plan.per) : 0);
+      cut(b, sg, ct, s0 == 0 && rest > 0 ? 1 + (int)div64(rest + per - 1, per) : 0);
       return;
     }
     s0 = 0;
@@ -407,6 +396,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
   const int i0 = blockIdx.x;
   const auto rec = const_space(P->cuts + i0);
   const int n = uni(rec->parts);
+  if (blockIdx.y == 0) clear_loose_tokens(P, blockIdx.x, gridDim.x);
   if (n <= 0) return;
   const int ct = uni(rec->tile), sg = uni(rec->head);
   const PagedSeq e = paged_seq_uniform(P, rec->b);
@@ -478,11 +468,17 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
   }
 }
 
+// Waves per SIMD that the register budget is cut for.  Two (256 registers): the
+// accumulators then stay in ordinary registers, where with one wave's budget
+// the compiler keeps them in the other half of the file and copies them to
+// and fro in every step.
+constexpr int packed_occ(int D, int RC) { return D == 128 && RC > 16 ? 1 : 2; }
+
 #define FNA2_PACKED(D, RC)                                                                     \
-  __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC(const PagedParams) {    \
+  __global__ __launch_bounds__(64, packed_occ(D, RC)) void paged_packed_d##D##_c##RC(const PagedParams) {    \
     packed_body<D, RC, false>();                                                               \
   }                                                                                            \
-  __global__ __launch_bounds__(64, 1) void paged_packed_d##D##_c##RC##_f16(const PagedParams) { \
+  __global__ __launch_bounds__(64, packed_occ(D, RC)) void paged_packed_d##D##_c##RC##_f16(const PagedParams) { \
     packed_body<D, RC, true>();                                                                \
   }
 FNA2_PACKED(64, 0)
@@ -524,8 +520,7 @@ hipError_t launch_paged_packed(const PagedParams& P, int rc, hipStream_t s) {
 }
 
 hipError_t launch_paged_merge(const PagedParams& P, hipStream_t s) {
-  if (P.waves <= 1) return hipSuccess;
-  const dim3 grid((uint32_t)(P.waves - 1), (uint32_t)(P.gsub * P.tpt));
+  const dim3 grid((uint32_t)P.waves, (uint32_t)(P.gsub * P.tpt));
   if (P.D == 64)
     hipLaunchKernelGGL(P.f16 ? (paged_merge_kernel<64, true>) : (paged_merge_kernel<64, false>), grid, dim3(256), 0, s, P);
   else

@@ -7,6 +7,23 @@
 
 namespace fna2 {
 
+// The page ids of a part of a sequence, 64 at a time in a register's lanes: a
+// step reads its own with no memory access, so none waits in the steps' way
+// (a scalar load a step ahead did: its counter is the LDS reads' too).
+struct PageIds {
+  const int* row;  // of the block table
+  int ids, base, last;
+  // Pages base .. base + 63; `last` is the last one that holds rows (-1: none).
+  __device__ __forceinline__ void load(int lane, int first) {
+    base = first;
+    ids = last >= 0 ? row[min(first + lane, last)] : -1;
+  }
+  __device__ __forceinline__ int at(int lane, int page) {
+    if (page - base >= 64) load(lane, page);
+    return __builtin_amdgcn_readlane(ids, page - base);
+  }
+};
+
 // e^(x) in powers of two for the weight of an accumulator, never zero: an
 // infinity in it stays one (a sum's start, x = -inf, holds zeros).
 __device__ __forceinline__ float weight2(float x) {
@@ -32,13 +49,20 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
 // the zeroing of those.
 template <int KB, bool F16>
 __device__ __forceinline__ bool tile_odd(const uint8_t* tile, int lane) {
-  uint32_t odd = 0;
+  // (the largest exponents, and one comparison: a comparison a word would take
+  // a pair of scalar registers each)
+  constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+  uint32_t lo = 0, hi = 0;
 #pragma unroll
   for (int i = 0; i < KB; ++i) {
     const u32x4 w = *(const u32x4*)(tile + 1024 * i + 16 * lane);
-    odd |= odd_bits<F16>(w[0]) | odd_bits<F16>(w[1]) | odd_bits<F16>(w[2]) | odd_bits<F16>(w[3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      lo = max(lo, w[j] & E);
+      hi = max(hi, w[j] & (E << 16));
+    }
   }
-  return __builtin_amdgcn_ballot_w64(odd != 0) != 0;
+  return __builtin_amdgcn_ballot_w64(lo == E || hi == (E << 16)) != 0;
 }
 template <int KB, bool F16>
 __device__ __forceinline__ void tile_clean(uint8_t* tile, int lane) {

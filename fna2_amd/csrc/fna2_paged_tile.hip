@@ -61,22 +61,6 @@ __device__ __forceinline__ void tile_body() {
   const int TB = 128 / hw;
   const int hblk = cdiv(P->group, hw);  // blocks of heads of a KV head
 
-  // Tokens of no sequence: zeros.
-  {
-    const int t0 = min(max(uni(*const_space(P->cu)), 0), P->T);
-    const int t1 = min(max(uni(*const_space(P->cu + P->N)), t0), P->T);
-    const int64_t rows = (int64_t)(t0 + P->T - t1) * P->H;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + wv; i < rows; i += (int64_t)gridDim.x * 4) {
-      const int h = (int)(i % P->H);
-      int t = (int)(i / P->H);
-      if (t >= t0) t += t1 - t0;
-      uint16_t* o = (uint16_t*)P->o.ptr + (int64_t)t * P->o.ss + (int64_t)h * P->o.sh;
-      if (lane < D / 8) st16(o + 8 * lane, u32x4{0, 0, 0, 0});
-      if (lane == 0 && P->lse.ptr)
-        ((float*)P->lse.ptr)[(int64_t)t * P->lse.ss + (int64_t)h * P->lse.sh] = kNegInf;
-    }
-  }
-
   const int run = run_of(blockIdx.x, gridDim.x);
   int64_t left, per;  // units of this run still to do, and of a run
   int b, hb, qt, s0;
@@ -85,19 +69,20 @@ __device__ __forceinline__ void tile_body() {
     if (threadIdx.x == 0) P->cuts[run] = PagedCut{seq, head, tile, parts};
   };
   {
-    const TilePlan plan(P, lane);
-    per = plan.per;
+    auto units = [&](const PagedSeq& s) { return TilePlan::units(P, s); };
+    SeqWork<decltype(units)> work(P, lane, units);
+    per = run_units(P, work.total);
     const int64_t u = (int64_t)run * per;
-    left = min(plan.total - u, per);
+    left = min(work.total - u, per);
     if (left <= 0) {
       cut(0, 0, 0, 0);
       return;
     }
-    const PagedAt at = wave_locate(P, lane, u, [&](const PagedSeq& s) { return TilePlan::units(P, s); });
+    const PagedAt at = work.seek(P, lane, u);
     b = at.b;
-    e = paged_seq_uniform(P, b);
+    e = at.s;
     const int64_t hu = TilePlan::head_units(P, e);
-    hb = uni((int)(at.rem / hu));
+    hb = uni((int)div64(at.rem, hu));
     int64_t r = at.rem - hb * hu;
     qt = uni(TilePlan::find(P, e, r));
     s0 = uni((int)r);
@@ -142,29 +127,28 @@ __device__ __forceinline__ void tile_body() {
     const uint32_t rrb = (uint32_t)P->rk.ss * 2u;
     const int rchunks = P->R / 8, group = P->group, HG = P->H_G;
 
+    // Page and row within it of this wave's row group of the next tile.
+    PageIds ids;
+    ids.row = trow;
+    ids.last = k_end > 0 ? page_of(P->ps_mul, P->ps_shift, k_end - 1) : -1;
+    int row = 32 * s0 + 16 * rg;
+    int page = page_of(P->ps_mul, P->ps_shift, row), poff = row - page * ps;
     // Rows of the part in pages that are not there (rare) are masked.
     bool gone = false;
     {
-      const int p1 = k_end > 32 * s0 ? (k_end - 1) / ps : -1;
-      for (int p = 32 * s0 / ps + lane; p <= p1; p += 64)
-        gone |= (uint32_t)trow[p] >= (uint32_t)npages;
+      const int first = page_of(P->ps_mul, P->ps_shift, 32 * s0);
+      for (int p = first; p <= ids.last; p += 64) {
+        ids.load(lane, p);
+        gone |= (uint32_t)ids.ids >= (uint32_t)npages;
+      }
       gone = __builtin_amdgcn_ballot_w64(gone) != 0;
+      if (ids.last - first >= 64 || ids.last < first) ids.load(lane, first);
     }
-
-    // Page of this wave's row group of the next tile.  Its id is loaded a step
-    // ahead and looked at only when the tile is issued, so that no step waits
-    // for it.
-    int row = 32 * s0 + 16 * rg;
-    int page = row / ps, poff = row - page * ps;
-    const int page_last = k_end > 0 ? (k_end - 1) / ps : -1;
-    int pid = -1;
-    auto look = [&]() {
-      if (page_last >= 0) pid = *const_space(trow + min(page, page_last));
-    };
     auto issue = [&](uint8_t* base) {
-      const bool in = (uint32_t)uni(pid) < (uint32_t)npages;
+      const int pid = row < k_end ? ids.at(lane, page) : -1;
+      const bool in = (uint32_t)pid < (uint32_t)npages;
       const int rows = in ? clamp_rows(k_end - row, 16) : 0;
-      const int64_t id = in ? uni(pid) : 0;
+      const int64_t id = in ? pid : 0;
       const auto rk_ = make_rsrc((const uint8_t*)(kpool + id * ksb) + (uint64_t)(uint32_t)poff * krb,
                                  (uint32_t)rows * krb);
       const auto rv_ = make_rsrc((const uint8_t*)(vpool + id * vsb) + (uint64_t)(uint32_t)poff * vrb,
@@ -205,10 +189,8 @@ __device__ __forceinline__ void tile_body() {
         poff -= ps;
         ++page;
       }
-      look();
     };
 
-    look();
     issue(stage0);
     __builtin_amdgcn_sched_barrier(0);
 
@@ -305,7 +287,7 @@ __device__ __forceinline__ void tile_body() {
         if (gone) {
           for (int g = 0; g < C::G; ++g) {
             const int r = kbase + 16 * g;
-            if (r >= k_end || (uint32_t)uni(*const_space(trow + r / ps)) < (uint32_t)npages) continue;
+            if (r >= k_end || (uint32_t)uni(*const_space(trow + page_of(kargs()->ps_mul, kargs()->ps_shift, r))) < (uint32_t)npages) continue;
 #pragma unroll
             for (int kb2 = 0; kb2 < BN / 32; ++kb2)
 #pragma unroll
@@ -418,7 +400,7 @@ __device__ __forceinline__ void tile_body() {
     left -= s1 - s0;
     if (left <= 0) {
       const int rest = steps - s1;
-      cut(b, hb, qt, s0 == 0 && rest > 0 ? 1 + (int)((rest + per - 1) / per) : 0);
+      cut(b, hb, qt, s0 == 0 && rest > 0 ? 1 + (int)div64(rest + per - 1, per) : 0);
       return;
     }
     s0 = 0;
@@ -443,6 +425,7 @@ __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedParams
   const int i0 = blockIdx.x;
   const auto rec = const_space(P->cuts + i0);
   const int n = uni(rec->parts);
+  if (blockIdx.y == 0) clear_loose_tokens(P, blockIdx.x, gridDim.x);
   if (n <= 0) return;
   const int hb = uni(rec->head), qt = uni(rec->tile);
   const PagedSeq e = paged_seq_uniform(P, rec->b);
@@ -558,8 +541,8 @@ hipError_t launch_paged_tile(const PagedParams& P, int rpl, hipStream_t s) {
   if (!k) return hipErrorInvalidValue;
   hipLaunchKernelGGL(k, dim3((uint32_t)P.waves), dim3(256), 0, s, P);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || P.waves <= 1) return e;
-  const dim3 grid((uint32_t)(P.waves - 1), (uint32_t)(P.D / 32));
+  if (e != hipSuccess) return e;
+  const dim3 grid((uint32_t)P.waves, (uint32_t)(P.D / 32));
   void (*m)(const PagedParams) =
       P.D == 64 ? (P.f16 ? paged_tile_merge_kernel<64, true> : paged_tile_merge_kernel<64, false>)
                 : (P.f16 ? paged_tile_merge_kernel<128, true> : paged_tile_merge_kernel<128, false>);

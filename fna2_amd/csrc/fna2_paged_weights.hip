@@ -45,7 +45,7 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
   const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
   const int col = lane & 31, hl = lane >> 5;
   auto units = [&](const PagedSeq& s) { return s.lq > 0 ? (int64_t)P->H_KV * cdiv(s.lk, 128) : 0; };
-  const int64_t total = uni64(wave_total(P, lane, units));
+  SeqWork<decltype(units)> work(P, lane, units);
   const RowLane rdl(lane);
   const int gsub = P->gsub, tpt = P->tpt;
   const int lrow = lane >> 2, lch = (lane & 3) ^ swz4(lane >> 2);
@@ -57,12 +57,12 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
   const uint32_t qand = P->qa == 0.f ? 0u : 0xffffffffu;
   const float c2 = P->c2;
 
-  for (int64_t id = blockIdx.x; id < total; id += gridDim.x) {
+  for (int64_t id = blockIdx.x; id < work.total; id += gridDim.x) {
     P = kargs();
-    const PagedAt at = wave_locate(P, lane, id, units);
-    const PagedSeq e = paged_seq_uniform(P, at.b);
+    const PagedAt at = work.seek(P, lane, id);
+    const PagedSeq e = at.s;
     const int nkb = cdiv(e.lk, 128);
-    const int kvh = uni((int)(at.rem / nkb));
+    const int kvh = uni((int)div64(at.rem, nkb));
     const int kb = 128 * (int)(at.rem - (int64_t)kvh * nkb);
     const int k0 = kb + 32 * wv, key = k0 + col, off = e.lk - e.lq;
     const bool causal = P->causal != 0;
