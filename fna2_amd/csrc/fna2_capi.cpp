@@ -1391,7 +1391,8 @@ void fill_cache(fna2::PagedParams& K, const fna2_paged_cache& c) {
 // R_k tile, so chunks that fill 64 or 128 tokens anyway take 2 heads or one.
 struct PagedPlan {
   bool tile;
-  int gsub, nsub, tpt, rc, hw, waves, min_steps;
+  int gsub, nsub, tpt, rc, hw, waves, min_steps, merge_runs;
+  bool merge_by_part;
   size_t ml, cuts, bytes;  // offsets of the (max, sum) pairs and the cuts; workspace
 };
 PagedPlan paged_plan(const fna2_paged_cache& c) {
@@ -1421,10 +1422,15 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
     k.bytes = k.cuts + align_up((size_t)k.waves * sizeof(fna2::PagedCut));
     return k;
   }
-  k.min_steps = 4;
+  k.min_steps = 1;
   const int64_t tiles = ((int64_t)c.total_q / k.tpt + c.batch) * c.heads_kv * k.nsub;
   k.waves = (int)std::min(256. * fna2::paged_waves_per_cu(c.head_dim, k.rc),
                           std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
+  // Few tiles in many parts: a workgroup of the merge for every column, and few
+  // of them for the runs in between.
+  const int64_t parts = k.waves / std::max<int64_t>(tiles, 1);
+  k.merge_by_part = parts > 8 || k.gsub * k.tpt <= 4;
+  k.merge_runs = (int)std::min<int64_t>(std::max<int64_t>(parts / 2, 1), 64);
   const size_t rows = 2 * (size_t)k.waves * (size_t)(k.gsub * k.tpt);
   k.ml = align_up(rows * (size_t)c.head_dim * 4u);
   k.cuts = k.ml + align_up(rows * 8u);
@@ -1497,6 +1503,8 @@ int fna2_paged_attn(const fna2_paged_attn_args* a, void* stream_ptr) {
   K.tpt = k.tpt;
   K.waves = k.waves;
   K.min_steps = k.min_steps;
+  K.merge_runs = k.merge_runs;
+  K.merge_by_part = k.merge_by_part;
   K.hw = k.hw;
   K.part = (float*)a->workspace;
   K.ml = (float*)((char*)a->workspace + k.ml);

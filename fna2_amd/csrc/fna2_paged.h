@@ -34,9 +34,11 @@ struct PagedParams {
   // tpt tokens are the columns of a tile; nsub such groups a KV head.
   int gsub, nsub, tpt;
   int waves;      // resident waves (workgroups of the tile kernel) that share the work
-  int min_steps;  // key steps a wave takes at least
+  int min_steps;  // tile kernel: key steps a run takes at least
   int hw;         // tile kernel: query heads of a KV head that a workgroup's waves take
   struct PagedCut* cuts;  // [waves]
+  int merge_runs;     // runs that a workgroup of the merge looks through (<= 64)
+  int merge_by_part;  // ... with a workgroup for every column
   float* part;    // [2 * waves] slots of unnormalised numerators of split tiles
   float* ml;      // [2 * waves][columns of a tile] (max, sum)
 };
@@ -181,9 +183,10 @@ __device__ __forceinline__ int small_div(int x, int d) {
   return (x * (65536 / d + 1)) >> 16;
 }
 
-// The units of a run: an equal share for each of the resident waves (workgroups).
-__device__ __forceinline__ int64_t run_units(KArg P, int64_t total) {
-  return max(div64(total + P->waves - 1, P->waves), (int64_t)P->min_steps);
+// The units of a run: an equal share for each of the resident waves
+// (workgroups), `least` at least.
+__device__ __forceinline__ int64_t run_units(KArg P, int64_t total, int64_t least) {
+  return max(div64(total + P->waves - 1, P->waves), least);
 }
 
 // The packed kernel's units: key steps of 32 rows of a column tile.
@@ -264,6 +267,7 @@ struct PagedAppendParams {
   const float* wq;
   const float* wk;
   float eps;
+  int share;  // waves of a token (set by the launch)
 };
 hipError_t launch_paged_append(const PagedAppendParams& P, hipStream_t s);
 

@@ -77,7 +77,10 @@ __device__ __forceinline__ void packed_body() {
   {
     auto units = [&](const PagedSeq& s) { return PackedPlan::units(P, s); };
     SeqWork<decltype(units)> work(P, lane, units);
-    per = run_units(P, work.total);
+    // One step a run while the parts are few, else two.  (us, one step, two,
+    // four: 128 steps x 2 columns 10.6, 11.8, 14.9; 640 x 4 13.9, 15.0, 19.9;
+    // 1024 x 4 16.6, 14.5, 15.3; 512 x 24 20.8, 17.6, 21.5)
+    per = run_units(P, work.total, work.total * cols <= 3000 ? 1 : 2);
     const int64_t u = (int64_t)blockIdx.x * per;
     left = min(work.total - u, per);
     if (left <= 0) {
@@ -381,10 +384,12 @@ __device__ __forceinline__ void packed_body() {
   }
 }
 
-// Joins the parts of a tile that runs cut: workgroup (i, y) columns y, y +
-// gridDim.y, ... of the tile that run i's end cuts.  The parts' weights first
-// (their maxima and sums), then D / 4 lanes a row and as many parts at once as
-// the workgroup then holds, four deep.  The parts' order is that of the runs.
+// Joins the parts of the tiles that runs cut: workgroup (x, y) those of runs
+// x merge_runs .. + merge_runs - 1 (of which most cut no tile, or not first, where a
+// tile has many parts), columns y, y + gridDim.y, ...  D / 4 lanes hold a row,
+// so the workgroup NG rows at once: with a workgroup for every column NG parts of it,
+// four deep; else NG columns, each of whose lanes walk its parts.  The order of the
+// sums goes by the parts alone.
 constexpr int kMergeParts = 2048;  // at most one part for each resident wave
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
@@ -393,11 +398,15 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
   __shared__ float wt[kMergeParts];
   __shared__ float part[NG][D];
   __shared__ float red[4], red2[4];
-  const int i0 = blockIdx.x;
+  if (blockIdx.y == 0) clear_loose_tokens(P, blockIdx.x, gridDim.x);
+  const int mr = P->merge_runs, r0 = blockIdx.x * mr + (threadIdx.x & 63);
+  uint64_t todo = __builtin_amdgcn_ballot_w64(
+      (int)(threadIdx.x & 63) < mr && r0 < P->waves && P->cuts[min(r0, P->waves - 1)].parts > 0);
+  while (todo) {
+  const int i0 = blockIdx.x * mr + uni(__builtin_ctzll(todo));
+  todo &= todo - 1;
   const auto rec = const_space(P->cuts + i0);
   const int n = uni(rec->parts);
-  if (blockIdx.y == 0) clear_loose_tokens(P, blockIdx.x, gridDim.x);
-  if (n <= 0) return;
   const int ct = uni(rec->tile), sg = uni(rec->head);
   const PagedSeq e = paged_seq_uniform(P, rec->b);
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
@@ -407,6 +416,48 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
   const int grp = threadIdx.x / LPR, f = 4 * (threadIdx.x % LPR);
   const float c2 = P->c2;
   auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * i0 + 1 : 2 * (i0 + j)); };
+  if (n <= LPR && (int)gridDim.y < cols) {
+    const int c = blockIdx.y + gridDim.y * grp;  // (gridDim.y * NG >= cols)
+    const int l = threadIdx.x % LPR;
+    const int tk = c / P->gsub, hc = c - tk * P->gsub, tok = ct * P->tpt + tk;
+    const bool on = c < cols && tok < e.lq && hc < nh;
+    f32x2 ml = {kNegInf, 0.f};
+    if (on && l < n) ml = *(const f32x2*)(P->ml + 2 * (slot(l) * cols + c));
+    const float* src = P->part + (int64_t)(on ? c : 0) * D + f;
+    float m = ml[0];
+#pragma unroll
+    for (int k = LPR / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    const float ref = m == kNegInf ? 0.f : m;
+    const float w = weight2((ml[0] - ref) * c2);
+    float sum = ml[1] * w;
+#pragma unroll
+    for (int k = LPR / 2; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < n; j0 += 4) {
+      f32x4_t x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (on && j0 + k < n) x[k] = *(const f32x4_t*)(src + slot(j0 + k) * cols * D);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float wj = __shfl(w, min(j0 + k, n - 1), LPR);
+        if (j0 + k < n) o += wj * x[k];
+      }
+    }
+    if (!on) continue;
+    const float inv = 1.f / (sum + 1e-6f);
+    uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)(h0 + hc) * P->o.sh;
+    u32x2 val;
+    val[0] = pack_e<F16>(o[0] * inv, o[1] * inv);
+    val[1] = pack_e<F16>(o[2] * inv, o[3] * inv);
+    *(u32x2*)(orow + f) = val;
+    if (l == 0 && P->lse.ptr)
+      ((float*)P->lse.ptr)[(int64_t)(e.q0 + tok) * P->lse.ss + (int64_t)(h0 + hc) * P->lse.sh] =
+          m == kNegInf ? kNegInf : m * P->c + __builtin_amdgcn_logf(sum + 1e-6f) * kLn2;
+    continue;
+  }
   for (int c = blockIdx.y; c < cols; c += gridDim.y) {
     const int tk = c / P->gsub, hc = c - tk * P->gsub, tok = ct * P->tpt + tk;
     if (tok >= e.lq || hc >= nh) continue;  // (uniform)
@@ -466,6 +517,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
     }
     __syncthreads();
   }
+  }  // (the next tile)
 }
 
 // Waves per SIMD that the register budget is cut for.  Two (256 registers): the
@@ -520,7 +572,9 @@ hipError_t launch_paged_packed(const PagedParams& P, int rc, hipStream_t s) {
 }
 
 hipError_t launch_paged_merge(const PagedParams& P, hipStream_t s) {
-  const dim3 grid((uint32_t)P.waves, (uint32_t)(P.gsub * P.tpt));
+  const int cols = P.gsub * P.tpt, rows = 256 / (P.D / 4);
+  const dim3 grid((uint32_t)((P.waves + P.merge_runs - 1) / P.merge_runs),
+                  (uint32_t)(P.merge_by_part ? cols : (cols + rows - 1) / rows));
   if (P.D == 64)
     hipLaunchKernelGGL(P.f16 ? (paged_merge_kernel<64, true>) : (paged_merge_kernel<64, false>), grid, dim3(256), 0, s, P);
   else

@@ -20,28 +20,28 @@ namespace {
 // once, then walk the token's rows, LPR = D / 16 lanes a row, each with 8
 // values of the first half and the matching 8 of the second.  Bound by
 // reading and writing every row once.
-constexpr int kAppWaves = 4;
+//
+// A workgroup takes one token at a time (few tokens: a wave of it each, see
+// launch_paged_append), its waves the token's rows in turn, two passes of rows in
+// flight; every wave forms the cos and sin that its lanes' columns need.
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));  // (norm weights anywhere)
+constexpr int kAppWaves = 4, kAppAhead = 2;
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const PagedAppendParams A) {
-  constexpr int LPR = D / 16, HALF = D / 2, RPP = 64 / LPR;  // rows a pass
+  constexpr int LPR = D / 16, HALF = D / 2, RPP = 64 / LPR;  // rows a pass of a wave
   const PagedParams& P = A.p;
   __shared__ float table[kAppWaves][2 * HALF];
   const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
   float* cs = table[wv];
   const int i = lane % LPR, lrow = lane / LPR, col = 8 * i;
   const auto cu = const_space(P.cu);
-  const int nv = P.H + P.H_KV, nr = nv + P.H_KV, per = nr + P.H_G;
-  float wn[2][16];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    wn[0][e] = A.wq ? A.wq[col + e] : 1.f;
-    wn[0][8 + e] = A.wq ? A.wq[HALF + col + e] : 1.f;
-    wn[1][e] = A.wk ? A.wk[col + e] : 1.f;
-    wn[1][8 + e] = A.wk ? A.wk[HALF + col + e] : 1.f;
-  }
+  const int nv = P.H + P.H_KV, nr = nv + P.H_KV;  // q and k rows; and v rows
+  const int share = A.share;                      // waves of a token
+  const int sub = wv % share;
   const double inv = A.inv_freq && lane < HALF ? (double)A.inv_freq[lane] : 0.0;
+  const int step = gridDim.x * (kAppWaves / share);
 
-  for (int t = blockIdx.x * kAppWaves + wv; t < P.T; t += gridDim.x * kAppWaves) {
+  for (int t = blockIdx.x * (kAppWaves / share) + wv / share; t < P.T; t += step) {
     // the token's sequence: the last b with cu[b] <= t
     int lo = -1, hi = P.N;
     if (uni(cu[P.N]) <= t) lo = P.N;
@@ -52,111 +52,125 @@ __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const Page
         else hi = mid;
       }
     const bool inside = lo >= 0 && lo < P.N;
-    int row = -1;
+    int row = -1, pr = 0;
     int64_t page = -1;
-    int pr = 0;
     if (inside) {
       const PagedSeq e = paged_seq_uniform(kargs(), lo);
       row = e.lk - e.lq + (t - e.q0);
       if (row >= 0 && row < e.lk) {
-        const int pg = row / P.ps;
+        const int pg = page_of(P.ps_mul, P.ps_shift, row);
         pr = row - pg * P.ps;
         const int id = uni(*const_space(P.table + (int64_t)lo * P.tstride + pg));
         if ((uint32_t)id < (uint32_t)P.npages) page = id;
       }
     }
+    // Source and destination of row r of the token (q, k, then v rows).
+    u32x4 a[kAppAhead], b[kAppAhead];
+    uint16_t* dst[kAppAhead];
+    auto load = [&](int r0) {
+#pragma unroll
+      for (int p = 0; p < kAppAhead; ++p) {
+        const int r = r0 + p * RPP * share + lrow;
+        const bool isq = r < P.H, isk = !isq && r < nv;
+        const int h = isq ? r : isk ? r - P.H : r - nv;
+        dst[p] = nullptr;
+        a[p] = b[p] = u32x4{0, 0, 0, 0};
+        if (r >= nr) continue;
+        const uint16_t* src;
+        if (isq) {
+          src = (const uint16_t*)P.q.ptr + (int64_t)t * P.q.ss + (int64_t)h * P.q.sh;
+          dst[p] = (uint16_t*)P.o.ptr + (int64_t)t * P.o.ss + (int64_t)h * P.o.sh;
+        } else {
+          const TView& n = isk ? A.kn : A.vn;
+          const TView& d = isk ? P.k : P.v;
+          src = (const uint16_t*)n.ptr + (int64_t)t * n.ss + (int64_t)h * n.sh;
+          if (page >= 0) dst[p] = (uint16_t*)d.ptr + page * d.sb + (int64_t)h * d.sh + (int64_t)pr * d.ss;
+        }
+        if (dst[p]) {
+          a[p] = ld16(src + col);
+          b[p] = ld16(src + HALF + col);
+        }
+      }
+    };
+    load(sub * RPP);
     const bool turn = inside && A.inv_freq;
+    float co[8], si[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) co[e] = 1.f, si[e] = 0.f;
     if (turn) {
       const int pos = A.pos ? uni(*const_space(A.pos + t)) : row;
       if (lane < HALF) {
         // in turns, reduced to half a turn either way
         const double x = (double)pos * inv * 0.15915494309189533577;
-        const float a = (float)((x - __builtin_rint(x)) * 6.28318530717958647693);
+        const float ang = (float)((x - __builtin_rint(x)) * 6.28318530717958647693);
         float s, c;
-        sincosf(a, &s, &c);
+        sincosf(ang, &s, &c);
         cs[lane] = c;
         cs[HALF + lane] = s;
       }
       // (one wave's own LDS: its reads follow its writes in order)
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-    }
-    float co[8], si[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      co[e] = turn ? cs[col + e] : 1.f;
-      si[e] = turn ? cs[HALF + col + e] : 0.f;
-    }
-    if (turn) {
+      for (int e = 0; e < 8; ++e) co[e] = cs[col + e], si[e] = cs[HALF + col + e];
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
-    for (int r0 = 0; r0 < nr; r0 += RPP) {
-      const int r = r0 + lrow;
-      const bool isq = r < P.H, isk = !isq && r < nv, have = r < nr;
-      const int h = isq ? r : isk ? r - P.H : r - nv;
-      u32x4 a = {0, 0, 0, 0}, b = a;
-      uint16_t* dst = nullptr;
-      if (have) {
-        const uint16_t* src;
-        if (isq) {
-          src = (const uint16_t*)P.q.ptr + (int64_t)t * P.q.ss + (int64_t)h * P.q.sh;
-          dst = (uint16_t*)P.o.ptr + (int64_t)t * P.o.ss + (int64_t)h * P.o.sh;
-        } else {
-          const TView& n = isk ? A.kn : A.vn;
-          const TView& d = isk ? P.k : P.v;
-          src = (const uint16_t*)n.ptr + (int64_t)t * n.ss + (int64_t)h * n.sh;
-          if (page >= 0) dst = (uint16_t*)d.ptr + page * d.sb + (int64_t)h * d.sh + (int64_t)pr * d.ss;
+    for (int r0 = sub * RPP; r0 < nr; r0 += kAppAhead * RPP * share) {
+#pragma unroll
+      for (int p = 0; p < kAppAhead; ++p) {
+        const int r = r0 + p * RPP * share + lrow;
+        const bool isq = r < P.H, isk = !isq && r < nv;
+        const float* w = isq ? A.wq : A.wk;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = elt_lo<F16>(a[p][e]), x[2 * e + 1] = elt_hi<F16>(a[p][e]);
+          x[8 + 2 * e] = elt_lo<F16>(b[p][e]), x[8 + 2 * e + 1] = elt_hi<F16>(b[p][e]);
         }
-        if (dst) {
-          a = ld16(src + col);
-          b = ld16(src + HALF + col);
-        }
-      }
-      const bool norm = isq ? A.wq != nullptr : A.wk != nullptr;
-      float x[16];
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = elt_lo<F16>(a[e]), x[2 * e + 1] = elt_hi<F16>(a[e]);
-        x[8 + 2 * e] = elt_lo<F16>(b[e]), x[8 + 2 * e + 1] = elt_hi<F16>(b[e]);
-      }
-      float ss = 0.f;
+        for (int e = 0; e < 16; ++e) ss += x[e] * x[e];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ss += x[e] * x[e];
+        for (int m = 1; m < LPR; m <<= 1) ss += __shfl_xor(ss, m);
+        if (!dst[p]) continue;
+        if (inside && (isq || isk) && (w || turn)) {
+          if (w) {
+            const float rs = rsqrtf(ss * (1.f / D) + A.eps);
 #pragma unroll
-      for (int m = 1; m < LPR; m <<= 1) ss += __shfl_xor(ss, m);
-      if (inside && (isq || isk)) {
-        if (norm) {
-          const float rs = rsqrtf(ss * (1.f / D) + A.eps);
-          const float* w = wn[0];
+            for (int e = 0; e < 2; ++e) {
+              const f32x4_u w1 = *(const f32x4_u*)(w + col + 4 * e);
+              const f32x4_u w2 = *(const f32x4_u*)(w + HALF + col + 4 * e);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = x[e] * rs * (isq ? wn[0][e] : wn[1][e]);
-          (void)w;
-        }
-        if (norm || turn) {
+              for (int k = 0; k < 4; ++k) x[4 * e + k] *= rs * w1[k], x[8 + 4 * e + k] *= rs * w2[k];
+            }
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p0 = x[2 * e], p1 = x[2 * e + 1], q0 = x[8 + 2 * e], q1 = x[8 + 2 * e + 1];
-            const float c0 = co[2 * e], c1 = co[2 * e + 1], s0 = si[2 * e], s1 = si[2 * e + 1];
-            a[e] = pack_e<F16>(turn ? p0 * c0 - q0 * s0 : p0, turn ? p1 * c1 - q1 * s1 : p1);
-            b[e] = pack_e<F16>(turn ? q0 * c0 + p0 * s0 : q0, turn ? q1 * c1 + p1 * s1 : q1);
+            float y[4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float p1 = x[2 * e + k], p2 = x[8 + 2 * e + k], c = co[2 * e + k], s = si[2 * e + k];
+              y[k] = turn ? p1 * c - p2 * s : p1;
+              y[2 + k] = turn ? p2 * c + p1 * s : p2;
+            }
+            a[p][e] = pack_e<F16>(y[0], y[1]);
+            b[p][e] = pack_e<F16>(y[2], y[3]);
           }
         }
+        st16(dst[p] + col, a[p]);
+        st16(dst[p] + HALF + col, b[p]);
       }
-      if (dst) {
-        st16(dst + col, a);
-        st16(dst + HALF + col, b);
-      }
+      if (r0 + kAppAhead * RPP * share < nr) load(r0 + kAppAhead * RPP * share);
     }
     if (P.H_G > 0 && page >= 0) {
       const int cr = P.R / 8, n = P.H_G * cr;
-      for (int j = lane; j < n; j += 64) {
+      for (int j = sub * 64 + lane; j < n; j += 64 * share) {
         const int h = j / cr, ch = j - h * cr;
         st16((uint16_t*)P.rk.ptr + page * P.rk.sb + (int64_t)h * P.rk.sh + (int64_t)pr * P.rk.ss + 8 * ch,
              ld16((const uint16_t*)A.rkn.ptr + (int64_t)t * A.rkn.ss + (int64_t)h * A.rkn.sh + 8 * ch));
       }
     }
-    (void)per;
   }
 }
 
@@ -402,10 +416,15 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
 
 }  // namespace
 
-hipError_t launch_paged_append(const PagedAppendParams& A, hipStream_t s) {
+hipError_t launch_paged_append(const PagedAppendParams& A_, hipStream_t s) {
+  PagedAppendParams A = A_;
   const PagedParams& P = A.p;
   if (P.T <= 0) return hipSuccess;
-  const dim3 grid((uint32_t)std::min((P.T + kAppWaves - 1) / kAppWaves, 4096));
+  // Few tokens (a decode step): all four waves of a workgroup on each, which
+  // shortens the chain; many: one wave each.
+  A.share = P.T <= 2048 ? 4 : 1;
+  const int per = kAppWaves / A.share;
+  const dim3 grid((uint32_t)std::min((P.T + per - 1) / per, 4096));
   void (*k)(const PagedAppendParams) =
       P.D == 64 ? (P.f16 ? paged_append_kernel<64, true> : paged_append_kernel<64, false>)
                 : (P.f16 ? paged_append_kernel<128, true> : paged_append_kernel<128, false>);

@@ -71,7 +71,7 @@ __device__ __forceinline__ void tile_body() {
   {
     auto units = [&](const PagedSeq& s) { return TilePlan::units(P, s); };
     SeqWork<decltype(units)> work(P, lane, units);
-    per = run_units(P, work.total);
+    per = run_units(P, work.total, P->min_steps);
     const int64_t u = (int64_t)run * per;
     left = min(work.total - u, per);
     if (left <= 0) {
