@@ -1388,7 +1388,10 @@ void fill_cache(fna2::PagedParams& K, const fna2_paged_cache& c) {
 // the longest chunk fits one tile.  Tile kernel (`tile`) for longer ones: hw
 // heads of a KV head (up to 4) times 128 / hw tokens, so that short chunks of
 // grouped heads still read K and V once; with ranks each head brings its own
-// R_k tile, so chunks that fill 64 or 128 tokens anyway take 2 heads or one.
+// R_k tile, so chunks that fill 64 or 128 tokens anyway take 2 heads or one (us, 1,
+// 2, 4 heads of 4: 1024 tokens over 16384 rows, rank 64 351, 368, 414; 100 over
+// 4000, rank 32 57, 50, 56; 2 x 600 over 8000, d = 64, rank 16 133, 135, 148; not
+// always: 512 over 2000, rank 32 55, 53, 46).
 struct PagedPlan {
   bool tile;
   int gsub, nsub, tpt, rc, hw, waves, min_steps, merge_runs;
@@ -1412,7 +1415,10 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
     const int64_t mean = cdiv64(c.total_q, std::max(c.batch, 1));
     k.hw = group >= 3 ? 4 : group;
     if (rpl > 0 && mean >= 64) k.hw = std::min(k.hw, mean >= 128 ? 1 : 2);
-    k.min_steps = 8;
+    // Four steps a run at least: a part of a tile is written and read as 64 KB
+    // (us, 2, 4, 8 steps: 100 tokens over 100 rows, 16 heads 15.7, 16.6, 24.8; 1024 over
+    // 1024 51.8, 37.3, 43.3; 2 x 64 over 1000, 16/4 heads 34.0, 28.2, 23.7)
+    k.min_steps = 4;
     const int64_t tiles = ((int64_t)c.total_q / (128 / k.hw) + c.batch) * c.heads_kv * ((group + k.hw - 1) / k.hw);
     k.waves = (int)std::min(256. * fna2::paged_tile_per_cu(c.head_dim, rpl, k.hw),
                             std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
