@@ -184,7 +184,7 @@ __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const Page
 // own.  Bound by the latency of its passes, not by memory: a wave keeps up to
 // 512 weights in registers over all of them.  (8 bits a pass: the first digit of positive
 // weights is their exponent's, a few bins that all lanes count in.)
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelAhead = 8;
+constexpr int kSelAhead = 8;
 constexpr int kSelBins = 2048;
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (w != w) return 0xffffffffu;
@@ -202,7 +202,11 @@ __device__ __forceinline__ int wave_scan(int x, int lane) {
   return x;
 }
 
+// kSelThreads: 1024, or 256 where no sequence holds more rows than those keep in
+// registers.
+template <int kSelThreads>
 __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEvictParams E) {
+  constexpr int kSelWaves = kSelThreads / 64, kBins = kSelBins / kSelThreads;  // bins a thread
   const PagedParams& P = E.p;
   __shared__ int hist[kSelBins];
   __shared__ int wsum[kSelWaves];
@@ -263,15 +267,20 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEv
       }
       __syncthreads();
       // The digit d whose rows, with those of larger digits, reach `need`: a
-      // thread has the two bins 2047 - 2 tid and the one below.
-      const int h0 = hist[2047 - 2 * tid], h1 = hist[2046 - 2 * tid];
-      int s = wave_scan(h0 + h1, lane);
+      // thread has kBins bins, from the largest digits down.
+      int h[kBins], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kBins; ++i) mine += h[i] = hist[kSelBins - 1 - kBins * tid - i];
+      int s = wave_scan(mine, lane);
       if (lane == 63) wsum[wv] = s;
       __syncthreads();
       for (int i = 0; i < wv; ++i) s += wsum[i];
-      const int before = s - h0 - h1;
-      if (before < need && before + h0 >= need) pick[0] = 2047 - 2 * tid, pick[1] = before;
-      if (before + h0 < need && s >= need) pick[0] = 2046 - 2 * tid, pick[1] = before + h0;
+      int before = s - mine;
+#pragma unroll
+      for (int i = 0; i < kBins; ++i) {
+        if (before < need && before + h[i] >= need) pick[0] = kSelBins - 1 - kBins * tid - i, pick[1] = before;
+        before += h[i];
+      }
       __syncthreads();
       prefix |= (uint32_t)pick[0] << shift;
       mask |= digit << shift;
@@ -365,7 +374,7 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
   const int* trow = P.table + (int64_t)b * P.tstride;
   // lanes a row: the chunks, rounded up to a power of two
   const int lanes = chunks > 8 ? 16 : chunks > 4 ? 8 : chunks > 2 ? 4 : chunks;
-  const int c = threadIdx.x & (lanes - 1), row0 = threadIdx.x / lanes, stride = kCompactThreads / lanes;
+  const int c = threadIdx.x & (lanes - 1), row0 = threadIdx.x / lanes, stride = blockDim.x / lanes;
   const int round = stride * kCompactAhead;
   uint16_t* base = (uint16_t*)t.ptr + (int64_t)h * t.sh + 8 * (kStrip * strip + c);
   auto place = [&](int j) -> uint16_t* {
@@ -433,7 +442,11 @@ hipError_t launch_paged_append(const PagedAppendParams& A_, hipStream_t s) {
 }
 
 hipError_t launch_paged_select(const PagedEvictParams& E, hipStream_t s) {
-  hipLaunchKernelGGL(paged_select_kernel, dim3((uint32_t)(E.p.N * E.p.H_KV)), dim3(kSelThreads), 0, s, E);
+  const dim3 grid((uint32_t)(E.p.N * E.p.H_KV));
+  if ((int64_t)E.p.width * E.p.ps <= 256 * kSelAhead)
+    hipLaunchKernelGGL(paged_select_kernel<256>, grid, dim3(256), 0, s, E);
+  else
+    hipLaunchKernelGGL(paged_select_kernel<1024>, grid, dim3(1024), 0, s, E);
   return hipGetLastError();
 }
 
@@ -441,7 +454,9 @@ hipError_t launch_paged_compact(const PagedEvictParams& E, hipStream_t s) {
   const PagedParams& P = E.p;
   const int64_t per = 2 * (int64_t)P.H_KV * (P.D / (8 * kStrip)) +
                       (P.H_G > 0 ? (int64_t)P.H_G * cdiv(P.R, 8 * kStrip) : 0);
-  hipLaunchKernelGGL(paged_compact_kernel, dim3((uint32_t)(per * P.N)), dim3(kCompactThreads), 0, s, E);
+  // (a small budget is one round of fewer waves: 8 lanes a row, kCompactAhead rows each)
+  const int threads = std::min(kCompactThreads, std::max(64, cdiv(2 * std::min(E.budget, 1 << 20), 64) * 64));
+  hipLaunchKernelGGL(paged_compact_kernel, dim3((uint32_t)(per * P.N)), dim3((uint32_t)threads), 0, s, E);
   return hipGetLastError();
 }
 
