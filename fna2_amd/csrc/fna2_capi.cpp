@@ -1415,6 +1415,8 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
     const int64_t mean = cdiv64(c.total_q, std::max(c.batch, 1));
     k.hw = group >= 3 ? 4 : group;
     if (rpl > 0 && mean >= 64) k.hw = std::min(k.hw, mean >= 128 ? 1 : 2);
+    // (long chunks: no wave without a head; short ones read K and V more often instead)
+    while (mean >= 64 && group % k.hw) k.hw /= 2;
     // Four steps a run at least: a part of a tile is written and read as 64 KB
     // (us, 2, 4, 8 steps: 100 tokens over 100 rows, 16 heads 15.7, 16.6, 24.8; 1024 over
     // 1024 51.8, 37.3, 43.3; 2 x 64 over 1000, 16/4 heads 34.0, 28.2, 23.7)
@@ -1423,6 +1425,7 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
     k.waves = (int)std::min(256. * fna2::paged_tile_per_cu(c.head_dim, rpl, k.hw),
                             std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
     k.waves = (int)cdiv64(k.waves, 8) * 8;  // (whole turns of the XCDs)
+    k.merge_by_part = k.waves / std::max<int64_t>(tiles, 1) > 8;
     k.ml = align_up(2 * (size_t)k.waves * fna2::paged_tile_slot(c.head_dim));
     k.cuts = k.ml + align_up(2 * (size_t)k.waves * 128 * 8u);
     k.bytes = k.cuts + align_up((size_t)k.waves * sizeof(fna2::PagedCut));

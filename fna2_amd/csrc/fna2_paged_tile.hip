@@ -414,13 +414,19 @@ __device__ __forceinline__ void tile_body() {
   }
 }
 
-// Joins the parts of a tile that runs cut: workgroup (i, d) takes 32 features
-// of the tile that run i's end cuts; a wave the tokens of one wave of the tile, four
-// parts at a time.  Parts come in the order of the runs.
+// Joins the parts of a tile that runs cut: workgroup (i, y) takes 32 features
+// of the tile that run i's end cuts, four parts at a time.  A wave takes the tokens
+// of one wave of the tile; where a tile has many parts (by_part) the
+// workgroup does, its waves every fourth group of parts each, joined in LDS.  The
+// order of the sums goes by the parts alone.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedParams) {
   KArg P = kargs();
-  const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6), d = blockIdx.y;
+  __shared__ f32x4_t part[4][4][64];
+  __shared__ float stat[4][2][32];
+  const int lane = threadIdx.x & 63, own = uni(threadIdx.x >> 6);
+  const bool by_part = P->merge_by_part != 0;
+  const int d = blockIdx.y % (D / 32), wv = by_part ? blockIdx.y / (D / 32) : own;
   const int l32 = lane & 31, hl = lane >> 5;
   const int i0 = blockIdx.x;
   const auto rec = const_space(P->cuts + i0);
@@ -431,7 +437,7 @@ __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedParams
   const PagedSeq e = paged_seq_uniform(P, rec->b);
   const int hblk = cdiv(P->group, P->hw), kvh = hb / hblk, h_in = (hb - kvh * hblk) * P->hw + wv % P->hw;
   const int tok = qt * TilePlan::tokens(P) + 32 * (wv / P->hw) + l32;
-  if (tok >= e.lq || h_in >= P->group) return;
+  const bool live = tok < e.lq && h_in < P->group;
   const int h = kvh * P->group + h_in;
   const float c2 = P->c2;
   float M = kNegInf, L = 0.f;
@@ -439,36 +445,56 @@ __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedParams
 #pragma unroll
   for (int g = 0; g < 4; ++g) o[g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   constexpr int U = 4;  // parts in flight
-  for (int j0 = 0; j0 < n; j0 += U) {
-    f32x4_t x[U][4];
-    f32x2 ml[U];
+  if (live) {
+    for (int j0 = by_part ? U * own : 0; j0 < n; j0 += by_part ? 4 * U : U) {
+      f32x4_t x[U][4];
+      f32x2 ml[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int j = min(j0 + k, n - 1);  // (past the last: weighed 0 below)
-      const int64_t slot = (int64_t)(j == 0 ? 2 * i0 + 1 : 2 * (i0 + j)) * 4 + wv;
-      const float* src = P->part + slot * 32 * D + d * 1024 + 4 * lane;
-      ml[k] = *(const f32x2*)(P->ml + 2 * (slot * 32 + l32));
+      for (int k = 0; k < U; ++k) {
+        const int j = min(j0 + k, n - 1);  // (past the last: not added below)
+        const int64_t slot = (int64_t)(j == 0 ? 2 * i0 + 1 : 2 * (i0 + j)) * 4 + wv;
+        const float* src = P->part + slot * 32 * D + d * 1024 + 4 * lane;
+        ml[k] = *(const f32x2*)(P->ml + 2 * (slot * 32 + l32));
 #pragma unroll
-      for (int g = 0; g < 4; ++g) x[k][g] = *(const f32x4_t*)(src + g * 256);
+        for (int g = 0; g < 4; ++g) x[k][g] = *(const f32x4_t*)(src + g * 256);
+      }
+      float m = M;
+#pragma unroll
+      for (int k = 0; k < U; ++k) m = fmaxf(m, ml[k][0]);
+      const float ref = m == kNegInf ? 0.f : m;
+      const float wa = weight2((M - ref) * c2);
+      L *= wa;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) o[g] *= wa;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (j0 + k >= n) break;  // (uniform)
+        const float wb = weight2((ml[k][0] - ref) * c2);
+        L += ml[k][1] * wb;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) o[g] += x[k][g] * wb;
+      }
+      M = m;
     }
-    float m = M;
-#pragma unroll
-    for (int k = 0; k < U; ++k) m = fmaxf(m, ml[k][0]);
-    const float ref = m == kNegInf ? 0.f : m;
-    const float wa = weight2((M - ref) * c2);
-    L *= wa;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) o[g] *= wa;
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (j0 + k >= n) break;  // (uniform)
-      const float wb = weight2((ml[k][0] - ref) * c2);
-      L += ml[k][1] * wb;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) o[g] += x[k][g] * wb;
-    }
-    M = m;
   }
+  if (by_part) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) part[own][g][lane] = o[g];
+    if (hl == 0) stat[own][0][l32] = M, stat[own][1][l32] = L;
+    __syncthreads();
+    if (own != 0) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float mw = stat[w][0][l32], m = fmaxf(M, mw);
+      const float ref = m == kNegInf ? 0.f : m;
+      const float wa = weight2((M - ref) * c2), wb = weight2((mw - ref) * c2);
+      L = L * wa + stat[w][1][l32] * wb;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) o[g] = o[g] * wa + part[w][g][lane] * wb;
+      M = m;
+    }
+  }
+  if (!live) return;
   const float inv = 1.f / (L + 1e-6f);
   uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)h * P->o.sh;
 #pragma unroll
@@ -542,7 +568,7 @@ hipError_t launch_paged_tile(const PagedParams& P, int rpl, hipStream_t s) {
   hipLaunchKernelGGL(k, dim3((uint32_t)P.waves), dim3(256), 0, s, P);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const dim3 grid((uint32_t)P.waves, (uint32_t)(P.D / 32));
+  const dim3 grid((uint32_t)P.waves, (uint32_t)(P.D / 32 * (P.merge_by_part ? 4 : 1)));
   void (*m)(const PagedParams) =
       P.D == 64 ? (P.f16 ? paged_tile_merge_kernel<64, true> : paged_tile_merge_kernel<64, false>)
                 : (P.f16 ? paged_tile_merge_kernel<128, true> : paged_tile_merge_kernel<128, false>);
