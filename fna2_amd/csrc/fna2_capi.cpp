@@ -1562,6 +1562,11 @@ int fna2_paged_weights(const fna2_paged_weights_args* w, void* stream) {
   K.p.nsub = k.tile ? K.p.group : k.nsub;
   K.p.tpt = k.tile ? 32 : k.tpt;
   const int rc = k.tile ? fna2::paged_rank_chunks(K.p.R / 8) : k.rc;
+  if (!k.tile) {
+    const double steps = (double)c.batch * c.heads_kv * (double)std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);
+    K.p.waves = K.grid = (int)std::min(steps, 256. * fna2::paged_glance_per_cu(c.head_dim, rc));
+    return fna2::launch_paged_glance(K, rc, (hipStream_t)stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
+  }
   const int64_t blocks = (int64_t)c.batch * c.heads_kv * std::max<int64_t>(cdiv64(cached_rows(c), 128), 1);
   K.grid = (int)std::min<int64_t>(blocks, 256 * fna2::paged_weigh_per_cu(rc));
   if (fna2::launch_paged_weights(K, rc, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;

@@ -257,6 +257,8 @@ struct PagedWeightsParams {
   int grid;
 };
 int paged_weigh_per_cu(int rc);  // resident workgroups
+int paged_glance_per_cu(int D, int rc);  // ... waves of the kernel for short chunks
+hipError_t launch_paged_glance(const PagedWeightsParams& P, int rc, hipStream_t s);
 hipError_t launch_paged_weights(const PagedWeightsParams& P, int rc, hipStream_t s);
 
 struct PagedAppendParams {

@@ -476,6 +476,30 @@ def test_hidden_rows_never_reach_a_result(gpu, lq, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,HKV,HG,R", [(4, 4, 4, 8), (6, 2, 4, 8), (4, 2, 4, 24), (32, 1, 20, 64),
+                                        (40, 1, 0, 0)])
+@pytest.mark.parametrize("lq", [[1, 1], [5, 3], [40, 33]])
+def test_weights_past_garbage(gpu, lq, H, HKV, HG, R):
+    """The rows' weights with NaN in every row that is no sequence's, behind odd
+    numbers of rank chunks and in pages next to the used ones."""
+    c = Case(lq, [75, 61], H, HKV, HG, 64, R, 16, device=gpu)
+    ref = torch.zeros(2, HKV, c.width * 16, device=gpu)
+    c.attend(key_weights=ref)
+    check_attend(c)
+    named = torch.zeros(c.P, 16, dtype=torch.bool)
+    for b in range(2):
+        for j in range(c.lk[b]):
+            named[c.slot(b, j)] = True
+    hole = ~named.to(gpu)
+    for pool in (c.k, c.v, c.rk):
+        if pool is not None:
+            pool.masked_fill_(hole[:, None, :, None], float("nan"))
+    acc = torch.zeros_like(ref)
+    c.attend(key_weights=acc)
+    assert torch.equal(acc, ref)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lq", [[1, 1], [40, 9]])
 def test_infinite_values_stay_infinite(gpu, lq):
     c = Case(lq, [75, 61], 4, 2, 0, 64, 0, 16, device=gpu)
