@@ -1556,19 +1556,23 @@ int fna2_paged_weights(const fna2_paged_weights_args* w, void* stream) {
   K.w_sb = w->stride_b;
   K.w_sh = w->stride_h;
   K.cap = w->capacity;
-  // Row tiles: the packed kernel's columns where it runs, else 32 tokens of a head.
   const PagedPlan k = paged_plan(c);
-  K.p.gsub = k.tile ? 1 : k.gsub;
-  K.p.nsub = k.tile ? K.p.group : k.nsub;
-  K.p.tpt = k.tile ? 32 : k.tpt;
-  const int rc = k.tile ? fna2::paged_rank_chunks(K.p.R / 8) : k.rc;
-  if (!k.tile) {
-    const double steps = (double)c.batch * c.heads_kv * (double)std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);
-    K.p.waves = K.grid = (int)std::min(steps, 256. * fna2::paged_glance_per_cu(c.head_dim, rc));
-    return fna2::launch_paged_glance(K, rc, (hipStream_t)stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
+  const int64_t rows = std::max<int64_t>(cached_rows(c), 1), heads = (int64_t)c.batch * c.heads_kv;
+  if (!k.tile) {  // row tiles as the packed kernel's columns
+    K.p.gsub = k.gsub;
+    K.p.nsub = k.nsub;
+    K.p.tpt = k.tpt;
+    K.p.waves = K.grid = (int)std::min((double)heads * (double)cdiv64(rows, 32),
+                                       256. * fna2::paged_glance_per_cu(c.head_dim, k.rc));
+    return fna2::launch_paged_glance(K, k.rc, (hipStream_t)stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
   }
-  const int64_t blocks = (int64_t)c.batch * c.heads_kv * std::max<int64_t>(cdiv64(cached_rows(c), 128), 1);
-  K.grid = (int)std::min<int64_t>(blocks, 256 * fna2::paged_weigh_per_cu(rc));
+  const int rc = fna2::paged_rank_chunks(K.p.R / 8);
+  const int64_t resident = 256 * fna2::paged_weigh_per_cu(c.head_dim, rc);
+  // Where blocks of 128 keys leave workgroups without one: 64 keys, whose row tiles
+  // two waves share (us, 128 and 64 keys: 32 blocks of 100 tokens 9.2, 7.1; 128
+  // of 256 38.4, 29.6; 512 of 1024 123, 115; but 1920 of 107 31, 43).
+  K.key_waves = heads * cdiv64(rows, 128) <= resident ? 2 : 4;
+  K.grid = (int)std::min<int64_t>(heads * cdiv64(rows, 32 * K.key_waves), resident);
   if (fna2::launch_paged_weights(K, rc, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
   return FNA2_OK;
 }

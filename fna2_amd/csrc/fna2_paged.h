@@ -255,8 +255,9 @@ struct PagedWeightsParams {
   int64_t w_sb, w_sh;
   int cap;
   int grid;
+  int key_waves;  // kernel for long chunks: waves of a workgroup on keys of their own, 4 or 2
 };
-int paged_weigh_per_cu(int rc);  // resident workgroups
+int paged_weigh_per_cu(int D, int rc);  // resident workgroups
 int paged_glance_per_cu(int D, int rc);  // ... waves of the kernel for short chunks
 hipError_t launch_paged_glance(const PagedWeightsParams& P, int rc, hipStream_t s);
 hipError_t launch_paged_weights(const PagedWeightsParams& P, int rc, hipStream_t s);

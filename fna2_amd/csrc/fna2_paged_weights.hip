@@ -2,26 +2,28 @@
 //
 //     W_j += sum over the chunk's tokens i and the KV head's query heads h of
 //            e^{S_hij - LSE_hi},
-// S as in fna2_paged_attn.hip, whose LSE this takes.
+// S as in fna2_paged_attn.hip, whose LSE this takes.  Two kernels, for the two of
+// the attention; in both keys are the columns of S = Q K^T, so that a lane
+// sums its key's weights in registers, in fp32 and in a fixed order, and adds them
+// to W once.
 //
-// The transpose of the attention's loop: a wave keeps 32 keys (K, and R_k of the
-// heads at hand, in registers) as the columns of S = Q K^T and walks the
-// chunk's rows, so that a lane sums its key's weights in registers, in fp32 and
-// in a fixed order.  A row tile is 32 (token, head) pairs: tpt tokens of gsub
-// heads, as the packed kernel's columns for short chunks, 32 tokens of one
-// head for longer ones.  The four waves of a workgroup share the row
-// tiles, which come through a two-stage LDS ring by DMA (rows past the chunk as
-// zeros), with each row's -LSE log2(e) (-inf: it sees nothing, or is none) and last
-// visible key beside them.  Blocks of 128 keys go round over the workgroups.
-//
-// Long chunks are bound by the matrix cores and the exponentials.
+// Long chunks (weigh kernel): a wave keeps 32 keys (K, and R_k of the head at
+// hand) in registers and walks the chunk's row tiles, 32 tokens of one head
+// each, which the workgroup's four waves share.  They come through a two-stage LDS
+// ring by DMA, two tiles a stage (rows past the chunk as zeros), with each row's
+// -LSE log2(e) (-inf: it sees nothing, or is none).  Blocks of 128 keys, or of 64
+// with the tiles halved between two waves, go round over the workgroups.
+// Bound by the exponentials: 16 of a lane's take 16 cycles each, and 8 more for scale
+// and sum, against 96 for the products of a tile at d = 64, R = 16.  2 chunks of 509
+// tokens over 7001 rows, 16 heads: 36 us, 1.9 10^12 weights a second.
 //
 // Short chunks (glance kernel, where the packed kernel runs): usually one row
 // tile holds the chunk, so a wave keeps that in registers instead and streams
 // keys, 32 at a time in a run of its own, the next ones' K and R_k on their way
-// while it works on these.  Bound by reading K (and R_k) once.  (With row tiles
-// through LDS: 45 sequences of 10,730 rows, 8 heads of 64, 484 us with the
-// attention.)
+// while it works on these.  Bound by reading K (and R_k) once: one token
+// of each of 16 sequences of up to 8192 rows, 8 KV heads of 128, 32.6 us.  (With row
+// tiles through LDS 38 us; 45 sequences of up to 10730, 8 heads of 64, with the attention
+// 484 us, now 331.)
 #include <algorithm>
 
 #include "fna2_kernels.h"
@@ -37,28 +39,28 @@ struct WeighCfg {
   static constexpr int QBYTES = 32 * D * 2, RBYTES = 32 * RC * 16;
   static constexpr int NQ = QBYTES / 4096;            // DMA instructions per wave and tile
   static constexpr int NR = (RBYTES / 1024 + 3) / 4;
+  static constexpr int U = 2;  // row tiles between two barriers
 };
 
 template <int D, int RC, bool F16>
 __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
   using C = WeighCfg<D, RC>;
-  __shared__ __attribute__((aligned(1024))) uint8_t st0[C::QBYTES + C::RBYTES];
-  __shared__ __attribute__((aligned(1024))) uint8_t st1[C::QBYTES + C::RBYTES];
-  // a row tile's -LSE log2(e), and the last keys that its rows see
-  __shared__ __attribute__((aligned(16))) float nl0[32], nl1[32];
-  __shared__ __attribute__((aligned(16))) int lim0[32], lim1[32];
+  constexpr int U = C::U, TILE = C::QBYTES + C::RBYTES;
+  __shared__ __attribute__((aligned(1024))) uint8_t st0[U * TILE], st1[U * TILE];
+  __shared__ __attribute__((aligned(16))) float nl0[32 * U], nl1[32 * U];  // rows' -LSE log2(e)
+  __shared__ float half[64];
   KArg P = kargs();
   const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
   const int col = lane & 31, hl = lane >> 5;
-  auto units = [&](const PagedSeq& s) { return s.lq > 0 ? (int64_t)P->H_KV * cdiv(s.lk, 128) : 0; };
+  // Keys of a workgroup: 32 for each of kw waves; with kw = 2 the waves behind
+  // take the second tile of each stage.
+  const int kw = W.key_waves, keys = 32 * kw;
+  auto units = [&](const PagedSeq& s) { return s.lq > 0 ? (int64_t)P->H_KV * cdiv(s.lk, keys) : 0; };
   SeqWork<decltype(units)> work(P, lane, units);
   const RowLane rdl(lane);
-  const int gsub = P->gsub, tpt = P->tpt;
   const int lrow = lane >> 2, lch = (lane & 3) ^ swz4(lane >> 2);
   // DMA slot wv + 4 j of a tile: column group (wv + 4 j) / 2, rows 16 (wv % 2) ..
-  const int drow = 16 * (wv & 1) + lrow;       // the row this lane fetches
-  const int dtk = drow / gsub, dhc = drow - dtk * gsub;
-  const int ltk = col / gsub, lhc = col - ltk * gsub;  // the row whose LSE this lane fetches
+  const int drow = 16 * (wv & 1) + lrow;  // the row this lane fetches
   const uint32_t qxor = P->qa < 0.f ? 0x80008000u : 0u;
   const uint32_t qand = P->qa == 0.f ? 0u : 0xffffffffu;
   const float c2 = P->c2;
@@ -67,14 +69,14 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
     P = kargs();
     const PagedAt at = work.seek(P, lane, id);
     const PagedSeq e = at.s;
-    const int nkb = cdiv(e.lk, 128);
+    const int nkb = cdiv(e.lk, keys);
     const int kvh = uni((int)div64(at.rem, nkb));
-    const int kb = 128 * (int)(at.rem - (int64_t)kvh * nkb);
-    const int k0 = kb + 32 * wv, key = k0 + col, off = e.lk - e.lq;
+    const int kb = keys * (int)(at.rem - (int64_t)kvh * nkb);
+    const int k0 = kb + 32 * (wv & (kw - 1)), key = k0 + col, off = e.lk - e.lq;
     const bool causal = P->causal != 0;
     int page = -1, r = 0;
     if (key < e.lk && key < W.cap) {
-      const int pg = key / P->ps;
+      const int pg = page_of(P->ps_mul, P->ps_shift, key);
       page = P->table[(int64_t)at.b * P->tstride + pg];
       r = key - pg * P->ps;
       if ((uint32_t)page >= (uint32_t)P->npages) page = -1;
@@ -84,22 +86,20 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
     float* wp = W.w + (int64_t)at.b * W.w_sb + (int64_t)kvh * W.w_sh + key;
     const int64_t id64 = here ? page : 0;
 
-    // row tiles: token tile tt0 + n % ntt of subgroup n / ntt
-    const int tt0 = causal ? max(kb - off, 0) / tpt : 0;  // earlier tokens see none of the keys
-    const int ntt = cdiv(e.lq, tpt) - tt0, n = P->nsub * ntt;
-    const int hkv0 = kvh * P->group, group = P->group, HG = P->H_G;
+    // row tiles: tokens 32 tt .. of query head h of the KV head's
+    const int tt0 = causal ? max(kb - off, 0) / 32 : 0;  // earlier tokens see none of the keys
+    const int tt1 = cdiv(e.lq, 32), n = P->group * (tt1 - tt0);
+    const int hkv0 = kvh * P->group, HG = P->H_G;
     const int crr = P->R / 8;
-    const uint32_t qss = (uint32_t)P->q.ss * 2u, qsh = (uint32_t)P->q.sh * 2u;
-    const uint32_t rss = (uint32_t)P->rq.ss * 2u, rsh = (uint32_t)P->rq.sh * 2u;
+    const uint32_t qss = (uint32_t)P->q.ss * 2u, rss = (uint32_t)P->rq.ss * 2u;
     const uint8_t* const qbase = (const uint8_t*)P->q.ptr + (int64_t)e.q0 * P->q.ss * 2 + (int64_t)hkv0 * P->q.sh * 2;
     const uint8_t* const rbase = (const uint8_t*)P->rq.ptr + (int64_t)e.q0 * P->rq.ss * 2 + (int64_t)hkv0 * P->rq.sh * 2;
     const float* const lse = (const float*)P->lse.ptr + (int64_t)e.q0 * P->lse.ss + (int64_t)hkv0 * P->lse.sh;
-    const int64_t lss = P->lse.ss, lsh = P->lse.sh;
-    auto issue = [&](int sub, int tt, uint8_t* base) {
-      const int h0 = sub * gsub, t0 = tt * tpt;
-      const bool on = dtk < tpt && t0 + dtk < e.lq && h0 + dhc < group;
-      const uint32_t vo = on ? (uint32_t)dtk * qss + (uint32_t)dhc * qsh + 16u * lch : kOOB;
-      const auto rs = make_rsrc(qbase + (int64_t)t0 * qss + (int64_t)h0 * qsh, 0x7ffffff0u);
+    const int64_t qsh = P->q.sh * 2, rsh = P->rq.sh * 2, lss = P->lse.ss, lsh = P->lse.sh;
+    auto issue = [&](int h, int tt, uint8_t* base) {
+      const bool on = 32 * tt + drow < e.lq;
+      const uint32_t vo = on ? (uint32_t)drow * qss + 16u * lch : kOOB;
+      const auto rs = make_rsrc(qbase + (int64_t)(32 * tt) * qss + h * qsh, 0x7ffffff0u);
 #pragma unroll
       for (int j = 0; j < C::NQ; ++j) {
         const int slot = wv + 4 * j;
@@ -107,37 +107,42 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
                                                  vo + 64u * (slot >> 1), 0, 0, 0);
       }
       if constexpr (RC > 0) {
-        // (the row's own head's chunks only: R_q block diagonal)
-        const bool g = on && hkv0 + h0 + dhc < HG;
-        const auto rr = make_rsrc(HG > 0 ? rbase + (int64_t)t0 * rss + (int64_t)h0 * rsh : qbase, 0x7ffffff0u);
+        const bool g = on && hkv0 + h < HG;
+        const auto rr = make_rsrc(HG > 0 ? rbase + (int64_t)(32 * tt) * rss + h * rsh : qbase, 0x7ffffff0u);
 #pragma unroll
         for (int j = 0; j < C::NR; ++j) {
           const int slot = wv + 4 * j;
           if (C::RBYTES / 1024 % 4 == 0 || slot < C::RBYTES / 1024) {
-            const int c = 4 * (slot >> 1) + lch - dhc * crr;
+            const int c = 4 * (slot >> 1) + lch;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 rr, (lds_void*)(base + C::QBYTES + slot * 1024), 16,
-                g && c >= 0 && c < crr ? (uint32_t)dtk * rss + (uint32_t)dhc * rsh + 16u * c : kOOB, 0, 0, 0);
+                g && c < crr ? (uint32_t)drow * rss + 16u * c : kOOB, 0, 0, 0);
           }
         }
       }
     };
-    // a tile's LSE (of row `col`), by wave 0
-    auto fetch = [&](int sub, int tt) {
-      const int tok = tt * tpt + ltk, h = sub * gsub + lhc;
-      return ltk < tpt && tok < e.lq && h < group ? lse[(int64_t)tok * lss + (int64_t)h * lsh] : kNegInf;
-    };
-    auto put = [&](int tt, float l, float* nl, int* lim) {
-      if (hl == 0) {
-        nl[col] = l == kNegInf ? kNegInf : -l * kLog2e;
-        lim[col] = causal ? off + tt * tpt + ltk : e.lk;
+    // A stage's U tiles; wave u loads the LSE of the u-th, and put() stores it.
+    int fh = 0, ft = tt0, left = n;  // next tile to fetch; tiles not yet fetched
+    float lnext = kNegInf;
+    auto fill = [&](uint8_t* base) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u >= left) break;
+        issue(fh, ft, base + u * TILE);
+        if (wv == u) {
+          const int tok = 32 * ft + col;
+          lnext = tok < e.lq ? lse[(int64_t)tok * lss + fh * lsh] : kNegInf;
+        }
+        if (++ft == tt1) ft = tt0, ++fh;
       }
+      left -= U;
+    };
+    auto put = [&](float* nl) {
+      if (wv < U && hl == 0) nl[32 * wv + col] = lnext == kNegInf ? kNegInf : -lnext * kLog2e;
     };
 
     ring_barrier<0>();  // the ring's last tiles are read
-    issue(0, tt0, st0);
-    float lnext = 0.f;
-    if (wv == 0) lnext = fetch(0, tt0);
+    fill(st0);
     // K (B of S = Q K^T): lane holds K[key][16 s + 8 hl .. +7]
     bf16x8 kreg[C::KSD];
     {
@@ -151,7 +156,7 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
     }
     float old = 0.f;
     if (here && hl == 0) old = *wp;
-    if (wv == 0) put(tt0, lnext, nl0, lim0);
+    put(nl0);
 #pragma unroll
     for (int s = 0; s < C::KSD; ++s) {
       u32x4 w = as_u32x4(kreg[s]);
@@ -161,106 +166,104 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
     }
 
     bf16x8 rkreg[C::KSR > 0 ? C::KSR : 1];
-    float bh[16];
+    float bh = 0.f;
     float sum = 0.f;
-    int sub = 0, tt = tt0;  // of the tile at hand
-    auto step = [&](int t, const uint8_t* cur, const float* nl, const int* lim, uint8_t* nxt,
-                    float* nl_nxt, int* lim_nxt) {
+    int h = 0, tt = tt0, held = -1;  // the tile at hand; the head whose R_k is held
+    auto step = [&](int t, const uint8_t* cur, const float* nl, uint8_t* nxt, float* nl_nxt) {
       ring_barrier<0>();
-      const bool more = t + 1 < n;
-      const int sub1 = tt + 1 < tt0 + ntt ? sub : sub + 1, tt1 = sub1 == sub ? tt + 1 : tt0;
-      if (more) {
-        issue(sub1, tt1, nxt);
-        if (wv == 0) lnext = fetch(sub1, tt1);
-      }
+      const bool more = left > 0;
+      if (more) fill(nxt);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (RC > 0) {
-        if (tt == tt0) {  // a new subgroup: its R_k, and each row's graph scale
-          const int h0 = hkv0 + sub * gsub;
-          const uint16_t* rrow = (const uint16_t*)P->rk.ptr + id64 * P->rk.sb + (int64_t)h0 * P->rk.sh + (int64_t)r * P->rk.ss;
-          const int gg = min(max(min(HG - h0, group - sub * gsub), 0), gsub);
 #pragma unroll
-          for (int s = 0; s < C::KSR; ++s) {
-            const int c = 2 * s + hl, hh = gsub == 1 ? 0 : c / crr;
-            u32x4 w = {0, 0, 0, 0};
-            if (here && c < gg * crr) w = ld16(rrow + (int64_t)hh * P->rk.sh + 8 * (c - hh * crr));
-            rkreg[s] = as_bf16x8(w);
-          }
+      for (int u = 0; u < U; ++u) {
+        if (t + u < n && (kw == 4 || u == wv >> 1)) {
+          if constexpr (RC > 0) {
+            if (h != held) {
+              held = h;
+              bh = hkv0 + h < HG ? P->gs[hkv0 + h] / P->c : 0.f;
+              const uint16_t* rrow = (const uint16_t*)P->rk.ptr + id64 * P->rk.sb + (int64_t)(hkv0 + h) * P->rk.sh + (int64_t)r * P->rk.ss;
 #pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int row = 8 * (v >> 2) + 4 * hl + (v & 3), hc = gsub == 1 ? 0 : row % gsub;
-            bh[v] = hc < gg ? P->gs[h0 + hc] / P->c : 0.f;
-          }
-        }
-      }
-      if (any && (!causal || k0 <= off + tt * tpt + tpt - 1)) {
-        f32x16 acc = f32x16{};
-        if constexpr (RC > 0) {
-#pragma unroll
-          for (int s = 0; s < C::KSR; ++s)
-            acc = mfma32(row_read<32>(cur + C::QBYTES, rdl, 0, s), rkreg[s], acc);
-#pragma unroll
-          for (int v = 0; v < 16; ++v) acc[v] *= bh[v];
-        }
-#pragma unroll
-        for (int s = 0; s < C::KSD; ++s)
-          acc = mfma_e<F16>(row_read<32>(cur, rdl, 0, s), kreg[s], acc);
-        float part = 0.f;
-        if (causal && k0 + 31 > off + tt * tpt) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4_t a = *(const f32x4_t*)(nl + 8 * q + 4 * hl);
-            const u32x4 m = *(const u32x4*)(lim + 8 * q + 4 * hl);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * q + i], c2, a[i]));
-              part += key <= (int)m[i] && a[i] != kNegInf ? p : 0.f;
+              for (int s = 0; s < C::KSR; ++s) {
+                const int c = 2 * s + hl;
+                u32x4 w = {0, 0, 0, 0};
+                if (here && hkv0 + h < HG && c < crr) w = ld16(rrow + 8 * c);
+                rkreg[s] = as_bf16x8(w);
+              }
             }
           }
-        } else {
+          if (any && (!causal || k0 <= off + 32 * tt + 31)) {
+            f32x16 acc = f32x16{};
+            if constexpr (RC > 0) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4_t a = *(const f32x4_t*)(nl + 8 * q + 4 * hl);
+              for (int s = 0; s < C::KSR; ++s)
+                acc = mfma32(row_read<32>(cur + u * TILE + C::QBYTES, rdl, 0, s), rkreg[s], acc);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              part += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * q + i], c2, a[i]));
+              for (int v = 0; v < 16; ++v) acc[v] *= bh;
+            }
+#pragma unroll
+            for (int s = 0; s < C::KSD; ++s)
+              acc = mfma_e<F16>(row_read<32>(cur + u * TILE, rdl, 0, s), kreg[s], acc);
+            float part = 0.f;
+            if (causal && k0 + 31 > off + 32 * tt) {
+              const int first = key - off - 32 * tt;  // the first row that sees the key
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const f32x4_t a = *(const f32x4_t*)(nl + 32 * u + 8 * q + 4 * hl);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * q + i], c2, a[i]));
+                  part += 8 * q + 4 * hl + i >= first && a[i] != kNegInf ? p : 0.f;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const f32x4_t a = *(const f32x4_t*)(nl + 32 * u + 8 * q + 4 * hl);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  part += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[4 * q + i], c2, a[i]));
+              }
+            }
+            sum += part;
           }
         }
-        sum += part;
+        if (++tt == tt1) tt = tt0, ++h;
       }
-      if (more && wv == 0) put(tt1, lnext, nl_nxt, lim_nxt);
-      sub = sub1;
-      tt = tt1;
+      if (more) put(nl_nxt);
     };
-    for (int t = 0; t < n; t += 2) {
-      step(t, st0, nl0, lim0, st1, nl1, lim1);
-      if (t + 1 < n) step(t + 1, st1, nl1, lim1, st0, nl0, lim0);
+    for (int t = 0; t < n; t += 2 * U) {
+      step(t, st0, nl0, st1, nl1);
+      if (t + U < n) step(t + U, st1, nl1, st0, nl0);
     }
     sum = wave_pair_sum(sum);
+    if (kw == 2) {
+      // (the next block's first barrier lies between these reads and its writes)
+      if (wv >= 2 && hl == 0) half[32 * (wv & 1) + col] = sum;
+      __syncthreads();
+      if (wv >= 2) continue;
+      sum += half[32 * wv + col];
+    }
     if (here && hl == 0) *wp = old + sum;
   }
 }
 
-// Workgroups of a CU, by the registers that R_k takes.
-constexpr int weigh_occ(int rc) { return rc == 0 ? 4 : rc <= 16 ? 3 : 2; }
+// Workgroups of a CU, by the registers that K and R_k take.  (Four at d = 128, R =
+// 32 spill: 31 us become 36.)
+constexpr int weigh_occ(int D, int rc) { return rc == 0 || (D == 64 && rc <= 4) ? 4 : 3; }
 
 #define FNA2_WEIGH(D, RC)                                                                           \
-  __global__ __launch_bounds__(256, weigh_occ(RC)) void paged_weigh_d##D##_c##RC(const PagedWeightsParams W) {  \
+  __global__ __launch_bounds__(256, weigh_occ(D, RC)) void paged_weigh_d##D##_c##RC(const PagedWeightsParams W) {  \
     weigh_body<D, RC, false>(W);                                                                    \
   }                                                                                                 \
-  __global__ __launch_bounds__(256, weigh_occ(RC)) void paged_weigh_d##D##_c##RC##_f16(const PagedWeightsParams W) { \
+  __global__ __launch_bounds__(256, weigh_occ(D, RC)) void paged_weigh_d##D##_c##RC##_f16(const PagedWeightsParams W) { \
     weigh_body<D, RC, true>(W);                                                                     \
   }
 FNA2_WEIGH(64, 0)
 FNA2_WEIGH(64, 4)
 FNA2_WEIGH(64, 8)
-FNA2_WEIGH(64, 16)
-FNA2_WEIGH(64, 32)
 FNA2_WEIGH(128, 0)
 FNA2_WEIGH(128, 4)
 FNA2_WEIGH(128, 8)
-FNA2_WEIGH(128, 16)
-FNA2_WEIGH(128, 32)
 #undef FNA2_WEIGH
 
 
@@ -483,18 +486,16 @@ FNA2_GLANCE(128, 32)
 
 }  // namespace
 
-int paged_weigh_per_cu(int rc) { return weigh_occ(rc); }
+int paged_weigh_per_cu(int D, int rc) { return weigh_occ(D, rc); }
 
 hipError_t launch_paged_weights(const PagedWeightsParams& W, int rc, hipStream_t s) {
   const PagedParams& P = W.p;
   void (*k)(const PagedWeightsParams) = nullptr;
 #define FNA2_WEIGH_OF(D, RC) (P.f16 ? paged_weigh_d##D##_c##RC##_f16 : paged_weigh_d##D##_c##RC)
   if (P.D == 64)
-    k = rc == 0 ? FNA2_WEIGH_OF(64, 0) : rc == 4 ? FNA2_WEIGH_OF(64, 4) : rc == 8 ? FNA2_WEIGH_OF(64, 8)
-      : rc == 16 ? FNA2_WEIGH_OF(64, 16) : rc == 32 ? FNA2_WEIGH_OF(64, 32) : nullptr;
+    k = rc == 0 ? FNA2_WEIGH_OF(64, 0) : rc == 4 ? FNA2_WEIGH_OF(64, 4) : rc == 8 ? FNA2_WEIGH_OF(64, 8) : nullptr;
   if (P.D == 128)
-    k = rc == 0 ? FNA2_WEIGH_OF(128, 0) : rc == 4 ? FNA2_WEIGH_OF(128, 4) : rc == 8 ? FNA2_WEIGH_OF(128, 8)
-      : rc == 16 ? FNA2_WEIGH_OF(128, 16) : rc == 32 ? FNA2_WEIGH_OF(128, 32) : nullptr;
+    k = rc == 0 ? FNA2_WEIGH_OF(128, 0) : rc == 4 ? FNA2_WEIGH_OF(128, 4) : rc == 8 ? FNA2_WEIGH_OF(128, 8) : nullptr;
 #undef FNA2_WEIGH_OF
   if (!k) return hipErrorInvalidValue;
   hipLaunchKernelGGL(k, dim3((uint32_t)W.grid), dim3(256), 0, s, W);

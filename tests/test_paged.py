@@ -500,6 +500,15 @@ def test_weights_past_garbage(gpu, lq, H, HKV, HG, R):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,R", [(64, 0), (64, 16), (128, 64), (128, 40)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_weights_under_a_wide_table(gpu, causal, D, R):
+    """Tables that hold thousands of rows: larger blocks of keys."""
+    check_attend(Case([40, 133], [300, 400], 8, 4, 7 if R else 0, D, R, 256, device=gpu, width=70),
+                 causal=causal)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lq", [[1, 1], [40, 9]])
 def test_infinite_values_stay_infinite(gpu, lq):
     c = Case(lq, [75, 61], 4, 2, 0, 64, 0, 16, device=gpu)
