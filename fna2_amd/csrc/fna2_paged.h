@@ -283,6 +283,7 @@ struct PagedEvictParams {
   float* w_out;
   int* kept;
   int* new_lens;
+  int strip;  // (set by the launch)
 };
 hipError_t launch_paged_select(const PagedEvictParams& P, hipStream_t s);
 hipError_t launch_paged_compact(const PagedEvictParams& P, hipStream_t s);

@@ -334,18 +334,21 @@ __global__ __launch_bounds__(kSelThreads) void paged_select_kernel(const PagedEv
 }
 
 // Compaction in place: row kept[r] becomes row r (kept[r] >= r, increasing).
-// A workgroup takes one strip of 64 bytes of the rows of one (sequence, head) of
-// K, V or R_k, in rounds of some hundred rows: all of a round's loads, a barrier,
-// all of its stores.  Rows stored so lie before every row that is still to be
-// loaded, so no other copy is needed.  A round's chain (kept row, its page, the row)
-// is as long as for a few rows, so rounds are as large as the registers
-// allow: 16 waves of 8 loads of 16 rows, 128 KB in flight, and the next
-// round's rows and pages are looked up while this one's are under way.
+// A workgroup takes one strip (128 bytes, or less) of the rows of one (sequence,
+// head) of K, V or R_k, in rounds of some hundred rows: all of a round's loads, a
+// barrier, all of its stores.  Rows stored so lie before every row that is still to
+// be loaded, so no other copy is needed.  A round's chain (kept row, its page, the
+// row) is as long as for a few rows, so rounds are as large as the registers allow:
+// 16 waves of 4 loads of 8 rows, 64 KB in flight, and the next round's rows
+// and pages are looked up while this one's are under way.  32 sequences of up to
+// 8192 rows to 4096 (8 KV heads of 128, 32 of R_k's 32): 284 us, 4.1 TB/s.  Where few
+// strips leave CUs without one they are narrower, and the rounds fewer (2 sequences
+// of 1201 rows to 1000, 4 KV heads of 64: 10.6 us become 8.0).
 constexpr int kCompactThreads = 1024, kCompactAhead = 4;
-constexpr int kStrip = 8;  // 16-byte chunks of a strip, at most
 __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const PagedEvictParams E) {
   const PagedParams& P = E.p;
-  const int kstrips = P.D / (8 * kStrip), rstrips = P.H_G > 0 ? cdiv(P.R, 8 * kStrip) : 0;
+  const int width = E.strip;  // 16-byte chunks of a strip, at most
+  const int kstrips = P.D / (8 * width), rstrips = P.H_G > 0 ? cdiv(P.R, 8 * width) : 0;
   const int per = 2 * P.H_KV * kstrips + P.H_G * rstrips;  // strips of a sequence
   const int b = blockIdx.x / per;
   int x = blockIdx.x - b * per;
@@ -359,13 +362,13 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
     x -= which * nk;
     h = kvh = x / kstrips;
     strip = x - h * kstrips;
-    chunks = kStrip;
+    chunks = width;
   } else {
     x -= 2 * nk;
     h = x / rstrips;
     kvh = h / P.group;
     strip = x - h * rstrips;
-    chunks = min(P.R / 8 - kStrip * strip, kStrip);
+    chunks = min(P.R / 8 - width * strip, width);
   }
   const TView& t = which == 0 ? P.k : which == 1 ? P.v : P.rk;
   const int64_t sb = t.sb, ss = t.ss;
@@ -376,7 +379,7 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
   const int lanes = chunks > 8 ? 16 : chunks > 4 ? 8 : chunks > 2 ? 4 : chunks;
   const int c = threadIdx.x & (lanes - 1), row0 = threadIdx.x / lanes, stride = blockDim.x / lanes;
   const int round = stride * kCompactAhead;
-  uint16_t* base = (uint16_t*)t.ptr + (int64_t)h * t.sh + 8 * (kStrip * strip + c);
+  uint16_t* base = (uint16_t*)t.ptr + (int64_t)h * t.sh + 8 * (width * strip + c);
   auto place = [&](int j) -> uint16_t* {
     const int pg = j / ps;
     const int id = trow[pg];
@@ -450,13 +453,19 @@ hipError_t launch_paged_select(const PagedEvictParams& E, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_paged_compact(const PagedEvictParams& E, hipStream_t s) {
+hipError_t launch_paged_compact(const PagedEvictParams& E_, hipStream_t s) {
+  PagedEvictParams E = E_;
   const PagedParams& P = E.p;
-  const int64_t per = 2 * (int64_t)P.H_KV * (P.D / (8 * kStrip)) +
-                      (P.H_G > 0 ? (int64_t)P.H_G * cdiv(P.R, 8 * kStrip) : 0);
-  // (a small budget is one round of fewer waves: 8 lanes a row, kCompactAhead rows each)
-  const int threads = std::min(kCompactThreads, std::max(64, cdiv(2 * std::min(E.budget, 1 << 20), 64) * 64));
-  hipLaunchKernelGGL(paged_compact_kernel, dim3((uint32_t)(per * P.N)), dim3((uint32_t)threads), 0, s, E);
+  auto strips = [&] {
+    return 2 * (int64_t)P.H_KV * (P.D / (8 * E.strip)) + (P.H_G > 0 ? (int64_t)P.H_G * cdiv(P.R, 8 * E.strip) : 0);
+  };
+  E.strip = 8;
+  while (E.strip > 2 && 2 * strips() * P.N <= 512 && E.budget > kCompactAhead * kCompactThreads / E.strip)
+    E.strip /= 2;
+  // (a small budget is one round of fewer waves)
+  const int rows = cdiv(std::min(E.budget, 1 << 20), kCompactAhead);
+  const int threads = std::min(kCompactThreads, cdiv(rows * E.strip, 64) * 64);
+  hipLaunchKernelGGL(paged_compact_kernel, dim3((uint32_t)(strips() * P.N)), dim3((uint32_t)threads), 0, s, E);
   return hipGetLastError();
 }
 
