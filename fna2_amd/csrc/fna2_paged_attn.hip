@@ -23,8 +23,14 @@
 // Pages.  A step's rows come as two groups of 16, each within one page
 // (page_size is a multiple of 16), DMA'd to LDS through descriptors of their
 // own that end with the sequence: what lies behind its last row, or in a
-// page that is not there, is never read and comes as zeros.  The page ids
-// are read a step ahead.
+// page that is not there, is never read and comes as zeros.  64 page ids at a time
+// lie in the lanes of a register.
+//
+// Bound by reading K, V and R_k once: 64 sequences of 4096 rows, one token each, 16
+// heads over 16 KV heads of 128, R = 32, 410 us, 5.9 TB/s (a large copy, read and written, 5.1 TB/s).
+// Few sequences are bound by the latency of the chain lengths, page ids, first
+// rows, parts, merge: 2 of 500 rows, 8 heads of 64, 7.5 us and 4.5 us for the merge.
+// A ring of three stages gained nothing over two: the other waves cover the loads.
 #include <algorithm>
 
 #include "fna2_kernels.h"
@@ -403,121 +409,121 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams) {
   uint64_t todo = __builtin_amdgcn_ballot_w64(
       (int)(threadIdx.x & 63) < mr && r0 < P->waves && P->cuts[min(r0, P->waves - 1)].parts > 0);
   while (todo) {
-  const int i0 = blockIdx.x * mr + uni(__builtin_ctzll(todo));
-  todo &= todo - 1;
-  const auto rec = const_space(P->cuts + i0);
-  const int n = uni(rec->parts);
-  const int ct = uni(rec->tile), sg = uni(rec->head);
-  const PagedSeq e = paged_seq_uniform(P, rec->b);
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int kvh = sg / P->nsub, h_in = (sg - kvh * P->nsub) * P->gsub;
-  const int nh = min(P->gsub, P->group - h_in), h0 = kvh * P->group + h_in;
-  const int cols = P->gsub * P->tpt;
-  const int grp = threadIdx.x / LPR, f = 4 * (threadIdx.x % LPR);
-  const float c2 = P->c2;
-  auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * i0 + 1 : 2 * (i0 + j)); };
-  if (n <= LPR && (int)gridDim.y < cols) {
-    const int c = blockIdx.y + gridDim.y * grp;  // (gridDim.y * NG >= cols)
-    const int l = threadIdx.x % LPR;
-    const int tk = c / P->gsub, hc = c - tk * P->gsub, tok = ct * P->tpt + tk;
-    const bool on = c < cols && tok < e.lq && hc < nh;
-    f32x2 ml = {kNegInf, 0.f};
-    if (on && l < n) ml = *(const f32x2*)(P->ml + 2 * (slot(l) * cols + c));
-    const float* src = P->part + (int64_t)(on ? c : 0) * D + f;
-    float m = ml[0];
+    const int i0 = blockIdx.x * mr + uni(__builtin_ctzll(todo));
+    todo &= todo - 1;
+    const auto rec = const_space(P->cuts + i0);
+    const int n = uni(rec->parts);
+    const int ct = uni(rec->tile), sg = uni(rec->head);
+    const PagedSeq e = paged_seq_uniform(P, rec->b);
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int kvh = sg / P->nsub, h_in = (sg - kvh * P->nsub) * P->gsub;
+    const int nh = min(P->gsub, P->group - h_in), h0 = kvh * P->group + h_in;
+    const int cols = P->gsub * P->tpt;
+    const int grp = threadIdx.x / LPR, f = 4 * (threadIdx.x % LPR);
+    const float c2 = P->c2;
+    auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * i0 + 1 : 2 * (i0 + j)); };
+    if (n <= LPR && (int)gridDim.y < cols) {
+      const int c = blockIdx.y + gridDim.y * grp;  // (gridDim.y * NG >= cols)
+      const int l = threadIdx.x % LPR;
+      const int tk = c / P->gsub, hc = c - tk * P->gsub, tok = ct * P->tpt + tk;
+      const bool on = c < cols && tok < e.lq && hc < nh;
+      f32x2 ml = {kNegInf, 0.f};
+      if (on && l < n) ml = *(const f32x2*)(P->ml + 2 * (slot(l) * cols + c));
+      const float* src = P->part + (int64_t)(on ? c : 0) * D + f;
+      float m = ml[0];
 #pragma unroll
-    for (int k = LPR / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-    const float ref = m == kNegInf ? 0.f : m;
-    const float w = weight2((ml[0] - ref) * c2);
-    float sum = ml[1] * w;
+      for (int k = LPR / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+      const float ref = m == kNegInf ? 0.f : m;
+      const float w = weight2((ml[0] - ref) * c2);
+      float sum = ml[1] * w;
 #pragma unroll
-    for (int k = LPR / 2; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int j0 = 0; j0 < n; j0 += 4) {
+      for (int k = LPR / 2; k > 0; k >>= 1) sum += __shfl_xor(sum, k);
+      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+      for (int j0 = 0; j0 < n; j0 += 4) {
+        f32x4_t x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          if (on && j0 + k < n) x[k] = *(const f32x4_t*)(src + slot(j0 + k) * cols * D);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float wj = __shfl(w, min(j0 + k, n - 1), LPR);
+          if (j0 + k < n) o += wj * x[k];
+        }
+      }
+      if (!on) continue;
+      const float inv = 1.f / (sum + 1e-6f);
+      uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)(h0 + hc) * P->o.sh;
+      u32x2 val;
+      val[0] = pack_e<F16>(o[0] * inv, o[1] * inv);
+      val[1] = pack_e<F16>(o[2] * inv, o[3] * inv);
+      *(u32x2*)(orow + f) = val;
+      if (l == 0 && P->lse.ptr)
+        ((float*)P->lse.ptr)[(int64_t)(e.q0 + tok) * P->lse.ss + (int64_t)(h0 + hc) * P->lse.sh] =
+            m == kNegInf ? kNegInf : m * P->c + __builtin_amdgcn_logf(sum + 1e-6f) * kLn2;
+      continue;
+    }
+    for (int c = blockIdx.y; c < cols; c += gridDim.y) {
+      const int tk = c / P->gsub, hc = c - tk * P->gsub, tok = ct * P->tpt + tk;
+      if (tok >= e.lq || hc >= nh) continue;  // (uniform)
+      const float* src = P->part + (int64_t)c * D + f;
       f32x4_t x[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        x[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        if (on && j0 + k < n) x[k] = *(const f32x4_t*)(src + slot(j0 + k) * cols * D);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float wj = __shfl(w, min(j0 + k, n - 1), LPR);
-        if (j0 + k < n) o += wj * x[k];
-      }
-    }
-    if (!on) continue;
-    const float inv = 1.f / (sum + 1e-6f);
-    uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)(h0 + hc) * P->o.sh;
-    u32x2 val;
-    val[0] = pack_e<F16>(o[0] * inv, o[1] * inv);
-    val[1] = pack_e<F16>(o[2] * inv, o[3] * inv);
-    *(u32x2*)(orow + f) = val;
-    if (l == 0 && P->lse.ptr)
-      ((float*)P->lse.ptr)[(int64_t)(e.q0 + tok) * P->lse.ss + (int64_t)(h0 + hc) * P->lse.sh] =
-          m == kNegInf ? kNegInf : m * P->c + __builtin_amdgcn_logf(sum + 1e-6f) * kLn2;
-    continue;
-  }
-  for (int c = blockIdx.y; c < cols; c += gridDim.y) {
-    const int tk = c / P->gsub, hc = c - tk * P->gsub, tok = ct * P->tpt + tk;
-    if (tok >= e.lq || hc >= nh) continue;  // (uniform)
-    const float* src = P->part + (int64_t)c * D + f;
-    f32x4_t x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int j = grp + k * NG;
-      if (j < n) x[k] = *(const f32x4_t*)(src + slot(j) * cols * D);
-    }
-    float m = kNegInf;
-    for (int j = threadIdx.x; j < n; j += 256) m = fmaxf(m, P->ml[2 * (slot(j) * cols + c)]);
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-    if (lane == 0) red[wv] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float ref = m == kNegInf ? 0.f : m;
-    float l = 0.f;
-    for (int j = threadIdx.x; j < n; j += 256) {
-      const f32x2 ml = *(const f32x2*)(P->ml + 2 * (slot(j) * cols + c));
-      const float w = weight2((ml[0] - ref) * c2);
-      wt[j] = w;
-      l += ml[1] * w;
-    }
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) l += __shfl_xor(l, k);
-    if (lane == 0) red2[wv] = l;
-    __syncthreads();
-    l = (red2[0] + red2[1]) + (red2[2] + red2[3]);
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int base = 0; base < n; base += 4 * NG) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int j = base + grp + k * NG;
-        if (j < n) o += wt[j] * x[k];
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int j = base + grp + (4 + k) * NG;
+        const int j = grp + k * NG;
         if (j < n) x[k] = *(const f32x4_t*)(src + slot(j) * cols * D);
       }
-    }
-    *(f32x4_t*)(&part[grp][f]) = o;
-    __syncthreads();
-    const float inv = 1.f / (l + 1e-6f);
-    if (threadIdx.x < D / 2) {
-      const int d = 2 * threadIdx.x;
-      float y0 = 0.f, y1 = 0.f;
+      float m = kNegInf;
+      for (int j = threadIdx.x; j < n; j += 256) m = fmaxf(m, P->ml[2 * (slot(j) * cols + c)]);
 #pragma unroll
-      for (int g = 0; g < NG; ++g) y0 += part[g][d], y1 += part[g][d + 1];
-      uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)(h0 + hc) * P->o.sh;
-      *(uint32_t*)(orow + d) = pack_e<F16>(y0 * inv, y1 * inv);
-      if (d == 0 && P->lse.ptr)
-        ((float*)P->lse.ptr)[(int64_t)(e.q0 + tok) * P->lse.ss + (int64_t)(h0 + hc) * P->lse.sh] =
-            m == kNegInf ? kNegInf : m * P->c + __builtin_amdgcn_logf(l + 1e-6f) * kLn2;
+      for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+      if (lane == 0) red[wv] = m;
+      __syncthreads();
+      m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+      const float ref = m == kNegInf ? 0.f : m;
+      float l = 0.f;
+      for (int j = threadIdx.x; j < n; j += 256) {
+        const f32x2 ml = *(const f32x2*)(P->ml + 2 * (slot(j) * cols + c));
+        const float w = weight2((ml[0] - ref) * c2);
+        wt[j] = w;
+        l += ml[1] * w;
+      }
+#pragma unroll
+      for (int k = 32; k > 0; k >>= 1) l += __shfl_xor(l, k);
+      if (lane == 0) red2[wv] = l;
+      __syncthreads();
+      l = (red2[0] + red2[1]) + (red2[2] + red2[3]);
+      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+      for (int base = 0; base < n; base += 4 * NG) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = base + grp + k * NG;
+          if (j < n) o += wt[j] * x[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = base + grp + (4 + k) * NG;
+          if (j < n) x[k] = *(const f32x4_t*)(src + slot(j) * cols * D);
+        }
+      }
+      *(f32x4_t*)(&part[grp][f]) = o;
+      __syncthreads();
+      const float inv = 1.f / (l + 1e-6f);
+      if (threadIdx.x < D / 2) {
+        const int d = 2 * threadIdx.x;
+        float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) y0 += part[g][d], y1 += part[g][d + 1];
+        uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)(e.q0 + tok) * P->o.ss + (int64_t)(h0 + hc) * P->o.sh;
+        *(uint32_t*)(orow + d) = pack_e<F16>(y0 * inv, y1 * inv);
+        if (d == 0 && P->lse.ptr)
+          ((float*)P->lse.ptr)[(int64_t)(e.q0 + tok) * P->lse.ss + (int64_t)(h0 + hc) * P->lse.sh] =
+              m == kNegInf ? kNegInf : m * P->c + __builtin_amdgcn_logf(l + 1e-6f) * kLn2;
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
-  }  // (the next tile)
 }
 
 // Waves per SIMD that the register budget is cut for.  Two (256 registers): the
