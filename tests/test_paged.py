@@ -897,6 +897,54 @@ def test_serving_steps_with_eviction(gpu, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lq", [[1, 1], [3, 0], [40, 3]])
+def test_caches_without_rows(gpu, lq):
+    """Lengths of zero, tables of no width, pools of no page: outputs 0, LSE
+    -inf, weights and pools as they were."""
+    def nothing(c):
+        acc = torch.rand(2, 2, 48, device=gpu)
+        before = acc.clone()
+        out, lse = c.attend(return_lse=True, key_weights=acc)
+        assert (out == 0).all() and (lse == -math.inf).all() and torch.equal(acc, before)
+        k = c.k.clone()
+        q = paged.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, c.rkn, c.rk)
+        assert torch.equal(q, c.q) and torch.equal(c.k, k)
+        kept, lens, w = paged.paged_evict(c.k, c.v, c.table, c.lens, acc, 4, 1, 1, c.rk, 4)
+        assert torch.equal(c.k, k) and kept.shape == (2, 2, 4) and w.shape == acc.shape
+        return lens
+
+    make = lambda: Case(lq, [0, 0], 4, 2, 3, 64, 8, 16, device=gpu)
+    assert (nothing(make()) == 0).all()
+    c = make()
+    c.lens += 60
+    c.table = c.table[:, :0]
+    assert (nothing(c) == 0).all()
+    c = make()
+    c.lens += 20
+    c.k, c.v, c.rk = c.k[:0], c.v[:0], c.rk[:0]
+    assert (nothing(c) == 4).all()
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(gpu):
+    """Calls on two streams: each has a workspace of its own."""
+    a = Case([1, 1], [3000, 900], 4, 2, 3, 64, 16, 16, device=gpu, seed=1)
+    b = Case([90, 2], [2000, 700], 4, 2, 3, 64, 16, 16, device=gpu, seed=2)
+    want = [x.attend(return_lse=True) for x in (a, b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for i, (x, s) in enumerate(zip((a, b), streams)):
+            with torch.cuda.stream(s):
+                got[i].append(x.attend(return_lse=True))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w[0], o) and torch.equal(w[1], l) for o, l in g)
+
+
+@pytest.mark.gpu
 def test_other_streams_and_graphs(gpu):
     """A step on a stream of its own, captured into a graph and replayed on
     new inputs and lengths, with eager work between the replays."""
