@@ -225,6 +225,8 @@ class PagedAttnArgs(ctypes.Structure):
         ("lse", Tensor),
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
+        ("scores", ctypes.c_void_p),
+        ("scores_bytes", ctypes.c_size_t),
     ]
 
 
@@ -292,6 +294,7 @@ SIGNATURES = {
     "fna2_decode_rows": (ctypes.c_int, [ctypes.POINTER(DecodeRowsArgs), ctypes.c_void_p]),
     "fna2_check_paged_attn": (ctypes.c_int, [ctypes.POINTER(PagedAttnArgs)]),
     "fna2_paged_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
+    "fna2_paged_scores_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
     "fna2_paged_attn": (ctypes.c_int, [ctypes.POINTER(PagedAttnArgs), ctypes.c_void_p]),
     "fna2_check_paged_weights": (ctypes.c_int, [ctypes.POINTER(PagedWeightsArgs)]),
     "fna2_paged_weights": (ctypes.c_int, [ctypes.POINTER(PagedWeightsArgs), ctypes.c_void_p]),

@@ -1447,6 +1447,26 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
   return k;
 }
 
+// Scores that the packed kernel leaves for the weights, 4 bytes a row and column,
+// written and read: where that is at most a quarter of the rows' K and R_k, which
+// the weights' kernel reads otherwise, and fits 512 MB.  (us, attention and weights,
+// from K and from the scores, one token each: 16 sequences of up to 8192 rows, 4 heads
+// a KV head of 128, 109, 98; 45 of 10730, 1 of 64, R = 8, 336, 259.  4 tokens of 2
+// heads, 16 of 4000, R = 32, 116, 103: a column more costs 1.4 there, and K 23.)
+size_t paged_scores(const fna2_paged_cache& c, const PagedPlan& k) {
+  const int64_t cols = (int64_t)k.nsub * k.gsub * k.tpt;
+  const int64_t rows = cdiv64(cached_rows(c), 32) * 32;
+  const int64_t row = 2 * (c.head_dim + (int64_t)c.heads_graph * c.rank / c.heads_kv);
+  if (k.tile || 32 * cols > row) return 0;
+  const double bytes = 4. * cols * (double)rows * c.heads_kv * c.batch;
+  return bytes <= 512. * 1048576. ? (size_t)bytes : 0;
+}
+void fill_scores(fna2::PagedParams& K, const fna2_paged_attn_args& a, const PagedPlan& k) {
+  if (!a.scores || paged_scores(a.c, k) == 0) return;
+  K.scores = (float*)a.scores;
+  K.srows = (int)(cdiv64(cached_rows(a.c), 32) * 32);
+}
+
 int check_paged_attn_common(const fna2_paged_attn_args& a) {
   FNA2_TRY(check_paged_cache(a.c, true));
   if (!std::isfinite(a.softmax_scale)) return FNA2_E_SCALE;
@@ -1462,6 +1482,8 @@ int check_paged_attn_common(const fna2_paged_attn_args& a) {
   }
   if (a.lse.ptr && (!aligned(a.lse.ptr, 4) || a.lse.stride_s < 0 || a.lse.stride_h < 0))
     return FNA2_E_STRIDE;
+  if (a.scores && (!aligned(a.scores, 16) || a.scores_bytes < paged_scores(a.c, paged_plan(a.c))))
+    return FNA2_E_WORKSPACE;
   return FNA2_OK;
 }
 
@@ -1497,6 +1519,11 @@ size_t fna2_paged_attn_workspace_bytes(const fna2_paged_attn_args* a) {
   return paged_plan(a->c).bytes;
 }
 
+size_t fna2_paged_scores_bytes(const fna2_paged_attn_args* a) {
+  if (fna2_check_paged_attn(a) != FNA2_OK || a->c.total_q == 0) return 0;
+  return paged_scores(a->c, paged_plan(a->c));
+}
+
 int fna2_paged_attn(const fna2_paged_attn_args* a, void* stream_ptr) {
   FNA2_TRY(fna2_check_paged_attn(a));
   if (a->c.total_q == 0) return FNA2_OK;
@@ -1522,6 +1549,7 @@ int fna2_paged_attn(const fna2_paged_attn_args* a, void* stream_ptr) {
     const int rpl = fna2::padded_rank32(K.H_G, K.R);
     return fna2::launch_paged_tile(K, rpl, stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
   }
+  fill_scores(K, *a, k);
   if (fna2::launch_paged_packed(K, k.rc, stream) != hipSuccess) return FNA2_E_LAUNCH;
   if (fna2::launch_paged_merge(K, stream) != hipSuccess) return FNA2_E_LAUNCH;
   return FNA2_OK;
@@ -1559,6 +1587,7 @@ int fna2_paged_weights(const fna2_paged_weights_args* w, void* stream) {
   const PagedPlan k = paged_plan(c);
   const int64_t rows = std::max<int64_t>(cached_rows(c), 1), heads = (int64_t)c.batch * c.heads_kv;
   if (!k.tile) {  // row tiles as the packed kernel's columns
+    fill_scores(K.p, w->attn, k);
     K.p.gsub = k.gsub;
     K.p.nsub = k.nsub;
     K.p.tpt = k.tpt;

@@ -41,6 +41,10 @@ struct PagedParams {
   int merge_by_part;  // ... with a workgroup for every column
   float* part;    // [2 * waves] slots of unnormalised numerators of split tiles
   float* ml;      // [2 * waves][columns of a tile] (max, sum)
+  // Scores that the packed kernel leaves for the weights: [N][H_KV * nsub][columns
+  // of a tile][srows], of the sequences whose chunk one tile holds; or null.
+  float* scores;
+  int srows;  // rows of the table, rounded up to 32
 };
 
 // The kernels read their parameters where the launch put them, through a
@@ -53,6 +57,11 @@ __device__ __forceinline__ KArg kargs() {
   KArg p = (KArg)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
   return p;
+}
+
+// The scores of group `sg` (kvh * nsub + sub) of sequence b.
+__device__ __forceinline__ float* paged_scores(KArg P, int b, int sg) {
+  return P->scores + ((int64_t)b * (P->H_KV * P->nsub) + sg) * (P->gsub * P->tpt) * P->srows;
 }
 
 // A sequence's tokens and rows, clamped so that no access leaves [0, T) or

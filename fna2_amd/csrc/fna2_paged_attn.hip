@@ -236,13 +236,21 @@ __device__ __forceinline__ void packed_body() {
       }
     }
 
+    // Scores kept for the rows' weights.
+    const bool keep = P->scores && e.lq <= P->tpt;
+    float* const srow = keep ? paged_scores(P, b, sg) + (int64_t)min(col, cols - 1) * P->srows + 4 * hl : nullptr;
+    bool stored = false;  // the newest four memory instructions are a step's scores
+
     f32x16 oacc[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) oacc[d] = f32x16{};
     float m_i = kNegInf, l_i = 0.f;
 
     auto step = [&](int t, uint8_t* cur_st, uint8_t* nxt_st) {
-      paged_wait<0>();
+      // (loads and stores end in order: those before the scores have)
+      if (stored) paged_wait<4>();
+      else paged_wait<0>();
+      stored = false;
       const int gone_now = gone;
       gone = issue(t + 1, nxt_st);  // (past the run: zeros, from no memory)
       __builtin_amdgcn_sched_barrier(0);
@@ -276,6 +284,14 @@ __device__ __forceinline__ void packed_body() {
           const bool dead = key > lim || ((gone_now >> (v >> 3)) & 1);
           acc[v] = dead ? kNegInf : acc[v];
         }
+      }
+      if (keep) {
+        if (col < cols) {  // (column 0 always is: four stores)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *(f32x4_t*)(srow + kbase + 8 * g) = f32x4_t{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+        }
+        stored = true;
       }
       float mx = kNegInf;
 #pragma unroll

@@ -21,9 +21,10 @@
 // tile holds the chunk, so a wave keeps that in registers instead and streams
 // keys, 32 at a time in a run of its own, the next ones' K and R_k on their way
 // while it works on these.  Bound by reading K (and R_k) once: one token
-// of each of 16 sequences of up to 8192 rows, 8 KV heads of 128, 32.6 us.  (With row
-// tiles through LDS 38 us; 45 sequences of up to 10730, 8 heads of 64, with the attention
-// 484 us, now 331.)
+// of each of 16 sequences of up to 8192 rows, 8 KV heads of 128, 32.6 us (with row
+// tiles through LDS 38 us).  Where the attention left its scores, a few columns of
+// them, the wave sums over those instead and reads no K: 10.3 us, and 12 us more in
+// the attention.
 #include <algorithm>
 
 #include "fna2_kernels.h"
@@ -310,141 +311,178 @@ __device__ __forceinline__ void glance_body(const PagedWeightsParams& W) {
     const uint16_t* const rpool = (const uint16_t*)P->rk.ptr;
     const int64_t ksb = P->k.sb, kss = P->k.ss, rsb = P->rk.sb, rss = P->rk.ss, rsh = P->rk.sh;
 
-    // Row tile i: Q (A of S = Q K^T), and for the rows of this lane's registers
-    // -LSE log2(e) and graph scale.
-    bf16x8 qreg[KSD + KSR];
-    float nl[16], bh[KSR > 0 ? 16 : 1];
-    int h0 = h00, gg = 0, lim0 = 0;
-    auto rows = [&](int i) {
-      const int sub = nsub == 1 ? 0 : i / nct, t0 = (i - sub * nct) * tpt;
-      h0 = h00 + sub * gsub;
-      gg = KSR > 0 ? min(max(min(HG - h0, group - sub * gsub), 0), gsub) : 0;
-      lim0 = off + t0;
-      const bool on = tk < tpt && t0 + tk < e.lq && hc < min(gsub, group - sub * gsub);
-      const int64_t t = e.q0 + (on ? t0 + tk : 0);
-      const int h = h0 + (on ? hc : 0);
-      const uint16_t* qrow = (const uint16_t*)P->q.ptr + t * P->q.ss + (int64_t)h * P->q.sh + 8 * hl;
+    // The attention has left the scores: four steps at a time, the columns in
+    // turn between the halves of the wave.
+    if (P->scores && e.lq <= tpt) {
+      const int64_t srows = P->srows;
+      for (int s = step; s < s1; s += 4) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f}, old[4];
 #pragma unroll
-      for (int s = 0; s < KSD; ++s) {
-        u32x4 w = ld16(qrow + 16 * s);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = (w[k] & (on ? qand : 0u)) ^ qxor;
-        qreg[s] = as_bf16x8(w);
-      }
-      if constexpr (KSR > 0) {
-        const uint16_t* rrow = (const uint16_t*)P->rq.ptr + t * P->rq.ss + (int64_t)h * P->rq.sh;
-#pragma unroll
-        for (int s = 0; s < KSR; ++s) {
-          const int c = 2 * s + hl - hc * crr;  // this row's own head's chunks only
-          u32x4 w = {0, 0, 0, 0};
-          if (on && hc < gg && c >= 0 && c < crr) w = ld16(rrow + 8 * c);
-          qreg[KSD + s] = as_bf16x8(w);
+        for (int k = 0; k < 4; ++k) {
+          const int key = 32 * (s + k) + col;
+          old[k] = hl == 0 && key <= last && key < W.cap ? wrow[key] : 0.f;
         }
-      }
-      float l = kNegInf, g = 0.f;
-      if (on) l = ((const float*)P->lse.ptr)[t * P->lse.ss + (int64_t)h * P->lse.sh];
-      if (KSR > 0 && hc < gg) g = P->gs[h0 + hc] / P->c;
-      l = l == kNegInf ? kNegInf : -l * kLog2e;
+        for (int sub = 0; sub < nsub; ++sub) {
+          const float* sc = paged_scores(P, b, kvh * nsub + sub) + 32 * s + col;
+          const int nh = min(gsub, group - sub * gsub);
+#pragma unroll 2
+          for (int c = hl; c < e.lq * gsub; c += 2) {
+            const int t = small_div(c, gsub), h = c - t * gsub;
+            if (h >= nh) continue;
+            float x[4];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int row = 8 * (v >> 2) + 4 * hl + (v & 3);
-        nl[v] = __shfl(l, row);
-        if constexpr (KSR > 0) bh[v] = __shfl(g, row);
-      }
-    };
-    // The page of this lane's key of step s, and the key's row in it.  A key that is
-    // not there reads the pool's first row instead, and its sum is dropped.
-    auto find = [&](int s, int& id, int& row) {
-      const int key = 32 * s + col;
-      id = -1, row = 0;
-      if (key <= last && key < W.cap) {
-        const int pg = page_of(P->ps_mul, P->ps_shift, key);
-        id = trow[pg];
-        row = key - pg * ps;
-      }
-    };
-    bf16x8 k[KSD], rk[KSR > 0 ? KSR : 1];
-    float old = 0.f;
-    bool here = false;
-    auto load_k = [&](int s, int id, int row) {
-      here = (uint32_t)id < (uint32_t)npages;
-      const uint16_t* p = kpool + (here ? (int64_t)id * ksb + (int64_t)row * kss : 0) + 8 * hl;
+            for (int k = 0; k < 4; ++k) x[k] = s + k < s1 ? sc[c * srows + 32 * k] : kNegInf;
+            const float l = ((const float*)P->lse.ptr)[(int64_t)(e.q0 + t) * P->lse.ss +
+                                                       (int64_t)(h00 + sub * gsub + h) * P->lse.sh];
 #pragma unroll
-      for (int i = 0; i < KSD; ++i) k[i] = as_bf16x8(ld16(p + 16 * i));
-      here = here && hl == 0;
-      if (here) old = wrow[32 * s + col];
-    };
-    auto load_r = [&](int id, int row) {
-      if constexpr (KSR > 0) {
-        if (gg > 0) {
-          const bool in = (uint32_t)id < (uint32_t)npages;
-          const uint16_t* p = rpool + (in ? (int64_t)id * rsb + (int64_t)row * rss : 0) + (int64_t)h0 * rsh;
-          int cr = crr;
-          asm volatile("" : "+s"(cr));  // (offsets found again each time, not kept)
-#pragma unroll
-          for (int s = 0; s < KSR; ++s) {
-            int c = 2 * s + hl;
-            c = c < gg * cr ? c : 0;  // (R_q's chunk is zero there)
-            const int hh = small_div(c, cr);
-            rk[s] = as_bf16x8(ld16(p + (int64_t)hh * rsh + 8 * (c - hh * cr)));
+            for (int k = 0; k < 4; ++k)
+              sum[k] += l == kNegInf ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(x[k], c2, -l * kLog2e));
           }
         }
-      }
-    };
-
-    int id, row, id1, row1, held = -1;
-    find(step, id, row);
-    load_k(step, id, row);
-    find(step + 1, id1, row1);
-    float sum = 0.f;
-    for (int s = step, i = 0; s < s1;) {
-      if (held != i) {
-        rows(i);
-        load_r(id, row);
-        held = i;
-      }
-      f32x16 acc = f32x16{};
-      if constexpr (KSR > 0) {
-        if (gg > 0) {
 #pragma unroll
-          for (int j = 0; j < KSR; ++j) acc = mfma32(qreg[KSD + j], rk[j], acc);
-#pragma unroll
-          for (int v = 0; v < 16; ++v) acc[v] *= bh[v];
+        for (int k = 0; k < 4; ++k) {
+          const int key = 32 * (s + k) + col;
+          sum[k] = wave_pair_sum(sum[k]);
+          if (hl == 0 && key <= last && key < W.cap) wrow[key] = old[k] + sum[k];
         }
       }
+    } else {
+      // Row tile i: Q (A of S = Q K^T), and for the rows of this lane's registers
+      // -LSE log2(e) and graph scale.
+      bf16x8 qreg[KSD + KSR];
+      float nl[16], bh[KSR > 0 ? 16 : 1];
+      int h0 = h00, gg = 0, lim0 = 0;
+      auto rows = [&](int i) {
+        const int sub = nsub == 1 ? 0 : i / nct, t0 = (i - sub * nct) * tpt;
+        h0 = h00 + sub * gsub;
+        gg = KSR > 0 ? min(max(min(HG - h0, group - sub * gsub), 0), gsub) : 0;
+        lim0 = off + t0;
+        const bool on = tk < tpt && t0 + tk < e.lq && hc < min(gsub, group - sub * gsub);
+        const int64_t t = e.q0 + (on ? t0 + tk : 0);
+        const int h = h0 + (on ? hc : 0);
+        const uint16_t* qrow = (const uint16_t*)P->q.ptr + t * P->q.ss + (int64_t)h * P->q.sh + 8 * hl;
 #pragma unroll
-      for (int j = 0; j < KSD; ++j) acc = mfma_e<F16>(qreg[j], k[j], acc);
-      // The next step's rows, into the registers that are read.
-      const bool put = here;
-      const float before = old;
-      const int s0 = s;
-      const bool turn = i + 1 == n;
-      if (turn) {
-        ++s, i = 0;
-        if (s < s1) {
-          id = id1, row = row1;
-          load_k(s, id, row);
-          if (n == 1) load_r(id, row);
-          find(s + 1, id1, row1);
+        for (int s = 0; s < KSD; ++s) {
+          u32x4 w = ld16(qrow + 16 * s);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = (w[k] & (on ? qand : 0u)) ^ qxor;
+          qreg[s] = as_bf16x8(w);
         }
-      } else {
-        ++i;
-      }
-      if (causal && 32 * s0 + 31 > lim0) {
+        if constexpr (KSR > 0) {
+          const uint16_t* rrow = (const uint16_t*)P->rq.ptr + t * P->rq.ss + (int64_t)h * P->rq.sh;
+#pragma unroll
+          for (int s = 0; s < KSR; ++s) {
+            const int c = 2 * s + hl - hc * crr;  // this row's own head's chunks only
+            u32x4 w = {0, 0, 0, 0};
+            if (on && hc < gg && c >= 0 && c < crr) w = ld16(rrow + 8 * c);
+            qreg[KSD + s] = as_bf16x8(w);
+          }
+        }
+        float l = kNegInf, g = 0.f;
+        if (on) l = ((const float*)P->lse.ptr)[t * P->lse.ss + (int64_t)h * P->lse.sh];
+        if (KSR > 0 && hc < gg) g = P->gs[h0 + hc] / P->c;
+        l = l == kNegInf ? kNegInf : -l * kLog2e;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const int rw = 8 * (v >> 2) + 4 * hl + (v & 3);
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], c2, nl[v]));
-          sum += 32 * s0 + col <= lim0 + small_div(rw, gsub) && nl[v] != kNegInf ? p : 0.f;
+          const int row = 8 * (v >> 2) + 4 * hl + (v & 3);
+          nl[v] = __shfl(l, row);
+          if constexpr (KSR > 0) bh[v] = __shfl(g, row);
         }
-      } else {
+      };
+      // The page of this lane's key of step s, and the key's row in it.  A key that is
+      // not there reads the pool's first row instead, and its sum is dropped.
+      auto find = [&](int s, int& id, int& row) {
+        const int key = 32 * s + col;
+        id = -1, row = 0;
+        if (key <= last && key < W.cap) {
+          const int pg = page_of(P->ps_mul, P->ps_shift, key);
+          id = trow[pg];
+          row = key - pg * ps;
+        }
+      };
+      bf16x8 k[KSD], rk[KSR > 0 ? KSR : 1];
+      float old = 0.f;
+      bool here = false;
+      auto load_k = [&](int s, int id, int row) {
+        here = (uint32_t)id < (uint32_t)npages;
+        const uint16_t* p = kpool + (here ? (int64_t)id * ksb + (int64_t)row * kss : 0) + 8 * hl;
 #pragma unroll
-        for (int v = 0; v < 16; ++v) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], c2, nl[v]));
-      }
-      if (turn) {
-        sum = wave_pair_sum(sum);
-        if (put) wrow[32 * s0 + col] = before + sum;
-        sum = 0.f;
+        for (int i = 0; i < KSD; ++i) k[i] = as_bf16x8(ld16(p + 16 * i));
+        here = here && hl == 0;
+        if (here) old = wrow[32 * s + col];
+      };
+      auto load_r = [&](int id, int row) {
+        if constexpr (KSR > 0) {
+          if (gg > 0) {
+            const bool in = (uint32_t)id < (uint32_t)npages;
+            const uint16_t* p = rpool + (in ? (int64_t)id * rsb + (int64_t)row * rss : 0) + (int64_t)h0 * rsh;
+            int cr = crr;
+            asm volatile("" : "+s"(cr));  // (offsets found again each time, not kept)
+#pragma unroll
+            for (int s = 0; s < KSR; ++s) {
+              int c = 2 * s + hl;
+              c = c < gg * cr ? c : 0;  // (R_q's chunk is zero there)
+              const int hh = small_div(c, cr);
+              rk[s] = as_bf16x8(ld16(p + (int64_t)hh * rsh + 8 * (c - hh * cr)));
+            }
+          }
+        }
+      };
+
+      int id, row, id1, row1, held = -1;
+      find(step, id, row);
+      load_k(step, id, row);
+      find(step + 1, id1, row1);
+      float sum = 0.f;
+      for (int s = step, i = 0; s < s1;) {
+        if (held != i) {
+          rows(i);
+          load_r(id, row);
+          held = i;
+        }
+        f32x16 acc = f32x16{};
+        if constexpr (KSR > 0) {
+          if (gg > 0) {
+#pragma unroll
+            for (int j = 0; j < KSR; ++j) acc = mfma32(qreg[KSD + j], rk[j], acc);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[v] *= bh[v];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < KSD; ++j) acc = mfma_e<F16>(qreg[j], k[j], acc);
+        // The next step's rows, into the registers that are read.
+        const bool put = here;
+        const float before = old;
+        const int s0 = s;
+        const bool turn = i + 1 == n;
+        if (turn) {
+          ++s, i = 0;
+          if (s < s1) {
+            id = id1, row = row1;
+            load_k(s, id, row);
+            if (n == 1) load_r(id, row);
+            find(s + 1, id1, row1);
+          }
+        } else {
+          ++i;
+        }
+        if (causal && 32 * s0 + 31 > lim0) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int rw = 8 * (v >> 2) + 4 * hl + (v & 3);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], c2, nl[v]));
+            sum += 32 * s0 + col <= lim0 + small_div(rw, gsub) && nl[v] != kNegInf ? p : 0.f;
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], c2, nl[v]));
+        }
+        if (turn) {
+          sum = wave_pair_sum(sum);
+          if (put) wrow[32 * s0 + col] = before + sum;
+          sum = 0.f;
+        }
       }
     }
     left -= s1 - step;

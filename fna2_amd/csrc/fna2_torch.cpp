@@ -51,6 +51,7 @@ struct Lib {
   decltype(&fna2_rope_bwd_workspace_bytes) rope_bwd_workspace_bytes;
   decltype(&fna2_check_paged_attn) check_paged_attn;
   decltype(&fna2_paged_attn_workspace_bytes) paged_attn_workspace_bytes;
+  decltype(&fna2_paged_scores_bytes) paged_scores_bytes;
   decltype(&fna2_paged_attn) paged_attn;
   decltype(&fna2_check_paged_weights) check_paged_weights;
   decltype(&fna2_paged_weights) paged_weights;
@@ -88,6 +89,7 @@ void bind(const std::map<std::string, uintptr_t>& f, py::object error) {
   FNA2_BIND(rope_bwd_workspace_bytes);
   FNA2_BIND(check_paged_attn);
   FNA2_BIND(paged_attn_workspace_bytes);
+  FNA2_BIND(paged_scores_bytes);
   FNA2_BIND(paged_attn);
   FNA2_BIND(check_paged_weights);
   FNA2_BIND(paged_weights);
@@ -696,6 +698,15 @@ std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
   }
   a.q = view(q, true);
   a.out = view(out, true);
+  Tensor scores;
+  if (w.defined()) {
+    const size_t bytes = L.paged_scores_bytes(&a);
+    if (bytes > 0) {
+      scores = bytes_on(bytes, q);
+      a.scores = scores.data_ptr();
+      a.scores_bytes = bytes;
+    }
+  }
   wa.attn = a;
   if (L.check_paged_attn(&a) != FNA2_OK ||
       (w.defined() && L.check_paged_weights(&wa) != FNA2_OK))

@@ -222,8 +222,12 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     a.q, a.out = _t3(q), _t3(out)
     lib = _capi.lib()
     _capi.raise_for(lib.fna2_check_paged_attn(ctypes.byref(a)), what)
-    wa = None
+    wa = scores = None
     if w is not None:
+        nbytes = lib.fna2_paged_scores_bytes(ctypes.byref(a))
+        if nbytes:
+            scores = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            a.scores, a.scores_bytes = scores.data_ptr(), nbytes
         wa = _capi.PagedWeightsArgs()
         wa.attn = a
         wa.key_weights = w.data_ptr()
@@ -238,7 +242,7 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
             if wa is not None:
                 _capi.raise_for(lib.fna2_paged_weights(ctypes.byref(wa), _stream(dev)), what)
                 _bump(w)
-    del keep, cu, gs
+    del keep, cu, gs, scores
     return (out, lse) if return_lse else out
 
 

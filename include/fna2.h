@@ -361,11 +361,16 @@ typedef struct fna2_paged_attn_args {
   fna2_tensor lse;     /* fp32 [T, H], written; ptr NULL: not computed         */
   void* workspace;     /* fna2_paged_attn_workspace_bytes, 16-byte aligned     */
   size_t workspace_bytes;
+  void* scores;        /* NULL, or fna2_paged_scores_bytes for a               */
+  size_t scores_bytes; /* fna2_paged_weights call to follow, 16-byte aligned   */
 } fna2_paged_attn_args;
 
 /* Host-only validation; no GPU call. */
 int fna2_check_paged_attn(const fna2_paged_attn_args* args);
 size_t fna2_paged_attn_workspace_bytes(const fna2_paged_attn_args* args);
+/* Bytes of the scores that fna2_paged_weights can take from the attention instead
+ * of forming them again; 0 where that would not be faster. */
+size_t fna2_paged_scores_bytes(const fna2_paged_attn_args* args);
 /* One launch, and a second that joins the parts of split rows. */
 int fna2_paged_attn(const fna2_paged_attn_args* args, void* hip_stream);
 
@@ -373,8 +378,8 @@ int fna2_paged_attn(const fna2_paged_attn_args* args, void* hip_stream);
  *     key_weights[b][kvh][j] += sum over b's tokens i and the query heads h of
  *                               KV head kvh of exp(S_hij - lse[i][h])
  * in fp32, in a fixed order (no atomics).  attn: the call's arguments, its
- * lse written (out and workspace unused).  Rows at or past `capacity` have no
- * weight. */
+ * lse and scores (if given) written, nothing it read changed since (out and
+ * workspace unused).  Rows at or past `capacity` have no weight. */
 typedef struct fna2_paged_weights_args {
   fna2_paged_attn_args attn;
   float* key_weights;          /* [N][H_KV][capacity], added to               */

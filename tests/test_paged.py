@@ -235,6 +235,25 @@ def test_check_paged_weights_codes(lib):
     assert code(capacity=0, key_weights=None) == "FNA2_OK"
 
 
+def test_check_paged_scores(lib):
+    """The scores' size: columns by rows where few columns serve a row, else 0;
+    a buffer that is too small or not aligned is refused."""
+    import ctypes
+    size = lambda a: lib.fna2_paged_scores_bytes(ctypes.byref(a))
+    one = _attn(max_seqlen_q=1)
+    assert size(one) == 4 * 4 * (8 * 64) * 4 * 4  # sequences, KV heads, rows, columns, bytes
+    assert size(_attn(max_seqlen_q=8)) == 0 and size(_attn(max_seqlen_q=16)) == 0
+    assert size(_attn(max_seqlen_q=1, table_width=1 << 20, table_stride=1 << 20)) == 0
+    assert size(_attn(max_seqlen_q=1, table_width=0)) == 0
+    for over, want in ((dict(scores=FAKE, scores_bytes=size(one)), "FNA2_OK"),
+                       (dict(scores=FAKE, scores_bytes=size(one) - 1), "FNA2_E_WORKSPACE"),
+                       (dict(scores=FAKE + 8, scores_bytes=size(one)), "FNA2_E_WORKSPACE")):
+        a = _attn(max_seqlen_q=1)
+        for k, v in over.items():
+            setattr(a, k, v)
+        assert _st(lib.fna2_check_paged_attn(ctypes.byref(a))) == want
+
+
 def test_check_paged_append_codes(lib):
     def code(**over):
         a = _capi.PagedAppendArgs()
@@ -497,6 +516,40 @@ def test_weights_past_garbage(gpu, lq, H, HKV, HG, R):
     acc = torch.zeros_like(ref)
     c.attend(key_weights=acc)
     assert torch.equal(acc, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("case", [c for c in ATTEND if max(c[0]) <= 9],
+                         ids=lambda c: f"q{c[0]}-k{c[1]}-h{c[2]}.{c[3]}.{c[4]}")
+def test_weights_without_the_scores(gpu, lib, monkeypatch, case, causal):
+    """The rows' weights from K, where the attention left no scores: right, and
+    past garbage (NaN in the rows that are no sequence's) the same bits."""
+    monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+    monkeypatch.setattr(lib, "fna2_paged_scores_bytes", lambda a: 0)
+    c = Case(*case, seed=3, device=gpu)
+    check_attend(c, causal=causal)
+    ref = torch.zeros(c.N, c.HKV, c.width * c.ps, device=gpu)
+    c.attend(key_weights=ref, is_causal=causal)
+    named = torch.zeros(c.P, c.ps, dtype=torch.bool)
+    for b in range(c.N):
+        for j in range(c.lk[b]):
+            named[c.slot(b, j)] = True
+    hole = ~named.to(gpu)
+    for pool in (c.k, c.v, c.rk):
+        if pool is not None:
+            pool.masked_fill_(hole[:, None, :, None], float("nan"))
+    acc = torch.zeros_like(ref)
+    c.attend(key_weights=acc, is_causal=causal)
+    assert torch.equal(acc, ref)
+
+
+@pytest.mark.gpu
+def test_scores_serve_the_short_chunks_only(gpu):
+    """A hint below the longest chunk: the sequences that one tile holds take
+    the scores, the others K; long caches in several runs."""
+    check_attend(Case([1, 7, 0, 2], [700, 400, 90, 33], 8, 4, 5, 64, 16, 16, device=gpu), hint=1)
+    check_attend(Case([3, 40, 2], [500, 300, 2], 4, 2, 0, 128, 0, 32, FP, device=gpu), hint=3)
 
 
 @pytest.mark.gpu
