@@ -701,10 +701,13 @@ std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
   Tensor scores;
   if (w.defined()) {
     const size_t bytes = L.paged_scores_bytes(&a);
-    if (bytes > 0) {
-      scores = bytes_on(bytes, q);
-      a.scores = scores.data_ptr();
-      a.scores_bytes = bytes;
+    try {  // (without the room the weights read K again)
+      if (bytes > 0) {
+        scores = bytes_on(bytes, q);
+        a.scores = scores.data_ptr();
+        a.scores_bytes = bytes;
+      }
+    } catch (const c10::OutOfMemoryError&) {
     }
   }
   wa.attn = a;

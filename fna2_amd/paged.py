@@ -224,10 +224,15 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     _capi.raise_for(lib.fna2_check_paged_attn(ctypes.byref(a)), what)
     wa = scores = None
     if w is not None:
+        # (with room for the scores, where they save a second reading of K and
+        # the memory is there)
         nbytes = lib.fna2_paged_scores_bytes(ctypes.byref(a))
-        if nbytes:
-            scores = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            a.scores, a.scores_bytes = scores.data_ptr(), nbytes
+        try:
+            if nbytes:
+                scores = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+                a.scores, a.scores_bytes = scores.data_ptr(), nbytes
+        except torch.OutOfMemoryError:
+            pass
         wa = _capi.PagedWeightsArgs()
         wa.attn = a
         wa.key_weights = w.data_ptr()

@@ -545,6 +545,25 @@ def test_weights_without_the_scores(gpu, lib, monkeypatch, case, causal):
 
 
 @pytest.mark.gpu
+def test_weights_where_the_scores_do_not_fit(gpu, lib, monkeypatch):
+    """No memory for the scores: the weights come from K."""
+    c = Case([1, 1], [300, 77], 8, 2, 6, 128, 32, 32, device=gpu)
+    monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+    refused, empty = [], torch.empty
+
+    def full(*size, **kw):
+        if kw.get("dtype") is torch.uint8 and not refused:
+            refused.append(size)
+            raise torch.OutOfMemoryError("full")
+        return empty(*size, **kw)
+
+    monkeypatch.setattr(torch, "empty", full)
+    check_attend(c)
+    # (N, HKV, rows, columns, bytes)
+    assert refused == [(2 * 2 * c.width * c.ps * 4 * 4,)]
+
+
+@pytest.mark.gpu
 def test_scores_serve_the_short_chunks_only(gpu):
     """A hint below the longest chunk: the sequences that one tile holds take
     the scores, the others K; long caches in several runs."""
