@@ -300,6 +300,8 @@ SIGNATURES = {
     "fna2_paged_weights": (ctypes.c_int, [ctypes.POINTER(PagedWeightsArgs), ctypes.c_void_p]),
     "fna2_check_paged_append": (ctypes.c_int, [ctypes.POINTER(PagedAppendArgs)]),
     "fna2_paged_append": (ctypes.c_int, [ctypes.POINTER(PagedAppendArgs), ctypes.c_void_p]),
+    "fna2_paged_append_shifted": (ctypes.c_int, [ctypes.POINTER(PagedAppendArgs), ctypes.c_void_p,
+                                                 ctypes.c_void_p]),
     "fna2_check_paged_evict": (ctypes.c_int, [ctypes.POINTER(PagedEvictArgs)]),
     "fna2_paged_evict": (ctypes.c_int, [ctypes.POINTER(PagedEvictArgs), ctypes.c_void_p]),
 }

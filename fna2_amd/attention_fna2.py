@@ -766,7 +766,7 @@ class NaylisAttention(nn.Module):
             cos, sin = cos[pos][:, None], sin[pos][:, None]
             q, k = self.rope.rotate(q, cos, sin), self.rope.rotate(k, cos, sin)
         q = paged_append(q, k, v, cache.k, cache.v, t.block_table, t.seqlens, cu, r_k, cache.r_k,
-                         inv, t.positions if inv is not None else None, wq, wk, eps)
+                         inv, None, wq, wk, eps, t.position_shift if inv is not None else None)
         out = flash_naylis_paged(q, cache.k, cache.v, t.block_table, t.seqlens, cu, max_q, r_q,
                                  cache.r_k, self.graph_scale, softmax_scale=self._attn_scale(),
                                  key_weights=cache.key_weights)

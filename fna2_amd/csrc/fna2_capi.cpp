@@ -1619,8 +1619,9 @@ int fna2_check_paged_append(const fna2_paged_append_args* a) {
   return FNA2_OK;
 }
 
-int fna2_paged_append(const fna2_paged_append_args* a, void* stream) {
+int fna2_paged_append_shifted(const fna2_paged_append_args* a, const int32_t* shift, void* stream) {
   FNA2_TRY(fna2_check_paged_append(a));
+  if (!aligned(shift, 4)) return FNA2_E_STRIDE;
   if (a->c.total_q == 0) return FNA2_OK;
   FNA2_TRY(check_device());
   fna2::PagedAppendParams K;
@@ -1632,12 +1633,17 @@ int fna2_paged_append(const fna2_paged_append_args* a, void* stream) {
   K.vn = view(a->v);
   K.rkn = view(a->r_k);
   K.pos = a->positions;
+  K.shift = shift;
   K.inv_freq = a->inv_freq;
   K.wq = a->norm_q;
   K.wk = a->norm_k;
   K.eps = a->eps;
   if (fna2::launch_paged_append(K, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
   return FNA2_OK;
+}
+
+int fna2_paged_append(const fna2_paged_append_args* a, void* stream) {
+  return fna2_paged_append_shifted(a, nullptr, stream);
 }
 
 int fna2_check_paged_evict(const fna2_paged_evict_args* a) {

@@ -275,6 +275,7 @@ struct PagedAppendParams {
   PagedParams p;  // q, k, v pools and the chunk; o is q_out
   TView kn, vn, rkn;  // the new rows [T, heads, .]
   const int* pos;
+  const int* shift;  // [N] added to a sequence's positions, or null
   const float* inv_freq;
   const float* wq;
   const float* wk;

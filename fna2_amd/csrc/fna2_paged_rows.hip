@@ -51,11 +51,12 @@ __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const Page
         else hi = mid;
       }
     const bool inside = lo >= 0 && lo < P.N;
-    int row = -1, pr = 0;
+    int row = -1, pr = 0, shift = 0;
     int64_t page = -1;
     if (inside) {
       const PagedSeq e = paged_seq_uniform(kargs(), lo);
       row = e.lk - e.lq + (t - e.q0);
+      if (A.shift) shift = uni(*const_space(A.shift + lo));
       if (row >= 0 && row < e.lk) {
         const int pg = page_of(P.ps_mul, P.ps_shift, row);
         pr = row - pg * P.ps;
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const Page
 #pragma unroll
     for (int e = 0; e < 8; ++e) co[e] = 1.f, si[e] = 0.f;
     if (turn) {
-      const int pos = A.pos ? uni(*const_space(A.pos + t)) : row;
+      const int64_t pos = (int64_t)(A.pos ? uni(*const_space(A.pos + t)) : row) + shift;
       if (lane < HALF) {
         // in turns, reduced to half a turn either way
         const double x = (double)pos * inv * 0.15915494309189533577;

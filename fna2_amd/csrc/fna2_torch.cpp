@@ -55,7 +55,7 @@ struct Lib {
   decltype(&fna2_paged_attn) paged_attn;
   decltype(&fna2_check_paged_weights) check_paged_weights;
   decltype(&fna2_paged_weights) paged_weights;
-  decltype(&fna2_paged_append) paged_append;
+  decltype(&fna2_paged_append_shifted) paged_append_shifted;
   decltype(&fna2_paged_evict) paged_evict;
 };
 Lib L{};
@@ -93,7 +93,7 @@ void bind(const std::map<std::string, uintptr_t>& f, py::object error) {
   FNA2_BIND(paged_attn);
   FNA2_BIND(check_paged_weights);
   FNA2_BIND(paged_weights);
-  FNA2_BIND(paged_append);
+  FNA2_BIND(paged_append_shifted);
   FNA2_BIND(paged_evict);
 #undef FNA2_BIND
 }
@@ -734,9 +734,9 @@ OptTensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const 
                        const Tensor& vp, const Tensor& table, const Tensor& lens, const Tensor& cu,
                        const OptTensor& rk_, const OptTensor& rkp_, const OptTensor& inv_,
                        const OptTensor& pos_, const OptTensor& nq, const OptTensor& nk,
-                       double eps) {
-  const Tensor &rk = opt(rk_), &pos = opt(pos_);
-  if (!L.paged_append || !q.defined() || !q.is_cuda() || q.dim() != 3) return std::nullopt;
+                       double eps, const OptTensor& shift_) {
+  const Tensor &rk = opt(rk_), &pos = opt(pos_), &shift = opt(shift_);
+  if (!L.paged_append_shifted || !q.defined() || !q.is_cuda() || q.dim() != 3) return std::nullopt;
   const c10::Device dev = q.device();
   const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
   fna2_paged_append_args a{};
@@ -757,6 +757,11 @@ OptTensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const 
       return std::nullopt;
     a.positions = pos.data_ptr<int32_t>();
   }
+  if (shift.defined()) {
+    if (!inv_.has_value() || !int32_on(shift, dev) || shift.dim() != 1 ||
+        shift.numel() != a.c.batch)
+      return std::nullopt;
+  }
   Tensor vec[3];
   auto fp32 = [&](const OptTensor& t, int64_t n, Tensor& keep, const float*& p) {
     if (!t.has_value()) return true;
@@ -776,7 +781,9 @@ OptTensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const 
   a.k = view(k, true);
   a.v = view(v, true);
   a.q_out = view(out, true);
-  if (!launched(L.paged_append(&a, stream_of(dev)), "paged_append")) return std::nullopt;
+  const int32_t* by = shift.defined() ? shift.data_ptr<int32_t>() : nullptr;
+  if (!launched(L.paged_append_shifted(&a, by, stream_of(dev)), "paged_append"))
+    return std::nullopt;
   written({&kp, &vp, &opt(rkp_)});
   return out;
 }
@@ -825,6 +832,10 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("rope_fwd", &rope_fwd, Free());
   m.def("rope_bwd", &rope_bwd, Free());
   m.def("paged_attn", &paged_attn, Free());
-  m.def("paged_append", &paged_append, Free());
+  m.def("paged_append", &paged_append, Free(), py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"), py::arg("seqlens_k"),
+        py::arg("cu_seqlens_q"), py::arg("r_k"), py::arg("rk_pages"), py::arg("inv_freq"),
+        py::arg("positions"), py::arg("norm_q"), py::arg("norm_k"), py::arg("eps"),
+        py::arg("position_shift") = py::none());
   m.def("paged_evict", &paged_evict, Free());
 }

@@ -258,7 +258,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
                  inv_freq: Optional[torch.Tensor] = None,
                  positions: Optional[torch.Tensor] = None,
                  norm_q: Optional[torch.Tensor] = None, norm_k: Optional[torch.Tensor] = None,
-                 eps: float = 1e-6) -> torch.Tensor:
+                 eps: float = 1e-6, position_shift: Optional[torch.Tensor] = None
+                 ) -> torch.Tensor:
     """The new tokens' rows, in one launch: q ``[T, H, D]`` and k ``[T, H_KV,
     D]`` RMS-normalised by ``norm_q`` / ``norm_k`` ``[D]`` (each optional) and
     rotated by ``inv_freq`` ``[D / 2]`` (optional), k, v and r_k ``[T, H_G, R]``
@@ -266,15 +267,17 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
 
     The chain is evaluated in fp32 (the angle in fp64) and rounded once, as
     ``rope_varlen`` with a norm does.  A token's position is its cache row, or
-    ``positions[t]`` (int32): after an eviction the two differ.  ``seqlens_k``
-    counts the rows after the append.  Rows before 0 or past the table are not
+    ``positions[t]`` (int32), plus ``position_shift[b]`` (int32 ``[N]``) of its
+    sequence: after an eviction a sequence's rows and positions differ by a
+    number.  ``seqlens_k`` counts the rows after the append.  Rows before 0 or past the table are not
     stored; tokens of no sequence keep their q and store nothing.  Pages that
     are written may belong to one sequence only."""
     what = "paged_append"
     nat = _capi.native_or_none() if q.is_cuda else None
     if nat is not None:
         done = nat.paged_append(q, k, v, k_pages, v_pages, block_table, seqlens_k, cu_seqlens_q,
-                                r_k, rk_pages, inv_freq, positions, norm_q, norm_k, float(eps))
+                                r_k, rk_pages, inv_freq, positions, norm_q, norm_k, float(eps),
+                                position_shift)
         if done is not None:
             return done
     assert q.dim() == 3 and k.dim() == 3, f"{what}: q [T, H, D] and k [T, H_KV, D] expected"
@@ -307,6 +310,11 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
         assert inv is not None, f"{what}: positions need inv_freq"
         pos = _ints(positions, dev)
         assert pos.shape == (T,), f"{what}: positions must hold one position a token"
+    shift = None
+    if position_shift is not None:
+        assert inv is not None, f"{what}: position_shift needs inv_freq"
+        shift = _ints(position_shift, dev)
+        assert shift.shape == (c.batch,), f"{what}: position_shift must hold one number a sequence"
     for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("rk_pages", rk_pages)):
         if t is not None:
             _written(t, name)
@@ -320,7 +328,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     lib = _capi.lib()
     _capi.raise_for(lib.fna2_check_paged_append(ctypes.byref(a)), what)
     with torch.cuda.device(dev):
-        _capi.raise_for(lib.fna2_paged_append(ctypes.byref(a), _stream(dev)), what)
+        _capi.raise_for(lib.fna2_paged_append_shifted(
+            ctypes.byref(a), None if shift is None else shift.data_ptr(), _stream(dev)), what)
     _bump(k_pages, v_pages, rk_pages if H_G else None)
     del keep, cu
     return out
@@ -396,12 +405,16 @@ class PageTable:
     """Which pages hold the rows of which sequence: one for all the layers of
     a model, whose pools (``PagedKVCache``) all have its pages.
 
-    ``block_table`` ``[sequences, max_pages]`` and ``seqlens`` ``[sequences]``
-    (int32) are on the device and written in place, so that captured graphs
-    read the step at hand.  ``extend(counts)`` takes in the new tokens of a step;
-    ``cu_seqlens_q``, ``max_seqlen_q``, ``total_q`` and ``positions`` then
-    describe them for every layer.  The bookkeeping is the host's: nothing is
-    read back from the device."""
+    ``extend(counts)`` takes in the new tokens of a step; ``block_table``
+    ``[sequences, max_pages]``, ``seqlens`` and ``position_shift``
+    ``[sequences]`` and ``cu_seqlens_q`` (int32) then describe them for every
+    layer.  These are on the device and written in place, so that captured
+    graphs read the step at hand (of as many tokens as the captured one).
+    ``max_seqlen_q`` and ``total_q`` are numbers.  A token's position is its row
+    plus its sequence's ``position_shift``, the rows that ``truncate`` took away
+    before it; ``positions`` are those of the step's tokens one by one, a tensor
+    of this step only.  The bookkeeping is the host's: nothing is read back from
+    the device."""
 
     def __init__(self, sequences: int, num_pages: int, page_size: int = 64,
                  max_pages: Optional[int] = None, device=None):
@@ -415,17 +428,29 @@ class PageTable:
         self._free = list(range(num_pages - 1, -1, -1))
         self._host = torch.full((sequences, self.width), -1, dtype=torch.int32)
         self.block_table = self._host.to(device)
-        self.seqlens = torch.zeros(sequences, dtype=torch.int32, device=device)
-        self.cu_seqlens_q = torch.zeros(sequences + 1, dtype=torch.int32, device=device)
+        self._cu = [0] * (sequences + 1)
+        # [seqlens | position_shift | cu_seqlens_q], uploaded in one copy
+        self._step = torch.zeros(3 * sequences + 1, dtype=torch.int32, device=device)
+        self.seqlens, self.position_shift, self.cu_seqlens_q = self._step.split(
+            [sequences, sequences, sequences + 1])
         self.max_seqlen_q = self.total_q = 0
-        self.positions: Optional[torch.Tensor] = None  # [total_q]; None: a token's row
+        self._positions: Optional[Sequence[int]] = None
 
     @property
     def free_pages(self) -> int:
         return len(self._free)
 
+    @property
+    def positions(self) -> Optional[torch.Tensor]:
+        """[total_q] int32: the positions of the last ``extend``'s tokens, a new
+        tensor; None: a token's row, in every sequence."""
+        if self._positions is None:
+            return None
+        return torch.tensor(self._positions, dtype=torch.int32, device=self.seqlens.device)
+
     def _upload(self, table: bool) -> None:
-        self.seqlens.copy_(torch.tensor(self.rows, dtype=torch.int32))
+        shift = [p - r for r, p in zip(self.rows, self.next_position)]
+        self._step.copy_(torch.tensor(self.rows + shift + self._cu, dtype=torch.int32))
         if table:
             self.block_table.copy_(self._host)
 
@@ -463,10 +488,9 @@ class PageTable:
                 pos += range(self.next_position[b], self.next_position[b] + c)
             self.rows[b] += c
             self.next_position[b] += c
-        self.cu_seqlens_q.copy_(torch.tensor(cu, dtype=torch.int32))
+        self._cu = cu
         self.total_q, self.max_seqlen_q = cu[-1], max(counts, default=0)
-        self.positions = torch.tensor(pos, dtype=torch.int32, device=self.seqlens.device) \
-            if moved else None
+        self._positions = pos if moved else None
         self._upload(any(more))
 
     def truncate(self, budget: int) -> None:

@@ -410,6 +410,11 @@ typedef struct fna2_paged_append_args {
 
 int fna2_check_paged_append(const fna2_paged_append_args* args);
 int fna2_paged_append(const fna2_paged_append_args* args, void* hip_stream);
+/* ... with position_shift[b] ([N] int32 on the device, or NULL) added to the
+ * positions of sequence b: after an eviction a sequence's rows and positions
+ * differ by a number. */
+int fna2_paged_append_shifted(const fna2_paged_append_args* args, const int32_t* position_shift,
+                              void* hip_stream);
 
 /* Eviction: of every sequence with more than `budget` rows each KV head keeps
  * the first `first`, the last `recent` and, between them, the budget - first

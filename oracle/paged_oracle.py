@@ -80,7 +80,7 @@ def norm_rope(x, weight, pos, inv_freq, eps):
 
 
 def append(q, k, v, k_pages, v_pages, table, lens, cu, r_k=None, rk_pages=None, inv_freq=None,
-           positions=None, norm_q=None, norm_k=None, eps=1e-6):
+           positions=None, norm_q=None, norm_k=None, eps=1e-6, position_shift=None):
     """(q_out, k_pages, v_pages, rk_pages) after the append."""
     q, k, v, rk = map(_np, (q, k, v, r_k))
     kp, vp, rkp = (None if t is None else _np(t).copy() for t in (k_pages, v_pages, rk_pages))
@@ -96,6 +96,7 @@ def append(q, k, v, k_pages, v_pages, table, lens, cu, r_k=None, rk_pages=None, 
         for i in range(m):
             t, row = int(cu[b]) + i, n - m + i
             at = row if pos is None else int(pos[t])
+            at += 0 if position_shift is None else int(position_shift[b])
             out[t] = norm_rope(q[t], wq, at, inv, eps)
             if not 0 <= row < cap:
                 continue

@@ -1055,3 +1055,49 @@ def test_other_streams_and_graphs(gpu):
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(w, acc), i
         assert all(torch.equal(a, b) for a, b in zip(ev, ev2)), i
+
+
+# ── Positions that run ahead of the rows ─────────────────────────────────────
+
+def test_check_paged_append_position_shift(lib):
+    a = _capi.PagedAppendArgs()
+    a.c = _cache_args(heads_graph=0)
+    a.q = a.q_out = _capi.Tensor(FAKE, 0, 16 * 128, 128)
+    a.k = a.v = _capi.Tensor(FAKE, 0, 4 * 128, 128)
+    a.inv_freq, a.eps = FAKE, 1e-6
+    # (refused before anything is asked of a device)
+    assert _st(lib.fna2_paged_append_shifted(ctypes.byref(a), FAKE + 2, None)) == "FNA2_E_STRIDE"
+    a.c.total_q = 0
+    assert _st(lib.fna2_paged_append_shifted(ctypes.byref(a), FAKE + 4, None)) == "FNA2_OK"
+    assert _st(lib.fna2_paged_append_shifted(ctypes.byref(a), None, None)) == "FNA2_OK"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("lq", [[1, 1, 1], [5, 0, 33]])
+def test_append_position_shift(gpu, monkeypatch, lq, given, native):
+    """A sequence's positions are its rows (or the positions given) plus a number."""
+    if not native:
+        monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+    c = Case(lq, [40, 9, 33], 4, 2, 3, 128, 8, 16, FP, seed=7, device=gpu, head=1, tail=2)
+    g = torch.Generator().manual_seed(2)
+    inv = 10000.0 ** (-torch.arange(0, 128, 2).float() / 128)
+    shift = torch.tensor([100000, 0, 77], dtype=torch.int32)
+    pos = torch.randint(0, 5000, (c.T,), generator=g).to(torch.int32) if given else None
+    w = 1 + 0.2 * torch.randn(128, generator=g)
+    ref = PO.append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, c.rkn, c.rk, inv, pos, w, w,
+                    position_shift=shift)
+    w = w.to(gpu)
+    got = paged.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, c.rkn, c.rk,
+                             inv.to(gpu), None if pos is None else pos.to(gpu), w, w,
+                             position_shift=shift.to(gpu) if native else shift)
+    for a, b in ((got, ref[0]), (c.k, ref[1])):
+        a = a.double().cpu().numpy()
+        assert (np.abs(a - b) <= HALF[FP] * np.abs(b) + 1e-5).all()
+    with pytest.raises(AssertionError, match="position_shift"):
+        paged.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, inv_freq=inv.to(gpu),
+                           position_shift=shift[:2].to(gpu))
+    with pytest.raises(AssertionError, match="position_shift"):
+        paged.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu,
+                           position_shift=shift.to(gpu))

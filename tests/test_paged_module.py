@@ -214,3 +214,136 @@ def test_two_layers_with_eviction(gpu):
         for c in cs:
             c.forget(1)
             assert (c.key_weights[1] == 0).all()
+
+
+# ── Positions that run ahead of the rows ─────────────────────────────────────
+
+def test_page_table_writes_a_step_in_place():
+    """What a captured step reads keeps its place through every call, and the
+    positions of tokens are rows plus the shift."""
+    t = PageTable(3, 12, page_size=16, max_pages=6)
+    names = ("block_table", "seqlens", "position_shift", "cu_seqlens_q")
+    held = {n: getattr(t, n) for n in names}
+    place = {n: x.data_ptr() for n, x in held.items()}
+    t.extend([50, 10, 0])
+    assert t.position_shift.tolist() == [0, 0, 0]
+    t.truncate(20)
+    assert t.position_shift.tolist() == [30, 0, 0] and t.cu_seqlens_q.tolist() == [0, 50, 60, 60]
+    t.extend([2, 1, 3])
+    assert t.position_shift.tolist() == [30, 0, 0] and t.seqlens.tolist() == [22, 11, 3]
+    assert t.positions.tolist() == [50, 51, 10, 0, 1, 2]
+    t.truncate(8)
+    assert t.position_shift.tolist() == [44, 3, 0]
+    t.extend([1, 1, 1])
+    assert t.positions.tolist() == [52, 11, 3] and t.cu_seqlens_q.tolist() == [0, 1, 2, 3]
+    t.release(0)
+    assert t.position_shift.tolist() == [0, 3, 0] and t.seqlens.tolist() == [0, 9, 4]
+    for n in names:
+        assert getattr(t, n) is held[n] and held[n].data_ptr() == place[n]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("when", ["before", "after"])
+@pytest.mark.parametrize("kw", [dict(), dict(use_rope=False)])
+def test_a_graph_follows_the_table_through_eviction(gpu, kw, when):
+    """A step captured before any eviction, or after one, replayed while more
+    follow: positions go on counting past the rows, as in eager steps of a second
+    cache."""
+    m = _layer(gpu, **kw)
+    t = PageTable(2, 40, page_size=16, device=gpu)
+    a, b = _cache(m, t, weigh=True), _cache(m, t, weigh=True)
+    g = torch.Generator().manual_seed(2)
+    x0 = torch.randn(2, 40, 512, generator=g).bfloat16().to(gpu)
+
+    def evict(budget):
+        b.key_weights.copy_(a.key_weights)
+        kept = [c.evict(budget, recent=4, first=1, heads=8) for c in (a, b)]
+        assert torch.equal(*kept)
+        t.truncate(budget)
+
+    with torch.no_grad():
+        t.extend([40, 40])
+        for c in (a, b):
+            m(x0, past_kv=c)
+        if when == "after":
+            evict(33)
+        t.extend([1, 1])
+        x = torch.randn(2, 1, 512, generator=g).bfloat16().to(gpu)
+        for _ in range(2):  # (the same rows again: nothing changes but the weights)
+            m(x, past_kv=a)
+        m(x, past_kv=b)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, _ = m(x, past_kv=a)
+        for i in range(24):
+            if i % 6 == 3:
+                evict(32 - i // 2)
+            t.extend([1, 1])
+            x.copy_(torch.randn(2, 1, 512, generator=g).bfloat16())
+            want, _ = m(x, past_kv=b)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), i
+            assert torch.equal(a.k, b.k), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_steps_after_an_eviction(gpu, graph):
+    """The rows that were kept are the cache's, each new token's key is rotated
+    for its position (not its row), and a step's output is the attention of its
+    query, so rotated, over them.
+
+    Keys: half a step and 1e-5 for the fp32 chain.  Outputs: the rotated q, P, the
+    attention's output and the layer's, each by at most 2^-8 of the value."""
+    from oracle import paged_oracle as PO
+    m = _layer(gpu)
+    t = PageTable(2, 12, page_size=16, device=gpu)
+    c = _cache(m, t, weigh=True)
+    g = torch.Generator().manual_seed(4)
+    inv = m.rope.inv_freq.double().cpu().numpy()
+    f64 = lambda y: y.detach().double().cpu().numpy()
+    rows = lambda pool, b: torch.stack([pool[t.pages[b][j // 16], :, j % 16] for j in range(t.rows[b])])
+    x = torch.zeros(2, 512, dtype=torch.bfloat16, device=gpu)
+    with torch.no_grad():
+        t.extend([60, 41])
+        m(torch.randn(101, 512, generator=g).bfloat16().to(gpu), past_kv=c)
+        t.extend([1, 1])
+        x.copy_(torch.randn(2, 512, generator=g).bfloat16())
+        m(x, past_kv=c)
+        if graph:
+            cg = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(cg):
+                yg, _ = m(x, past_kv=c)
+        before = [[rows(p, b) for p in (c.k, c.v, c.r_k)] for b in range(2)]
+        kept = c.evict(48, recent=8, first=2, heads=8)
+        t.truncate(48)
+        for b in range(2):
+            n = t.rows[b]
+            for p, old in zip((c.k, c.v), before[b]):
+                for h in range(2):
+                    assert torch.equal(rows(p, b)[:, h], old[kept[b, h, :n].long(), h])
+            for h in range(8):
+                assert torch.equal(rows(c.r_k, b)[:, h], before[b][2][kept[b, h // 4, :n].long(), h])
+        for step in range(4):
+            t.extend([1, 1])
+            x.copy_(torch.randn(2, 512, generator=g).bfloat16())
+            if graph:
+                cg.replay()
+                y = yg
+            else:
+                y, _ = m(x, past_kv=c)
+            q, k, _, r_q, _ = m._project(x)
+            pos = [61 + step, 42 + step]
+            assert t.positions.tolist() == pos
+            qs = []
+            for b in range(2):
+                want = PO.norm_rope(f64(k[b]), f64(m.k_norm.weight), pos[b], inv, m.k_norm.eps)
+                got = f64(rows(c.k, b)[-1])
+                assert (abs(got - want) <= 2.0 ** -8 * abs(want) + 1e-5).all(), (step, b)
+                qs.append(PO.norm_rope(f64(q[b]), f64(m.q_norm.weight), pos[b], inv, m.q_norm.eps))
+            out = PO.attend(torch.stack([torch.from_numpy(z) for z in qs]), c.k, c.v, t.block_table,
+                            t.seqlens, t.cu_seqlens_q, r_q, c.r_k, m.graph_scale)[0]
+            ref = out.reshape(2, 512) @ f64(m.out_proj.weight).T
+            assert rel_norm(y, ref) < 4 * 2.0 ** -8, step
