@@ -192,6 +192,13 @@ class RotaryPositionalEmbedding(nn.Module):
             self._cos, self._sin, self._cache_key = ang.cos(), ang.sin(), key
         return self._cos, self._sin
 
+    def _at(self, pos: torch.Tensor, dtype):
+        """cos / sin of the positions ``pos`` [n], rounded as the rows of
+        ``_table``, which has room for positions that the host knows only."""
+        ang = torch.outer(pos.to(dtype), self.inv_freq.to(device=pos.device, dtype=dtype))
+        ang = torch.cat((ang, ang), dim=-1)
+        return ang.cos(), ang.sin()
+
     @staticmethod
     def _rotate_half(x: torch.Tensor) -> torch.Tensor:
         h = x.shape[-1] // 2
@@ -755,15 +762,8 @@ class NaylisAttention(nn.Module):
             wq, wk, eps = self.q_norm.weight, self.k_norm.weight, self.q_norm.eps
             inv = None if self.rope is None else self.rope.inv_freq
         elif self.rope is not None:  # rounded as rope_varlen rounds without a norm
-            pos = t.positions
-            if pos is None:
-                rows = torch.arange(x2.shape[0], device=x.device)
-                b = torch.searchsorted(cu[1:].contiguous(), rows.to(cu.dtype), right=True)
-                b = b.clamp(max=t.seqlens.shape[0] - 1)
-                pos = rows - cu[b + 1] + t.seqlens[b]
-            cos, sin = self.rope._table(max(t.next_position, default=0), q.device, q.dtype)
-            pos = pos.long().clamp(0, cos.shape[0] - 1)
-            cos, sin = cos[pos][:, None], sin[pos][:, None]
+            cos, sin = self.rope._at(t.token_positions(x2.shape[0], cu), q.dtype)
+            cos, sin = cos[:, None], sin[:, None]
             q, k = self.rope.rotate(q, cos, sin), self.rope.rotate(k, cos, sin)
         q = paged_append(q, k, v, cache.k, cache.v, t.block_table, t.seqlens, cu, r_k, cache.r_k,
                          inv, None, wq, wk, eps, t.position_shift if inv is not None else None)

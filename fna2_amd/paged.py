@@ -448,6 +448,18 @@ class PageTable:
             return None
         return torch.tensor(self._positions, dtype=torch.int32, device=self.seqlens.device)
 
+    def token_positions(self, tokens: int, cu_seqlens_q: Optional[torch.Tensor] = None
+                        ) -> torch.Tensor:
+        """[tokens] positions of a step's packed tokens, formed on the device from
+        what this table keeps there, so that a captured step forms its own anew.
+        (Tokens of no sequence: any number.)"""
+        row = torch.arange(tokens, device=self.seqlens.device)
+        if not self.rows:
+            return row
+        cu = self.cu_seqlens_q if cu_seqlens_q is None else _ints(cu_seqlens_q, row.device)
+        b = torch.searchsorted(cu[1:], row.to(cu.dtype), right=True).clamp(max=len(self.rows) - 1)
+        return row - cu[b + 1] + self.seqlens[b] + self.position_shift[b]
+
     def _upload(self, table: bool) -> None:
         shift = [p - r for r, p in zip(self.rows, self.next_position)]
         self._step.copy_(torch.tensor(self.rows + shift + self._cu, dtype=torch.int32))

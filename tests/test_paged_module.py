@@ -347,3 +347,98 @@ def test_steps_after_an_eviction(gpu, graph):
                             t.seqlens, t.cu_seqlens_q, r_q, c.r_k, m.graph_scale)[0]
             ref = out.reshape(2, 512) @ f64(m.out_proj.weight).T
             assert rel_norm(y, ref) < 4 * 2.0 ** -8, step
+
+
+def test_positions_of_packed_tokens():
+    t = PageTable(3, 12, page_size=16, max_pages=6)
+    t.extend([50, 10, 0])
+    t.truncate(20)
+    t.extend([2, 0, 3])
+    assert t.token_positions(5).tolist() == t.positions.tolist() == [50, 51, 0, 1, 2]
+    # tokens of no sequence before and behind
+    cu = torch.tensor([2, 4, 4, 7])
+    assert t.token_positions(9, cu)[2:7].tolist() == [50, 51, 0, 1, 2]
+    assert t.token_positions(0).shape == (0,)
+    assert PageTable(0, 4, page_size=16).token_positions(3).shape == (3,)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rotation_at_positions_is_the_tables(dtype):
+    """Row by row the same bits, at positions that the type rounds as well."""
+    from fna2_amd.attention_fna2 import RotaryPositionalEmbedding
+    rope = RotaryPositionalEmbedding(64)
+    for device in ["cpu"] + (["cuda"] if torch.cuda.is_available() else []):
+        table = rope._table(3001, torch.device(device), dtype)
+        pos = torch.tensor([0, 1, 255, 256, 257, 1000, 1001, 2049, 3000, 5], device=device)
+        for ids in (pos, pos.int()):
+            for a, b in zip(rope._at(ids, dtype), table):
+                assert torch.equal(a, b[pos])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(use_qk_norm=False), dict()])
+def test_a_graph_at_positions_past_its_capture(gpu, kw):
+    """A step captured early and replayed far past it, with evictions, and with
+    the layer's own table growing between."""
+    m = _layer(gpu, **kw)
+    t = PageTable(2, 40, page_size=16, device=gpu)
+    a, b = _cache(m, t, weigh=True), _cache(m, t, weigh=True)
+    g = torch.Generator().manual_seed(3)
+    x0 = torch.randn(12, 512, generator=g).bfloat16().to(gpu)
+    with torch.no_grad():
+        t.extend([7, 5])
+        for c in (a, b):
+            m(x0, past_kv=c)
+        t.extend([1, 1])
+        x = torch.randn(2, 512, generator=g).bfloat16().to(gpu)
+        for _ in range(2):
+            m(x, past_kv=a)
+        m(x, past_kv=b)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, _ = m(x, past_kv=a)
+        for i in range(60):
+            if i % 25 == 20:
+                b.key_weights.copy_(a.key_weights)
+                for c in (a, b):
+                    c.evict(16, recent=4, first=1, heads=8)
+                t.truncate(16)
+            if i % 20 == 10:
+                m.rope._table(100 + 10 * i, gpu, torch.bfloat16)
+            t.extend([1, 1])
+            x.copy_(torch.randn(2, 512, generator=g).bfloat16())
+            want, _ = m(x, past_kv=b)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), i
+            assert torch.equal(a.k, b.k), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(use_qk_norm=False), dict()])
+def test_a_padded_step(gpu, kw):
+    """cu_seqlens_q of the caller's, with tokens of no sequence around the
+    others, after an eviction: what the step without them gives.
+
+    The projections of differing numbers of rows may round to other neighbours
+    (2^-7), and after them the rotation (2^-8, without a norm three times): in 5 of 55
+    rows a cache, a third of 2^-7 + 6 * 2^-8 of its norm."""
+    m = _layer(gpu, **kw)
+    t = PageTable(2, 40, page_size=16, device=gpu)
+    a, b = _cache(m, t, weigh=True), _cache(m, t, weigh=True)
+    g = torch.Generator().manual_seed(3)
+    x0 = torch.randn(80, 512, generator=g).bfloat16().to(gpu)
+    with torch.no_grad():
+        t.extend([50, 30])
+        for c in (a, b):
+            m(x0, past_kv=c)
+            c.evict(25, heads=8)
+        t.truncate(25)
+        t.extend([1, 4])
+        x = torch.randn(9, 512, generator=g).bfloat16().to(gpu)
+        want, _ = m(x[2:7], past_kv=a)
+        cu = torch.tensor([2, 3, 7], dtype=torch.int32, device=gpu)
+        got, _ = m(x, past_kv=b, cu_seqlens_q=cu)
+    assert rel_norm(got[2:7], want.double().cpu().numpy()) < 5 * 2.0 ** -8
+    assert rel_norm(b.k, a.k.double().cpu().numpy()) < 8 / 3 * 2.0 ** -8
