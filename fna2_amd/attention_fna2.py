@@ -753,18 +753,25 @@ class NaylisAttention(nn.Module):
             raise ValueError(f"{x2.shape[0]} tokens, but the PageTable was extended by {t.total_q}")
         q, k, v, r_q, r_k = self._project(x2)
         orig_dtype = q.dtype
-        if q.dtype != cache.k.dtype:
-            q, k, v = (y.to(cache.k.dtype) for y in (q, k, v))
         wq = wk = inv = None
         eps = 1e-6
-        if self.use_qk_norm:  # with the rotation in the append's launch, in fp32
+        if self.use_qk_norm and q.dtype == cache.k.dtype:
+            # with the rotation in the append's launch: in fp32, rounded once
             assert self.q_norm.eps == self.k_norm.eps
             wq, wk, eps = self.q_norm.weight, self.k_norm.weight, self.q_norm.eps
             inv = None if self.rope is None else self.rope.inv_freq
-        elif self.rope is not None:  # rounded as rope_varlen rounds without a norm
-            cos, sin = self.rope._at(t.token_positions(x2.shape[0], cu), q.dtype)
-            cos, sin = cos[:, None], sin[:, None]
-            q, k = self.rope.rotate(q, cos, sin), self.rope.rotate(k, cos, sin)
+        else:
+            # Other activations than the cache's (fp32): the same chain, rounded to
+            # the cache's type behind it.  Without a norm the rotation rounds as
+            # rope_varlen does, in the activations' type.
+            if self.use_qk_norm:
+                q, k = self.q_norm(q.float()), self.k_norm(k.float())
+            if self.rope is not None:
+                cos, sin = self.rope._at(t.token_positions(x2.shape[0], cu),
+                                         torch.float64 if self.use_qk_norm else q.dtype)
+                cos, sin = cos[:, None].to(q.dtype), sin[:, None].to(q.dtype)
+                q, k = self.rope.rotate(q, cos, sin), self.rope.rotate(k, cos, sin)
+        q, k, v = (y.to(cache.k.dtype) for y in (q, k, v))
         q = paged_append(q, k, v, cache.k, cache.v, t.block_table, t.seqlens, cu, r_k, cache.r_k,
                          inv, None, wq, wk, eps, t.position_shift if inv is not None else None)
         out = flash_naylis_paged(q, cache.k, cache.v, t.block_table, t.seqlens, cu, max_q, r_q,

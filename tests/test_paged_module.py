@@ -442,3 +442,61 @@ def test_a_padded_step(gpu, kw):
         got, _ = m(x, past_kv=b, cu_seqlens_q=cu)
     assert rel_norm(got[2:7], want.double().cpu().numpy()) < 5 * 2.0 ** -8
     assert rel_norm(b.k, a.k.double().cpu().numpy()) < 8 / 3 * 2.0 ** -8
+
+
+# ── Activations of another type than the cache's ─────────────────────────────
+
+def _prompt_and_steps(m, gpu, x, splits, **kw):
+    """x [T, E] served as one sequence in pieces: (outputs, the cache, its table)."""
+    t = PageTable(1, x.shape[0] // 16 + 2, page_size=16, device=gpu)
+    c = _cache(m, t, **kw)
+    out, at = [], 0
+    with torch.no_grad():
+        for n in splits:
+            t.extend([n])
+            out.append(m(x[at:at + n], past_kv=c)[0])
+            at += n
+    return torch.cat(out), c, t
+
+
+def _rows_of(c, n, pool):
+    ids = c.table.block_table[0, : -(-n // c.table.page_size)].long()
+    return pool[ids].transpose(1, 2).reshape(-1, pool.shape[1], pool.shape[3])[:n]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cached", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("norm", [True, False])
+def test_an_fp32_layer_on_pages(gpu, norm, cached):
+    """fp32 activations are normalised and rotated in fp32 and rounded once, to
+    the cache's type: the cached keys are within half a step of the definition, and
+    (bf16) the layer gives what its own forward does, also far along.
+
+    Keys: 1e-5 on top for the fp32 chain of values of order one.  Without a norm the
+    angles are the fp32 products that the layer's table holds."""
+    m = _layer(gpu, torch.float32, use_qk_norm=norm)
+    g = torch.Generator().manual_seed(5)
+    if norm:
+        with torch.no_grad():
+            m.k_norm.weight.copy_(1 + 0.2 * torch.randn(64, generator=g))
+    n = 1100
+    x = torch.randn(n, 512, generator=g).to(gpu)
+    y, c, _ = _prompt_and_steps(m, gpu, x, [1000, 98, 1, 1], dtype=cached)
+    assert y.dtype == torch.float32
+    with torch.no_grad():
+        k = torch.cat([m._project(p)[1] for p in torch.split(x, [1000, 98, 1, 1])]).double().cpu()
+        ref, _ = m(x, cu_seqlens_q=torch.tensor([0, n], dtype=torch.int32, device=gpu), max_seqlen_q=n)
+    if norm:
+        k = k / torch.sqrt(k.square().mean(-1, keepdim=True) + m.k_norm.eps) * m.k_norm.weight.double().cpu()
+        ang = torch.outer(torch.arange(n).double(), m.rope.inv_freq.double().cpu())
+    else:
+        ang = torch.outer(torch.arange(n).float(), m.rope.inv_freq.float().cpu()).double()
+    a, b = k.chunk(2, -1)
+    cos, sin = ang.cos()[:, None], ang.sin()[:, None]
+    want = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+    got = _rows_of(c, n, c.k).double().cpu()
+    half = torch.finfo(cached).eps / 2
+    assert ((got - want).abs() <= half * want.abs() + 1e-5).all()
+    if cached == torch.bfloat16:
+        # (the rotated q and k, P and the attention's output, each half a step)
+        assert rel_norm(y, ref.double().cpu().numpy()) < 4 * 2.0 ** -8
