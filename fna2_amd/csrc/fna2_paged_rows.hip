@@ -55,7 +55,9 @@ __global__ __launch_bounds__(64 * kAppWaves) void paged_append_kernel(const Page
     int64_t page = -1;
     if (inside) {
       const PagedSeq e = paged_seq_uniform(kargs(), lo);
-      row = e.lk - e.lq + (t - e.q0);
+      // (a sequence past its table: its tokens keep their rows, and those that
+      // the table does not have are not stored)
+      row = max(uni(*const_space(P.lens + lo)), 0) - e.lq + (t - e.q0);
       if (A.shift) shift = uni(*const_space(A.shift + lo));
       if (row >= 0 && row < e.lk) {
         const int pg = page_of(P.ps_mul, P.ps_shift, row);

@@ -14,7 +14,10 @@ The new tokens of a call are packed, as in ``flash_naylis_attn``'s varlen
 mode: tokens ``[cu_seqlens_q[b], cu_seqlens_q[b + 1])`` belong to sequence b.
 They are the last rows of its cache: ``seqlens_k[b]`` counts the rows in use,
 theirs included.  One token a sequence is a decode step, a piece of a prompt a
-prefill, and one call may hold both, and sequences without a token.
+prefill, and one call may hold both, and sequences without a token.  A length
+past the rows that the table has room for: the append stores the tokens whose
+rows the table has, at those rows, and drops the others; the other calls take
+the length to be that number of rows.
 
 A step of a server is ``paged_append`` (q and k normalised and rotated, k, v
 and R_k into their pages), then ``flash_naylis_paged``; where the cache has
@@ -269,9 +272,10 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
     ``rope_varlen`` with a norm does.  A token's position is its cache row, or
     ``positions[t]`` (int32), plus ``position_shift[b]`` (int32 ``[N]``) of its
     sequence: after an eviction a sequence's rows and positions differ by a
-    number.  ``seqlens_k`` counts the rows after the append.  Rows before 0 or past the table are not
-    stored; tokens of no sequence keep their q and store nothing.  Pages that
-    are written may belong to one sequence only."""
+    number.  ``seqlens_k`` counts the rows after the append.  Rows before 0 or
+    past the table are not stored (no other row gives way to them); tokens of no
+    sequence keep their q and store nothing.  Pages that are written may belong
+    to one sequence only."""
     what = "paged_append"
     nat = _capi.native_or_none() if q.is_cuda else None
     if nat is not None:

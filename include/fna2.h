@@ -325,7 +325,10 @@ int fna2_decode_rows(const fna2_decode_rows_args* args, void* hip_stream);
  * cu_seqlens_q[b+1]) of [T, heads, f] belong to sequence b (any number, none
  * included) and are the last of the seqlens_k[b] rows that its cache holds,
  * theirs included: token i of lq sits at row seqlens_k[b] - lq + i.
- * seqlens_k is clamped to [0, table_width * page_size]. */
+ * seqlens_k below 0 is 0.  Past table_width * page_size, the rows that the
+ * table has room for, the append stores the tokens whose rows the table has, at
+ * those rows, and drops the others; every other call takes the length to be
+ * that size, and with it, causal, the chunk to be the last lq of those rows. */
 typedef struct fna2_paged_cache {
   int32_t dtype;        /* FNA2_BF16 or FNA2_F16: q, k, v, out; R_q, R_k bf16   */
   int32_t batch;        /* N sequences                                          */
@@ -396,7 +399,7 @@ int fna2_paged_weights(const fna2_paged_weights_args* args, void* hip_stream);
  * given; y as in fna2_rope_args), in fp32 (the angle in fp64) with one
  * rounding; q to q_out [T, H, D], k, v and r_k to their pages.  Tokens of no
  * sequence: q copied, nothing stored.  Rows before 0 or past the table: not
- * stored. */
+ * stored, and no row is moved for them. */
 typedef struct fna2_paged_append_args {
   fna2_paged_cache c;          /* (max_seqlen_q unused)                         */
   fna2_tensor q, k, v, r_k;    /* [T, H, D], [T, H_KV, D] x 2, [T, H_G, R]     */

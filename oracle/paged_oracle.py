@@ -91,7 +91,7 @@ def append(q, k, v, k_pages, v_pages, table, lens, cu, r_k=None, rk_pages=None, 
     cap = table.shape[1] * ps
     out = q.copy()
     for b in range(len(lens)):
-        n = min(max(int(lens[b]), 0), cap)
+        n = max(int(lens[b]), 0)
         m = int(cu[b + 1] - cu[b])
         for i in range(m):
             t, row = int(cu[b]) + i, n - m + i

@@ -1101,3 +1101,49 @@ def test_append_position_shift(gpu, monkeypatch, lq, given, native):
     with pytest.raises(AssertionError, match="position_shift"):
         paged.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu,
                            position_shift=shift.to(gpu))
+
+
+# ── A chunk that outgrows its table ──────────────────────────────────────────
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[100, 30], [70, 10 ** 8], [2 ** 31 - 1, 64]])
+def test_append_past_the_table(gpu, lens):
+    """A chunk that outgrows its table: the tokens whose rows the table holds are
+    stored at those rows, the others are not, and no older row is touched."""
+    c = Case([50, 20], [64, 64], 4, 2, 3, 64, 16, 16, device=gpu, width=4, seed=6)
+    c.lens = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    before = c.k.clone(), c.v.clone(), c.rk.clone()
+    ref = PO.append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, c.rkn, c.rk)
+    q = paged.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, c.rkn, c.rk)
+    for a, b in zip((q, c.k, c.v, c.rk), ref):
+        assert (a.double().cpu().numpy() == b).all()
+    for b, m in enumerate(c.lq):
+        for j in range(min(max(lens[b] - m, 0), 64)):
+            p, r = c.slot(b, j)
+            for pool, old in zip((c.k, c.v, c.rk), before):
+                assert torch.equal(pool[p, :, r], old[p, :, r]), (b, j)
+
+
+@pytest.mark.gpu
+def test_append_past_the_table_keeps_positions(gpu):
+    """... and each token is rotated for its own row, stored or not."""
+    c = Case([50, 20], [64, 64], 4, 2, 0, 64, 0, 16, device=gpu, width=4, seed=6)
+    c.lens = torch.tensor([100, 70], dtype=torch.int32, device=gpu)
+    inv = 10000.0 ** (-torch.arange(0, 64, 2).float() / 64)
+    ref = PO.append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, inv_freq=inv)
+    q = paged.paged_append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu, inv_freq=inv.to(gpu))
+    for a, b in zip((q, c.k, c.v), ref):
+        a = a.double().cpu().numpy()
+        assert (np.abs(a - b) <= HALF[c.dtype] * np.abs(b) + 1e-5).all()
+
+
+def test_oracle_append_past_the_table():
+    """Row by row: token i of m belongs to row lens - m + i, and is stored where
+    the table has that row."""
+    c = Case([50], [64], 2, 1, 0, 64, 0, 16, width=4)
+    c.lens[0] = 100
+    _, kp, vp, _ = PO.append(c.q, c.kn, c.vn, c.k, c.v, c.table, c.lens, c.cu)
+    for j in range(64):
+        p, r = c.slot(0, j)
+        want = c.kn[j - 50] if j >= 50 else c.k[p, :, r]
+        assert (kp[p, :, r] == want.double().numpy()).all()
