@@ -10,8 +10,10 @@
 // Long chunks (weigh kernel): a wave keeps 32 keys (K, and R_k of the head at
 // hand) in registers and walks the chunk's row tiles, 32 tokens of one head
 // each, which the workgroup's four waves share.  They come through a two-stage LDS
-// ring by DMA, two tiles a stage (rows past the chunk as zeros), with each row's
-// -LSE log2(e) (-inf: it sees nothing, or is none).  Blocks of 128 keys, or of 64
+// ring by DMA, two tiles a stage, with each row's -LSE log2(e) (-inf: it sees nothing,
+// or is none).  Rows of a tile that no token fills, here and below, repeat the tile's
+// first one: e^{S - inf} is then 0 where that row's own weight is a number, while zeros
+// times an infinity in K or R_k would be NaN in the key's sum.  Blocks of 128 keys, or of 64
 // with the tiles halved between two waves, go round over the workgroups.
 // Bound by the exponentials: 16 of a lane's take 16 cycles each, and 8 more for scale
 // and sum, against 96 for the products of a tile at d = 64, R = 16.  2 chunks of 509
@@ -98,8 +100,8 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
     const float* const lse = (const float*)P->lse.ptr + (int64_t)e.q0 * P->lse.ss + (int64_t)hkv0 * P->lse.sh;
     const int64_t qsh = P->q.sh * 2, rsh = P->rq.sh * 2, lss = P->lse.ss, lsh = P->lse.sh;
     auto issue = [&](int h, int tt, uint8_t* base) {
-      const bool on = 32 * tt + drow < e.lq;
-      const uint32_t vo = on ? (uint32_t)drow * qss + 16u * lch : kOOB;
+      const uint32_t row = 32 * tt + drow < e.lq ? drow : 0;
+      const uint32_t vo = row * qss + 16u * lch;
       const auto rs = make_rsrc(qbase + (int64_t)(32 * tt) * qss + h * qsh, 0x7ffffff0u);
 #pragma unroll
       for (int j = 0; j < C::NQ; ++j) {
@@ -108,7 +110,7 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
                                                  vo + 64u * (slot >> 1), 0, 0, 0);
       }
       if constexpr (RC > 0) {
-        const bool g = on && hkv0 + h < HG;
+        const bool g = hkv0 + h < HG;
         const auto rr = make_rsrc(HG > 0 ? rbase + (int64_t)(32 * tt) * rss + h * rsh : qbase, 0x7ffffff0u);
 #pragma unroll
         for (int j = 0; j < C::NR; ++j) {
@@ -117,7 +119,7 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
             const int c = 4 * (slot >> 1) + lch;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 rr, (lds_void*)(base + C::QBYTES + slot * 1024), 16,
-                g && c < crr ? (uint32_t)drow * rss + 16u * c : kOOB, 0, 0, 0);
+                g && c < crr ? row * rss + 16u * c : kOOB, 0, 0, 0);
           }
         }
       }
@@ -358,29 +360,29 @@ __device__ __forceinline__ void glance_body(const PagedWeightsParams& W) {
         gg = KSR > 0 ? min(max(min(HG - h0, group - sub * gsub), 0), gsub) : 0;
         lim0 = off + t0;
         const bool on = tk < tpt && t0 + tk < e.lq && hc < min(gsub, group - sub * gsub);
-        const int64_t t = e.q0 + (on ? t0 + tk : 0);
-        const int h = h0 + (on ? hc : 0);
+        const int64_t t = e.q0 + t0 + (on ? tk : 0);
+        const int hr = on ? hc : 0, h = h0 + hr;
         const uint16_t* qrow = (const uint16_t*)P->q.ptr + t * P->q.ss + (int64_t)h * P->q.sh + 8 * hl;
 #pragma unroll
         for (int s = 0; s < KSD; ++s) {
           u32x4 w = ld16(qrow + 16 * s);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = (w[k] & (on ? qand : 0u)) ^ qxor;
+          for (int k = 0; k < 4; ++k) w[k] = (w[k] & qand) ^ qxor;
           qreg[s] = as_bf16x8(w);
         }
         if constexpr (KSR > 0) {
           const uint16_t* rrow = (const uint16_t*)P->rq.ptr + t * P->rq.ss + (int64_t)h * P->rq.sh;
 #pragma unroll
           for (int s = 0; s < KSR; ++s) {
-            const int c = 2 * s + hl - hc * crr;  // this row's own head's chunks only
+            const int c = 2 * s + hl - hr * crr;  // this row's own head's chunks only
             u32x4 w = {0, 0, 0, 0};
-            if (on && hc < gg && c >= 0 && c < crr) w = ld16(rrow + 8 * c);
+            if (hr < gg && c >= 0 && c < crr) w = ld16(rrow + 8 * c);
             qreg[KSD + s] = as_bf16x8(w);
           }
         }
         float l = kNegInf, g = 0.f;
         if (on) l = ((const float*)P->lse.ptr)[t * P->lse.ss + (int64_t)h * P->lse.sh];
-        if (KSR > 0 && hc < gg) g = P->gs[h0 + hc] / P->c;
+        if (KSR > 0 && hr < gg) g = P->gs[h] / P->c;
         l = l == kNegInf ? kNegInf : -l * kLog2e;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {

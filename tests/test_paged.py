@@ -1147,3 +1147,25 @@ def test_oracle_append_past_the_table():
         p, r = c.slot(0, j)
         want = c.kn[j - 50] if j >= 50 else c.k[p, :, r]
         assert (kp[p, :, r] == want.double().numpy()).all()
+
+
+# ── Infinities ───────────────────────────────────────────────────────────────
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("scores", [True, False])
+@pytest.mark.parametrize("lq", [[1, 1], [5, 3], [40, 33]])
+@pytest.mark.parametrize("H,HKV,HG,R", [(4, 2, 3, 16), (4, 4, 4, 8), (6, 2, 0, 0)])
+def test_weights_of_rows_with_infinite_keys(gpu, lib, monkeypatch, H, HKV, HG, R, lq, scores, causal):
+    """A visible row whose score is minus infinity for every token and head weighs
+    0: rows of a tile that no token fills do not add to it."""
+    if not scores:
+        monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+        monkeypatch.setattr(lib, "fna2_paged_scores_bytes", lambda a: 0)
+    c = Case(lq, [75, 61], H, HKV, HG, 64, R, 16, device=gpu, seed=9)
+    c.q[:, :, 5] = -c.q[:, :, 5].abs() - 0.25
+    for b in range(2):
+        for j in (0, 2):
+            p, r = c.slot(b, j)
+            c.k[p, :, r, 5] = float("inf")
+    check_attend(c, causal=causal)
