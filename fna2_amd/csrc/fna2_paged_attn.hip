@@ -246,7 +246,8 @@ __device__ __forceinline__ void packed_body() {
     for (int d = 0; d < D / 32; ++d) oacc[d] = f32x16{};
     float m_i = kNegInf, l_i = 0.f;
 
-    auto step = [&](int t, uint8_t* cur_st, uint8_t* nxt_st) {
+    auto step = [&](auto apart, int t, uint8_t* cur_st, uint8_t* nxt_st) {
+      constexpr bool APART = decltype(apart)::value;
       // (loads and stores end in order: those before the scores have)
       if (stored) paged_wait<4>();
       else paged_wait<0>();
@@ -266,11 +267,28 @@ __device__ __forceinline__ void packed_body() {
       const uint8_t* rl = kl + C::KBYTES;
       const uint8_t* vl = rl + C::RBYTES;
       f32x16 acc = f32x16{};
-      if constexpr (RC > 0) {
+      if constexpr (RC > 0 && !APART) {
 #pragma unroll
         for (int s = 0; s < C::KSR; ++s)
           if (s < nrs) acc = mfma32(row_read<kPagBN>(rl, rdl, 0, s), qreg[C::KSD + s], acc);
         acc *= bh;
+      }
+      if constexpr (APART) {  // a chain for each head, without the others' ranks
+        const int cr = uni(kargs()->R / 8);
+#pragma unroll 1
+        for (int hh = 0; hh * cr < uni(rch); ++hh) {
+          f32x16 own = f32x16{};
+#pragma unroll
+          for (int s = 0; s < C::KSR; ++s) {
+            const int c = 2 * s + hl - hh * cr;
+            u32x4 w = as_u32x4(row_read<kPagBN>(rl, rdl, 0, s));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = c >= 0 && c < cr ? w[i] : 0u;
+            own = mfma32(as_bf16x8(w), qreg[C::KSD + s], own);
+          }
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[v] = hc == hh ? own[v] * bh : acc[v];
+        }
       }
 #pragma unroll
       for (int s = 0; s < C::KSD; ++s)
@@ -349,10 +367,34 @@ __device__ __forceinline__ void packed_body() {
     };
 
     for (int t = s0; t < s1; t += 2) {
-      step(t, st0, st1);
-      if (t + 1 < s1) step(t + 1, st1, st0);
+      step(std::false_type{}, t, st0, st1);
+      if (t + 1 < s1) step(std::false_type{}, t + 1, st1, st0);
     }
     paged_wait<0>();  // no DMA may still write when the ring is used again, or the wave ends
+    // R_q's zeros keep the heads of a tile apart, but not from an infinity or a NaN in
+    // another's R_k row, which times zero is NaN.  Where a sum is NaN the part is done
+    // again, a rank chain for each head (in the step itself: 50 scalar registers more
+    // spilled).
+    if constexpr (RC > 0) {
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(live && l_i != l_i) != 0 && rch > 0, 0)) {
+        KArg p = kargs();
+        page = page_of(p->ps_mul, p->ps_shift, 32 * s0), poff = 32 * s0 - page * ps;
+        ids.load(lane, page);
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) oacc[d] = f32x16{};
+        m_i = kNegInf, l_i = 0.f;
+        stored = false;
+        gone = issue(s0, st0);
+        uint8_t *cur = st0, *nxt = st1;
+#pragma unroll 1
+        for (int t = s0; t < s1; ++t) {
+          step(std::true_type{}, t, cur, nxt);
+          uint8_t* const was = cur;
+          cur = nxt, nxt = was;
+        }
+        paged_wait<0>();
+      }
+    }
 
     P = kargs();
     const float l_tot = wave_pair_sum(l_i);

@@ -431,6 +431,44 @@ __device__ __forceinline__ void glance_body(const PagedWeightsParams& W) {
         }
       };
 
+      // The sum of this lane's rows of tile `i` for key 32 s + col, a product at a
+      // time: each head meets its own ranks only (in the tile an infinity or a NaN in
+      // another head's R_k comes as NaN, times a zero of R_q's).
+      auto one_by_one = [&](int s) {
+        int id, row;
+        find(s, id, row);
+        const int key = 32 * s + col, t0 = lim0 - off, hs = min(gsub, group - (h0 - h00));
+        float part = 0.f;
+        if ((uint32_t)id >= (uint32_t)npages) return part;
+        auto dot = [](auto f16, const uint16_t* x, const uint16_t* y, int n) {
+          constexpr bool F = decltype(f16)::value;
+          float d = 0.f;
+#pragma unroll 1
+          for (int c = 0; c < n; c += 8) {
+            const u32x4 a = ld16(x + c), b = ld16(y + c);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) d += elt_lo<F>(a[k]) * elt_lo<F>(b[k]) + elt_hi<F>(a[k]) * elt_hi<F>(b[k]);
+          }
+          return d;
+        };
+#pragma unroll 1
+        for (int v = 0; v < 16; ++v) {
+          const int rw = 8 * (v >> 2) + 4 * hl + (v & 3), t = small_div(rw, gsub), h = rw - t * gsub;
+          if (t >= tpt || t0 + t >= e.lq || h >= hs || (causal && key > lim0 + t)) continue;
+          const int64_t tok = e.q0 + t0 + t;
+          const float l = ((const float*)P->lse.ptr)[tok * P->lse.ss + (int64_t)(h0 + h) * P->lse.sh];
+          if (l == kNegInf) continue;
+          float x = P->qa * dot(std::integral_constant<bool, F16>{}, (const uint16_t*)P->q.ptr + tok * P->q.ss + (int64_t)(h0 + h) * P->q.sh,
+                                kpool + (int64_t)id * ksb + (int64_t)row * kss, D);
+          if (h < gg)
+            x += P->gs[h0 + h] / P->c *
+                 dot(std::false_type{}, (const uint16_t*)P->rq.ptr + tok * P->rq.ss + (int64_t)(h0 + h) * P->rq.sh,
+                     rpool + (int64_t)id * rsb + (int64_t)row * rss + (int64_t)(h0 + h) * rsh, P->R);
+          part += __builtin_amdgcn_exp2f(__builtin_fmaf(x, c2, -l * kLog2e));
+        }
+        return part;
+      };
+
       int id, row, id1, row1, held = -1;
       find(step, id, row);
       load_k(step, id, row);
@@ -469,17 +507,23 @@ __device__ __forceinline__ void glance_body(const PagedWeightsParams& W) {
         } else {
           ++i;
         }
+        float part = 0.f;
         if (causal && 32 * s0 + 31 > lim0) {
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
             const int rw = 8 * (v >> 2) + 4 * hl + (v & 3);
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], c2, nl[v]));
-            sum += 32 * s0 + col <= lim0 + small_div(rw, gsub) && nl[v] != kNegInf ? p : 0.f;
+            part += 32 * s0 + col <= lim0 + small_div(rw, gsub) && nl[v] != kNegInf ? p : 0.f;
           }
         } else {
 #pragma unroll
-          for (int v = 0; v < 16; ++v) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], c2, nl[v]));
+          for (int v = 0; v < 16; ++v) part += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v], c2, nl[v]));
         }
+        if constexpr (KSR > 0) {
+          if (__builtin_expect(gg > 0 && __builtin_amdgcn_ballot_w64(part != part) != 0, 0))
+            if (part != part) part = one_by_one(s0);
+        }
+        sum += part;
         if (turn) {
           sum = wave_pair_sum(sum);
           if (put) wrow[32 * s0 + col] = before + sum;

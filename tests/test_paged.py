@@ -1169,3 +1169,48 @@ def test_weights_of_rows_with_infinite_keys(gpu, lib, monkeypatch, H, HKV, HG, R
             p, r = c.slot(b, j)
             c.k[p, :, r, 5] = float("inf")
     check_attend(c, causal=causal)
+
+
+def _odd_rank_rows(c, value):
+    """R_k of graph head 1 holds `value` in one feature of a visible row of each
+    sequence; R_q's feature and the scale are such that an infinity times them
+    is minus infinity: head 1 gives the row no weight, the others are as ever."""
+    c.rq[:, 1, 3] = -c.rq[:, 1, 3].abs() - 0.25
+    c.gs[1] = 1.5
+    for b in range(c.N):
+        p, r = c.slot(b, min(2, c.lk[b] - c.lq[b]))
+        c.rk[p, 1, r, 3] = value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scores", [True, False])
+@pytest.mark.parametrize("hint", [None, 1, 10 ** 6])
+@pytest.mark.parametrize("lq", [[1, 1], [5, 3], [40, 33]])
+@pytest.mark.parametrize("H,HKV,HG,D,R", [(4, 1, 3, 64, 8), (8, 2, 6, 128, 16), (12, 4, 12, 64, 24),
+                                          (32, 1, 20, 64, 64)])
+def test_infinite_ranks_stay_with_their_head(gpu, lib, monkeypatch, H, HKV, HG, D, R, lq, hint, scores):
+    """Heads share a column tile with their ranks side by side; a row's infinity in
+    one head's R_k reaches neither the other graph heads' results nor the vanilla
+    heads', nor the rows' weights, whatever the kernel."""
+    if not scores:
+        monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+        monkeypatch.setattr(lib, "fna2_paged_scores_bytes", lambda a: 0)
+    c = Case(lq, [75, 61], H, HKV, HG, D, R, 16, device=gpu, seed=8)
+    _odd_rank_rows(c, float("inf"))
+    check_attend(c, hint=hint)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hint", [None, 1, 10 ** 6])
+@pytest.mark.parametrize("lq", [[1, 1], [5, 3], [40, 33]])
+def test_nan_ranks_stay_with_their_head(gpu, lq, hint):
+    c = Case(lq, [75, 61], 4, 1, 3, 64, 16, 16, device=gpu, seed=8)
+    _odd_rank_rows(c, float("nan"))
+    ref, lse, _, mag = c.oracle()
+    out, got = c.attend(hint, return_lse=True)
+    assert torch.isnan(out[:, 1]).all()
+    for x in (ref, lse, mag):
+        x[:, 1] = 0.0
+    out[:, 1], got[:, 1] = 0.0, 0.0
+    close_out(c, out, ref, mag)
+    assert np.abs(got.double().cpu().numpy() - lse).max() <= 1e-4
