@@ -656,6 +656,7 @@ std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
   const Tensor &rq = opt(rq_), &w = opt(w_);
   Tensor gs = opt(gs_);
   if (!L.paged_attn || !q.defined() || !q.is_cuda() || q.dim() != 3) return std::nullopt;
+  if (!rq.defined() && (rkp_.has_value() || gs_.has_value())) return std::nullopt;
   const c10::Device dev = q.device();
   const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
   fna2_paged_attn_args a{};

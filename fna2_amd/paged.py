@@ -163,7 +163,8 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     """Attention of packed chunks of new tokens over a paged cache.
 
     q ``[T, H, D]`` (bf16 or fp16, as the pools), r_q ``[T, H_G, R]`` bf16,
-    graph_scale ``[H_G]``.  ``max_seqlen_q`` is a hint of the longest chunk (it
+    graph_scale ``[H_G]`` (the bias: r_q, rk_pages and graph_scale, or none of
+    them).  ``max_seqlen_q`` is a hint of the longest chunk (it
     picks the kernels, not the result).  Causal: token i of a chunk of lq sees
     rows ``0 .. seqlens_k - lq + i``; not causal: all ``seqlens_k``.  Hidden rows
     do not reach a token's result, whatever they hold; a token that sees no row,
@@ -188,7 +189,10 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     dev = k_pages.device
     T, H, D = q.shape
     H_G = R = 0
-    if r_q is not None:
+    if r_q is None:
+        assert rk_pages is None and graph_scale is None, \
+            f"{what}: rk_pages and graph_scale need r_q"
+    else:
         assert rk_pages is not None and graph_scale is not None, \
             f"{what}: r_q needs rk_pages and graph_scale"
         assert r_q.dim() == 3, f"{what}: r_q must be [T, H_G, R]"

@@ -1214,3 +1214,18 @@ def test_nan_ranks_stay_with_their_head(gpu, lq, hint):
     out[:, 1], got[:, 1] = 0.0, 0.0
     close_out(c, out, ref, mag)
     assert np.abs(got.double().cpu().numpy() - lse).max() <= 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_a_bias_without_its_queries_is_refused(gpu, monkeypatch, native):
+    """R_k pages or a graph scale without R_q: an attention without the bias would
+    not be what was asked for."""
+    if not native:
+        monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+    c = Case([3, 1], [70, 80], 4, 2, 4, 64, 16, 16, device=gpu)
+    args = (c.q, c.k, c.v, c.table, c.lens, c.cu, 3)
+    for kw in (dict(rk_pages=c.rk, graph_scale=c.gs), dict(rk_pages=c.rk), dict(graph_scale=c.gs)):
+        with pytest.raises(AssertionError, match="r_q"):
+            paged.flash_naylis_paged(*args, **kw)
+    paged.flash_naylis_paged(*args)
