@@ -226,6 +226,13 @@ class RotaryPositionalEmbedding(nn.Module):
         return rope_varlen(q, k, cu_seqlens, self.inv_freq, norm_q, norm_k, eps, grad_slab)
 
 
+def _plain(m: Optional[nn.Module], cls) -> bool:
+    """Whether a module is absent, or ``cls`` itself with no hook on it."""
+    return m is None or (type(m) is cls and not m._forward_hooks and not m._forward_pre_hooks and
+                         "forward" not in vars(m) and
+                         not nn.modules.module._has_any_global_hook())
+
+
 def _stacked_view(ws) -> Optional[torch.Tensor]:
     """The weights as one [sum rows, E] matrix when they are consecutive row
     blocks of one buffer (no copy), else None."""
@@ -755,7 +762,8 @@ class NaylisAttention(nn.Module):
         orig_dtype = q.dtype
         wq = wk = inv = None
         eps = 1e-6
-        if self.use_qk_norm and q.dtype == cache.k.dtype:
+        called = not self._plain_norm_rope()  # replaced or hooked modules: called as such
+        if self.use_qk_norm and q.dtype == cache.k.dtype and not called:
             # with the rotation in the append's launch: in fp32, rounded once
             assert self.q_norm.eps == self.k_norm.eps
             wq, wk, eps = self.q_norm.weight, self.k_norm.weight, self.q_norm.eps
@@ -764,11 +772,15 @@ class NaylisAttention(nn.Module):
             # Other activations than the cache's (fp32): the same chain, rounded to
             # the cache's type behind it.  Without a norm the rotation rounds as
             # rope_varlen does, in the activations' type.
+            if self.use_qk_norm and not called:
+                q, k = q.float(), k.float()
             if self.use_qk_norm:
-                q, k = self.q_norm(q.float()), self.k_norm(k.float())
-            if self.rope is not None:
-                cos, sin = self.rope._at(t.token_positions(x2.shape[0], cu),
-                                         torch.float64 if self.use_qk_norm else q.dtype)
+                q, k = self.q_norm(q), self.k_norm(k)
+            if not _plain(self.rope, RotaryPositionalEmbedding):
+                q, k = self._rotate_called(q, k, t, cu_seqlens_q)
+            elif self.rope is not None:
+                cos, sin = self.rope._at(t.token_positions(x2.shape[0], cu), torch.float64
+                                         if self.use_qk_norm and not called else q.dtype)
                 cos, sin = cos[:, None].to(q.dtype), sin[:, None].to(q.dtype)
                 q, k = self.rope.rotate(q, cos, sin), self.rope.rotate(k, cos, sin)
         q, k, v = (y.to(cache.k.dtype) for y in (q, k, v))
@@ -779,6 +791,31 @@ class NaylisAttention(nn.Module):
                                  key_weights=cache.key_weights)
         y = self._finish(out.view(x2.shape[0], self.embed_dim), orig_dtype)
         return y.view(*lead, self.embed_dim), (cache if use_kv_cache else None)
+
+    def _rotate_called(self, q, k, table: PageTable, cu_seqlens_q):
+        """q [T, H, D], k [T, H_KV, D] through a rope module that is not this
+        file's as it stands, sequence by sequence: it takes its position from
+        the host, so such a step cannot be captured."""
+        if q.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a replaced or hooked rope takes positions from the host: its "
+                               "paged steps cannot be captured into a graph")
+        cu = table._cu if cu_seqlens_q is None else cu_seqlens_q.tolist()
+        qs, ks = [q[:cu[0]]], [k[:cu[0]]]
+        for s, e, after in zip(cu, cu[1:], table.next_position):
+            if s < e:
+                if after < e - s:
+                    raise ValueError("a sequence has fewer positions than new tokens")
+                rows = lambda x: x[s:e].transpose(0, 1)[None]
+                out = self.rope(rows(q), rows(k), position_offset=after - (e - s))
+                for x, y in zip((qs, ks), out):
+                    x.append(y[0].transpose(0, 1))
+        return torch.cat(qs + [q[cu[-1]:]]), torch.cat(ks + [k[cu[-1]:]])
+
+    def _plain_norm_rope(self) -> bool:
+        """Whether q_norm, k_norm and rope are this file's modules as they stand,
+        whose work a launch may do in their place."""
+        return (_plain(self.q_norm, RMSNorm) and _plain(self.k_norm, RMSNorm) and
+                _plain(self.rope, RotaryPositionalEmbedding))
 
     def _decode_rows(self, q, k, v, r_k, cache: StaticKVCache) -> Optional[torch.Tensor]:
         """The step's QK-RMSNorm, rotation and cache append in one launch:
@@ -791,13 +828,9 @@ class NaylisAttention(nn.Module):
         if (torch.is_grad_enabled() or not _fna2_plain_eager(q) or
                 torch.is_autocast_enabled(q.device.type) or
                 type(cache) is not StaticKVCache or n >= cache.capacity or
-                (cache.r_k is None) != (r_k is None) or nn.modules.module._has_any_global_hook()):
+                (cache.r_k is None) != (r_k is None) or not self._plain_norm_rope()):
             return None
         qn, kn, rope = self.q_norm, self.k_norm, self.rope
-        for m, cls in ((qn, RMSNorm), (kn, RMSNorm), (rope, RotaryPositionalEmbedding)):
-            if m is not None and (type(m) is not cls or m._forward_hooks or
-                                  m._forward_pre_hooks or "forward" in vars(m)):
-                return None  # a replaced or hooked module is called as such
         wq, wk = None if qn is None else qn.weight, None if kn is None else kn.weight
         nat = _capi.native_or_none() if q.is_cuda else None
         if nat is None or q.dtype != torch.bfloat16 or any(

@@ -500,3 +500,94 @@ def test_an_fp32_layer_on_pages(gpu, norm, cached):
     if cached == torch.bfloat16:
         # (the rotated q and k, P and the attention's output, each half a step)
         assert rel_norm(y, ref.double().cpu().numpy()) < 4 * 2.0 ** -8
+
+
+# ── Hooked and replaced modules ──────────────────────────────────────────────
+
+def _twice(mod, args, out):
+    return tuple(2 * o for o in out) if isinstance(out, tuple) else 2 * out
+
+
+def _same(mod, args, out):
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rope", [True, False])
+def test_hooked_and_replaced_norms_are_called(gpu, rope):
+    """A hook on k_norm, or a class of its own in its place, takes part as in
+    the layer's other steps: twice its output is what weights of twice the size give."""
+    from fna2_amd.attention_fna2 import RMSNorm
+
+    class Twice(RMSNorm):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    x = torch.randn(70, 512, generator=torch.Generator().manual_seed(1)).bfloat16().to(gpu)
+    run = lambda m: _prompt_and_steps(m, gpu, x, [60, 9, 1])[0]
+    hooked, replaced, doubled, plain = (_layer(gpu, use_rope=rope) for _ in range(4))
+    hooked.k_norm.register_forward_hook(_twice)
+    own = Twice(64).to(gpu).bfloat16()
+    own.load_state_dict(replaced.k_norm.state_dict())
+    replaced.k_norm = own
+    doubled.k_norm.register_forward_hook(_same)
+    with torch.no_grad():
+        doubled.k_norm.weight.mul_(2)
+    want = run(doubled)
+    assert torch.equal(run(hooked), want) and torch.equal(run(replaced), want)
+    assert not torch.equal(run(plain), want)
+
+
+@pytest.mark.gpu
+def test_hooked_and_replaced_rotations_are_called(gpu):
+    from fna2_amd.attention_fna2 import RotaryPositionalEmbedding
+
+    class Twice(RotaryPositionalEmbedding):
+        def forward(self, q, k, position_offset=0):
+            q, k = super().forward(q, k, position_offset)
+            return 2 * q, 2 * k
+
+    x = torch.randn(70, 512, generator=torch.Generator().manual_seed(1)).bfloat16().to(gpu)
+    run = lambda m: _prompt_and_steps(m, gpu, x, [60, 9, 1])[0]
+    hooked, replaced, doubled, plain = (_layer(gpu, use_qk_norm=False) for _ in range(4))
+    hooked.rope.register_forward_hook(_twice)
+    replaced.rope = Twice(64, 256).to(gpu).bfloat16()
+    replaced.rope.inv_freq = hooked.rope.inv_freq.clone()
+    with torch.no_grad():
+        doubled.q_proj.weight.mul_(2)
+        doubled.k_proj.weight.mul_(2)
+    want = run(doubled)
+    assert torch.equal(run(hooked), want) and torch.equal(run(replaced), want)
+    assert not torch.equal(run(plain), want)
+
+
+@pytest.mark.gpu
+def test_a_hooked_rotation_after_an_eviction(gpu):
+    """Its positions are the tokens', not their rows; a step of it is not captured."""
+    hooked, plain = _layer(gpu, use_qk_norm=False), _layer(gpu, use_qk_norm=False)
+    seen = []
+    hooked.rope.register_forward_hook(
+        lambda mod, args, kw, out: seen.append(kw["position_offset"]), with_kwargs=True)
+    g = torch.Generator().manual_seed(6)
+    t = PageTable(2, 12, page_size=16, device=gpu)
+    caches = [_cache(m, t, weigh=True) for m in (hooked, plain)]
+    x0 = torch.randn(70, 512, generator=g).bfloat16().to(gpu)
+    x = torch.randn(7, 512, generator=g).bfloat16().to(gpu)
+    cu = torch.tensor([1, 3, 6], dtype=torch.int32, device=gpu)
+    with torch.no_grad():
+        t.extend([40, 30])
+        got = [m(x0, past_kv=c)[0] for m, c in zip((hooked, plain), caches)]
+        assert torch.equal(*got) and seen == [0, 0]
+        caches[1].key_weights.copy_(caches[0].key_weights)
+        for c in caches:
+            c.evict(20, heads=8)
+        t.truncate(20)
+        t.extend([2, 3])
+        got = [m(x, past_kv=c, cu_seqlens_q=cu)[0] for m, c in zip((hooked, plain), caches)]
+        assert torch.equal(*got) and seen[2:] == [40, 30]
+        assert torch.equal(caches[0].k, caches[1].k)
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="captured"):
+            with torch.cuda.graph(graph):
+                hooked(x, past_kv=caches[0], cu_seqlens_q=cu)
+    torch.cuda.synchronize()
