@@ -1326,6 +1326,36 @@ int check_pool(const fna2_tensor& t, int64_t feat) {
   return FNA2_OK;
 }
 
+// Rows of `feat` elements at the sums of multiples of some strides, that a call
+// writes: strides, from the smallest up, must step over all that lies below.
+struct Axis {
+  int64_t stride, size;
+};
+template <size_t N>
+int check_disjoint(Axis (&&a)[N], int64_t feat) {
+  std::sort(a, a + N, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
+  for (const Axis& x : a)
+    if (x.size <= 0) return FNA2_OK;
+  __int128 span = feat;
+  for (const Axis& x : a) {
+    if (x.size == 1) continue;
+    if (x.stride < span) return FNA2_E_STRIDE;
+    span += (__int128)x.stride * (x.size - 1);
+  }
+  return FNA2_OK;
+}
+
+// The pools of a call that writes them: no two rows share memory.
+int check_written_pools(const fna2_paged_cache& c) {
+  if (c.batch == 0 || c.table_width == 0 || c.num_pages == 0) return FNA2_OK;  // none is written
+  auto one = [&](const fna2_tensor& t, int64_t heads, int64_t feat) {
+    return check_disjoint({{t.stride_b, c.num_pages}, {t.stride_h, heads}, {t.stride_s, c.page_size}}, feat);
+  };
+  FNA2_TRY(one(c.k_pages, c.heads_kv, c.head_dim));
+  FNA2_TRY(one(c.v_pages, c.heads_kv, c.head_dim));
+  return c.heads_graph > 0 ? one(c.rk_pages, c.heads_graph, c.rank) : FNA2_OK;
+}
+
 int check_paged_cache(const fna2_paged_cache& c, bool chunk) {
   if (c.dtype != FNA2_BF16 && c.dtype != FNA2_F16) return FNA2_E_DTYPE;
   if (c.head_dim != 64 && c.head_dim != 128) return FNA2_E_HEAD_DIM;
@@ -1566,10 +1596,7 @@ int fna2_check_paged_weights(const fna2_paged_weights_args* w) {
     if (t->ptr && (32 * t->stride_s + g * t->stride_h) * 2 > kOff31) return FNA2_E_SHAPE;
   if (!w->attn.lse.ptr || !w->key_weights) return FNA2_E_NULL;
   if (!aligned(w->key_weights, 4)) return FNA2_E_STRIDE;
-  if ((w->attn.c.heads_kv > 1 && w->stride_h < w->capacity) ||
-      (w->attn.c.batch > 1 && w->stride_b < w->capacity))
-    return FNA2_E_STRIDE;
-  return FNA2_OK;
+  return check_disjoint({{w->stride_b, w->attn.c.batch}, {w->stride_h, w->attn.c.heads_kv}}, w->capacity);
 }
 
 int fna2_paged_weights(const fna2_paged_weights_args* w, void* stream) {
@@ -1609,6 +1636,7 @@ int fna2_paged_weights(const fna2_paged_weights_args* w, void* stream) {
 int fna2_check_paged_append(const fna2_paged_append_args* a) {
   if (!a) return FNA2_E_NULL;
   FNA2_TRY(check_paged_cache(a->c, true));
+  FNA2_TRY(check_written_pools(a->c));
   if ((a->norm_q || a->norm_k) && !std::isfinite(a->eps)) return FNA2_E_SCALE;
   for (const void* p : {(const void*)a->norm_q, (const void*)a->norm_k, (const void*)a->inv_freq,
                         (const void*)a->positions})
@@ -1649,6 +1677,7 @@ int fna2_paged_append(const fna2_paged_append_args* a, void* stream) {
 int fna2_check_paged_evict(const fna2_paged_evict_args* a) {
   if (!a) return FNA2_E_NULL;
   FNA2_TRY(check_paged_cache(a->c, false));
+  FNA2_TRY(check_written_pools(a->c));
   if (a->budget < 0 || a->recent < 0 || a->first < 0 || a->capacity < 0) return FNA2_E_SHAPE;
   if ((int64_t)a->recent + a->first > a->budget || a->budget > kMaxCached) return FNA2_E_SHAPE;
   if (a->stride_b < 0 || a->stride_h < 0) return FNA2_E_STRIDE;

@@ -745,6 +745,7 @@ OptTensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const 
       rk_.has_value() != rkp_.has_value() || !paged_cache(a.c, kp, vp, rkp_, table, lens, &cu, H))
     return std::nullopt;
   const auto dt = kp.scalar_type();
+  if (kp.data_ptr() == vp.data_ptr()) return std::nullopt;
   if (kp.size(3) != D || !new_rows(q, dev, dt, T, H, D) ||
       !new_rows(k, dev, dt, T, a.c.heads_kv, D) || !new_rows(v, dev, dt, T, a.c.heads_kv, D))
     return std::nullopt;
@@ -798,6 +799,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(
       recent + first > budget || !paged_cache(a.c, kp, vp, rkp_, table, lens, nullptr, heads))
     return std::nullopt;
   const c10::Device dev = kp.device();
+  if (kp.data_ptr() == vp.data_ptr()) return std::nullopt;
   if (!plain(w, dev) || w.scalar_type() != at::kFloat || w.dim() != 3 || w.size(0) != a.c.batch ||
       w.size(1) != a.c.heads_kv || w.stride(2) != 1 || w.size(2) > INT32_MAX)
     return std::nullopt;

@@ -8,7 +8,9 @@ of 16) anywhere in a pool: row j of sequence b is row ``j % page_size`` of page
 ``[pages, H_KV, page_size, D]`` and, with the graph bias, ``rk_pages``
 ``[pages, H_G, page_size, R]``, with any strides but a unit feature stride and
 16-byte aligned rows.  A row whose page id is outside the pool is not there:
-it is neither read nor written.  Sequences may share pages for reading.
+it is neither read nor written.  Sequences may share pages for reading.  Pools
+that a call writes (``paged_append``, ``paged_evict``) hold no two rows in one
+memory: expanded ones are refused.
 
 The new tokens of a call are packed, as in ``flash_naylis_attn``'s varlen
 mode: tokens ``[cu_seqlens_q[b], cu_seqlens_q[b + 1])`` belong to sequence b.
@@ -80,6 +82,14 @@ def _written(t: torch.Tensor, name: str) -> None:
     assert not t.requires_grad, f"{name} is written in place and cannot require a gradient"
     if t.is_inference() and not torch.is_inference_mode_enabled():
         raise RuntimeError(f"{name}: an inference tensor is written in inference mode only")
+
+
+def _written_pools(what: str, k_pages, v_pages, rk_pages) -> None:
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("rk_pages", rk_pages)):
+        if t is not None:
+            _written(t, name)
+    assert k_pages.numel() == 0 or k_pages.data_ptr() != v_pages.data_ptr(), \
+        f"{what}: k_pages and v_pages are one memory, and both are written"
 
 
 def _bump(*ts: Optional[torch.Tensor]) -> None:
@@ -323,9 +333,7 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: tor
         assert inv is not None, f"{what}: position_shift needs inv_freq"
         shift = _ints(position_shift, dev)
         assert shift.shape == (c.batch,), f"{what}: position_shift must hold one number a sequence"
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("rk_pages", rk_pages)):
-        if t is not None:
-            _written(t, name)
+    _written_pools(what, k_pages, v_pages, rk_pages)
     out = torch.empty((T, H, D), dtype=dt, device=dev)
     a.q, a.k, a.v, a.q_out = _t3(q), _t3(k), _t3(v), _t3(out)
     a.positions = None if pos is None else pos.data_ptr()
@@ -383,9 +391,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     assert w.device == dev, f"{what}: key_weights is on another device"
     if w.stride(2) != 1 and w.shape[2] > 1:
         w = w.contiguous()
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages), ("rk_pages", rk_pages)):
-        if t is not None:
-            _written(t, name)
+    _written_pools(what, k_pages, v_pages, rk_pages)
     assert 0 <= int(budget) < 1 << 31 and 0 <= int(recent) and 0 <= int(first) and \
         int(recent) + int(first) <= int(budget), f"{what}: 0 <= first + recent <= budget expected"
     N, hkv = c.batch, c.heads_kv

@@ -319,7 +319,9 @@ int fna2_decode_rows(const fna2_decode_rows_args* args, void* hip_stream);
  *     ptr + page*stride_b + head*stride_h + row*stride_s + f
  * (element strides, feature stride 1, rows 16-byte aligned).  A row whose
  * page id is outside [0, num_pages) is not there: it is neither read nor
- * written.  Pages may be shared by sequences for reading.
+ * written.  Pages may be shared by sequences for reading.  A pool that a call
+ * writes must have strides under which no two of its rows overlap, and share no
+ * memory with another.
  *
  * The new tokens of a call are packed: tokens [cu_seqlens_q[b],
  * cu_seqlens_q[b+1]) of [T, heads, f] belong to sequence b (any number, none

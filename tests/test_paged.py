@@ -1229,3 +1229,62 @@ def test_a_bias_without_its_queries_is_refused(gpu, monkeypatch, native):
         with pytest.raises(AssertionError, match="r_q"):
             paged.flash_naylis_paged(*args, **kw)
     paged.flash_naylis_paged(*args)
+
+
+# ── Rows that share memory ───────────────────────────────────────────────────
+
+def test_check_written_rows_do_not_overlap(lib):
+    """What a call writes, the pools of append and evict and the weights, has no two
+    rows in one memory; pools that are only read may."""
+    T = _capi.Tensor
+
+    def codes(**over):
+        ap, ev = _capi.PagedAppendArgs(), _capi.PagedEvictArgs()
+        ap.c, ev.c = _cache_args(**over), _cache_args(**over)
+        ap.q = ap.q_out = T(FAKE, 0, 16 * 128, 128)
+        ap.k = ap.v = T(FAKE, 0, 4 * 128, 128)
+        ap.r_k = T(FAKE, 0, 12 * 32, 32)
+        ev.budget, ev.capacity, ev.stride_b, ev.stride_h = 100, 512, 2048, 512
+        ev.key_weights, ev.weights_out, ev.kept, ev.new_lens = FAKE, 2 * FAKE, FAKE, FAKE
+        return [_st(f(ctypes.byref(a))) for f, a in ((lib.fna2_check_paged_append, ap),
+                                                     (lib.fna2_check_paged_evict, ev),
+                                                     (lib.fna2_check_paged_attn, _attn(**over)))]
+    fine, shared = ["FNA2_OK"] * 3, ["FNA2_E_STRIDE", "FNA2_E_STRIDE", "FNA2_OK"]
+    assert codes() == fine
+    assert codes(k_pages=T(FAKE, 64 * 4 * 128, 4 * 128, 128)) == fine      # rows of all heads together
+    assert codes(k_pages=T(FAKE, 64 * 128, 128, 50 * 64 * 128)) == fine    # heads outermost
+    assert codes(v_pages=T(FAKE, 2 * 4 * 64 * 128, 2 * 128, 2 * 64 * 128)) == fine  # K and V by turns
+    assert codes(k_pages=T(FAKE, 0, 128, 64 * 128)) == shared              # one page, many times
+    assert codes(v_pages=T(FAKE, 4 * 64 * 128, 128, 0)) == shared          # one head for all
+    assert codes(v_pages=T(FAKE, 64 * 128, 128, 64 * 128)) == shared       # pages that overlap
+    assert codes(rk_pages=T(FAKE, 12 * 64 * 32, 32, 63 * 32)) == shared
+    assert codes(rk_pages=T(FAKE, 11 * 64 * 32, 32, 64 * 32)) == shared
+    assert codes(v_pages=T(FAKE, 0, 128, 64 * 128), num_pages=1) == fine
+
+    w = _capi.PagedWeightsArgs()
+    w.attn, w.key_weights, w.capacity = _attn(), FAKE, 512
+    for (w.stride_b, w.stride_h), want in (((2048, 512), "FNA2_OK"), ((512, 2048), "FNA2_OK"),
+                                           ((512, 512), "FNA2_E_STRIDE"), ((1024, 512), "FNA2_E_STRIDE"),
+                                           ((512, 1536), "FNA2_E_STRIDE"), ((2047, 512), "FNA2_E_STRIDE")):
+        assert _st(lib.fna2_check_paged_weights(ctypes.byref(w))) == want, (w.stride_b, w.stride_h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_pools_that_share_memory_are_read_only(gpu, monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+    c = Case([3, 1], [70, 80], 4, 2, 4, 64, 16, 16, device=gpu)
+    w = torch.zeros(2, 2, 96, device=gpu)
+    v = c.v.clone()
+    for k_pages, v_pages in ((c.k, c.k), (c.k[:1].expand_as(c.k), c.v), (c.k, c.v[:, :1].expand_as(c.v))):
+        with pytest.raises((AssertionError, RuntimeError)):
+            paged.paged_append(c.q, c.kn, c.vn, k_pages, v_pages, c.table, c.lens, c.cu)
+        with pytest.raises((AssertionError, RuntimeError)):
+            paged.paged_evict(k_pages, v_pages, c.table, c.lens, w, 10)
+    assert torch.equal(c.v, v)
+    # read, they are what they show
+    c.v = c.v[:, :1].expand_as(c.v)
+    check_attend(c)
+    c.k = c.v
+    check_attend(c)
