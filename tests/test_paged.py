@@ -1288,3 +1288,21 @@ def test_pools_that_share_memory_are_read_only(gpu, monkeypatch, native):
     check_attend(c)
     c.k = c.v
     check_attend(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scores", [True, False])
+@pytest.mark.parametrize("dtype,H,HKV,HG,D,R,lq", [(FP, 4, 1, 3, 128, 32, [1, 4]), (BF, 6, 2, 4, 64, 8, [3, 1]),
+                                                   (FP, 8, 2, 8, 64, 40, [9, 2]), (BF, 16, 2, 16, 128, 64, [2, 1])])
+def test_infinite_ranks_in_a_split_cache(gpu, lib, monkeypatch, dtype, H, HKV, HG, D, R, lq, scores):
+    """... and where runs cut the tile: only the run that holds the row is done again,
+    and its part joins the others'."""
+    if not scores:
+        monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+        monkeypatch.setattr(lib, "fna2_paged_scores_bytes", lambda a: 0)
+    c = Case(lq, [900, 400], H, HKV, HG, D, R, 48, dtype, device=gpu, seed=10)
+    _odd_rank_rows(c, float("inf"))
+    for j in (500, 333):
+        p, r = c.slot(0, j)
+        c.rk[p, 1, r, 3] = float("inf")
+    check_attend(c)
