@@ -29,7 +29,9 @@
 // Bound by reading K, V and R_k once: 64 sequences of 4096 rows, one token each, 16
 // heads over 16 KV heads of 128, R = 32, 410 us, 5.9 TB/s (a large copy, read and written, 5.1 TB/s).
 // Few sequences are bound by the latency of the chain lengths, page ids, first
-// rows, parts, merge: 2 of 500 rows, 8 heads of 64, 7.5 us and 4.5 us for the merge.
+// rows, parts, merge: 2 of 500 rows, 8 heads of 64, 7.7 us and 4.6 us for the merge.
+// A few drafted tokens (5 for 16 ragged sequences of up to 2500 rows, 16 heads over 4,
+// R = 24) are as well: 25.6 and 7.8 us, 2.8 TB/s from three waves a CU.
 // A ring of three stages gained nothing over two: the other waves cover the loads.
 #include <algorithm>
 
@@ -60,7 +62,6 @@ struct PackCfg {
   static constexpr int STAGE = 2 * KBYTES + RBYTES;
   static constexpr int NG = CD / 4;      // column groups of a K / V tile
   static constexpr int NR = RC / 4;      // ... of an Rk tile
-  static constexpr int OPS = 4 * NG + 2 * NR;  // VMEM instructions per step
 };
 
 template <int D, int RC, bool F16>

@@ -358,7 +358,7 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Pa
   const int lk = min(max(uni(*const_space(P.lens + b)), 0), P.width * P.ps);
   const int budget = E.budget;
   if (lk <= budget) return;
-  int h, kvh, strip, chunks;  // head, its KV head, 64-byte strip, 16-byte chunks of it
+  int h, kvh, strip, chunks;  // head, its KV head, strip of the row, 16-byte chunks of it
   const int nk = P.H_KV * kstrips;
   const int which = x < nk ? 0 : x < 2 * nk ? 1 : 2;
   if (which < 2) {

@@ -17,9 +17,14 @@
 //
 // Bound by the matrix cores and, between their products, by the exponentials and the
 // rounding of P: 1024 tokens over 16,384 rows, 32 heads over 8 KV heads of 128, R = 64,
-// 346 us with the merge of the parts, 0.96 10^15 operations a second of the 1.23 10^15
-// of a large matrix product.  A step of 256 tokens beside 32 decoding sequences over
-// 4096 rows is bound by reading K, V and R_k: 122 us and 12 us.  P is rounded once, off by
+// 346 to 362 us with the merge of the parts, up to 0.96 10^15 operations a second of the
+// 1.23 10^15 of a large matrix product (matrix cores 52% of the cycles, at the 1.85 GHz
+// that the power leaves; spread evenly at 2.4 GHz products 132 us, other vector
+// instructions 125).  A step of 256 tokens beside 32 decoding sequences over 4096 rows
+// is bound by reading K, V and R_k (5.7 TB/s): 123 us and 12 us.  At d = 64, R = 16
+// (2 chunks of 509 tokens over 7001 rows, 16 heads) by neither, 48 us and 9: products
+// 10 us, vector instructions 19, waves waiting 37% of their time on two workgroups a CU,
+// and the ranks padded to 32.  P is rounded once, off by
 // half a step (bf16 2^-8) of each p at most, on top of the output's own rounding (1.4 times
 // the error of an output alone); in two parts the products with V would double.
 #include <algorithm>
@@ -520,7 +525,7 @@ __global__ __launch_bounds__(256) void paged_tile_merge_kernel(const PagedParams
 // Waves per SIMD that the register budget is cut for, and workgroups of a CU.
 // Three where one head's ranks or none come with d = 128: such tiles are long,
 // bound by the matrix cores, and a third workgroup fills the others' waits
-// (1024-token piece, rank 64: 346 us, two 351).  Two for the others: the third
+// (1024-token piece, rank 64, in turn: 346 us, two 351).  Two for the others: the third
 // costs spilled registers (mixed step, 4 heads of rank 32: 146 us, two 133; d =
 // 64, rank 16, 509-token pieces with their weights: 103, 97).  A third ring
 // stage in the room that leaves: 136 and 99.

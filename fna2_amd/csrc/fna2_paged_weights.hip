@@ -15,9 +15,14 @@
 // first one: e^{S - inf} is then 0 where that row's own weight is a number, while zeros
 // times an infinity in K or R_k would be NaN in the key's sum.  Blocks of 128 keys, or of 64
 // with the tiles halved between two waves, go round over the workgroups.
-// Bound by the exponentials: 16 of a lane's take 16 cycles each, and 8 more for scale
-// and sum, against 96 for the products of a tile at d = 64, R = 16.  2 chunks of 509
-// tokens over 7001 rows, 16 heads: 36 us, 1.9 10^12 weights a second.
+// Bound by the blocks' uneven rounds and their starts, not by a pipe: 2 chunks of 509
+// tokens over 7001 rows, 16 heads of 64, R = 16, 36 us, 2.1 10^12 weights a second.  A
+// tile's 1024 weights take 384 cycles of a SIMD's vector instructions (16 exponentials
+// of 16, scale and sum 8 each) and 192 of its products (6 of 32), which over the whole
+// chip would be 6.5 10^12 a second; counted, all vector instructions spread evenly
+// would take 18 us, the exponentials 8 of them, and the products 6.  But 1360
+// blocks for 1024 resident workgroups are two rounds, the second a third full, and a
+// block begins with a chain of page id, K row and R_k row for its 11 to 16 tiles.
 //
 // Short chunks (glance kernel, where the packed kernel runs): usually one row
 // tile holds the chunk, so a wave keeps that in registers instead and streams

@@ -28,8 +28,12 @@ calls added up.
 
 The reference's multi-token step against a cache runs PyTorch SDPA without
 the bias, or fails with it (FNA2/attention_fna2.py:412-429, :445-473).  All
-lengths and tables stay on the device: no call synchronises, and every call
-can be captured into a graph.  Forward only (no autograd).  There is no
+lengths and tables stay on the device: none of the three functions
+synchronises (given device tensors), and each can be captured into a graph.  How
+they run (parts, buffers) goes by the table's width, not by the lengths, which the
+host does not know: a table not much wider than its sequences' pages serves them
+best.  ``PageTable`` keeps its books on the host, and each of its methods waits for
+the stream while it uploads them.  Forward only (no autograd).  There is no
 fallback: without the HIP library, or off the GPU, the calls raise.
 """
 from __future__ import annotations
@@ -428,7 +432,8 @@ class PageTable:
     plus its sequence's ``position_shift``, the rows that ``truncate`` took away
     before it; ``positions`` are those of the step's tokens one by one, a tensor
     of this step only.  The bookkeeping is the host's: nothing is read back from
-    the device."""
+    the device, but each upload (one, and the block table where pages changed)
+    waits for the stream's earlier work."""
 
     def __init__(self, sequences: int, num_pages: int, page_size: int = 64,
                  max_pages: Optional[int] = None, device=None):
