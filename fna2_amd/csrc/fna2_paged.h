@@ -65,17 +65,21 @@ __device__ __forceinline__ float* paged_scores(KArg P, int b, int sg) {
 }
 
 // A sequence's tokens and rows, clamped so that no access leaves [0, T) or
-// its row of the table.
+// its row of the table.  off: the first token's row, lk - lq; more where the
+// sequence has outgrown its table (whose rows the tokens past it all see).
 struct PagedSeq {
-  int q0, lq, lk;
+  int q0, lq, lk, off;
 };
-__device__ __forceinline__ PagedSeq paged_clamp(KArg P, int qs, int qe, int lk) {
+__device__ __forceinline__ PagedSeq paged_clamp(KArg P, int qs, int qe, int len) {
   PagedSeq s;
   qs = min(max(qs, 0), P->T);
   qe = min(max(qe, qs), P->T);
   s.q0 = qs;
   s.lq = qe - qs;
-  s.lk = min(max(lk, 0), P->width * P->ps);
+  const int rows = P->width * P->ps;
+  len = max(len, 0);
+  s.lk = min(len, rows);
+  s.off = min(len - s.lq, rows);
   return s;
 }
 __device__ __forceinline__ PagedSeq paged_seq(KArg P, int b) {
@@ -133,7 +137,7 @@ struct SeqWork {
   PagedSeq s;
   __device__ __forceinline__ void scan(KArg P, int lane, int b0, int64_t before) {
     const int b = b0 + lane;
-    s = PagedSeq{0, 0, 0};
+    s = PagedSeq{0, 0, 0, 0};
     if (b < P->N) s = paged_seq(P, b);
     base = before;
     mine = b < P->N ? units(s) : 0;
@@ -161,7 +165,7 @@ struct SeqWork {
     at.b = b0 + l;
     at.rem = u - lane64(end - mine, l);
     at.s = PagedSeq{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.lq, l),
-                    __builtin_amdgcn_readlane(s.lk, l)};
+                    __builtin_amdgcn_readlane(s.lk, l), __builtin_amdgcn_readlane(s.off, l)};
     return at;
   }
 };
@@ -218,14 +222,21 @@ struct TilePlan {
   // Units of tiles 0 .. m - 1, none of them the sequence's last.
   __device__ __forceinline__ static int64_t before(KArg P, const PagedSeq& s, int m) {
     if (!P->causal) return (int64_t)m * max(cdiv(s.lk, 32), 1);
-    const int t = 4 / P->hw, off = s.lk - s.lq;
+    const int t = 4 / P->hw, off = s.off;
+    if (off + m * tokens(P) > s.lk) {  // (the last ones of a sequence past its table see all its rows)
+      const int n = min(max(s.lk - off, 0) / tokens(P), m);
+      return before_end(t, off, n) + (int64_t)(m - n) * max(cdiv(s.lk, 32), 1);
+    }
+    return before_end(t, off, m);
+  }
+  __device__ __forceinline__ static int64_t before_end(int t, int off, int m) {
     const int64_t a = off >= 0 ? (off + 31) / 32 : -(-off / 32);  // ceil(off / 32)
     const int64_t n0 = a > 0 ? 0 : min((int64_t)m, -a / t);       // tiles that see no row
     return n0 + a * (m - n0) + t * ((int64_t)m * (m + 1) - n0 * (n0 + 1)) / 2;
   }
   __device__ __forceinline__ static int steps(KArg P, const PagedSeq& s, int i) {
     int vis = s.lk;
-    if (P->causal) vis = min(vis, s.lk - s.lq + (i + 1) * tokens(P));
+    if (P->causal) vis = min(vis, s.off + (i + 1) * tokens(P));
     return max(cdiv(max(vis, 0), 32), 1);
   }
   __device__ __forceinline__ static int64_t head_units(KArg P, const PagedSeq& s) {

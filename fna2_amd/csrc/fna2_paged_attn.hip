@@ -126,7 +126,7 @@ __device__ __forceinline__ void packed_body() {
     const int rch = gg * crr, nrs = cdiv(rch, 2);
     const int tok = ct * P->tpt + tk;
     const bool live = tk < P->tpt && tok < e.lq && hc < nh;
-    const int off = e.lk - e.lq;
+    const int off = e.off;
     // last key that this column, and that every column, sees
     const int lim = min(causal ? off + tok : e.lk, e.lk - 1);
     const int lim_all = causal ? min(off + ct * P->tpt, e.lk - 1) : e.lk - 1;

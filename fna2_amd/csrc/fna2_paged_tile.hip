@@ -118,7 +118,7 @@ __device__ __forceinline__ void tile_body() {
     const int s1 = (int)min((int64_t)steps, s0 + left);
     const int kvh = hb / hblk, h_in = (hb - kvh * hblk) * hw + wv % hw;
     const int h = kvh * P->group + min(h_in, P->group - 1);
-    const int off = e.lk - e.lq;
+    const int off = e.off;
     const int tok0 = qt * TB + 32 * (wv / hw);  // this wave's first token
     const bool idle = tok0 >= e.lq || h_in >= P->group;
     const int tok_last = min(tok0 + 31, e.lq - 1);

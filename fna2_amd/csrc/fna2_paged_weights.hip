@@ -80,7 +80,7 @@ __device__ __forceinline__ void weigh_body(const PagedWeightsParams& W) {
     const int nkb = cdiv(e.lk, keys);
     const int kvh = uni((int)div64(at.rem, nkb));
     const int kb = keys * (int)(at.rem - (int64_t)kvh * nkb);
-    const int k0 = kb + 32 * (wv & (kw - 1)), key = k0 + col, off = e.lk - e.lq;
+    const int k0 = kb + 32 * (wv & (kw - 1)), key = k0 + col, off = e.off;
     const bool causal = P->causal != 0;
     int page = -1, r = 0;
     if (key < e.lk && key < W.cap) {
@@ -309,7 +309,7 @@ __device__ __forceinline__ void glance_body(const PagedWeightsParams& W) {
     const bool causal = P->causal != 0;
     const float c2 = P->c2;
     const int s1 = (int)min((int64_t)steps, step + left);
-    const int off = e.lk - e.lq, ps = P->ps, npages = P->npages, HG = P->H_G, group = P->group;
+    const int off = e.off, ps = P->ps, npages = P->npages, HG = P->H_G, group = P->group;
     const int h00 = kvh * group, nct = cdiv(e.lq, tpt), n = nsub * nct;
     const int last = min(32 * s1, e.lk) - 1;
     const int* trow = P->table + (int64_t)b * P->tstride;

@@ -16,10 +16,10 @@ The new tokens of a call are packed, as in ``flash_naylis_attn``'s varlen
 mode: tokens ``[cu_seqlens_q[b], cu_seqlens_q[b + 1])`` belong to sequence b.
 They are the last rows of its cache: ``seqlens_k[b]`` counts the rows in use,
 theirs included.  One token a sequence is a decode step, a piece of a prompt a
-prefill, and one call may hold both, and sequences without a token.  A length
-past the rows that the table has room for: the append stores the tokens whose
-rows the table has, at those rows, and drops the others; the other calls take
-the length to be that number of rows.
+prefill, and one call may hold both, and sequences without a token.  Rows
+past those that the table has room for are not there: the append drops their
+tokens, attention sees the rows before them, eviction takes the table's rows
+for all.
 
 A step of a server is ``paged_append`` (q and k normalised and rotated, k, v
 and R_k into their pages), then ``flash_naylis_paged``; where the cache has

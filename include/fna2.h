@@ -327,10 +327,10 @@ int fna2_decode_rows(const fna2_decode_rows_args* args, void* hip_stream);
  * cu_seqlens_q[b+1]) of [T, heads, f] belong to sequence b (any number, none
  * included) and are the last of the seqlens_k[b] rows that its cache holds,
  * theirs included: token i of lq sits at row seqlens_k[b] - lq + i.
- * seqlens_k below 0 is 0.  Past table_width * page_size, the rows that the
- * table has room for, the append stores the tokens whose rows the table has, at
- * those rows, and drops the others; every other call takes the length to be
- * that size, and with it, causal, the chunk to be the last lq of those rows. */
+ * seqlens_k below 0 is 0.  Rows at or past table_width * page_size, where the
+ * table ends, are not there: the append drops their tokens, attention sees the
+ * rows before them (causal: up to the token's own), and eviction takes the
+ * table's rows for all that there are. */
 typedef struct fna2_paged_cache {
   int32_t dtype;        /* FNA2_BF16 or FNA2_F16: q, k, v, out; R_q, R_k bf16   */
   int32_t batch;        /* N sequences                                          */

@@ -42,7 +42,8 @@ def attend(q, k_pages, v_pages, table, lens, cu, r_q=None, rk_pages=None, gs=Non
     out, lse, mag = np.zeros((T, H, D)), np.full((T, H), -np.inf), np.zeros((T, H, D))
     w = np.zeros((len(lens), hkv, cap))
     for b in range(len(lens)):
-        n = min(max(int(lens[b]), 0), cap)
+        length = max(int(lens[b]), 0)
+        n = min(length, cap)
         t0, m = int(cu[b]), int(cu[b + 1] - cu[b])
         for kv in range(hkv):
             K, there = rows_of(kp, table[b], kv, n, ps)
@@ -50,7 +51,7 @@ def attend(q, k_pages, v_pages, table, lens, cu, r_q=None, rk_pages=None, gs=Non
             for h in range(kv * g, (kv + 1) * g):
                 rk = rows_of(rkp, table[b], h, n, ps)[0] if h < hg else None
                 for i in range(m):
-                    see = there & ((np.arange(n) <= n - m + i) if causal else True)
+                    see = there & ((np.arange(n) <= length - m + i) if causal else True)
                     if not see.any():
                         continue
                     s = scale * (K[see] @ q[t0 + i, h])

@@ -1306,3 +1306,39 @@ def test_infinite_ranks_in_a_split_cache(gpu, lib, monkeypatch, dtype, H, HKV, H
         p, r = c.slot(0, j)
         c.rk[p, 1, r, 3] = float("inf")
     check_attend(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens", [[100, 30], [65, 10 ** 8], [2 ** 31 - 1, 64], [114, 70]])
+@pytest.mark.parametrize("lq", [[1, 1], [3, 5], [50, 20], [90, 1], [50, 300]])
+@pytest.mark.parametrize("H,HKV,HG,R", [(4, 2, 3, 16), (4, 1, 4, 64), (3, 3, 0, 0)])
+def test_attend_past_the_table(gpu, H, HKV, HG, R, lq, lens, causal):
+    """A chunk that has outgrown its table: a token sees the table's rows up to its
+    own row, which the table need not have."""
+    c = Case(lq, [64, 64], H, HKV, HG, 64, R, 16, device=gpu, width=4, seed=6)
+    c.lens = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    check_attend(c, causal=causal)
+
+
+@pytest.mark.gpu
+def test_a_chunk_past_its_table_is_the_wider_tables(gpu):
+    """Append and attention of a chunk whose last rows the table does not have: its
+    first tokens' results are those of a table with room for all."""
+    for lq in (20, 90):
+        wide = Case([lq], [64 + lq], 4, 2, 3, 64, 16, 16, device=gpu, seed=3)
+        inv = 10000.0 ** (-torch.arange(0, 64, 2, device=gpu).float() / 64)
+        room = (64 + lq // 2) // 16 * 16  # rows that the narrow table has
+        out = []
+        for table in (wide.table, wide.table[:, :room // 16]):
+            k, v, rk = wide.k.clone(), wide.v.clone(), wide.rk.clone()
+            q = paged.paged_append(wide.q, wide.kn, wide.vn, k, v, table, wide.lens, wide.cu,
+                                   wide.rkn, rk, inv)
+            y = paged.flash_naylis_paged(q, k, v, table, wide.lens, wide.cu, lq, r_q=wide.rq,
+                                         rk_pages=rk, graph_scale=wide.gs)
+            out.append((q, y[:room - 64]))
+        assert torch.equal(out[0][0], out[1][0])
+        h = HALF[BF]
+        a, b = (y.double() for _, y in out)
+        # (parts may be cut elsewhere: two roundings of the output, and of P)
+        assert ((a - b).abs() <= 2 * h * a.abs() + 2 * h * wide.v.double().abs().max()).all()
