@@ -1365,7 +1365,8 @@ int check_paged_cache(const fna2_paged_cache& c, bool chunk) {
   if (c.batch < 0 || c.total_q < 0 || c.max_seqlen_q < 0 || c.num_pages < 0) return FNA2_E_SHAPE;
   if (c.page_size <= 0 || c.page_size % 16 != 0) return FNA2_E_SHAPE;
   if (c.table_width < 0 || c.table_stride < 0 || cached_rows(c) > kMaxCached) return FNA2_E_SHAPE;
-  if (c.total_q > kMaxCached || c.batch > (1 << 20)) return FNA2_E_SHAPE;
+  // (a token's row, and the last of a tile's, behind a full table: int)
+  if (c.total_q > kMaxCached - 256 || c.batch > (1 << 20)) return FNA2_E_SHAPE;
   if (c.batch > 1 && c.table_stride < c.table_width) return FNA2_E_STRIDE;
   if (chunk && c.total_q > 0 && !c.cu_seqlens_q) return FNA2_E_SEQLENS;
   if (c.batch == 0) return FNA2_OK;

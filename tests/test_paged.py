@@ -1342,3 +1342,10 @@ def test_a_chunk_past_its_table_is_the_wider_tables(gpu):
         a, b = (y.double() for _, y in out)
         # (parts may be cut elsewhere: two roundings of the output, and of P)
         assert ((a - b).abs() <= 2 * h * a.abs() + 2 * h * wide.v.double().abs().max()).all()
+
+
+def test_check_paged_token_count(lib):
+    """A full table of 2^30 rows and the tokens behind it still count in 32 bits."""
+    for total, want in (((1 << 30) - 256, "FNA2_OK"), ((1 << 30) - 255, "FNA2_E_SHAPE")):
+        a = _attn(total_q=total, max_seqlen_q=total, table_width=1 << 24, table_stride=1 << 24)
+        assert _st(lib.fna2_check_paged_attn(ctypes.byref(a))) == want

@@ -367,12 +367,22 @@ def test_rotation_at_positions_is_the_tables(dtype):
     """Row by row the same bits, at positions that the type rounds as well."""
     from fna2_amd.attention_fna2 import RotaryPositionalEmbedding
     rope = RotaryPositionalEmbedding(64)
-    for device in ["cpu"] + (["cuda"] if torch.cuda.is_available() else []):
-        table = rope._table(3001, torch.device(device), dtype)
-        pos = torch.tensor([0, 1, 255, 256, 257, 1000, 1001, 2049, 3000, 5], device=device)
-        for ids in (pos, pos.int()):
-            for a, b in zip(rope._at(ids, dtype), table):
-                assert torch.equal(a, b[pos])
+    _rows_are_the_tables(rope, torch.device("cpu"), dtype)
+
+
+def _rows_are_the_tables(rope, device, dtype):
+    table = rope._table(3001, device, dtype)
+    pos = torch.tensor([0, 1, 255, 256, 257, 1000, 1001, 2049, 3000, 5], device=device)
+    for ids in (pos, pos.int()):
+        for a, b in zip(rope._at(ids, dtype), table):
+            assert torch.equal(a, b[pos])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rotation_at_positions_is_the_tables_on_the_gpu(gpu, dtype):
+    from fna2_amd.attention_fna2 import RotaryPositionalEmbedding
+    _rows_are_the_tables(RotaryPositionalEmbedding(64).to(gpu), gpu, dtype)
 
 
 @pytest.mark.gpu
