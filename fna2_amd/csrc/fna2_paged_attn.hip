@@ -323,7 +323,9 @@ __device__ __forceinline__ void packed_body() {
       // P in two parts (as the decode kernel): the first cut to the element
       // type, the second what that cut off, so that the result does not
       // depend on where a tile is split.  A part of a visible key is never
-      // zero (an infinite V stays infinite), a hidden key's both are.
+      // zero (an infinite V stays infinite), a hidden key's both are.  The second
+      // part's lowest bit, which sees to that, is 2^-24 in fp16 (p's scale: the
+      // largest is 1), which is then each key's error at most; in bf16 nothing.
       bf16x8 pb[2], pe[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
