@@ -230,6 +230,15 @@ class PagedAttnArgs(ctypes.Structure):
     ]
 
 
+class PagedSharedArgs(ctypes.Structure):
+    _fields_ = [
+        ("attn", PagedAttnArgs),
+        ("groups", ctypes.c_int32),
+        ("cu_groups", ctypes.c_void_p),
+        ("shared_rows", ctypes.c_void_p),
+    ]
+
+
 class PagedWeightsArgs(ctypes.Structure):
     _fields_ = [
         ("attn", PagedAttnArgs),
@@ -296,6 +305,9 @@ SIGNATURES = {
     "fna2_paged_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
     "fna2_paged_scores_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedAttnArgs)]),
     "fna2_paged_attn": (ctypes.c_int, [ctypes.POINTER(PagedAttnArgs), ctypes.c_void_p]),
+    "fna2_check_paged_shared": (ctypes.c_int, [ctypes.POINTER(PagedSharedArgs)]),
+    "fna2_paged_shared_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedSharedArgs)]),
+    "fna2_paged_shared": (ctypes.c_int, [ctypes.POINTER(PagedSharedArgs), ctypes.c_void_p]),
     "fna2_check_paged_weights": (ctypes.c_int, [ctypes.POINTER(PagedWeightsArgs)]),
     "fna2_paged_weights": (ctypes.c_int, [ctypes.POINTER(PagedWeightsArgs), ctypes.c_void_p]),
     "fna2_check_paged_append": (ctypes.c_int, [ctypes.POINTER(PagedAppendArgs)]),

@@ -10,7 +10,7 @@
 
 #include "fna2.h"
 #include "fna2_kernels.h"
-#include "fna2_paged.h"
+#include "fna2_paged_shared.h"
 #include "fna2_sched.h"
 
 namespace {
@@ -1478,6 +1478,42 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
   return k;
 }
 
+// The same for groups that share rows: the tile kernel, whatever the chunks' length,
+// since the shared rows have the tokens of a whole group.
+struct SharedPlan {
+  int hw, waves, min_steps;
+  size_t ml, seqs, ends, recs, whole, whole_ml, bytes;
+};
+SharedPlan shared_plan(const fna2_paged_shared_args& a) {
+  const fna2_paged_cache& c = a.attn.c;
+  SharedPlan k{};
+  const int group = c.heads / c.heads_kv, rpl = fna2::padded_rank32(c.heads_graph, c.rank);
+  k.hw = group >= 3 ? 4 : group;
+  k.min_steps = 4;
+  const int64_t blocks = (int64_t)c.heads_kv * ((group + k.hw - 1) / k.hw);
+  const int64_t steps = std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);
+  const int64_t tiles = (2 * ((int64_t)c.total_q / (128 / k.hw)) + c.batch + a.groups) * blocks;
+  k.waves = (int)std::min(256. * fna2::paged_tile_per_cu(c.head_dim, rpl, k.hw),
+                          std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
+  k.waves = (int)cdiv64(k.waves, 8) * 8;  // (whole turns of the XCDs)
+  const size_t virt = (size_t)c.batch + (size_t)a.groups, rows = 2 * (size_t)c.total_q * (size_t)c.heads;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align_up(bytes);
+    return here;
+  };
+  take(2 * (size_t)k.waves * fna2::paged_tile_slot(c.head_dim));
+  k.ml = take(2 * (size_t)k.waves * 128 * 8u);
+  k.seqs = take(virt * sizeof(fna2::SharedSeq));
+  k.ends = take(virt * 8u);
+  k.recs = take(2 * (size_t)blocks * (size_t)c.total_q * sizeof(fna2::SharedRec));
+  k.whole = take(rows * (size_t)c.head_dim * 4u);
+  k.whole_ml = take(rows * 8u);
+  k.bytes = at;
+  return k;
+}
+
 // Scores that the packed kernel leaves for the weights, 4 bytes a row and column,
 // written and read: where that is at most a quarter of the rows' K and R_k, which
 // the weights' kernel reads otherwise, and fits 512 MB.  (us, attention and weights,
@@ -1584,6 +1620,47 @@ int fna2_paged_attn(const fna2_paged_attn_args* a, void* stream_ptr) {
   if (fna2::launch_paged_packed(K, k.rc, stream) != hipSuccess) return FNA2_E_LAUNCH;
   if (fna2::launch_paged_merge(K, stream) != hipSuccess) return FNA2_E_LAUNCH;
   return FNA2_OK;
+}
+
+int fna2_check_paged_shared(const fna2_paged_shared_args* a) {
+  if (!a) return FNA2_E_NULL;
+  FNA2_TRY(fna2_check_paged_attn(&a->attn));
+  if (a->groups < 0 || a->groups > (1 << 20)) return FNA2_E_SHAPE;
+  if (a->groups > 0 && (!a->cu_groups || !a->shared_rows)) return FNA2_E_SEQLENS;
+  return FNA2_OK;
+}
+
+size_t fna2_paged_shared_workspace_bytes(const fna2_paged_shared_args* a) {
+  if (fna2_check_paged_shared(a) != FNA2_OK || a->attn.c.total_q == 0) return 0;
+  return shared_plan(*a).bytes;
+}
+
+int fna2_paged_shared(const fna2_paged_shared_args* a, void* stream_ptr) {
+  FNA2_TRY(fna2_check_paged_shared(a));
+  if (a->attn.c.total_q == 0) return FNA2_OK;
+  FNA2_TRY(check_device());
+  const SharedPlan k = shared_plan(*a);
+  char* const ws = (char*)a->attn.workspace;
+  if (!ws || a->attn.workspace_bytes < k.bytes || !aligned(ws, 16)) return FNA2_E_WORKSPACE;
+  fna2::PagedSharedParams S;
+  std::memset(&S, 0, sizeof(S));
+  fill_attn(S.p, a->attn);
+  S.p.waves = k.waves;
+  S.p.min_steps = k.min_steps;
+  S.p.hw = k.hw;
+  S.p.part = (float*)ws;
+  S.p.ml = (float*)(ws + k.ml);
+  S.G = a->groups;
+  S.V = a->groups + a->attn.c.batch;
+  S.cu_groups = a->cu_groups;
+  S.shared_rows = a->shared_rows;
+  S.seqs = (fna2::SharedSeq*)(ws + k.seqs);
+  S.ends = (int64_t*)(ws + k.ends);
+  S.recs = (fna2::SharedRec*)(ws + k.recs);
+  S.whole = (float*)(ws + k.whole);
+  S.whole_ml = (float*)(ws + k.whole_ml);
+  const int rpl = fna2::padded_rank32(S.p.H_G, S.p.R);
+  return fna2::launch_paged_shared(S, rpl, (hipStream_t)stream_ptr) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
 }
 
 int fna2_check_paged_weights(const fna2_paged_weights_args* w) {

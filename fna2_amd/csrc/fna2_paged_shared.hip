@@ -1,0 +1,266 @@
+// fna2_paged_shared.hip — attention over a paged cache in which groups of
+// sequences share their first rows.
+//
+// Rows that a group of sequences shares (one prompt, one document, many
+// questions) are attended to once for the tokens of all of them: softmax over
+// the shared rows and over a sequence's own are two parts of one, joined as
+// parts of rows are,
+//     m = max(m1, m2),  l = l1 e^{m1-m} + l2 e^{m2-m},
+//     O = (O1 e^{m1-m} + O2 e^{m2-m}) / (l + 1e-6).
+// A group shares the rows that lie before every chunk of its tokens, so that no
+// token's mask cuts them, in whole key steps of 32; what is left over is each
+// sequence's own.
+//
+// Three launches.  The plan (one workgroup) makes the list of virtual sequences:
+// the groups' shared rows, each of all the group's tokens, and the sequences'
+// own rows; and the sums of their key steps.  The tile kernel
+// (fna2_paged_tile_dev.h) takes equal runs of them.  A tile that runs cut, or
+// that is one of two for its tokens, leaves unnormalised parts; the join adds a
+// token's parts up in a fixed order.
+#include <algorithm>
+
+#include "fna2_paged_tile_dev.h"
+
+namespace fna2 {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+// One workgroup.  A wave per group: the rows that it shares; then all threads:
+// the units of the virtual sequences, added up.
+__global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(const PagedSharedParams) {
+  SArg S = sargs();
+  KArg P = &S->p;
+  const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
+  const int N = P->N, G = S->G, V = S->V;
+  SharedSeq* const seqs = S->seqs;
+  for (int b = threadIdx.x; b < N; b += kPlanThreads)
+    seqs[G + b] = SharedSeq{paged_seq(P, b), 0, b, kSharedAlone, 0};
+  __threadfence_block();
+  __syncthreads();
+  for (int g = wv; g < G; g += kPlanThreads / 64) {
+    const int c0 = min(max(uni(S->cu_groups[g]), 0), N);
+    const int c1 = min(max(uni(S->cu_groups[g + 1]), c0), N);
+    // the least number of rows before a chunk, the sequences that have one, and the first of them
+    int least = 0x7fffffff, first = c1, n = 0;
+    for (int b = c0 + lane; b < c1; b += 64) {
+      const PagedSeq s = seqs[G + b].s;
+      if (s.lq <= 0) continue;
+      least = min(least, s.off);
+      first = min(first, b);
+      ++n;
+    }
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) {
+      least = min(least, __shfl_xor(least, k));
+      first = min(first, __shfl_xor(first, k));
+      n += __shfl_xor(n, k);
+    }
+    int rows = min(least, uni(S->shared_rows[g]));
+    rows = n > 1 && rows > 0 ? rows & ~31 : 0;
+    SharedSeq pre = SharedSeq{PagedSeq{0, 0, 0, 0}, 0, 0, kSharedPrefix, 0};
+    if (rows > 0) {
+      pre.s.q0 = seqs[G + c0].s.q0;
+      const PagedSeq last = seqs[G + c1 - 1].s;
+      pre.s.lq = max(last.q0 + last.lq - pre.s.q0, 0);
+      pre.s.lk = pre.s.off = rows;
+      pre.table = first;
+      for (int b = c0 + lane; b < c1; b += 64) {
+        SharedSeq x = seqs[G + b];
+        if (x.s.lq <= 0) continue;
+        x.s.lk = max(x.s.lk - rows, 0);
+        x.s.off -= rows;
+        x.row0 = rows;
+        x.kind = kSharedOwn;
+        seqs[G + b] = x;
+      }
+    }
+    if (lane == 0) seqs[g] = pre;
+  }
+  __threadfence_block();
+  __syncthreads();
+  __shared__ int64_t sums[kPlanThreads / 64];
+  int64_t before = 0;
+  for (int v0 = 0; v0 < V; v0 += kPlanThreads) {
+    const int v = v0 + threadIdx.x;
+    const int64_t end = lane_scan64(v < V ? TilePlan::units(P, seqs[v].s) : 0);
+    if (lane == 63) sums[wv] = end;
+    __syncthreads();
+    int64_t mine = before;
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+      if (w < wv) mine += sums[w];
+      before += sums[w];
+    }
+    if (v < V) S->ends[v] = mine + end;
+    __syncthreads();
+  }
+}
+
+// The join: a workgroup takes 32 tokens, a query head and 32 features; its
+// waves every fourth group of four parts each.  Column = lane % 32, as in a
+// tile, so that the parts of tokens that are neighbours in a tile are read as they lie.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void paged_shared_join_kernel(const PagedSharedParams) {
+  SArg S = sargs();
+  KArg P = &S->p;
+  __shared__ f32x4_t part[4][4][64];
+  __shared__ float stat[4][2][32];
+  const int lane = threadIdx.x & 63, own = uni(threadIdx.x >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
+  const int h = uni(blockIdx.y / (D / 32)), d = uni(blockIdx.y % (D / 32));
+  const int tok = 32 * blockIdx.x + l32;
+  const int hw = P->hw, hblk = cdiv(P->group, hw);
+  const int kvh = h / P->group, h_in = h - kvh * P->group;
+  const int hb = kvh * hblk + h_in / hw, hin = h_in % hw;
+  const int t0 = min(max(uni(*const_space(P->cu)), 0), P->T);
+  const int t1 = min(max(uni(*const_space(P->cu + P->N)), t0), P->T);
+  const bool loose = tok < P->T && (tok < t0 || tok >= t1);
+  SharedRec a = {0, -1}, b = {0, 0};
+  if (tok >= t0 && tok < t1) a = S->recs[(int64_t)hb * P->T + tok];
+  const bool live = a.parts >= 0, two = live && (a.at & kSharedHas);
+  if (two) b = S->recs[(int64_t)(P->H_KV * hblk + hb) * P->T + tok];
+  const int na = live ? max(a.parts, 1) : 0, nb = two ? max(b.parts, 1) : 0, n = na + nb;
+  const float c2 = P->c2;
+  float M = kNegInf, L = 0.f;
+  f32x4_t o[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) o[g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;  // parts in flight
+  for (int j0 = U * own; __builtin_amdgcn_ballot_w64(j0 < n) != 0; j0 += 4 * U) {
+    f32x4_t x[U][4];
+    f32x2 ml[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      ml[k] = f32x2{kNegInf, 0.f};
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x[k][g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      int j = j0 + k;
+      if (j >= n) continue;
+      const bool second = j >= nb;  // the shared rows' parts first
+      if (second) j -= nb;
+      const SharedRec r = second ? a : b;
+      const float *src, *src_ml;
+      int step;
+      if (r.parts == 0) {
+        const int64_t row = ((int64_t)!second * P->T + tok) * P->H + h;
+        src = S->whole + row * D + 32 * d + 4 * hl;
+        src_ml = S->whole_ml + 2 * row;
+        step = 8;
+      } else {
+        const int run = min((r.at & 0xffff) + j, P->waves - 1), at = (r.at >> 16) & 0x7f;
+        const int wv = ((at >> 5) * hw + hin) & 3;
+        const int64_t slot = (2 * (int64_t)run + (j == 0 ? 1 : 0)) * 4 + wv;
+        src = P->part + slot * 32 * D + d * 1024 + 4 * ((at & 31) + 32 * hl);
+        src_ml = P->ml + 2 * (slot * 32 + (at & 31));
+        step = 256;
+      }
+      ml[k] = *(const f32x2*)src_ml;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x[k][g] = *(const f32x4_t*)(src + g * step);
+    }
+    float m = M;
+#pragma unroll
+    for (int k = 0; k < U; ++k) m = fmaxf(m, ml[k][0]);
+    const float ref = m == kNegInf ? 0.f : m;
+    const float wa = weight2((M - ref) * c2);
+    L *= wa;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) o[g] *= wa;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const float wb = weight2((ml[k][0] - ref) * c2);
+      L += ml[k][1] * wb;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) o[g] += x[k][g] * wb;
+    }
+    M = m;
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g) part[own][g][lane] = o[g];
+  if (hl == 0) stat[own][0][l32] = M, stat[own][1][l32] = L;
+  __syncthreads();
+  if (own != 0 || !(live || loose)) return;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) {
+    const float mw = stat[w][0][l32], m = fmaxf(M, mw);
+    const float ref = m == kNegInf ? 0.f : m;
+    const float wa = weight2((M - ref) * c2), wb = weight2((mw - ref) * c2);
+    L = L * wa + stat[w][1][l32] * wb;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) o[g] = o[g] * wa + part[w][g][lane] * wb;
+    M = m;
+  }
+  const float inv = 1.f / (L + 1e-6f);
+  uint16_t* orow = (uint16_t*)P->o.ptr + (int64_t)tok * P->o.ss + (int64_t)h * P->o.sh;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    u32x2 val;
+    val[0] = pack_e<F16>(o[g][0] * inv, o[g][1] * inv);
+    val[1] = pack_e<F16>(o[g][2] * inv, o[g][3] * inv);
+    *(u32x2*)(orow + d * 32 + 8 * g + 4 * hl) = val;
+  }
+  if (d == 0 && hl == 0 && P->lse.ptr)
+    ((float*)P->lse.ptr)[(int64_t)tok * P->lse.ss + (int64_t)h * P->lse.sh] =
+        M == kNegInf ? kNegInf : M * P->c + __builtin_amdgcn_logf(L + 1e-6f) * kLn2;
+}
+
+#define FNA2_SHARED(D, RPL, HW)                                                                   \
+  __global__ __launch_bounds__(256, tile_occ(D, RPL, HW)) void                                    \
+      paged_shared_d##D##_r##RPL##_h##HW(const PagedSharedParams) {                               \
+    tile_body<D, RPL, HW, false, true>();                                                         \
+  }                                                                                               \
+  __global__ __launch_bounds__(256, tile_occ(D, RPL, HW)) void                                    \
+      paged_shared_d##D##_r##RPL##_h##HW##_f16(const PagedSharedParams) {                         \
+    tile_body<D, RPL, HW, true, true>();                                                          \
+  }
+FNA2_SHARED(64, 0, 1)
+FNA2_SHARED(64, 32, 1)
+FNA2_SHARED(64, 32, 2)
+FNA2_SHARED(64, 32, 4)
+FNA2_SHARED(64, 64, 1)
+FNA2_SHARED(64, 64, 2)
+FNA2_SHARED(64, 64, 4)
+FNA2_SHARED(128, 0, 1)
+FNA2_SHARED(128, 32, 1)
+FNA2_SHARED(128, 32, 2)
+FNA2_SHARED(128, 32, 4)
+FNA2_SHARED(128, 64, 1)
+FNA2_SHARED(128, 64, 2)
+FNA2_SHARED(128, 64, 4)
+#undef FNA2_SHARED
+
+}  // namespace
+
+hipError_t launch_paged_shared(const PagedSharedParams& S, int rpl, hipStream_t s) {
+  const PagedParams& P = S.p;
+  void (*k)(const PagedSharedParams) = nullptr;
+#define FNA2_SHARED_OF(D, RPL, HW) \
+  (P.f16 ? paged_shared_d##D##_r##RPL##_h##HW##_f16 : paged_shared_d##D##_r##RPL##_h##HW)
+#define FNA2_SHARED_HW(D, RPL)                             \
+  (P.hw == 1   ? FNA2_SHARED_OF(D, RPL, 1)                 \
+   : P.hw == 2 ? FNA2_SHARED_OF(D, RPL, 2)                 \
+   : P.hw == 4 ? FNA2_SHARED_OF(D, RPL, 4)                 \
+               : nullptr)
+  if (P.D == 64)
+    k = rpl == 0 ? FNA2_SHARED_OF(64, 0, 1) : rpl == 32 ? FNA2_SHARED_HW(64, 32) : FNA2_SHARED_HW(64, 64);
+  if (P.D == 128)
+    k = rpl == 0 ? FNA2_SHARED_OF(128, 0, 1) : rpl == 32 ? FNA2_SHARED_HW(128, 32) : FNA2_SHARED_HW(128, 64);
+#undef FNA2_SHARED_HW
+#undef FNA2_SHARED_OF
+  if (!k) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(paged_shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, S);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(k, dim3((uint32_t)P.waves), dim3(256), 0, s, S);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const dim3 grid((uint32_t)((P.T + 31) / 32), (uint32_t)(P.H * (P.D / 32)));
+  void (*m)(const PagedSharedParams) =
+      P.D == 64 ? (P.f16 ? paged_shared_join_kernel<64, true> : paged_shared_join_kernel<64, false>)
+                : (P.f16 ? paged_shared_join_kernel<128, true> : paged_shared_join_kernel<128, false>);
+  hipLaunchKernelGGL(m, grid, dim3(256), 0, s, S);
+  return hipGetLastError();
+}
+
+}  // namespace fna2

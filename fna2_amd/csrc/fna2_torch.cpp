@@ -53,6 +53,9 @@ struct Lib {
   decltype(&fna2_paged_attn_workspace_bytes) paged_attn_workspace_bytes;
   decltype(&fna2_paged_scores_bytes) paged_scores_bytes;
   decltype(&fna2_paged_attn) paged_attn;
+  decltype(&fna2_check_paged_shared) check_paged_shared;
+  decltype(&fna2_paged_shared_workspace_bytes) paged_shared_workspace_bytes;
+  decltype(&fna2_paged_shared) paged_shared;
   decltype(&fna2_check_paged_weights) check_paged_weights;
   decltype(&fna2_paged_weights) paged_weights;
   decltype(&fna2_paged_append_shifted) paged_append_shifted;
@@ -91,6 +94,9 @@ void bind(const std::map<std::string, uintptr_t>& f, py::object error) {
   FNA2_BIND(paged_attn_workspace_bytes);
   FNA2_BIND(paged_scores_bytes);
   FNA2_BIND(paged_attn);
+  FNA2_BIND(check_paged_shared);
+  FNA2_BIND(paged_shared_workspace_bytes);
+  FNA2_BIND(paged_shared);
   FNA2_BIND(check_paged_weights);
   FNA2_BIND(paged_weights);
   FNA2_BIND(paged_append_shifted);
@@ -648,12 +654,15 @@ void written(std::initializer_list<const Tensor*> ts) {
     if (t && t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
-// flash_naylis_paged: (out, LSE or None).
+// flash_naylis_paged, and with cu_groups and shared_rows flash_naylis_shared:
+// (out, LSE or None).
 std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
     const Tensor& q, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lens,
     const Tensor& cu, int64_t max_q, const OptTensor& rq_, const OptTensor& rkp_,
-    const OptTensor& gs_, double scale, bool causal, const OptTensor& w_, bool want_lse) {
-  const Tensor &rq = opt(rq_), &w = opt(w_);
+    const OptTensor& gs_, double scale, bool causal, const OptTensor& w_, bool want_lse,
+    const OptTensor& groups_, const OptTensor& shared_) {
+  const Tensor &rq = opt(rq_), &w = opt(w_), &groups = opt(groups_), &shared = opt(shared_);
+  const char* const what = groups.defined() ? "flash_naylis_shared" : "flash_naylis_paged";
   Tensor gs = opt(gs_);
   if (!L.paged_attn || !q.defined() || !q.is_cuda() || q.dim() != 3) return std::nullopt;
   if (!rq.defined() && (rkp_.has_value() || gs_.has_value())) return std::nullopt;
@@ -678,6 +687,10 @@ std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
   a.c.max_seqlen_q = (int32_t)std::min(max_q, T);
   a.causal = causal;
   a.softmax_scale = (float)scale;
+  if (groups.defined() &&
+      (!int32_on(groups, dev) || !int32_on(shared, dev) || groups.dim() != 1 || shared.dim() != 1 ||
+       groups.numel() != shared.numel() + 1 || groups.numel() > INT32_MAX))
+    return std::nullopt;
   fna2_paged_weights_args wa{};
   if (w.defined()) {
     if (!plain(w, dev) || w.scalar_type() != at::kFloat || w.dim() != 3 ||
@@ -700,7 +713,7 @@ std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
   a.q = view(q, true);
   a.out = view(out, true);
   Tensor scores;
-  if (w.defined()) {
+  if (w.defined() && !groups.defined()) {
     const size_t bytes = L.paged_scores_bytes(&a);
     try {  // (without the room the weights read K again)
       if (bytes > 0) {
@@ -715,15 +728,25 @@ std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
   if (L.check_paged_attn(&a) != FNA2_OK ||
       (w.defined() && L.check_paged_weights(&wa) != FNA2_OK))
     return std::nullopt;
-  const size_t need = L.paged_attn_workspace_bytes(&a);
+  fna2_paged_shared_args sa{};
+  if (groups.defined()) {
+    sa.attn = a;
+    sa.groups = (int32_t)shared.numel();
+    sa.cu_groups = groups.data_ptr<int32_t>();
+    sa.shared_rows = shared.data_ptr<int32_t>();
+    if (L.check_paged_shared(&sa) != FNA2_OK) return std::nullopt;
+  }
+  const size_t need =
+      groups.defined() ? L.paged_shared_workspace_bytes(&sa) : L.paged_attn_workspace_bytes(&a);
   const Tensor ws = bytes_on(need, q);
-  a.workspace = ws.data_ptr();
-  a.workspace_bytes = need;
-  if (!launched(L.paged_attn(&a, stream_of(dev)), "flash_naylis_paged")) return std::nullopt;
+  a.workspace = sa.attn.workspace = ws.data_ptr();
+  a.workspace_bytes = sa.attn.workspace_bytes = need;
+  void* const stream = stream_of(dev);
+  if (!launched(groups.defined() ? L.paged_shared(&sa, stream) : L.paged_attn(&a, stream), what))
+    return std::nullopt;
   if (w.defined()) {
     // (checked above: what is left to fail is a launch)
-    if (!launched(L.paged_weights(&wa, stream_of(dev)), "flash_naylis_paged"))
-      launched(FNA2_E_LAUNCH, "flash_naylis_paged");
+    if (!launched(L.paged_weights(&wa, stream), what)) launched(FNA2_E_LAUNCH, what);
     written({&w});
   }
   if (!want_lse) lse.reset();
@@ -834,7 +857,12 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("decode_rows", &decode_rows, Free());
   m.def("rope_fwd", &rope_fwd, Free());
   m.def("rope_bwd", &rope_bwd, Free());
-  m.def("paged_attn", &paged_attn, Free());
+  m.def("paged_attn", &paged_attn, Free(), py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
+        py::arg("block_table"), py::arg("seqlens_k"), py::arg("cu_seqlens_q"),
+        py::arg("max_seqlen_q"), py::arg("r_q"), py::arg("rk_pages"), py::arg("graph_scale"),
+        py::arg("softmax_scale"), py::arg("is_causal"), py::arg("key_weights"),
+        py::arg("return_lse"), py::arg("cu_groups") = py::none(),
+        py::arg("shared_rows") = py::none());
   m.def("paged_append", &paged_append, Free(), py::arg("q"), py::arg("k"), py::arg("v"),
         py::arg("k_pages"), py::arg("v_pages"), py::arg("block_table"), py::arg("seqlens_k"),
         py::arg("cu_seqlens_q"), py::arg("r_k"), py::arg("rk_pages"), py::arg("inv_freq"),

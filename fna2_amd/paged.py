@@ -189,14 +189,55 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     the KV head, is added to it (rows at or past ``capacity`` are left out).
 
     Returns out ``[T, H, D]`` (and the fp32 LSE ``[T, H]``)."""
-    what = "flash_naylis_paged"
+    return _attention("flash_naylis_paged", q, k_pages, v_pages, block_table, seqlens_k,
+                      cu_seqlens_q, max_seqlen_q, r_q, rk_pages, graph_scale, softmax_scale,
+                      is_causal, key_weights, return_lse, None, None)
+
+
+def flash_naylis_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                        block_table: torch.Tensor, seqlens_k: torch.Tensor,
+                        cu_seqlens_q: torch.Tensor, max_seqlen_q: int, cu_groups: torch.Tensor,
+                        shared_rows: torch.Tensor, r_q: Optional[torch.Tensor] = None,
+                        rk_pages: Optional[torch.Tensor] = None,
+                        graph_scale: Optional[torch.Tensor] = None,
+                        softmax_scale: Optional[float] = None, is_causal: bool = True,
+                        key_weights: Optional[torch.Tensor] = None, return_lse: bool = False
+                        ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """``flash_naylis_paged`` of sequences that share their first rows: the same
+    arguments and result (sums in another order), with rows that a group of
+    sequences shares read and attended to once for the tokens of them all.
+
+    Group g is sequences ``cu_groups[g] .. cu_groups[g + 1] - 1`` (``cu_groups``
+    ``[G + 1]``, nondecreasing; sequences of no group share nothing), and the first
+    ``shared_rows[g]`` rows of each lie in the same pages: their rows of
+    ``block_table`` begin alike (``paged_groups`` finds such groups).  Of these
+    rows, those are shared that lie before every chunk of the group, in whole steps of
+    32, if two of its sequences have tokens; ``shared_rows`` may be larger or 0.
+    """
+    assert cu_groups is not None and shared_rows is not None, \
+        "flash_naylis_shared: cu_groups and shared_rows expected"
+    return _attention("flash_naylis_shared", q, k_pages, v_pages, block_table, seqlens_k,
+                      cu_seqlens_q, max_seqlen_q, r_q, rk_pages, graph_scale, softmax_scale,
+                      is_causal, key_weights, return_lse, cu_groups, shared_rows)
+
+
+def _groups(what: str, cu_groups, shared_rows, dev) -> Tuple[torch.Tensor, torch.Tensor]:
+    cg, rows = _ints(cu_groups, dev), _ints(shared_rows, dev)
+    assert cg.dim() == 1 and rows.dim() == 1 and cg.numel() == rows.numel() + 1, \
+        f"{what}: cu_groups must hold one entry a group and one more, shared_rows one a group"
+    return cg, rows
+
+
+def _attention(what, q, k_pages, v_pages, block_table, seqlens_k, cu_seqlens_q, max_seqlen_q, r_q,
+               rk_pages, graph_scale, softmax_scale, is_causal, key_weights, return_lse, cu_groups,
+               shared_rows):
     nat = _capi.native_or_none() if q.is_cuda else None
     if nat is not None:  # the native launch path (None: a call it leaves to the code below)
         done = nat.paged_attn(
             q, k_pages, v_pages, block_table, seqlens_k, cu_seqlens_q, int(max_seqlen_q), r_q,
             rk_pages, graph_scale,
             float(q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale),
-            bool(is_causal), key_weights, return_lse)
+            bool(is_causal), key_weights, return_lse, cu_groups, shared_rows)
         if done is not None:
             return done if return_lse else done[0]
     assert q.dim() == 3, f"{what}: q must be [T, H, D]"
@@ -243,11 +284,15 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     a.q, a.out = _t3(q), _t3(out)
     lib = _capi.lib()
     _capi.raise_for(lib.fna2_check_paged_attn(ctypes.byref(a)), what)
-    wa = scores = None
+    wa = scores = sa = None
+    if cu_groups is not None:
+        sa, groups = _capi.PagedSharedArgs(), _groups(what, cu_groups, shared_rows, dev)
+        sa.groups = groups[1].numel()
+        sa.cu_groups, sa.shared_rows = groups[0].data_ptr(), groups[1].data_ptr() or None
     if w is not None:
         # (with room for the scores, where they save a second reading of K and
         # the memory is there)
-        nbytes = lib.fna2_paged_scores_bytes(ctypes.byref(a))
+        nbytes = 0 if sa is not None else lib.fna2_paged_scores_bytes(ctypes.byref(a))
         try:
             if nbytes:
                 scores = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -259,16 +304,22 @@ def flash_naylis_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
         wa.key_weights = w.data_ptr()
         wa.stride_b, wa.stride_h, wa.capacity = w.stride(0), w.stride(1), w.shape[2]
         _capi.raise_for(lib.fna2_check_paged_weights(ctypes.byref(wa)), what)
+    call, size = lib.fna2_paged_attn, lib.fna2_paged_attn_workspace_bytes
+    if sa is not None:
+        sa.attn = a
+        _capi.raise_for(lib.fna2_check_paged_shared(ctypes.byref(sa)), what)
+        call, size = lib.fna2_paged_shared, lib.fna2_paged_shared_workspace_bytes
     if T > 0:
-        nbytes = lib.fna2_paged_attn_workspace_bytes(ctypes.byref(a))
+        args, at = (a, a) if sa is None else (sa, sa.attn)
+        nbytes = size(ctypes.byref(args))
         ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+        at.workspace, at.workspace_bytes = ws.data_ptr(), nbytes
         with torch.cuda.device(dev):
-            _capi.raise_for(lib.fna2_paged_attn(ctypes.byref(a), _stream(dev)), what)
+            _capi.raise_for(call(ctypes.byref(args), _stream(dev)), what)
             if wa is not None:
                 _capi.raise_for(lib.fna2_paged_weights(ctypes.byref(wa), _stream(dev)), what)
                 _bump(w)
-    del keep, cu, gs, scores
+    del keep, cu, gs, scores, sa
     return (out, lse) if return_lse else out
 
 

@@ -379,6 +379,26 @@ size_t fna2_paged_scores_bytes(const fna2_paged_attn_args* args);
 /* One launch, and a second that joins the parts of split rows. */
 int fna2_paged_attn(const fna2_paged_attn_args* args, void* hip_stream);
 
+/* fna2_paged_attn for sequences that share their first rows: the same result
+ * (up to the order of its sums), the shared rows read and attended to once for all tokens
+ * of a group.  Group g is sequences [cu_groups[g], cu_groups[g+1]) (in order, no sequence
+ * in two groups; the others share nothing); the first shared_rows[g] rows of each
+ * of them lie in the same pages, which their rows of the block table all name.
+ * Of these rows, those are shared that lie before every chunk of the group, in whole
+ * steps of 32, where two of its sequences have tokens. */
+typedef struct fna2_paged_shared_args {
+  fna2_paged_attn_args attn;    /* scores unused                                 */
+  int32_t groups;               /* G >= 0                                       */
+  const int32_t* cu_groups;     /* [G+1] device                                 */
+  const int32_t* shared_rows;   /* [G] device                                   */
+} fna2_paged_shared_args;
+
+/* Host-only validation; no GPU call. */
+int fna2_check_paged_shared(const fna2_paged_shared_args* args);
+size_t fna2_paged_shared_workspace_bytes(const fna2_paged_shared_args* args);
+/* Three launches: a plan, the tiles, the join of their parts. */
+int fna2_paged_shared(const fna2_paged_shared_args* args, void* hip_stream);
+
 /* The cached rows' attention weights of a fna2_paged_attn call:
  *     key_weights[b][kvh][j] += sum over b's tokens i and the query heads h of
  *                               KV head kvh of exp(S_hij - lse[i][h])
