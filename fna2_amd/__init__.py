@@ -27,11 +27,14 @@ from .paged import (  # noqa: F401
     flash_naylis_shared,
     paged_append,
     paged_evict,
+    paged_extend,
+    paged_groups,
+    paged_trim,
 )
-from .rope import rope_varlen  # noqa: F401
+from .rope import rope_varlen, rotary_embed, rotary_frequencies  # noqa: F401
 from . import ops  # noqa: F401,E402  (registers the fna2::fwd / fna2::bwd custom ops)
 
 __all__ = ["BLOCK_M", "BLOCK_N", "BLOCK_R", "FlashNaylisAttnFunc", "flash_naylis_attn",
            "flash_naylis_decode", "flash_naylis_paged", "flash_naylis_shared", "PagedKVCache",
-           "PageTable", "paged_append", "paged_evict",
-           "rope_varlen"]
+           "PageTable", "paged_append", "paged_evict", "paged_extend", "paged_groups", "paged_trim",
+           "rope_varlen", "rotary_embed", "rotary_frequencies"]

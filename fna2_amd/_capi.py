@@ -160,6 +160,20 @@ class RopeBwdArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("r", RopeArgs),
+        ("positions", ctypes.c_void_p),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class RotaryBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", RotaryArgs)] + RopeBwdArgs._fields_[1:]
+
+
 class DecodeArgs(ctypes.Structure):
     _fields_ = [
         ("batch", ctypes.c_int32),
@@ -275,6 +289,33 @@ class PagedEvictArgs(ctypes.Structure):
     ]
 
 
+class PagedBooks(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "table_width", "page_size", "capacity")] + [
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("seqlens", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p),
+    ]
+
+
+class PagedExtendArgs(ctypes.Structure):
+    _fields_ = [("b", PagedBooks), ("counts", ctypes.c_void_p),
+                ("position_shift", ctypes.c_void_p), ("total_q", ctypes.c_int32)] + [
+        (n, ctypes.c_void_p) for n in ("cu_seqlens_q", "new_lens", "new_free_count", "slots",
+                                       "sequences", "positions", "status")]
+
+
+class PagedTrimArgs(ctypes.Structure):
+    _fields_ = [("b", PagedBooks)] + [
+        (n, ctypes.c_void_p) for n in ("keep", "borrowed", "new_lens", "new_free_count")]
+
+
+class PagedGroupsArgs(ctypes.Structure):
+    _fields_ = [("b", PagedBooks)] + [
+        (n, ctypes.c_void_p) for n in ("cu_groups", "shared_rows", "workspace")]
+
+
 # Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
     "fna2_version": (ctypes.c_int, []),
@@ -295,6 +336,11 @@ SIGNATURES = {
     "fna2_rope_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(RopeArgs)]),
     "fna2_check_rope_bwd": (ctypes.c_int, [ctypes.POINTER(RopeBwdArgs)]),
     "fna2_rope_bwd": (ctypes.c_int, [ctypes.POINTER(RopeBwdArgs), ctypes.c_void_p]),
+    "fna2_check_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryArgs)]),
+    "fna2_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]),
+    "fna2_rotary_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(RotaryArgs)]),
+    "fna2_check_rotary_bwd": (ctypes.c_int, [ctypes.POINTER(RotaryBwdArgs)]),
+    "fna2_rotary_bwd": (ctypes.c_int, [ctypes.POINTER(RotaryBwdArgs), ctypes.c_void_p]),
     "fna2_check_decode": (ctypes.c_int, [ctypes.POINTER(DecodeArgs)]),
     "fna2_decode_num_splits": (ctypes.c_int, [ctypes.POINTER(DecodeArgs)]),
     "fna2_decode_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DecodeArgs)]),
@@ -316,6 +362,12 @@ SIGNATURES = {
                                                  ctypes.c_void_p]),
     "fna2_check_paged_evict": (ctypes.c_int, [ctypes.POINTER(PagedEvictArgs)]),
     "fna2_paged_evict": (ctypes.c_int, [ctypes.POINTER(PagedEvictArgs), ctypes.c_void_p]),
+    "fna2_check_paged_extend": (ctypes.c_int, [ctypes.POINTER(PagedExtendArgs)]),
+    "fna2_paged_extend": (ctypes.c_int, [ctypes.POINTER(PagedExtendArgs), ctypes.c_void_p]),
+    "fna2_check_paged_trim": (ctypes.c_int, [ctypes.POINTER(PagedTrimArgs)]),
+    "fna2_paged_trim": (ctypes.c_int, [ctypes.POINTER(PagedTrimArgs), ctypes.c_void_p]),
+    "fna2_check_paged_groups": (ctypes.c_int, [ctypes.POINTER(PagedGroupsArgs)]),
+    "fna2_paged_groups": (ctypes.c_int, [ctypes.POINTER(PagedGroupsArgs), ctypes.c_void_p]),
 }
 
 _lib = None

@@ -10,6 +10,7 @@
 
 #include "fna2.h"
 #include "fna2_kernels.h"
+#include "fna2_paged_books.h"
 #include "fna2_paged_shared.h"
 #include "fna2_sched.h"
 
@@ -1310,6 +1311,126 @@ int fna2_decode_rows(const fna2_decode_rows_args* a, void* stream) {
 
 }  // extern "C"
 
+// ── Rotary positions, the other layouts ───────────────────────────────────────
+
+namespace {
+
+int rotary_common(const fna2_rotary_args* a) {
+  if (!a) return FNA2_E_NULL;
+  fna2_rope_args r = a->r;
+  if (a->positions) {
+    if (r.cu_seqlens) return FNA2_E_SEQLENS;
+    r.cu_seqlens = a->positions;  // (the one or the other)
+  }
+  FNA2_TRY(rope_common(&r));
+  if (a->rotary_dim < 2 || a->rotary_dim > r.head_dim || a->rotary_dim % 2 != 0) return FNA2_E_HEAD_DIM;
+  if (a->interleaved != 0 && a->interleaved != 1) return FNA2_E_SHAPE;
+  if (!std::isfinite(a->scale)) return FNA2_E_SCALE;
+  return FNA2_OK;
+}
+
+fna2::RotaryParams rotary_params(const fna2_rotary_args* a) {
+  fna2::RotaryParams P;
+  std::memset(&P, 0, sizeof(P));
+  P.r = rope_params(&a->r);
+  P.rd = a->rotary_dim;
+  P.inter = a->interleaved;
+  P.scale = a->scale;
+  P.pos = a->positions;
+  return P;
+}
+
+size_t rotary_ws(const fna2_rotary_args* a) {
+  if (!(a->r.norm_q || a->r.norm_k) || rope_empty(&a->r)) return 0;
+  return align_up(sizeof(float) * 2u * (size_t)fna2::rotary_bwd_blocks(a->r.total_tokens) *
+                  (size_t)a->r.head_dim);
+}
+
+}  // namespace
+
+extern "C" {
+
+int fna2_check_rotary(const fna2_rotary_args* a) {
+  FNA2_TRY(rotary_common(a));
+  const fna2_rope_args* r = &a->r;
+  if (rope_empty(r)) return FNA2_OK;
+  const size_t es = rope_esize(r);
+  if (r->heads_q > 0) FNA2_TRY(rope_pair(r->q, r->q_out, r->total_tokens, r->heads_q, r->head_dim, es));
+  if (r->heads_k > 0) FNA2_TRY(rope_pair(r->k, r->k_out, r->total_tokens, r->heads_k, r->head_dim, es));
+  return FNA2_OK;
+}
+
+int fna2_rotary(const fna2_rotary_args* a, void* stream) {
+  FNA2_TRY(fna2_check_rotary(a));
+  if (rope_empty(&a->r)) return FNA2_OK;
+  FNA2_TRY(check_device());
+  fna2::RotaryParams P = rotary_params(a);
+  rope_out(P.r, a->r.q_out, a->r.k_out);
+  return fna2::launch_rotary(P, (hipStream_t)stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
+}
+
+size_t fna2_rotary_bwd_workspace_bytes(const fna2_rotary_args* a) {
+  return rotary_common(a) == FNA2_OK ? rotary_ws(a) : 0;
+}
+
+int fna2_check_rotary_bwd(const fna2_rotary_bwd_args* b) {
+  if (!b) return FNA2_E_NULL;
+  const fna2_rotary_args* a = &b->fwd;
+  const fna2_rope_args* r = &a->r;
+  FNA2_TRY(rotary_common(a));
+  if (rope_empty(r)) return FNA2_OK;
+  const int T = r->total_tokens, D = r->head_dim;
+  const size_t es = rope_esize(r);
+  const bool norm = r->norm_q || r->norm_k;
+  if (r->heads_q > 0) {
+    FNA2_TRY(rope_pair(b->dq_out, b->dq, T, r->heads_q, D, es));
+    if (norm) FNA2_TRY(rope_pair(r->q, b->dq, T, r->heads_q, D, es));
+    if (r->norm_q && !b->dnorm_q) return FNA2_E_NULL;
+  }
+  if (r->heads_k > 0) {
+    FNA2_TRY(rope_pair(b->dk_out, b->dk, T, r->heads_k, D, es));
+    if (norm) FNA2_TRY(rope_pair(r->k, b->dk, T, r->heads_k, D, es));
+    if (r->norm_k && !b->dnorm_k) return FNA2_E_NULL;
+  }
+  const size_t need = rotary_ws(a);
+  if (need && (!b->workspace || b->workspace_bytes < need)) return FNA2_E_WORKSPACE;
+  return FNA2_OK;
+}
+
+int fna2_rotary_bwd(const fna2_rotary_bwd_args* b, void* stream) {
+  FNA2_TRY(fna2_check_rotary_bwd(b));
+  const fna2_rotary_args* a = &b->fwd;
+  if (rope_empty(&a->r)) return FNA2_OK;
+  FNA2_TRY(check_device());
+  fna2::RotaryParams P = rotary_params(a);
+  rope_out(P.r, b->dq, b->dk);
+  P.r.gq = b->dq_out.ptr;
+  P.r.gk = b->dk_out.ptr;
+  P.r.gq_ss = b->dq_out.stride_s;
+  P.r.gq_sh = b->dq_out.stride_h;
+  P.r.gk_ss = b->dk_out.stride_s;
+  P.r.gk_sh = b->dk_out.stride_h;
+  hipError_t e;
+  if (!(P.r.wq || P.r.wk)) {  // the inverse rotation of the gradients
+    P.r.q = P.r.gq;
+    P.r.k = P.r.gk;
+    P.r.q_ss = P.r.gq_ss;
+    P.r.q_sh = P.r.gq_sh;
+    P.r.k_ss = P.r.gk_ss;
+    P.r.k_sh = P.r.gk_sh;
+    P.r.sign = -a->r.sign;
+    e = fna2::launch_rotary(P, (hipStream_t)stream);
+  } else {
+    P.r.part = (float*)b->workspace;
+    P.r.dwq = P.r.wq ? b->dnorm_q : nullptr;
+    P.r.dwk = P.r.wk ? b->dnorm_k : nullptr;
+    e = fna2::launch_rotary_norm_bwd(P, (hipStream_t)stream);
+  }
+  return e == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
+}
+
+}  // extern "C"
+
 // ── Paged cache ──────────────────────────────────────────────────────────────
 
 namespace {
@@ -1380,6 +1501,16 @@ int check_paged_cache(const fna2_paged_cache& c, bool chunk) {
   return FNA2_OK;
 }
 
+// page of row group n = row / 16 < 2^26: n / d, d = page_size / 16, as n m >> (26 + s) with
+// 2^s >= d and m = ceil(2^(26+s) / d): off by n (m d - 2^(26+s)) / (d 2^(26+s)) < 1 / d
+void fill_page_div(int page_size, uint32_t& mul, int& shift) {
+  const int64_t d = page_size / 16;
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  shift = 26 + s;
+  mul = (uint32_t)cdiv64((int64_t)1 << shift, d);
+}
+
 void fill_cache(fna2::PagedParams& K, const fna2_paged_cache& c) {
   K.N = c.batch;
   K.T = c.total_q;
@@ -1390,15 +1521,7 @@ void fill_cache(fna2::PagedParams& K, const fna2_paged_cache& c) {
   K.R = c.heads_graph > 0 ? c.rank : 0;
   K.group = c.heads / c.heads_kv;
   K.ps = c.page_size;
-  // page of row group n = row / 16 < 2^26: n / d, d = page_size / 16, as n m >> (26 + s) with
-  // 2^s >= d and m = ceil(2^(26+s) / d): off by n (m d - 2^(26+s)) / (d 2^(26+s)) < 1 / d
-  {
-    const int64_t d = c.page_size / 16;
-    int s = 0;
-    while (((int64_t)1 << s) < d) ++s;
-    K.ps_shift = 26 + s;
-    K.ps_mul = (uint32_t)cdiv64((int64_t)1 << K.ps_shift, d);
-  }
+  fill_page_div(c.page_size, K.ps_mul, K.ps_shift);
   K.npages = c.num_pages;
   K.width = c.table_width;
   K.tstride = c.table_stride;
@@ -1793,6 +1916,110 @@ int fna2_paged_evict(const fna2_paged_evict_args* a, void* stream) {
   if (K.budget > 0 && K.p.width > 0)
     if (fna2::launch_paged_compact(K, (hipStream_t)stream) != hipSuccess) return FNA2_E_LAUNCH;
   return FNA2_OK;
+}
+
+}  // extern "C"
+
+// ── The paged cache's books ───────────────────────────────────────────────────
+
+namespace {
+
+int check_books(const fna2_paged_books& b, bool stack) {
+  if (b.batch < 0 || b.batch > (1 << 20) || b.table_width < 0 || b.table_stride < 0) return FNA2_E_SHAPE;
+  if (b.page_size <= 0 || b.page_size % 16 != 0) return FNA2_E_SHAPE;
+  if ((int64_t)b.table_width * b.page_size > kMaxCached || b.capacity < 0) return FNA2_E_SHAPE;
+  if (b.batch > 1 && b.table_stride < b.table_width) return FNA2_E_STRIDE;
+  if (b.batch > 0 && b.table_width > 0 && !b.block_table) return FNA2_E_NULL;
+  if (!stack) return FNA2_OK;
+  if (b.batch > 0 && !b.seqlens) return FNA2_E_SEQLENS;
+  if (!b.free_count || (b.capacity > 0 && !b.free_pages)) return FNA2_E_NULL;
+  return FNA2_OK;
+}
+
+fna2::BooksParams books_params(const fna2_paged_books& b) {
+  fna2::BooksParams P;
+  std::memset(&P, 0, sizeof(P));
+  P.N = b.batch;
+  P.width = b.table_width;
+  P.ps = b.page_size;
+  P.cap = b.capacity;
+  fill_page_div(b.page_size, P.ps_mul, P.ps_shift);
+  P.tstride = b.table_stride;
+  P.table = b.block_table;
+  P.lens = b.seqlens;
+  P.free = b.free_pages;
+  P.nfree = b.free_count;
+  return P;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fna2_check_paged_extend(const fna2_paged_extend_args* a) {
+  if (!a) return FNA2_E_NULL;
+  FNA2_TRY(check_books(a->b, true));
+  if (a->total_q < 0 || a->total_q > kMaxCached - 256) return FNA2_E_SHAPE;
+  if (!a->cu_seqlens_q || !a->new_free_count || !a->status) return FNA2_E_NULL;
+  if (a->b.batch > 0 && (!a->counts || !a->new_lens)) return FNA2_E_NULL;
+  if (a->total_q > 0 && (!a->slots || !a->sequences || !a->positions)) return FNA2_E_NULL;
+  // (workgroups read these while others write)
+  if (a->new_lens == a->b.seqlens && a->b.batch > 0) return FNA2_E_ALIAS;
+  if (a->new_free_count == a->b.free_count) return FNA2_E_ALIAS;
+  return FNA2_OK;
+}
+
+int fna2_paged_extend(const fna2_paged_extend_args* a, void* stream) {
+  FNA2_TRY(fna2_check_paged_extend(a));
+  FNA2_TRY(check_device());
+  fna2::BooksParams P = books_params(a->b);
+  P.counts = a->counts;
+  P.shift = a->position_shift;
+  P.T = a->total_q;
+  P.cu = a->cu_seqlens_q;
+  P.new_lens = a->new_lens;
+  P.new_nfree = a->new_free_count;
+  P.slots = a->slots;
+  P.seq = a->sequences;
+  P.pos = a->positions;
+  P.status = a->status;
+  return fna2::launch_paged_extend(P, (hipStream_t)stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
+}
+
+int fna2_check_paged_trim(const fna2_paged_trim_args* a) {
+  if (!a) return FNA2_E_NULL;
+  FNA2_TRY(check_books(a->b, true));
+  if (!a->new_free_count || (a->b.batch > 0 && (!a->keep || !a->new_lens))) return FNA2_E_NULL;
+  return FNA2_OK;
+}
+
+int fna2_paged_trim(const fna2_paged_trim_args* a, void* stream) {
+  FNA2_TRY(fna2_check_paged_trim(a));
+  FNA2_TRY(check_device());
+  fna2::BooksParams P = books_params(a->b);
+  P.counts = a->keep;
+  P.borrowed = a->borrowed;
+  P.new_lens = a->new_lens;
+  P.new_nfree = a->new_free_count;
+  return fna2::launch_paged_trim(P, (hipStream_t)stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
+}
+
+int fna2_check_paged_groups(const fna2_paged_groups_args* a) {
+  if (!a) return FNA2_E_NULL;
+  FNA2_TRY(check_books(a->b, false));
+  if (!a->cu_groups) return FNA2_E_NULL;
+  if (a->b.batch > 0 && (!a->shared_rows || !a->workspace)) return FNA2_E_NULL;
+  return FNA2_OK;
+}
+
+int fna2_paged_groups(const fna2_paged_groups_args* a, void* stream) {
+  FNA2_TRY(fna2_check_paged_groups(a));
+  FNA2_TRY(check_device());
+  fna2::BooksParams P = books_params(a->b);
+  P.cu_groups = a->cu_groups;
+  P.shared_rows = a->shared_rows;
+  P.common = a->workspace;
+  return fna2::launch_paged_groups(P, (hipStream_t)stream) == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;
 }
 
 }  // extern "C"

@@ -109,6 +109,20 @@ struct RopeParams {
 int rope_bwd_blocks(int T);  // workgroups of the norm backward over T tokens
 hipError_t launch_rope(const RopeParams& P, hipStream_t s);
 hipError_t launch_rope_norm_bwd(const RopeParams& P, hipStream_t s);
+// dw from the partials of `nblocks` workgroups.
+hipError_t launch_rope_dw_reduce(const RopeParams& P, int nblocks, hipStream_t s);
+
+// Rotary positions in either layout, over rd features, scaled (fna2_rotary.hip).
+struct RotaryParams {
+  RopeParams r;    // cu unused with pos; inv_freq [rd / 2]
+  int rd, inter;
+  float scale;     // of the rotated features
+  const int* pos;  // [T], or null: the packed sequences'
+  int share;       // waves of a token (set by the launch)
+};
+int rotary_bwd_blocks(int T);
+hipError_t launch_rotary(const RotaryParams& P, hipStream_t s);
+hipError_t launch_rotary_norm_bwd(const RotaryParams& P, hipStream_t s);
 
 // One-token decode against a KV cache (fna2_decode.hip).  q, rq, o, lse:
 // row (b, h) at ptr + b * sb + h * sh; caches: row j of (b, h) at

@@ -1,0 +1,442 @@
+// fna2_rotary.hip — rotary positions in either layout, over part of the head,
+// scaled, at given positions or those of packed sequences; with the QK norm.
+//
+// Token at position p, row x of D features, rd of them rotated, f = inv_freq:
+//     n = x rsqrt(mean(x^2) + eps) w                   (rows with a norm)
+//     (u, v) -> s (u cos a_i - v sin a_i, v cos a_i + u sin a_i),  a_i = p f_i,
+// for the pairs i < rd / 2 of features (i, i + rd / 2) or, interleaved, (2i, 2i + 1); features
+// from rd on stay n.  The angle is formed and reduced in fp64 (in fp32 it is off by
+// 0.06 radians at position 10^6); the rest is fp32 with one rounding, at the store.
+// Backward, with g = s R(-a) dy for the rotated features:
+//     dx = r (w g - x r^2 mean(x w g)),  dw = sum of g x r,  r = rsqrt(mean(x^2) + eps),
+// and dx = g without a norm, which is the forward kernel with the angle's sign
+// changed.
+//
+// Bound by reading and writing every row once.  A lane owns two 16-byte chunks
+// of a row that hold whole pairs: the same chunk of both halves, or (interleaved) two
+// neighbours; LPR = D / (2 EPL) lanes a row.  Halves that do not begin on a chunk
+// (rd / 2 not a multiple of EPL) have their pairs in different lanes: those go
+// through LDS.  A wave forms the token's cos and sin once, a lane a pair.
+#include <algorithm>
+
+#include "fna2_rope_dev.h"
+
+namespace fna2 {
+
+namespace {
+
+constexpr int kRotHalf = 0, kRotInter = 1, kRotAny = 2;
+constexpr int kRotWaves = 4;
+constexpr int kRotPasses = 4;  // row passes whose loads are in flight together
+constexpr int kRotMaxHalf = 256;
+
+__device__ __forceinline__ void rot_wave_sync() {
+  // (one wave's own LDS: its reads follow its writes in order)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// LDS of a wave: the token's cos and sin, and (kRotAny) the rows of a pass.
+template <int DT, int MODE>
+struct RotShared {
+  float cos[kRotMaxHalf], sin[kRotMaxHalf];
+  float x[MODE == kRotAny ? 2 * Chunk<DT>::EPL * 64 : 1];
+};
+
+template <int DT, int MODE>
+struct RotLane {
+  static constexpr int EPL = Chunk<DT>::EPL, N = 2 * EPL;
+  RotShared<DT, MODE>& sh;
+  int lane, lpr, rpw, col, lrow, o1, o2, half;
+  double inv[kRotMaxHalf / 64];
+  float c[MODE == kRotAny ? N : EPL], s[MODE == kRotAny ? N : EPL];
+  int off[MODE == kRotAny ? N : 1];
+
+  __device__ __forceinline__ RotLane(const RotaryParams& P, RotShared<DT, MODE>& shared) : sh(shared) {
+    lane = threadIdx.x & 63;
+    lpr = P.r.D / N;
+    rpw = 64 / lpr;
+    lrow = lane / lpr;
+    col = (lane % lpr) * EPL;  // pairs col .. col + EPL - 1
+    half = P.rd / 2;
+    o1 = 2 * col, o2 = o1 + EPL;
+    if (MODE == kRotHalf) {
+      if (col < half) o1 = col, o2 = half + col;
+    }
+#pragma unroll
+    for (int k = 0; k < kRotMaxHalf / 64; ++k) {
+      const int i = lane + 64 * k;
+      inv[k] = i < half ? (double)P.r.inv_freq[i] : 0.;
+      sh.cos[i] = 1.f;
+      sh.sin[i] = 0.f;
+    }
+    if constexpr (MODE == kRotAny) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int f = o1 + e, pf = f < half ? f + half : f < P.rd ? f - half : f;
+        off[e] = pf % N * 64 + lane - lane % lpr + pf / N;
+      }
+    }
+  }
+  // The feature of this lane's value e.
+  __device__ __forceinline__ int feature(int e) const { return e < EPL ? o1 + e : o2 + e - EPL; }
+
+  // cos and sin of position p for the lane's pairs.
+  __device__ __forceinline__ void at(const RotaryParams& P, int p, float sign) {
+#pragma unroll
+    for (int k = 0; k < kRotMaxHalf / 64; ++k) {
+      const int i = lane + 64 * k;
+      if (i < half) {
+        // in turns, reduced to half a turn either way
+        const double x = (double)p * inv[k] * 0.15915494309189533577;
+        const float ang = (float)((x - __builtin_rint(x)) * 6.28318530717958647693);
+        float sv, cv;
+        sincosf(ang, &sv, &cv);
+        sh.cos[i] = cv * P.scale;
+        sh.sin[i] = sign * sv * P.scale;
+      }
+    }
+    rot_wave_sync();
+    if constexpr (MODE == kRotAny) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int f = o1 + e, i = f < half ? f : f < P.rd ? f - half : 0;
+        c[e] = sh.cos[i];
+        s[e] = f < half ? -sh.sin[i] : sh.sin[i];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) c[e] = sh.cos[col + e], s[e] = sh.sin[col + e];
+    }
+    rot_wave_sync();
+  }
+
+  // Rotates the lane's values.  (Every lane of the wave comes here.)
+  __device__ __forceinline__ void turn(float (&x)[N]) const {
+    if constexpr (MODE == kRotAny) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) sh.x[64 * e + lane] = x[e];
+      rot_wave_sync();
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float y = x[e] * c[e] + sh.x[off[e]] * s[e];
+        x[e] = o1 + e < 2 * half ? y : x[e];
+      }
+      rot_wave_sync();
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const int i = MODE == kRotInter ? 2 * e : e, j = MODE == kRotInter ? 2 * e + 1 : EPL + e;
+        const float u = x[i], v = x[j];
+        const bool in = MODE == kRotInter ? col + e < half : col < half;
+        x[i] = in ? u * c[e] - v * s[e] : u;
+        x[j] = in ? v * c[e] + u * s[e] : v;
+      }
+    }
+  }
+};
+
+// A wave's tokens, and the position of each (inside: it is rotated).
+struct RotTokens {
+  int t0, n, b;
+  __device__ __forceinline__ RotTokens(const RotaryParams& P, int unit) {
+    t0 = unit * P.r.tpw;
+    n = min(P.r.T - t0, P.r.tpw);
+    b = -1;
+    if (P.pos || n <= 0) return;
+    // Largest b with cu[b] <= t0 (b = -1: before the first sequence).
+    const auto cu = const_space(P.r.cu);
+    int lo = -1, hi = P.r.nseq;
+    if (uni(cu[hi]) <= t0) lo = hi;
+    else
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (uni(cu[mid]) <= t0) lo = mid;
+        else hi = mid;
+      }
+    b = lo;
+  }
+  __device__ __forceinline__ int position(const RotaryParams& P, int t, bool& inside) {
+    inside = true;
+    if (P.pos) return uni(*const_space(P.pos + t));
+    const auto cu = const_space(P.r.cu);
+    while (b < P.r.nseq && uni(cu[b + 1]) <= t) ++b;
+    inside = b >= 0 && b < P.r.nseq;
+    return inside ? t - uni(cu[b]) : 0;
+  }
+};
+
+template <int DT, int MODE, bool NORM>
+__global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(const RotaryParams P) {
+  using Ch = Chunk<DT>;
+  constexpr int EPL = Ch::EPL, N = 2 * EPL, ES = DT == kRopeF32 ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) RotShared<DT, MODE> shared[kRotWaves];
+  __shared__ float wsh[NORM ? 2 : 1][NORM ? 512 : 1];
+  const RopeParams& R = P.r;
+  const int wv = uni(threadIdx.x >> 6);
+  if constexpr (NORM) {
+    for (int d = threadIdx.x; d < R.D; d += 64 * kRotWaves) {
+      wsh[0][d] = R.wq ? R.wq[d] : 1.f;
+      wsh[1][d] = R.wk ? R.wk[d] : 1.f;
+    }
+    __syncthreads();
+  }
+  const int unit = blockIdx.x * kRotWaves + wv;
+  RotLane<DT, MODE> L(P, shared[wv]);
+  RotTokens tokens(P, unit / P.share);
+  const int sub = unit % P.share;  // of the waves that share a token's rows
+  const int nrows = R.Hq + R.Hk, step = L.rpw * P.share;
+  const float inv_d = 1.f / (float)R.D, sign = (float)R.sign;
+  const int r_first = L.lrow + sub * L.rpw;
+
+  for (int it = 0; it < tokens.n; ++it) {
+    const int t = tokens.t0 + it;
+    Raw<DT> x1[kRotPasses], x2[kRotPasses];
+    char* dst[kRotPasses];
+    bool same[kRotPasses];  // in place
+    auto load = [&](int r0) {
+#pragma unroll
+      for (int j = 0; j < kRotPasses; ++j) {
+        const int r = r0 + j * step;
+        dst[j] = nullptr;
+        x1[j].w = x2[j].w = u32x4{0u, 0u, 0u, 0u};
+        if (r >= nrows) continue;
+        const bool isq = r < R.Hq;
+        const int h = isq ? r : r - R.Hq;
+        const char* src = (const char*)(isq ? R.q : R.k) +
+                          ((int64_t)t * (isq ? R.q_ss : R.k_ss) + (int64_t)h * (isq ? R.q_sh : R.k_sh)) * ES;
+        dst[j] = (char*)(isq ? R.q_out : R.k_out) +
+                 ((int64_t)t * (isq ? R.qo_ss : R.ko_ss) + (int64_t)h * (isq ? R.qo_sh : R.ko_sh)) * ES;
+        same[j] = dst[j] == src;
+        x1[j].load(src + L.o1 * ES);
+        x2[j].load(src + L.o2 * ES);
+      }
+    };
+    load(r_first);
+    bool inside;
+    const int p = tokens.position(P, t, inside);
+    if (inside) L.at(P, p, sign);
+    for (int r0 = r_first;;) {
+#pragma unroll
+      for (int j = 0; j < kRotPasses; ++j) {
+        if (r0 - L.lrow + j * step >= nrows) continue;  // (the whole wave: the sums cross lanes)
+        if (!inside) {  // outside every sequence: unchanged
+          if (dst[j] && !same[j]) {
+            x1[j].store(dst[j] + L.o1 * ES);
+            x2[j].store(dst[j] + L.o2 * ES);
+          }
+          continue;
+        }
+        float x[N];
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x[e] = x1[j].get(e), x[EPL + e] = x2[j].get(e);
+        if constexpr (NORM) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < N; ++e) ss += x[e] * x[e];
+          ss = row_sum(ss, L.lpr);
+          const bool isq = r0 + j * step < R.Hq;
+          const bool has = isq ? R.wq != nullptr : R.wk != nullptr;
+          const float rs = has ? rsqrtf(ss * inv_d + R.eps) : 1.f;
+          const float* w = wsh[isq ? 0 : 1];
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) {
+            x[e] = x[e] * rs * w[L.o1 + e];
+            x[EPL + e] = x[EPL + e] * rs * w[L.o2 + e];
+          }
+        }
+        L.turn(x);
+        if (!dst[j]) continue;
+        Ch y1, y2;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) y1.v[e] = x[e], y2.v[e] = x[EPL + e];
+        y1.store(dst[j] + L.o1 * ES);
+        y2.store(dst[j] + L.o2 * ES);
+      }
+      r0 += kRotPasses * step;
+      if (r0 - L.lrow >= nrows) break;
+      load(r0);
+    }
+  }
+}
+
+// Backward of the normalised rotation.  Each workgroup writes its part of dw, in a
+// fixed order, to part[2][gridDim.x][D].
+template <int DT, int MODE>
+__global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotary_norm_bwd_kernel(
+    const RotaryParams P) {
+  using Ch = Chunk<DT>;
+  constexpr int EPL = Ch::EPL, N = 2 * EPL, ES = DT == kRopeF32 ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) RotShared<DT, MODE> shared[kRotWaves];
+  __shared__ float red[2][kRotWaves][512];
+  __shared__ float wsh[2][512];
+  const RopeParams& R = P.r;
+  const int wv = uni(threadIdx.x >> 6);
+  for (int d = threadIdx.x; d < R.D; d += 64 * kRotWaves) {
+    wsh[0][d] = R.wq ? R.wq[d] : 1.f;
+    wsh[1][d] = R.wk ? R.wk[d] : 1.f;
+  }
+  __syncthreads();
+  RotLane<DT, MODE> L(P, shared[wv]);
+  RotTokens tokens(P, blockIdx.x * kRotWaves + wv);
+  const float inv_d = 1.f / (float)R.D, sign = -(float)R.sign;
+  float dw[2][N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) dw[0][e] = dw[1][e] = 0.f;
+
+  for (int it = 0; it < tokens.n; ++it) {
+    const int t = tokens.t0 + it;
+    bool inside;
+    const int p = tokens.position(P, t, inside);
+    if (inside) L.at(P, p, sign);
+    auto rows = [&](auto side_, int r0) {
+      constexpr int side = decltype(side_)::value;
+      const int r = r0 + L.lrow;
+      const bool live = r < (side ? R.Hk : R.Hq);
+      Raw<DT> x1, x2, g1, g2;
+      x1.w = x2.w = g1.w = g2.w = u32x4{0u, 0u, 0u, 0u};
+      if (live) {
+        const char* x = (const char*)(side ? R.k : R.q) +
+                        ((int64_t)t * (side ? R.k_ss : R.q_ss) + (int64_t)r * (side ? R.k_sh : R.q_sh)) * ES;
+        const char* g = (const char*)(side ? R.gk : R.gq) +
+                        ((int64_t)t * (side ? R.gk_ss : R.gq_ss) + (int64_t)r * (side ? R.gk_sh : R.gq_sh)) * ES;
+        x1.load(x + L.o1 * ES);
+        x2.load(x + L.o2 * ES);
+        g1.load(g + L.o1 * ES);
+        g2.load(g + L.o2 * ES);
+      }
+      char* out = (char*)(side ? R.k_out : R.q_out) +
+                  ((int64_t)t * (side ? R.ko_ss : R.qo_ss) + (int64_t)r * (side ? R.ko_sh : R.qo_sh)) * ES;
+      if (!inside) {  // (the same for every lane)
+        if (live) {
+          g1.store(out + L.o1 * ES);
+          g2.store(out + L.o2 * ES);
+        }
+        return;
+      }
+      float y[N];
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) y[e] = g1.get(e), y[EPL + e] = g2.get(e);
+      L.turn(y);
+      if ((side ? R.wk : R.wq) != nullptr) {
+        float ss = 0.f, tw = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float u = e < EPL ? x1.get(e) : x2.get(e - EPL);
+          ss += u * u;
+          tw += u * wsh[side][L.feature(e)] * y[e];
+        }
+        // (a lane past the rows holds zeros; every lane joins the sums)
+        ss = row_sum(ss, L.lpr);
+        tw = row_sum(tw, L.lpr);
+        const float rr = rsqrtf(ss * inv_d + R.eps);
+        const float k3 = rr * rr * rr * tw * inv_d;
+        if (live) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float u = e < EPL ? x1.get(e) : x2.get(e - EPL);
+            dw[side][e] += u * rr * y[e];
+            y[e] = rr * wsh[side][L.feature(e)] * y[e] - u * k3;
+          }
+        }
+      }
+      if (live) {
+        Ch y1, y2;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) y1.v[e] = y[e], y2.v[e] = y[EPL + e];
+        y1.store(out + L.o1 * ES);
+        y2.store(out + L.o2 * ES);
+      }
+    };
+    for (int r = 0; r < R.Hq; r += L.rpw) rows(std::integral_constant<int, 0>{}, r);
+    for (int r = 0; r < R.Hk; r += L.rpw) rows(std::integral_constant<int, 1>{}, r);
+  }
+
+  // dw: lanes that share features, then the waves.
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    for (int m = L.lpr; m < 64; m <<= 1) {
+      dw[0][e] += __shfl_xor(dw[0][e], m);
+      dw[1][e] += __shfl_xor(dw[1][e], m);
+    }
+  if (L.lane < L.lpr) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      red[0][wv][L.feature(e)] = dw[0][e];
+      red[1][wv][L.feature(e)] = dw[1][e];
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < 2 * R.D; d += 64 * kRotWaves) {
+    const int which = d / R.D, dd = d - which * R.D;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRotWaves; ++w) v += red[which][w][dd];
+    R.part[((int64_t)which * gridDim.x + blockIdx.x) * R.D + dd] = v;
+  }
+}
+
+template <int DT>
+void launch_fwd(const RotaryParams& P, int mode, dim3 grid, hipStream_t s) {
+  const bool norm = P.r.wq || P.r.wk;
+  void (*k)(const RotaryParams) =
+      mode == kRotHalf    ? (norm ? rotary_kernel<DT, kRotHalf, true> : rotary_kernel<DT, kRotHalf, false>)
+      : mode == kRotInter ? (norm ? rotary_kernel<DT, kRotInter, true> : rotary_kernel<DT, kRotInter, false>)
+                          : (norm ? rotary_kernel<DT, kRotAny, true> : rotary_kernel<DT, kRotAny, false>);
+  hipLaunchKernelGGL(k, grid, dim3(64 * kRotWaves), 0, s, P);
+}
+template <int DT>
+void launch_bwd(const RotaryParams& P, int mode, dim3 grid, hipStream_t s) {
+  void (*k)(const RotaryParams) = mode == kRotHalf    ? rotary_norm_bwd_kernel<DT, kRotHalf>
+                                  : mode == kRotInter ? rotary_norm_bwd_kernel<DT, kRotInter>
+                                                      : rotary_norm_bwd_kernel<DT, kRotAny>;
+  hipLaunchKernelGGL(k, grid, dim3(64 * kRotWaves), 0, s, P);
+}
+
+int rot_mode(const RotaryParams& P) {
+  const int epl = P.r.dtype == kRopeF32 ? 4 : 8;
+  return P.inter ? kRotInter : (P.rd / 2) % epl == 0 ? kRotHalf : kRotAny;
+}
+int rot_tokens(int T) { return T <= 4096 ? 1 : T <= 12288 ? 2 : 4; }
+int rot_bwd_tokens(int T) { return T <= 1024 ? 1 : T <= 12288 ? 2 : 4; }
+
+}  // namespace
+
+int rotary_bwd_blocks(int T) {
+  const int tpw = rot_bwd_tokens(T);
+  return (int)(((int64_t)T + kRotWaves * tpw - 1) / (kRotWaves * tpw));
+}
+
+hipError_t launch_rotary(const RotaryParams& args, hipStream_t s) {
+  RotaryParams P = args;
+  if (P.r.T <= 0 || P.r.Hq + P.r.Hk <= 0) return hipSuccess;
+  P.r.tpw = rot_tokens(P.r.T);
+  P.share = P.r.T <= 1024 ? kRotWaves : 1;
+  const int64_t waves = ((int64_t)P.r.T + P.r.tpw - 1) / P.r.tpw * P.share;
+  const dim3 grid((uint32_t)((waves + kRotWaves - 1) / kRotWaves));
+  switch (P.r.dtype) {
+    case kRopeBF16: launch_fwd<kRopeBF16>(P, rot_mode(P), grid, s); break;
+    case kRopeF16: launch_fwd<kRopeF16>(P, rot_mode(P), grid, s); break;
+    case kRopeF32: launch_fwd<kRopeF32>(P, rot_mode(P), grid, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_rotary_norm_bwd(const RotaryParams& args, hipStream_t s) {
+  RotaryParams P = args;
+  if (P.r.T <= 0 || P.r.Hq + P.r.Hk <= 0) return hipSuccess;
+  P.r.tpw = rot_bwd_tokens(P.r.T);
+  const int nb = rotary_bwd_blocks(P.r.T);
+  const dim3 grid((uint32_t)nb);
+  switch (P.r.dtype) {
+    case kRopeBF16: launch_bwd<kRopeBF16>(P, rot_mode(P), grid, s); break;
+    case kRopeF16: launch_bwd<kRopeF16>(P, rot_mode(P), grid, s); break;
+    case kRopeF32: launch_bwd<kRopeF32>(P, rot_mode(P), grid, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  if (hipGetLastError() != hipSuccess) return hipErrorLaunchFailure;
+  return launch_rope_dw_reduce(P.r, nb, s);
+}
+
+}  // namespace fna2

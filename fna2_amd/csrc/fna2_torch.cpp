@@ -49,6 +49,9 @@ struct Lib {
   decltype(&fna2_rope_varlen) rope_varlen;
   decltype(&fna2_rope_bwd) rope_bwd;
   decltype(&fna2_rope_bwd_workspace_bytes) rope_bwd_workspace_bytes;
+  decltype(&fna2_rotary) rotary;
+  decltype(&fna2_rotary_bwd) rotary_bwd;
+  decltype(&fna2_rotary_bwd_workspace_bytes) rotary_bwd_workspace_bytes;
   decltype(&fna2_check_paged_attn) check_paged_attn;
   decltype(&fna2_paged_attn_workspace_bytes) paged_attn_workspace_bytes;
   decltype(&fna2_paged_scores_bytes) paged_scores_bytes;
@@ -60,6 +63,9 @@ struct Lib {
   decltype(&fna2_paged_weights) paged_weights;
   decltype(&fna2_paged_append_shifted) paged_append_shifted;
   decltype(&fna2_paged_evict) paged_evict;
+  decltype(&fna2_paged_extend) paged_extend;
+  decltype(&fna2_paged_trim) paged_trim;
+  decltype(&fna2_paged_groups) paged_groups;
 };
 Lib L{};
 
@@ -90,6 +96,9 @@ void bind(const std::map<std::string, uintptr_t>& f, py::object error) {
   FNA2_BIND(rope_varlen);
   FNA2_BIND(rope_bwd);
   FNA2_BIND(rope_bwd_workspace_bytes);
+  FNA2_BIND(rotary);
+  FNA2_BIND(rotary_bwd);
+  FNA2_BIND(rotary_bwd_workspace_bytes);
   FNA2_BIND(check_paged_attn);
   FNA2_BIND(paged_attn_workspace_bytes);
   FNA2_BIND(paged_scores_bytes);
@@ -101,6 +110,9 @@ void bind(const std::map<std::string, uintptr_t>& f, py::object error) {
   FNA2_BIND(paged_weights);
   FNA2_BIND(paged_append_shifted);
   FNA2_BIND(paged_evict);
+  FNA2_BIND(paged_extend);
+  FNA2_BIND(paged_trim);
+  FNA2_BIND(paged_groups);
 #undef FNA2_BIND
 }
 
@@ -495,9 +507,10 @@ OptTensor decode_rows(const Tensor& q, const Tensor& k, const Tensor& v, const O
 
 // The arguments rope_varlen's forward and backward share.  w: the norm
 // weights and inv_freq in fp32 (kept by the caller).
+// part: inv_freq may be of part of the head.
 bool rope_args(fna2_rope_args& a, const Tensor& q, const Tensor& k, const Tensor& cu,
                const Tensor& inv, int64_t sign, const OptTensor& nq, const OptTensor& nk,
-               double eps, Tensor (&w)[3]) {
+               double eps, Tensor (&w)[3], bool part = false) {
   if (!L.rope_varlen || !q.defined() || !q.is_cuda()) return false;
   const c10::Device dev = q.device();
   const auto dt = q.scalar_type();
@@ -506,7 +519,8 @@ bool rope_args(fna2_rope_args& a, const Tensor& q, const Tensor& k, const Tensor
     if (!plain(*t, dev) || t->dim() != 3 || t->scalar_type() != dt || !rows16(*t)) return false;
   const int64_t D = q.size(2);
   if (k.size(0) != q.size(0) || k.size(2) != D || q.size(0) > INT32_MAX) return false;
-  if (!int32_on(cu, dev) || !plain(inv, dev) || inv.numel() != D / 2 || !inv.is_floating_point())
+  if (!int32_on(cu, dev) || !plain(inv, dev) || (!part && inv.numel() != D / 2) ||
+      inv.numel() > D / 2 || !inv.is_floating_point())
     return false;
   w[2] = inv.to(at::kFloat).contiguous();
   const OptTensor* norms[2] = {&nq, &nk};
@@ -584,6 +598,81 @@ std::optional<std::tuple<Tensor, Tensor, OptTensor, OptTensor>> rope_bwd(
     b.workspace_bytes = need;
   }
   if (!launched(L.rope_bwd(&b, stream_of(dev)), "fna2_rope_bwd")) return std::nullopt;
+  return std::make_tuple(dq, dk, dn[0], dn[1]);
+}
+
+// rotary_embed's arguments: rope_args, with positions or cu_seqlens.
+bool rotary_args(fna2_rotary_args& a, const Tensor& q, const Tensor& k, const Tensor& inv,
+                 const OptTensor& pos, const OptTensor& cu, bool inter, double scale, int64_t sign,
+                 const OptTensor& nq, const OptTensor& nk, double eps, Tensor (&w)[3]) {
+  if (!L.rotary || pos.has_value() == cu.has_value()) return false;
+  const Tensor& where = pos.has_value() ? *pos : *cu;
+  if (!rope_args(a.r, q, k, where, inv, sign, nq, nk, eps, w, true) || where.dim() != 1) return false;
+  if (pos.has_value()) {
+    if (pos->numel() != q.size(0)) return false;
+    a.positions = a.r.cu_seqlens;
+    a.r.cu_seqlens = nullptr;
+    a.r.nseq = 0;
+  }
+  a.rotary_dim = (int32_t)(2 * inv.numel());
+  a.interleaved = inter;
+  a.scale = (float)scale;
+  return true;
+}
+
+// rotary_embed without gradients: (q, k).
+std::optional<std::tuple<Tensor, Tensor>> rotary_fwd(const Tensor& q, const Tensor& k,
+                                                     const Tensor& inv, const OptTensor& pos,
+                                                     const OptTensor& cu, bool inter, double scale,
+                                                     const OptTensor& nq, const OptTensor& nk,
+                                                     double eps) {
+  fna2_rotary_args a{};
+  Tensor w[3];
+  const c10::OptionalDeviceGuard guard(at::device_of(q));
+  if (!rotary_args(a, q, k, inv, pos, cu, inter, scale, 1, nq, nk, eps, w)) return std::nullopt;
+  const Tensor qo = at::empty_like(q, at::MemoryFormat::Contiguous);
+  const Tensor ko = at::empty_like(k, at::MemoryFormat::Contiguous);
+  a.r.q_out = view(qo, true);
+  a.r.k_out = view(ko, true);
+  if (!launched(L.rotary(&a, stream_of(q.device())), "rotary_embed")) return std::nullopt;
+  return std::make_tuple(qo, ko);
+}
+
+// rotary_embed's backward: (dq, dk, dnorm_q, dnorm_k).
+std::optional<std::tuple<Tensor, Tensor, OptTensor, OptTensor>> rotary_bwd(
+    const Tensor& dqo, const Tensor& dko, const Tensor& q, const Tensor& k, const Tensor& inv,
+    const OptTensor& pos, const OptTensor& cu, bool inter, double scale, const OptTensor& nq,
+    const OptTensor& nk, double eps, const OptTensor& dq_, const OptTensor& dk_) {
+  fna2_rotary_bwd_args b{};
+  Tensor w[3];
+  const c10::OptionalDeviceGuard guard(at::device_of(q));
+  if (!rotary_args(b.fwd, q, k, inv, pos, cu, inter, scale, 1, nq, nk, eps, w)) return std::nullopt;
+  const c10::Device dev = q.device();
+  auto like = [&](const Tensor& t, const Tensor& x) {
+    return plain(t, dev) && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes();
+  };
+  if (!like(dqo, q) || !like(dko, k) || !rows16(dqo) || !rows16(dko)) return std::nullopt;
+  if ((dq_.has_value() && !like(*dq_, q)) || (dk_.has_value() && !like(*dk_, k)))
+    return std::nullopt;
+  const Tensor dq = dq_.has_value() ? *dq_ : at::empty_like(q, at::MemoryFormat::Contiguous);
+  const Tensor dk = dk_.has_value() ? *dk_ : at::empty_like(k, at::MemoryFormat::Contiguous);
+  b.dq_out = view(dqo, true);
+  b.dk_out = view(dko, true);
+  b.dq = view(dq, true);
+  b.dk = view(dk, true);
+  OptTensor dn[2];
+  for (int i = 0; i < 2; ++i)
+    if (w[i].defined()) dn[i] = at::empty_like(w[i]);
+  b.dnorm_q = dn[0] ? dn[0]->data_ptr<float>() : nullptr;
+  b.dnorm_k = dn[1] ? dn[1]->data_ptr<float>() : nullptr;
+  const size_t need = L.rotary_bwd_workspace_bytes(&b.fwd);
+  Tensor ws;
+  if (need > 0) {
+    ws = bytes_on(need, q);
+    b.workspace = ws.data_ptr();
+    b.workspace_bytes = need;
+  }
+  if (!launched(L.rotary_bwd(&b, stream_of(dev)), "rotary_embed")) return std::nullopt;
   return std::make_tuple(dq, dk, dn[0], dn[1]);
 }
 
@@ -845,6 +934,114 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> paged_evict(
   return std::make_tuple(kept, new_lens, w_out);
 }
 
+// The books of a paged cache: block table (used in place), lengths and stack.
+bool paged_books(fna2_paged_books& b, const Tensor& table, int64_t page_size, const Tensor* lens,
+                 const Tensor* stack, const Tensor* count) {
+  if (!table.defined() || !table.is_cuda()) return false;
+  const c10::Device dev = table.device();
+  if (!plain(table, dev) || table.scalar_type() != at::kInt || table.dim() != 2 ||
+      table.stride(1) != 1 || table.stride(0) < table.size(1) || table.size(0) > INT32_MAX ||
+      table.size(1) > INT32_MAX || page_size <= 0 || page_size > INT32_MAX)
+    return false;
+  b.batch = (int32_t)table.size(0);
+  b.table_width = (int32_t)table.size(1);
+  b.page_size = (int32_t)page_size;
+  b.block_table = table.data_ptr<int32_t>();
+  b.table_stride = table.stride(0);
+  if (!lens) return true;
+  if (table.is_inference() && !c10::InferenceMode::is_enabled()) return false;
+  if (!int32_on(*lens, dev) || lens->dim() != 1 || lens->numel() != b.batch) return false;
+  if (!int32_on(*stack, dev) || stack->dim() != 1 || stack->numel() > INT32_MAX ||
+      (stack->is_inference() && !c10::InferenceMode::is_enabled()))
+    return false;
+  if (!int32_on(*count, dev) || count->numel() != 1) return false;
+  b.capacity = (int32_t)stack->numel();
+  b.seqlens = lens->data_ptr<int32_t>();
+  b.free_pages = stack->data_ptr<int32_t>();
+  b.free_count = count->data_ptr<int32_t>();
+  return true;
+}
+
+// One number a sequence, if given.
+bool per_sequence(const OptTensor& t, const fna2_paged_books& b, const c10::Device& dev,
+                  const int32_t*& p) {
+  if (!t.has_value()) return true;
+  if (!int32_on(*t, dev) || t->dim() != 1 || t->numel() != b.batch) return false;
+  p = t->data_ptr<int32_t>();
+  return true;
+}
+
+// paged_extend: the members of PagedStep.
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>> paged_extend(
+    const Tensor& table, const Tensor& lens, const OptTensor& counts, const Tensor& stack,
+    const Tensor& count, int64_t page_size, int64_t T, const OptTensor& shift) {
+  fna2_paged_extend_args a{};
+  if (!L.paged_extend || T < 0 || T > INT32_MAX || !counts.has_value() ||
+      !paged_books(a.b, table, page_size, &lens, &stack, &count))
+    return std::nullopt;
+  const c10::Device dev = table.device();
+  if (!per_sequence(counts, a.b, dev, a.counts) || !per_sequence(shift, a.b, dev, a.position_shift))
+    return std::nullopt;
+  const c10::DeviceGuard guard(dev);
+  // (one allocation for the small ones, each 16-byte aligned)
+  const int64_t N = a.b.batch, n1 = (N + 4) / 4 * 4, n2 = (N + 3) / 4 * 4;
+  const Tensor small = at::empty({n1 + n2 + 8}, table.options());
+  const Tensor cu = small.narrow(0, 0, N + 1), new_lens = small.narrow(0, n1, N);
+  const Tensor new_count = small.narrow(0, n1 + n2, 1), status = small.narrow(0, n1 + n2 + 4, 1);
+  const Tensor slots = at::empty({T}, table.options().dtype(at::kLong));
+  const Tensor seq = at::empty({T}, table.options()), pos = at::empty({T}, table.options());
+  a.total_q = (int32_t)T;
+  a.cu_seqlens_q = cu.data_ptr<int32_t>();
+  a.new_lens = new_lens.data_ptr<int32_t>();
+  a.new_free_count = new_count.data_ptr<int32_t>();
+  a.slots = slots.data_ptr<int64_t>();
+  a.sequences = seq.data_ptr<int32_t>();
+  a.positions = pos.data_ptr<int32_t>();
+  a.status = status.data_ptr<int32_t>();
+  if (!launched(L.paged_extend(&a, stream_of(dev)), "paged_extend")) return std::nullopt;
+  written({&table});
+  return std::make_tuple(cu, new_lens, new_count, slots, seq, pos, status);
+}
+
+// paged_trim: (new lengths, new count).
+std::optional<std::tuple<Tensor, Tensor>> paged_trim(const Tensor& table, const Tensor& lens,
+                                                     const OptTensor& keep, const Tensor& stack,
+                                                     const Tensor& count, int64_t page_size,
+                                                     const OptTensor& borrowed) {
+  fna2_paged_trim_args a{};
+  if (!L.paged_trim || !keep.has_value() ||
+      !paged_books(a.b, table, page_size, &lens, &stack, &count))
+    return std::nullopt;
+  const c10::Device dev = table.device();
+  if (!per_sequence(keep, a.b, dev, a.keep) || !per_sequence(borrowed, a.b, dev, a.borrowed))
+    return std::nullopt;
+  const c10::DeviceGuard guard(dev);
+  const Tensor new_lens = at::empty({a.b.batch}, table.options());
+  const Tensor new_count = at::empty({1}, table.options());
+  a.new_lens = new_lens.data_ptr<int32_t>();
+  a.new_free_count = new_count.data_ptr<int32_t>();
+  if (!launched(L.paged_trim(&a, stream_of(dev)), "paged_trim")) return std::nullopt;
+  written({&table, &stack});
+  return std::make_tuple(new_lens, new_count);
+}
+
+// paged_groups: (cu_groups, shared_rows).
+std::optional<std::tuple<Tensor, Tensor>> paged_groups(const Tensor& table, int64_t page_size) {
+  fna2_paged_groups_args a{};
+  if (!L.paged_groups || !paged_books(a.b, table, page_size, nullptr, nullptr, nullptr))
+    return std::nullopt;
+  const c10::Device dev = table.device();
+  const c10::DeviceGuard guard(dev);
+  const int64_t N = a.b.batch;
+  const Tensor cu = at::empty({N + 1}, table.options());
+  const Tensor rows = at::empty({N}, table.options()), ws = at::empty({N}, table.options());
+  a.cu_groups = cu.data_ptr<int32_t>();
+  a.shared_rows = rows.data_ptr<int32_t>();
+  a.workspace = ws.data_ptr<int32_t>();
+  if (!launched(L.paged_groups(&a, stream_of(dev)), "paged_groups")) return std::nullopt;
+  return std::make_tuple(cu, rows);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_binding, m) {
@@ -857,6 +1054,8 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("decode_rows", &decode_rows, Free());
   m.def("rope_fwd", &rope_fwd, Free());
   m.def("rope_bwd", &rope_bwd, Free());
+  m.def("rotary_fwd", &rotary_fwd, Free());
+  m.def("rotary_bwd", &rotary_bwd, Free());
   m.def("paged_attn", &paged_attn, Free(), py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
         py::arg("block_table"), py::arg("seqlens_k"), py::arg("cu_seqlens_q"),
         py::arg("max_seqlen_q"), py::arg("r_q"), py::arg("rk_pages"), py::arg("graph_scale"),
@@ -869,4 +1068,7 @@ PYBIND11_MODULE(_torch_binding, m) {
         py::arg("positions"), py::arg("norm_q"), py::arg("norm_k"), py::arg("eps"),
         py::arg("position_shift") = py::none());
   m.def("paged_evict", &paged_evict, Free());
+  m.def("paged_extend", &paged_extend, Free());
+  m.def("paged_trim", &paged_trim, Free());
+  m.def("paged_groups", &paged_groups, Free());
 }

@@ -39,7 +39,7 @@ fallback: without the HIP library, or off the GPU, the calls raise.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence, Tuple, Union
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -468,6 +468,165 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     _bump(k_pages, v_pages, rk_pages if H_G else None)
     del keep
     return kept, lens, w_out
+
+
+class PagedStep(NamedTuple):
+    """What ``paged_extend`` says of a step's tokens (all on the device)."""
+    cu_seqlens_q: torch.Tensor  # [N + 1] int32
+    seqlens: torch.Tensor       # [N] int32, the step's tokens included
+    free_count: torch.Tensor    # [1] int32
+    slots: torch.Tensor         # [T] int64: page * page_size + row in the page, or -1
+    sequences: torch.Tensor     # [T] int32, or -1
+    positions: torch.Tensor     # [T] int32
+    status: torch.Tensor        # [1] int32
+
+
+def _books(what: str, block_table, page_size, seqlens=None, free_pages=None, free_count=None):
+    """(PagedBooks, tensors kept alive): the table and the stack are used in place."""
+    _gpu(block_table, "block_table", what)
+    dev = block_table.device
+    assert block_table.dim() == 2 and block_table.dtype == torch.int32, \
+        f"{what}: block_table must be [sequences, pages] int32"
+    assert block_table.stride(1) == 1 or block_table.shape[1] <= 1, \
+        f"{what}: block_table needs contiguous rows"
+    b = _capi.PagedBooks()
+    b.batch, b.table_width = block_table.shape
+    b.page_size = int(page_size)
+    b.block_table = block_table.data_ptr() or None
+    b.table_stride = max(block_table.stride(0), b.table_width) if b.batch <= 1 else block_table.stride(0)
+    if seqlens is None:
+        return b, ()
+    lens = _ints(seqlens, dev)
+    assert lens.shape == (b.batch,), f"{what}: seqlens must hold one length a sequence"
+    _gpu(free_pages, "free_pages", what)
+    assert free_pages.device == dev and free_pages.dim() == 1 and \
+        free_pages.dtype == torch.int32 and free_pages.is_contiguous(), \
+        f"{what}: free_pages must be a contiguous int32 vector on the table's device"
+    count = _ints(free_count, dev)
+    assert count.numel() == 1, f"{what}: free_count must hold one number"
+    b.capacity = free_pages.numel()
+    b.seqlens, b.free_pages = lens.data_ptr() or None, free_pages.data_ptr() or None
+    b.free_count = count.data_ptr()
+    return b, (lens, count)
+
+
+def _per_sequence(what, name, t, N, dev) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    t = _ints(t, dev)
+    assert t.shape == (N,), f"{what}: {name} must hold one number a sequence"
+    return t
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr() or None
+
+
+def paged_extend(block_table: torch.Tensor, seqlens: torch.Tensor, counts: torch.Tensor,
+                 free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int, total_q: int,
+                 position_shift: Optional[torch.Tensor] = None) -> PagedStep:
+    """The books of a step, made on the GPU: ``counts[b]`` new tokens for sequence b
+    of ``seqlens[b]`` rows (both ``[N]`` int32; below 0: 0).  Pages that the new rows need
+    come off the top of the stack ``free_pages[:free_count]`` (int32), in the
+    order of the sequences, and go into ``block_table`` ``[N, width]`` (int32), which
+    is written in place; the lengths and the stack's count come as new tensors, and a
+    repeated call gives the same again.  ``total_q`` is the host's bound of the
+    step's tokens T, the length of what comes per token: its slot, its
+    sequence (-1 behind the last token) and its position, the row plus
+    ``position_shift[b]``.
+
+    All or nothing.  ``status`` is 0, or, with no page taken, no length changed and no
+    token in the step: the number of pages missing, -1 where a sequence outgrows its row of
+    the table, -2 where there are more than ``total_q`` tokens."""
+    what = "paged_extend"
+    nat = _capi.native_or_none() if block_table.is_cuda else None
+    if nat is not None:
+        done = nat.paged_extend(block_table, seqlens, counts, free_pages, free_count,
+                                int(page_size), int(total_q), position_shift)
+        if done is not None:
+            return PagedStep(*done)
+    b, keep = _books(what, block_table, page_size, seqlens, free_pages, free_count)
+    _written(block_table, "block_table")
+    N, dev, T = b.batch, block_table.device, int(total_q)
+    assert T >= 0, f"{what}: total_q must not be negative"
+    assert counts is not None, f"{what}: counts expected"
+    c = _per_sequence(what, "counts", counts, N, dev)
+    shift = _per_sequence(what, "position_shift", position_shift, N, dev)
+    new = lambda n, dt=torch.int32: torch.empty(n, dtype=dt, device=dev)
+    out = PagedStep(new(N + 1), new(N), new(1), new(T, torch.int64), new(T), new(T), new(1))
+    a = _capi.PagedExtendArgs()
+    a.b, a.counts, a.position_shift, a.total_q = b, _at(c), _at(shift), T
+    a.cu_seqlens_q, a.new_lens, a.new_free_count = (_at(t) for t in out[:3])
+    a.slots, a.sequences, a.positions, a.status = (_at(t) for t in out[3:])
+    lib = _capi.lib()
+    _capi.raise_for(lib.fna2_check_paged_extend(ctypes.byref(a)), what)
+    with torch.cuda.device(dev):
+        _capi.raise_for(lib.fna2_paged_extend(ctypes.byref(a), _stream(dev)), what)
+    _bump(block_table)
+    del keep
+    return out
+
+
+def paged_trim(block_table: torch.Tensor, seqlens: torch.Tensor, keep: torch.Tensor,
+               free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
+               borrowed: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Brings every sequence to ``min(seqlens[b], keep[b])`` rows (below 0: 0): one that is
+    done, one whose drafted tokens were refused, one that was evicted.  Entries of
+    ``block_table`` behind the pages that then hold rows become -1, and the
+    pages go back onto the stack (``free_pages``, room for them expected), sequence by
+    sequence, each one's last page first: but not the first ``borrowed[b]`` pages of a
+    sequence, which are another's.  ``block_table`` and ``free_pages`` are written
+    in place; returns the new lengths and the new count, both new tensors."""
+    what = "paged_trim"
+    nat = _capi.native_or_none() if block_table.is_cuda else None
+    if nat is not None:
+        done = nat.paged_trim(block_table, seqlens, keep, free_pages, free_count, int(page_size),
+                              borrowed)
+        if done is not None:
+            return done
+    b, alive = _books(what, block_table, page_size, seqlens, free_pages, free_count)
+    _written(block_table, "block_table")
+    _written(free_pages, "free_pages")
+    N, dev = b.batch, block_table.device
+    assert keep is not None, f"{what}: keep expected"
+    rows = _per_sequence(what, "keep", keep, N, dev)
+    lent = _per_sequence(what, "borrowed", borrowed, N, dev)
+    lens = torch.empty(N, dtype=torch.int32, device=dev)
+    count = torch.empty(1, dtype=torch.int32, device=dev)
+    a = _capi.PagedTrimArgs()
+    a.b, a.keep, a.borrowed, a.new_lens, a.new_free_count = b, _at(rows), _at(lent), _at(lens), _at(count)
+    lib = _capi.lib()
+    _capi.raise_for(lib.fna2_check_paged_trim(ctypes.byref(a)), what)
+    with torch.cuda.device(dev):
+        _capi.raise_for(lib.fna2_paged_trim(ctypes.byref(a), _stream(dev)), what)
+    _bump(block_table, free_pages)
+    del alive
+    return lens, count
+
+
+def paged_groups(block_table: torch.Tensor, page_size: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(cu_groups [N + 1], shared_rows [N])`` for ``flash_naylis_shared``: runs of
+    neighbouring sequences whose rows of ``block_table`` ``[N, width]`` (int32) begin with
+    the same page are a group, which shares the pages (none below 0) that all
+    its rows begin with; a sequence that shares with no neighbour is a group of its
+    own, with 0 rows.  Behind the last group ``cu_groups`` holds N and ``shared_rows`` 0."""
+    what = "paged_groups"
+    nat = _capi.native_or_none() if block_table.is_cuda else None
+    if nat is not None:
+        done = nat.paged_groups(block_table, int(page_size))
+        if done is not None:
+            return done
+    b, _ = _books(what, block_table, page_size)
+    N, dev = b.batch, block_table.device
+    new = lambda n: torch.empty(n, dtype=torch.int32, device=dev)
+    cu, rows, ws = new(N + 1), new(N), new(N)
+    a = _capi.PagedGroupsArgs()
+    a.b, a.cu_groups, a.shared_rows, a.workspace = b, _at(cu), _at(rows), _at(ws)
+    lib = _capi.lib()
+    _capi.raise_for(lib.fna2_check_paged_groups(ctypes.byref(a)), what)
+    with torch.cuda.device(dev):
+        _capi.raise_for(lib.fna2_paged_groups(ctypes.byref(a), _stream(dev)), what)
+    return cu, rows
 
 
 class PageTable:

@@ -227,6 +227,42 @@ int fna2_check_rope_bwd(const fna2_rope_bwd_args* args);
 /* Backward of fna2_rope_varlen (one launch without a norm, two with). */
 int fna2_rope_bwd(const fna2_rope_bwd_args* args, void* hip_stream);
 
+/* Rotary positions in either layout, over part of the head, scaled, at given
+ * positions; r as for fna2_rope_varlen (both tensors, the optional norm), but for:
+ *   r.inv_freq  [rotary_dim / 2]; the first rotary_dim features of a row are
+ *               rotated, in pairs (i, i + rotary_dim/2), or (2i, 2i+1) with
+ *               interleaved, by p * inv_freq[i], and multiplied by scale; the others
+ *               are only normalised;
+ *   positions   [T] device int32, and r.cu_seqlens NULL: a position for every token; or
+ *               NULL: the position in its sequence, as there.
+ * The chain is fp32 (the angle fp64) with one rounding, with a norm or
+ * without.  r.sign -1 rotates by -angle. */
+typedef struct fna2_rotary_args {
+  fna2_rope_args r;
+  const int32_t* positions;
+  int32_t rotary_dim;      /* even, in [2, head_dim]                           */
+  int32_t interleaved;     /* 0 or 1                                           */
+  float scale;             /* finite                                           */
+} fna2_rotary_args;
+
+int fna2_check_rotary(const fna2_rotary_args* args);
+int fna2_rotary(const fna2_rotary_args* args, void* hip_stream);
+
+/* Its backward; the tensors as in fna2_rope_bwd_args. */
+typedef struct fna2_rotary_bwd_args {
+  fna2_rotary_args fwd;
+  fna2_tensor dq_out, dk_out;   /* incoming gradients [T, H, D], [T, H_KV, D]  */
+  fna2_tensor dq, dk;           /* written                                     */
+  float* dnorm_q;               /* [D] fp32, written where fwd.r.norm_q        */
+  float* dnorm_k;
+  void* workspace;              /* fna2_rotary_bwd_workspace_bytes             */
+  size_t workspace_bytes;
+} fna2_rotary_bwd_args;
+
+size_t fna2_rotary_bwd_workspace_bytes(const fna2_rotary_args* args);
+int fna2_check_rotary_bwd(const fna2_rotary_bwd_args* args);
+int fna2_rotary_bwd(const fna2_rotary_bwd_args* args, void* hip_stream);
+
 /* One-token decode against a KV cache.  Sequence b has one new query row per
  * head and len_b cached rows (the new token's row included), all visible:
  *     S_j = softmax_scale <q_h, K_j> + [h < H_G] graph_scale[h] <rq_h, Rk_hj>
@@ -461,6 +497,74 @@ typedef struct fna2_paged_evict_args {
 
 int fna2_check_paged_evict(const fna2_paged_evict_args* args);
 int fna2_paged_evict(const fna2_paged_evict_args* args, void* hip_stream);
+
+/* The books of a paged cache on the device: the block table, the lengths, and a
+ * stack of the free pages, free_pages[0 .. *free_count), its top last. */
+typedef struct fna2_paged_books {
+  int32_t batch;               /* N sequences                                  */
+  int32_t table_width;         /* entries of a block table row                 */
+  int32_t page_size;           /* rows of a page: a multiple of 16             */
+  int32_t capacity;            /* entries that free_pages has room for         */
+  int32_t* block_table;        /* [N][table_stride], written in place          */
+  int64_t table_stride;
+  const int32_t* seqlens;      /* [N] rows in use (below 0: 0)                 */
+  int32_t* free_pages;         /* [capacity] (written by the trim)             */
+  const int32_t* free_count;   /* [1]                                          */
+} fna2_paged_books;
+
+/* Takes in counts[b] new tokens for every sequence b (below 0: 0): with have =
+ * ceil(len / page_size) pages, the ceil((len + count) / page_size) - have more ones come
+ * from the stack's top, in the order of the sequences, into the table's next entries.
+ * All or nothing: where the stack has too few pages, status is the number
+ * missing; where a sequence outgrows its table's row (or 2^30 rows), -1; where there are more
+ * than total_q tokens, -2: then no page is taken, the lengths stay, cu_seqlens_q
+ * is 0.  Otherwise status is 0.  One launch; nothing is read back. */
+typedef struct fna2_paged_extend_args {
+  fna2_paged_books b;
+  const int32_t* counts;         /* [N]                                        */
+  const int32_t* position_shift; /* [N], or NULL: 0                            */
+  int32_t total_q;               /* T: tokens that the step has room for       */
+  int32_t* cu_seqlens_q;         /* [N+1]: sums of the counts                  */
+  int32_t* new_lens;             /* [N]: not seqlens itself                    */
+  int32_t* new_free_count;       /* [1]: not free_count itself                 */
+  int64_t* slots;                /* [T]: page * page_size + row in it, or -1   */
+  int32_t* sequences;            /* [T], or -1 behind the last token           */
+  int32_t* positions;            /* [T]: row + position_shift, or 0            */
+  int32_t* status;               /* [1]                                        */
+} fna2_paged_extend_args;
+
+int fna2_check_paged_extend(const fna2_paged_extend_args* args);
+int fna2_paged_extend(const fna2_paged_extend_args* args, void* hip_stream);
+
+/* Brings every sequence to min(len, keep[b]) rows (keep below 0: 0).  The
+ * table's entries behind the pages that then hold rows become -1; their pages go
+ * back onto the stack (sequences in order, each one's last page first), but for
+ * the first borrowed[b] of a sequence's, which are another's. */
+typedef struct fna2_paged_trim_args {
+  fna2_paged_books b;
+  const int32_t* keep;           /* [N]                                        */
+  const int32_t* borrowed;       /* [N], or NULL: 0                            */
+  int32_t* new_lens;             /* [N]                                        */
+  int32_t* new_free_count;       /* [1]                                        */
+} fna2_paged_trim_args;
+
+int fna2_check_paged_trim(const fna2_paged_trim_args* args);
+int fna2_paged_trim(const fna2_paged_trim_args* args, void* hip_stream);
+
+/* The groups of fna2_paged_shared: runs of neighbouring sequences whose rows of the
+ * table begin with the same page; a group shares the entries (none below 0) that
+ * all of its rows begin with, page_size rows each.  Sequences that share with no
+ * neighbour are groups of one, with 0 rows.  (b: batch, table_width, page_size,
+ * block_table, table_stride; the others unused.) */
+typedef struct fna2_paged_groups_args {
+  fna2_paged_books b;
+  int32_t* cu_groups;            /* [N+1]: padded with N                       */
+  int32_t* shared_rows;          /* [N]: padded with 0                         */
+  int32_t* workspace;            /* [N]                                        */
+} fna2_paged_groups_args;
+
+int fna2_check_paged_groups(const fna2_paged_groups_args* args);
+int fna2_paged_groups(const fna2_paged_groups_args* args, void* hip_stream);
 
 /* ABI version (FNA2_ABI_VERSION). */
 int fna2_version(void);
