@@ -167,6 +167,7 @@ class RotaryArgs(ctypes.Structure):
         ("rotary_dim", ctypes.c_int32),
         ("interleaved", ctypes.c_int32),
         ("scale", ctypes.c_float),
+        ("norm_dtype", ctypes.c_int32),
     ]
 
 

@@ -1326,6 +1326,9 @@ int rotary_common(const fna2_rotary_args* a) {
   if (a->rotary_dim < 2 || a->rotary_dim > r.head_dim || a->rotary_dim % 2 != 0) return FNA2_E_HEAD_DIM;
   if (a->interleaved != 0 && a->interleaved != 1) return FNA2_E_SHAPE;
   if (!std::isfinite(a->scale)) return FNA2_E_SCALE;
+  if ((r.norm_q || r.norm_k) && a->norm_dtype != FNA2_BF16 && a->norm_dtype != FNA2_F16 &&
+      a->norm_dtype != FNA2_F32)
+    return FNA2_E_DTYPE;
   return FNA2_OK;
 }
 
@@ -1337,6 +1340,9 @@ fna2::RotaryParams rotary_params(const fna2_rotary_args* a) {
   P.inter = a->interleaved;
   P.scale = a->scale;
   P.pos = a->positions;
+  P.wdt = a->norm_dtype == FNA2_BF16  ? fna2::kRopeBF16
+          : a->norm_dtype == FNA2_F16 ? fna2::kRopeF16
+                                      : fna2::kRopeF32;
   return P;
 }
 
@@ -1422,8 +1428,8 @@ int fna2_rotary_bwd(const fna2_rotary_bwd_args* b, void* stream) {
     e = fna2::launch_rotary(P, (hipStream_t)stream);
   } else {
     P.r.part = (float*)b->workspace;
-    P.r.dwq = P.r.wq ? b->dnorm_q : nullptr;
-    P.r.dwk = P.r.wk ? b->dnorm_k : nullptr;
+    P.r.dwq = P.r.wq ? (float*)b->dnorm_q : nullptr;  // (of type wdt)
+    P.r.dwk = P.r.wk ? (float*)b->dnorm_k : nullptr;
     e = fna2::launch_rotary_norm_bwd(P, (hipStream_t)stream);
   }
   return e == hipSuccess ? FNA2_OK : FNA2_E_LAUNCH;

@@ -109,13 +109,11 @@ struct RopeParams {
 int rope_bwd_blocks(int T);  // workgroups of the norm backward over T tokens
 hipError_t launch_rope(const RopeParams& P, hipStream_t s);
 hipError_t launch_rope_norm_bwd(const RopeParams& P, hipStream_t s);
-// dw from the partials of `nblocks` workgroups.
-hipError_t launch_rope_dw_reduce(const RopeParams& P, int nblocks, hipStream_t s);
 
 // Rotary positions in either layout, over rd features, scaled (fna2_rotary.hip).
 struct RotaryParams {
-  RopeParams r;    // cu unused with pos; inv_freq [rd / 2]
-  int rd, inter;
+  RopeParams r;    // cu unused with pos; inv_freq [rd / 2]; wq, wk, dwq, dwk of type wdt
+  int rd, inter, wdt;
   float scale;     // of the rotated features
   const int* pos;  // [T], or null: the packed sequences'
   int share;       // waves of a token (set by the launch)

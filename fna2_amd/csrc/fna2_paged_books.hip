@@ -11,8 +11,8 @@ namespace fna2 {
 
 namespace {
 
-constexpr int kBooksThreads = 1024, kBooksWaves = kBooksThreads / 64;
-constexpr int kBooksChunk = 4096;  // sequences whose sums fit in LDS
+constexpr int kBooksThreads = 256, kBooksWaves = kBooksThreads / 64;
+constexpr int kBooksChunk = 1024;  // sequences whose sums are formed at once
 constexpr int kBooksEach = kBooksChunk / kBooksThreads;
 constexpr int kBooksMax = 1 << 30;  // rows of a sequence, tokens of a step
 
@@ -237,47 +237,50 @@ __global__ __launch_bounds__(256) void paged_common_kernel(const BooksParams P) 
 
 __global__ __launch_bounds__(kBooksThreads) void paged_groups_kernel(const BooksParams P) {
   __shared__ int64_t sums[2][kBooksWaves];
+  __shared__ int least[kBooksChunk + 1];
   BooksScan scan{sums};
   const int tid = threadIdx.x, N = P.N;
-  for (int g = tid; g < N; g += kBooksThreads) P.shared_rows[g] = 0x7fffffff;
-  __threadfence();
-  __syncthreads();
-  int before = 0;
+  int before = 0;      // groups that begin in the chunks before
+  int open = kBooksMax;  // the last of them: the least of its pairs so far
   for (int c0 = 0; c0 < N; c0 += kBooksChunk) {
     int64_t a[kBooksEach], b[kBooksEach];
     int c[kBooksEach];
 #pragma unroll
     for (int i = 0; i < kBooksEach; ++i) {
       const int s = c0 + kBooksEach * tid + i;
-      c[i] = s < N ? P.common[s] : 1;
+      c[i] = s < N ? P.common[s] : -1;
       a[i] = c[i] == 0;
       b[i] = 0;
+      least[kBooksEach * tid + i + 1] = kBooksMax;
     }
+    if (tid == 0) least[0] = open;
     scan.run(a, b);
 #pragma unroll
     for (int i = 0; i < kBooksEach; ++i) {
       const int s = c0 + kBooksEach * tid + i;
-      if (s >= N) continue;
-      const int starts = before + (int)a[i];  // ... before this one
-      if (c[i] == 0) P.cu_groups[starts] = s;
-      else atomicMin(P.shared_rows + starts - 1, c[i]);
+      if (c[i] == 0) P.cu_groups[before + (int)a[i]] = s;
+      else if (c[i] > 0) atomicMin(least + (int)a[i], c[i]);  // (the group that is open here)
     }
-    before += (int)scan.total[0];
+    const int n = (int)scan.total[0];
+    __syncthreads();
+    // groups before - 1 .. before + n - 2 are closed; the next goes on
+    for (int g = tid; g < n; g += kBooksThreads)
+      if (before + g > 0) P.shared_rows[before + g - 1] = least[g] == kBooksMax ? 0 : least[g] * P.ps;
+    open = least[n];
+    before += n;
+    __syncthreads();
   }
-  __threadfence();
-  __syncthreads();
-  for (int g = tid; g <= N; g += kBooksThreads) {
-    if (g >= before) P.cu_groups[g] = N;
-    if (g == N) continue;
-    const int n = __hip_atomic_load(P.shared_rows + g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    P.shared_rows[g] = n == 0x7fffffff ? 0 : n * P.ps;
+  if (tid == 0 && before > 0) P.shared_rows[before - 1] = open == kBooksMax ? 0 : open * P.ps;
+  for (int g = before + tid; g <= N; g += kBooksThreads) {
+    P.cu_groups[g] = N;
+    if (g < N) P.shared_rows[g] = 0;
   }
 }
 
 }  // namespace
 
 hipError_t launch_paged_extend(const BooksParams& P, hipStream_t s) {
-  const int grid = std::min(std::max((P.T + kBooksThreads - 1) / kBooksThreads, 1), 256);
+  const int grid = std::min(std::max((P.T + kBooksThreads - 1) / kBooksThreads, 1), 512);
   hipLaunchKernelGGL(paged_extend_kernel, dim3(grid), dim3(kBooksThreads), 0, s, P);
   return hipGetLastError();
 }

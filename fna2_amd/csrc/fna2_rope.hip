@@ -439,11 +439,7 @@ hipError_t launch_rope_norm_bwd(const RopeParams& args, hipStream_t s) {
     default: return hipErrorInvalidValue;
   }
   if (hipGetLastError() != hipSuccess) return hipErrorLaunchFailure;
-  return launch_rope_dw_reduce(P, nb, s);
-}
-
-hipError_t launch_rope_dw_reduce(const RopeParams& P, int nblocks, hipStream_t s) {
-  hipLaunchKernelGGL(rope_dw_reduce_kernel, dim3((2 * P.D + 63) / 64), dim3(1024), 0, s, P, nblocks);
+  hipLaunchKernelGGL(rope_dw_reduce_kernel, dim3((2 * P.D + 63) / 64), dim3(1024), 0, s, P, nb);
   return hipGetLastError();
 }
 

@@ -43,12 +43,29 @@ struct RotShared {
   float x[MODE == kRotAny ? 2 * Chunk<DT>::EPL * 64 : 1];
 };
 
+// The norm weights (1 for a side without) to LDS.
+__device__ __forceinline__ void rot_weights(const RotaryParams& P, float (*wsh)[512]) {
+  for (int i = threadIdx.x; i < 2 * P.r.D; i += 64 * kRotWaves) {
+    const int side = i >= P.r.D, d = i - side * P.r.D;
+    const void* w = side ? P.r.wk : P.r.wq;
+    float x = 1.f;
+    if (w) {
+      const uint16_t h = P.wdt == kRopeF32 ? 0 : ((const uint16_t*)w)[d];
+      x = P.wdt == kRopeF32   ? ((const float*)w)[d]
+          : P.wdt == kRopeF16 ? (float)__builtin_bit_cast(_Float16, h)
+                              : __builtin_bit_cast(float, (uint32_t)h << 16);
+    }
+    wsh[side][d] = x;
+  }
+  __syncthreads();
+}
+
 template <int DT, int MODE>
 struct RotLane {
   static constexpr int EPL = Chunk<DT>::EPL, N = 2 * EPL;
   RotShared<DT, MODE>& sh;
   int lane, lpr, rpw, col, lrow, o1, o2, half;
-  double inv[kRotMaxHalf / 64];
+  float inv;  // of pair `lane` (those from 64 on are read when used)
   float c[MODE == kRotAny ? N : EPL], s[MODE == kRotAny ? N : EPL];
   int off[MODE == kRotAny ? N : 1];
 
@@ -65,11 +82,10 @@ struct RotLane {
     }
 #pragma unroll
     for (int k = 0; k < kRotMaxHalf / 64; ++k) {
-      const int i = lane + 64 * k;
-      inv[k] = i < half ? (double)P.r.inv_freq[i] : 0.;
-      sh.cos[i] = 1.f;
-      sh.sin[i] = 0.f;
+      sh.cos[lane + 64 * k] = 1.f;
+      sh.sin[lane + 64 * k] = 0.f;
     }
+    inv = lane < half ? P.r.inv_freq[lane] : 0.f;
     if constexpr (MODE == kRotAny) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
@@ -83,15 +99,14 @@ struct RotLane {
 
   // cos and sin of position p for the lane's pairs.
   __device__ __forceinline__ void at(const RotaryParams& P, int p, float sign) {
-#pragma unroll
-    for (int k = 0; k < kRotMaxHalf / 64; ++k) {
-      const int i = lane + 64 * k;
+#pragma unroll 1
+    for (int i = lane; i - lane < half; i += 64) {
       if (i < half) {
         // in turns, reduced to half a turn either way
-        const double x = (double)p * inv[k] * 0.15915494309189533577;
-        const float ang = (float)((x - __builtin_rint(x)) * 6.28318530717958647693);
+        const float f = i < 64 ? inv : P.r.inv_freq[i];
+        const double x = (double)p * (double)f * 0.15915494309189533577;
         float sv, cv;
-        sincosf(ang, &sv, &cv);
+        sincospif((float)(2. * (x - __builtin_rint(x))), &sv, &cv);
         sh.cos[i] = cv * P.scale;
         sh.sin[i] = sign * sv * P.scale;
       }
@@ -167,95 +182,88 @@ struct RotTokens {
 };
 
 template <int DT, int MODE, bool NORM>
-__global__ __launch_bounds__(64 * kRotWaves) void rotary_kernel(const RotaryParams P) {
+__global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotary_kernel(const RotaryParams P) {
   using Ch = Chunk<DT>;
   constexpr int EPL = Ch::EPL, N = 2 * EPL, ES = DT == kRopeF32 ? 4 : 2;
   __shared__ __attribute__((aligned(16))) RotShared<DT, MODE> shared[kRotWaves];
   __shared__ float wsh[NORM ? 2 : 1][NORM ? 512 : 1];
   const RopeParams& R = P.r;
   const int wv = uni(threadIdx.x >> 6);
-  if constexpr (NORM) {
-    for (int d = threadIdx.x; d < R.D; d += 64 * kRotWaves) {
-      wsh[0][d] = R.wq ? R.wq[d] : 1.f;
-      wsh[1][d] = R.wk ? R.wk[d] : 1.f;
-    }
-    __syncthreads();
-  }
+  if constexpr (NORM) rot_weights(P, wsh);
   const int unit = blockIdx.x * kRotWaves + wv;
   RotLane<DT, MODE> L(P, shared[wv]);
   RotTokens tokens(P, unit / P.share);
-  const int sub = unit % P.share;  // of the waves that share a token's rows
-  const int nrows = R.Hq + R.Hk, step = L.rpw * P.share;
+  // Row passes of a wave, q's and then k's: `step` rows each with those of
+  // the waves that share the token.
+  const int step = L.rpw * P.share, nq = cdiv(R.Hq, step), passes = nq + cdiv(R.Hk, step);
+  const int first = unit % P.share * L.rpw + L.lrow;
+  const int batches = cdiv(passes, kRotPasses), batch = cdiv(passes, max(batches, 1));
   const float inv_d = 1.f / (float)R.D, sign = (float)R.sign;
-  const int r_first = L.lrow + sub * L.rpw;
+  const bool in_place = R.q == R.q_out && R.k == R.k_out;
 
   for (int it = 0; it < tokens.n; ++it) {
     const int t = tokens.t0 + it;
-    Raw<DT> x1[kRotPasses], x2[kRotPasses];
-    char* dst[kRotPasses];
-    bool same[kRotPasses];  // in place
-    auto load = [&](int r0) {
-#pragma unroll
-      for (int j = 0; j < kRotPasses; ++j) {
-        const int r = r0 + j * step;
-        dst[j] = nullptr;
-        x1[j].w = x2[j].w = u32x4{0u, 0u, 0u, 0u};
-        if (r >= nrows) continue;
-        const bool isq = r < R.Hq;
-        const int h = isq ? r : r - R.Hq;
-        const char* src = (const char*)(isq ? R.q : R.k) +
-                          ((int64_t)t * (isq ? R.q_ss : R.k_ss) + (int64_t)h * (isq ? R.q_sh : R.k_sh)) * ES;
-        dst[j] = (char*)(isq ? R.q_out : R.k_out) +
-                 ((int64_t)t * (isq ? R.qo_ss : R.ko_ss) + (int64_t)h * (isq ? R.qo_sh : R.ko_sh)) * ES;
-        same[j] = dst[j] == src;
-        x1[j].load(src + L.o1 * ES);
-        x2[j].load(src + L.o2 * ES);
-      }
-    };
-    load(r_first);
     bool inside;
     const int p = tokens.position(P, t, inside);
     if (inside) L.at(P, p, sign);
-    for (int r0 = r_first;;) {
+    else if (in_place) continue;
+#pragma unroll 1
+    for (int j0 = 0; j0 < passes; j0 += batch) {
+      Raw<DT> x1[kRotPasses], x2[kRotPasses];
 #pragma unroll
       for (int j = 0; j < kRotPasses; ++j) {
-        if (r0 - L.lrow + j * step >= nrows) continue;  // (the whole wave: the sums cross lanes)
-        if (!inside) {  // outside every sequence: unchanged
-          if (dst[j] && !same[j]) {
-            x1[j].store(dst[j] + L.o1 * ES);
-            x2[j].store(dst[j] + L.o2 * ES);
-          }
-          continue;
+        if (j >= batch || j0 + j >= passes) break;
+        const bool k = j0 + j >= nq;  // (the same for every lane)
+        const int r = (j0 + j - (k ? nq : 0)) * step + first;
+        x1[j].w = x2[j].w = u32x4{0u, 0u, 0u, 0u};
+        if (r < (k ? R.Hk : R.Hq)) {
+          const char* src = (const char*)(k ? R.k : R.q) + (int64_t)t * ((k ? R.k_ss : R.q_ss) * ES) +
+                            (int64_t)r * ((k ? R.k_sh : R.q_sh) * ES);
+          x1[j].load(src + L.o1 * ES);
+          x2[j].load(src + L.o2 * ES);
         }
-        float x[N];
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) x[e] = x1[j].get(e), x[EPL + e] = x2[j].get(e);
-        if constexpr (NORM) {
-          float ss = 0.f;
-#pragma unroll
-          for (int e = 0; e < N; ++e) ss += x[e] * x[e];
-          ss = row_sum(ss, L.lpr);
-          const bool isq = r0 + j * step < R.Hq;
-          const bool has = isq ? R.wq != nullptr : R.wk != nullptr;
-          const float rs = has ? rsqrtf(ss * inv_d + R.eps) : 1.f;
-          const float* w = wsh[isq ? 0 : 1];
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) {
-            x[e] = x[e] * rs * w[L.o1 + e];
-            x[EPL + e] = x[EPL + e] * rs * w[L.o2 + e];
-          }
-        }
-        L.turn(x);
-        if (!dst[j]) continue;
-        Ch y1, y2;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) y1.v[e] = x[e], y2.v[e] = x[EPL + e];
-        y1.store(dst[j] + L.o1 * ES);
-        y2.store(dst[j] + L.o2 * ES);
       }
-      r0 += kRotPasses * step;
-      if (r0 - L.lrow >= nrows) break;
-      load(r0);
+#pragma unroll
+      for (int j = 0; j < kRotPasses; ++j) {
+        if (j >= batch || j0 + j >= passes) break;
+        const bool k = j0 + j >= nq;
+        const int r = (j0 + j - (k ? nq : 0)) * step + first;
+        char* dst = (char*)(k ? R.k_out : R.q_out) + (int64_t)t * ((k ? R.ko_ss : R.qo_ss) * ES) +
+                    (int64_t)r * ((k ? R.ko_sh : R.qo_sh) * ES);
+        const bool live = r < (k ? R.Hk : R.Hq);
+        if (inside) {
+          float x[N];
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) x[e] = x1[j].get(e), x[EPL + e] = x2[j].get(e);
+          if constexpr (NORM) {
+            if ((k ? R.wk : R.wq) != nullptr) {
+              float ss = 0.f;
+#pragma unroll
+              for (int e = 0; e < N; ++e) ss += x[e] * x[e];
+              // (a lane past the rows holds zeros; every lane joins the sum)
+              const float rs = rsqrtf(row_sum(ss, L.lpr) * inv_d + R.eps);
+              const float* w = wsh[k];
+#pragma unroll
+              for (int e = 0; e < EPL; ++e) {
+                x[e] = x[e] * rs * w[L.o1 + e];
+                x[EPL + e] = x[EPL + e] * rs * w[L.o2 + e];
+              }
+            }
+          }
+          L.turn(x);
+          Ch y1, y2;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) y1.v[e] = x[e], y2.v[e] = x[EPL + e];
+          if (live) {
+            y1.store(dst + L.o1 * ES);
+            y2.store(dst + L.o2 * ES);
+          }
+        } else if (live) {
+          x1[j].store(dst + L.o1 * ES);
+          x2[j].store(dst + L.o2 * ES);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (one pass's values at a time: registers)
+      }
     }
   }
 }
@@ -272,11 +280,7 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
   __shared__ float wsh[2][512];
   const RopeParams& R = P.r;
   const int wv = uni(threadIdx.x >> 6);
-  for (int d = threadIdx.x; d < R.D; d += 64 * kRotWaves) {
-    wsh[0][d] = R.wq ? R.wq[d] : 1.f;
-    wsh[1][d] = R.wk ? R.wk[d] : 1.f;
-  }
-  __syncthreads();
+  rot_weights(P, wsh);
   RotLane<DT, MODE> L(P, shared[wv]);
   RotTokens tokens(P, blockIdx.x * kRotWaves + wv);
   const float inv_d = 1.f / (float)R.D, sign = -(float)R.sign;
@@ -329,6 +333,8 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
         // (a lane past the rows holds zeros; every lane joins the sums)
         ss = row_sum(ss, L.lpr);
         tw = row_sum(tw, L.lpr);
+        // (fp16, interleaved: the products below stay behind the sums, or 10 registers spill)
+        if constexpr (DT == kRopeF16) asm volatile("" : "+v"(ss));
         const float rr = rsqrtf(ss * inv_d + R.eps);
         const float k3 = rr * rr * rr * tw * inv_d;
         if (live) {
@@ -374,6 +380,39 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
     for (int w = 0; w < kRotWaves; ++w) v += red[which][w][dd];
     R.part[((int64_t)which * gridDim.x + blockIdx.x) * R.D + dd] = v;
   }
+}
+
+// dw = the workgroups' parts added up, in 64 bits and a fixed order: workgroup x
+// takes 64 of the 2 D columns, its 16 waves every 16th part each.
+__global__ __launch_bounds__(1024) void rotary_dw_kernel(const RotaryParams P, int nblocks) {
+  __shared__ double acc[16][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, D = P.r.D;
+  const int i = blockIdx.x * 64 + lane;
+  const bool ok = i < 2 * D;
+  const int side = ok && i >= D, d = ok ? i - side * D : 0;
+  const float* src = P.r.part + (int64_t)side * nblocks * D + d;
+  double v = 0.;
+  int b = wv;
+  for (; b + 7 * 16 < nblocks; b += 8 * 16) {  // eight loads in flight
+    float t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t[u] = src[(int64_t)(b + 16 * u) * D];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v += t[u];
+  }
+  for (; b < nblocks; b += 16) v += src[(int64_t)b * D];
+  acc[wv][lane] = v;
+  __syncthreads();
+  if (wv != 0 || !ok) return;
+  double sum = 0.;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) sum += acc[w][lane];
+  void* out = side ? P.r.dwk : P.r.dwq;
+  if (!out) return;
+  const float x = (float)sum;
+  if (P.wdt == kRopeF32) ((float*)out)[d] = x;
+  else if (P.wdt == kRopeF16) ((_Float16*)out)[d] = (_Float16)x;
+  else ((uint16_t*)out)[d] = (uint16_t)pack_bf16(x, 0.f);
 }
 
 template <int DT>
@@ -436,7 +475,8 @@ hipError_t launch_rotary_norm_bwd(const RotaryParams& args, hipStream_t s) {
     default: return hipErrorInvalidValue;
   }
   if (hipGetLastError() != hipSuccess) return hipErrorLaunchFailure;
-  return launch_rope_dw_reduce(P.r, nb, s);
+  hipLaunchKernelGGL(rotary_dw_kernel, dim3((2 * P.r.D + 63) / 64), dim3(1024), 0, s, P, nb);
+  return hipGetLastError();
 }
 
 }  // namespace fna2

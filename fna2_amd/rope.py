@@ -242,7 +242,16 @@ def _rotary_args(q, k, inv, pos, cu, inter, scale, wq, wk, eps) -> _capi.RotaryA
     if pos is not None:
         a.positions, a.r.cu_seqlens, a.r.nseq = pos.data_ptr(), None, 0
     a.rotary_dim, a.interleaved, a.scale = 2 * inv.numel(), int(bool(inter)), float(scale)
+    a.norm_dtype = _DTYPES[next((w.dtype for w in (wq, wk) if w is not None), torch.float32)]
     return a
+
+
+def _weights(wq, wk, dev):
+    """The norm weights as the kernel reads them: of one type, contiguous."""
+    dtypes = {w.dtype for w in (wq, wk) if w is not None}
+    dt = dtypes.pop() if len(dtypes) == 1 else torch.float32
+    return tuple(_on(w, dev, dt if dt in _DTYPES and not dtypes else torch.float32)
+                 for w in (wq, wk))
 
 
 def _on(t: Optional[torch.Tensor], dev, dtype) -> Optional[torch.Tensor]:
@@ -263,7 +272,7 @@ def rotary_embed_raw(q, k, inv_freq, positions=None, cu_seqlens=None, interleave
     q, k, dev = _usable(q), _usable(k), q.device
     inv, pos, cu = _on(inv_freq, dev, torch.float32), _on(positions, dev, torch.int32), \
         _on(cu_seqlens, dev, torch.int32)
-    wq, wk = _f32(norm_q, dev), _f32(norm_k, dev)
+    wq, wk = _weights(norm_q, norm_k, dev)
     a = _rotary_args(q, k, inv, pos, cu, interleaved, scale, wq, wk, eps)
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
@@ -288,7 +297,7 @@ def rotary_embed_bwd(dq_out, dk_out, q, k, inv_freq, positions=None, cu_seqlens=
     dq_out, dk_out = _usable(dq_out.to(q.dtype)), _usable(dk_out.to(k.dtype))
     inv, pos, cu = _on(inv_freq, dev, torch.float32), _on(positions, dev, torch.int32), \
         _on(cu_seqlens, dev, torch.int32)
-    wq, wk = _f32(norm_q, dev), _f32(norm_k, dev)
+    wq, wk = _weights(norm_q, norm_k, dev)
     b = _capi.RotaryBwdArgs()
     b.fwd = _rotary_args(q, k, inv, pos, cu, interleaved, scale, wq, wk, eps)
     if dq is None:
@@ -355,6 +364,11 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
     chain is evaluated in fp32, the angle in fp64, and rounded once.  Differentiable in
     q, k and the norm weights.  ``rotary_frequencies`` makes ``inv_freq`` and ``scale``."""
     args = (q, k, inv_freq, positions, cu_seqlens, norm_q, norm_k)
+    nat = _capi.native_or_none() if q.is_cuda and grad_slab is None else None
+    if nat is not None:
+        done = nat.rotary_embed(*args, bool(interleaved), float(scale), float(eps))
+        if done is not None:
+            return done
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (q, k, norm_q, norm_k)):
         return RotaryFunc.apply(*args, (bool(interleaved), float(scale), float(eps)), grad_slab)

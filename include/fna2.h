@@ -235,6 +235,7 @@ int fna2_rope_bwd(const fna2_rope_bwd_args* args, void* hip_stream);
  *               are only normalised;
  *   positions   [T] device int32, and r.cu_seqlens NULL: a position for every token; or
  *               NULL: the position in its sequence, as there.
+ *   r.norm_q, r.norm_k are of norm_dtype.
  * The chain is fp32 (the angle fp64) with one rounding, with a norm or
  * without.  r.sign -1 rotates by -angle. */
 typedef struct fna2_rotary_args {
@@ -243,6 +244,7 @@ typedef struct fna2_rotary_args {
   int32_t rotary_dim;      /* even, in [2, head_dim]                           */
   int32_t interleaved;     /* 0 or 1                                           */
   float scale;             /* finite                                           */
+  int32_t norm_dtype;      /* enum fna2_dtype, with a norm                     */
 } fna2_rotary_args;
 
 int fna2_check_rotary(const fna2_rotary_args* args);
@@ -253,8 +255,8 @@ typedef struct fna2_rotary_bwd_args {
   fna2_rotary_args fwd;
   fna2_tensor dq_out, dk_out;   /* incoming gradients [T, H, D], [T, H_KV, D]  */
   fna2_tensor dq, dk;           /* written                                     */
-  float* dnorm_q;               /* [D] fp32, written where fwd.r.norm_q        */
-  float* dnorm_k;
+  void* dnorm_q;                /* [D] of norm_dtype, written where fwd.r.norm_q */
+  void* dnorm_k;
   void* workspace;              /* fna2_rotary_bwd_workspace_bytes             */
   size_t workspace_bytes;
 } fna2_rotary_bwd_args;

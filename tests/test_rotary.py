@@ -313,6 +313,17 @@ def test_other_strides_dtypes_and_streams():
 
 
 @gpu
+@pytest.mark.parametrize("wdtype", [torch.float32, torch.float16, torch.bfloat16, torch.float64])
+def test_norm_weights_of_another_type(wdtype):
+    c = Case(40, 4, 2, 64, 32, True, torch.bfloat16, wdtype=wdtype)
+    HALF[torch.float64] = STEP[torch.float64] = 2.0 ** -24  # (rounded to fp32 on the way)
+    check_forward(c)
+    check_backward(c)
+    c.wk = c.wk.to(torch.float32)
+    check_backward(c)
+
+
+@gpu
 def test_captured():
     c = Case(70, 4, 2, 128, 64, True, torch.bfloat16)
     c.run()
@@ -378,6 +389,8 @@ def _args(**over):
     (dict(q_out=_capi.Tensor(FAKE, 0, 256, 64)), "FNA2_OK"),  # in place
     (dict(q=_capi.Tensor(FAKE + 2, 0, 256, 64)), "FNA2_E_STRIDE"),
     (dict(total_tokens=0, q=_capi.empty_tensor()), "FNA2_OK"),
+    (dict(norm_q=FAKE), "FNA2_E_DTYPE"),
+    (dict(norm_q=FAKE, norm_dtype=2), "FNA2_OK"),
 ])
 def test_check(over, code):
     lib = _capi.lib()
@@ -390,7 +403,7 @@ def test_check(over, code):
 def test_check_backward():
     lib = _capi.lib()
     b = _capi.RotaryBwdArgs()
-    b.fwd = _args(norm_q=FAKE)
+    b.fwd = _args(norm_q=FAKE, norm_dtype=3)
     b.dq_out, b.dk_out, b.dq, b.dk = b.fwd.r.q, b.fwd.r.k, b.fwd.r.q_out, b.fwd.r.k_out
     st = lambda: _capi.STATUS[lib.fna2_check_rotary_bwd(ctypes.byref(b))]
     assert st() == "FNA2_E_NULL"
