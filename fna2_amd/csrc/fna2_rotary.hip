@@ -36,6 +36,23 @@ __device__ __forceinline__ void rot_wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// Sum over the lpr lanes of a row, every lane of the wave taking part.  Moves between
+// lanes' registers up to 16 of them (row_sum's go through LDS).
+template <int CTRL>
+__device__ __forceinline__ float rot_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                                           0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float rot_row_sum(float v, int lpr) {
+  if (lpr >= 2) v = rot_add<0xb1>(v);    // quad_perm 1, 0, 3, 2
+  if (lpr >= 4) v = rot_add<0x4e>(v);    // quad_perm 2, 3, 0, 1
+  if (lpr >= 8) v = rot_add<0x141>(v);   // row_half_mirror
+  if (lpr >= 16) v = rot_add<0x140>(v);  // row_mirror
+  if (lpr >= 32) v += __shfl_xor(v, 16);
+  if (lpr >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+
 // LDS of a wave: the token's cos and sin, and (kRotAny) the rows of a pass.
 template <int DT, int MODE>
 struct RotShared {
@@ -193,23 +210,16 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
   const int unit = blockIdx.x * kRotWaves + wv;
   RotLane<DT, MODE> L(P, shared[wv]);
   RotTokens tokens(P, unit / P.share);
-  // Row passes of a wave, q's and then k's: `step` rows each with those of
-  // the waves that share the token.
-  const int step = L.rpw * P.share, nq = cdiv(R.Hq, step), passes = nq + cdiv(R.Hk, step);
-  const int first = unit % P.share * L.rpw + L.lrow;
+  // Row passes, q's and then k's, of the waves that share the token.
+  const int step = L.rpw * P.share, first = unit % P.share * L.rpw + L.lrow, nq = cdiv(R.Hq, step), passes = nq + cdiv(R.Hk, step);
   const int batches = cdiv(passes, kRotPasses), batch = cdiv(passes, max(batches, 1));
   const float inv_d = 1.f / (float)R.D, sign = (float)R.sign;
   const bool in_place = R.q == R.q_out && R.k == R.k_out;
 
   for (int it = 0; it < tokens.n; ++it) {
     const int t = tokens.t0 + it;
-    bool inside;
-    const int p = tokens.position(P, t, inside);
-    if (inside) L.at(P, p, sign);
-    else if (in_place) continue;
-#pragma unroll 1
-    for (int j0 = 0; j0 < passes; j0 += batch) {
-      Raw<DT> x1[kRotPasses], x2[kRotPasses];
+    Raw<DT> x1[kRotPasses], x2[kRotPasses];
+    auto load = [&](int j0) {
 #pragma unroll
       for (int j = 0; j < kRotPasses; ++j) {
         if (j >= batch || j0 + j >= passes) break;
@@ -223,6 +233,15 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
           x2[j].load(src + L.o2 * ES);
         }
       }
+    };
+    load(0);  // (ahead of the angles, which take as long)
+    bool inside;
+    const int p = tokens.position(P, t, inside);
+    if (inside) L.at(P, p, sign);
+    else if (in_place) continue;
+#pragma unroll 1
+    for (int j0 = 0; j0 < passes; j0 += batch) {
+      if (j0 > 0) load(j0);
 #pragma unroll
       for (int j = 0; j < kRotPasses; ++j) {
         if (j >= batch || j0 + j >= passes) break;
@@ -241,7 +260,7 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
 #pragma unroll
               for (int e = 0; e < N; ++e) ss += x[e] * x[e];
               // (a lane past the rows holds zeros; every lane joins the sum)
-              const float rs = rsqrtf(row_sum(ss, L.lpr) * inv_d + R.eps);
+              const float rs = rsqrtf(rot_row_sum(ss, L.lpr) * inv_d + R.eps);
               const float* w = wsh[k];
 #pragma unroll
               for (int e = 0; e < EPL; ++e) {
@@ -331,8 +350,8 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
           tw += u * wsh[side][L.feature(e)] * y[e];
         }
         // (a lane past the rows holds zeros; every lane joins the sums)
-        ss = row_sum(ss, L.lpr);
-        tw = row_sum(tw, L.lpr);
+        ss = rot_row_sum(ss, L.lpr);
+        tw = rot_row_sum(tw, L.lpr);
         // (fp16, interleaved: the products below stay behind the sums, or 10 registers spill)
         if constexpr (DT == kRopeF16) asm volatile("" : "+v"(ss));
         const float rr = rsqrtf(ss * inv_d + R.eps);
@@ -436,7 +455,17 @@ int rot_mode(const RotaryParams& P) {
   const int epl = P.r.dtype == kRopeF32 ? 4 : 8;
   return P.inter ? kRotInter : (P.rd / 2) % epl == 0 ? kRotHalf : kRotAny;
 }
-int rot_tokens(int T) { return T <= 4096 ? 1 : T <= 12288 ? 2 : 4; }
+// Consecutive tokens per wave, which share its start: one while the waves leave
+// the chip with room, or where a token has three passes of rows and more; four once
+// short ones fill it.  (us, 1 / 2 / 4 tokens, with norm: 16384 tokens x 32 heads of 128, four passes,
+// 52.8 / 53.9 / 54.6; x 12 of 64, one pass, 22.1 / 19.1 / 17.8; 8000 x 12 of 64 in fp32 13.0 / 12.1 /
+// 14.0; 2000 x 16 6.4 / 7.2 / 10.8.)  The backward leaves its part of dw as well: 1000 tokens x 40 18.8 /
+// 25.4 / 39.0, 8000 x 12 29.2 / 23.7 / 24.1, 16384 x 32 103 / 93 / 92.
+int rot_tokens(const RotaryParams& P) {
+  const int rpw = 64 * (P.r.dtype == kRopeF32 ? 8 : 16) / P.r.D;
+  if (P.r.T <= 256 || cdiv(P.r.Hq, rpw) + cdiv(P.r.Hk, rpw) >= 3) return 1;
+  return P.r.T <= 4096 ? 1 : P.r.T <= 12288 ? 2 : 4;
+}
 int rot_bwd_tokens(int T) { return T <= 1024 ? 1 : T <= 12288 ? 2 : 4; }
 
 }  // namespace
@@ -449,8 +478,10 @@ int rotary_bwd_blocks(int T) {
 hipError_t launch_rotary(const RotaryParams& args, hipStream_t s) {
   RotaryParams P = args;
   if (P.r.T <= 0 || P.r.Hq + P.r.Hk <= 0) return hipSuccess;
-  P.r.tpw = rot_tokens(P.r.T);
-  P.share = P.r.T <= 1024 ? kRotWaves : 1;
+  P.r.tpw = rot_tokens(P);
+  // Few tokens: the waves of a workgroup share each (us, 64 tokens x 40 rows of 128, one
+  // wave a token 7.0, four 5.0; 1000 8.5, 8.8; 16384 x 32 53, 83).
+  P.share = P.r.T <= 256 ? kRotWaves : 1;
   const int64_t waves = ((int64_t)P.r.T + P.r.tpw - 1) / P.r.tpw * P.share;
   const dim3 grid((uint32_t)((waves + kRotWaves - 1) / kRotWaves));
   switch (P.r.dtype) {
