@@ -1608,10 +1608,16 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
 }
 
 // The same for groups that share rows: the tile kernel, whatever the chunks' length,
-// since the shared rows have the tokens of a whole group.
+// since the shared rows have the tokens of a whole group, with up to 4 heads a tile, since
+// the own rows may have one token (us, 1, 2, 4 heads of 4: 64 tokens over 16384 shared and up
+// to 1000 own rows, rank 32 179, 127, 103; 16 x 128 over 8192, rank 64 345, 361, 350).  Runs are
+// equal in key steps and 8 for each tile that they begin, which takes as long as those: its
+// page ids, first rows, queries, and the part that it leaves (us, 0, 4, 8, 12: the 16 x 128
+// 852, 420, 378, 380; 16 x 64, rank 32 561, 227, 190, 188; 64 tokens, as above 117, 118, 116, 114;
+// 4 over 2000 18.2 with 8, 19.8 with 4).
 struct SharedPlan {
   int hw, waves, min_steps;
-  size_t ml, seqs, ends, recs, whole, whole_ml, bytes;
+  size_t ml, meta, groups, group_ends, seqs, ends, recs, whole, whole_ml, bytes;
 };
 SharedPlan shared_plan(const fna2_paged_shared_args& a) {
   const fna2_paged_cache& c = a.attn.c;
@@ -1634,6 +1640,9 @@ SharedPlan shared_plan(const fna2_paged_shared_args& a) {
   };
   take(2 * (size_t)k.waves * fna2::paged_tile_slot(c.head_dim));
   k.ml = take(2 * (size_t)k.waves * 128 * 8u);
+  k.meta = take(sizeof(fna2::SharedMeta));
+  k.groups = take((size_t)a.groups * sizeof(fna2::SharedGroup));
+  k.group_ends = take((size_t)a.groups * 8u);
   k.seqs = take(virt * sizeof(fna2::SharedSeq));
   k.ends = take(virt * 8u);
   k.recs = take(2 * (size_t)blocks * (size_t)c.total_q * sizeof(fna2::SharedRec));
@@ -1779,10 +1788,15 @@ int fna2_paged_shared(const fna2_paged_shared_args* a, void* stream_ptr) {
   S.p.hw = k.hw;
   S.p.part = (float*)ws;
   S.p.ml = (float*)(ws + k.ml);
+  S.start = 8;  // (see shared_plan)
+  S.small = a->groups <= fna2::kSharedSmall && a->attn.c.batch <= fna2::kSharedSmall;
   S.G = a->groups;
   S.V = a->groups + a->attn.c.batch;
   S.cu_groups = a->cu_groups;
   S.shared_rows = a->shared_rows;
+  S.meta = (fna2::SharedMeta*)(ws + k.meta);
+  S.groups = (fna2::SharedGroup*)(ws + k.groups);
+  S.group_ends = (int64_t*)(ws + k.group_ends);
   S.seqs = (fna2::SharedSeq*)(ws + k.seqs);
   S.ends = (int64_t*)(ws + k.ends);
   S.recs = (fna2::SharedRec*)(ws + k.recs);

@@ -11,12 +11,13 @@
 // token's mask cuts them, in whole key steps of 32; what is left over is each
 // sequence's own.
 //
-// Three launches.  The plan (one workgroup) makes the list of virtual sequences:
-// the groups' shared rows, each of all the group's tokens, and the sequences'
-// own rows; and the sums of their key steps.  The tile kernel
-// (fna2_paged_tile_dev.h) takes equal runs of them.  A tile that runs cut, or
-// that is one of two for its tokens, leaves unnormalised parts; the join adds a
-// token's parts up in a fixed order.
+// The plan forms the units, key steps of tiles of 128 (token, head) columns, of the
+// groups' shared rows with all the group's tokens and of the sequences' own rows, and cuts
+// them into equal runs: every workgroup for itself where 64 sequences and 64 groups at
+// most fit its LDS, else in a launch of its own.  The tile kernel
+// (fna2_paged_tile_dev.h) takes a run a workgroup.  A tile that runs cut, or
+// that is one of two for its tokens, leaves unnormalised parts; the join, another
+// launch, adds a token's parts up in a fixed order.
 #include <algorithm>
 
 #include "fna2_paged_tile_dev.h"
@@ -25,76 +26,12 @@ namespace fna2 {
 
 namespace {
 
+// The plan where a workgroup has no room for it in LDS.
 constexpr int kPlanThreads = 1024;
-
-// One workgroup.  A wave per group: the rows that it shares; then all threads:
-// the units of the virtual sequences, added up.
 __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(const PagedSharedParams) {
   SArg S = sargs();
-  KArg P = &S->p;
-  const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
-  const int N = P->N, G = S->G, V = S->V;
-  SharedSeq* const seqs = S->seqs;
-  for (int b = threadIdx.x; b < N; b += kPlanThreads)
-    seqs[G + b] = SharedSeq{paged_seq(P, b), 0, b, kSharedAlone, 0};
-  __threadfence_block();
-  __syncthreads();
-  for (int g = wv; g < G; g += kPlanThreads / 64) {
-    const int c0 = min(max(uni(S->cu_groups[g]), 0), N);
-    const int c1 = min(max(uni(S->cu_groups[g + 1]), c0), N);
-    // the least number of rows before a chunk, the sequences that have one, and the first of them
-    int least = 0x7fffffff, first = c1, n = 0;
-    for (int b = c0 + lane; b < c1; b += 64) {
-      const PagedSeq s = seqs[G + b].s;
-      if (s.lq <= 0) continue;
-      least = min(least, s.off);
-      first = min(first, b);
-      ++n;
-    }
-#pragma unroll
-    for (int k = 32; k > 0; k >>= 1) {
-      least = min(least, __shfl_xor(least, k));
-      first = min(first, __shfl_xor(first, k));
-      n += __shfl_xor(n, k);
-    }
-    int rows = min(least, uni(S->shared_rows[g]));
-    rows = n > 1 && rows > 0 ? rows & ~31 : 0;
-    SharedSeq pre = SharedSeq{PagedSeq{0, 0, 0, 0}, 0, 0, kSharedPrefix, 0};
-    if (rows > 0) {
-      pre.s.q0 = seqs[G + c0].s.q0;
-      const PagedSeq last = seqs[G + c1 - 1].s;
-      pre.s.lq = max(last.q0 + last.lq - pre.s.q0, 0);
-      pre.s.lk = pre.s.off = rows;
-      pre.table = first;
-      for (int b = c0 + lane; b < c1; b += 64) {
-        SharedSeq x = seqs[G + b];
-        if (x.s.lq <= 0) continue;
-        x.s.lk = max(x.s.lk - rows, 0);
-        x.s.off -= rows;
-        x.row0 = rows;
-        x.kind = kSharedOwn;
-        seqs[G + b] = x;
-      }
-    }
-    if (lane == 0) seqs[g] = pre;
-  }
-  __threadfence_block();
-  __syncthreads();
   __shared__ int64_t sums[kPlanThreads / 64];
-  int64_t before = 0;
-  for (int v0 = 0; v0 < V; v0 += kPlanThreads) {
-    const int v = v0 + threadIdx.x;
-    const int64_t end = lane_scan64(v < V ? TilePlan::units(P, seqs[v].s) : 0);
-    if (lane == 63) sums[wv] = end;
-    __syncthreads();
-    int64_t mine = before;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-      if (w < wv) mine += sums[w];
-      before += sums[w];
-    }
-    if (v < V) S->ends[v] = mine + end;
-    __syncthreads();
-  }
+  shared_plan<kPlanThreads>(S, SharedPlanRef{S->meta, S->groups, S->group_ends, S->seqs, S->ends}, sums);
 }
 
 // The join: a workgroup takes 32 tokens, a query head and 32 features; its
@@ -116,11 +53,17 @@ __global__ __launch_bounds__(256) void paged_shared_join_kernel(const PagedShare
   const int t0 = min(max(uni(*const_space(P->cu)), 0), P->T);
   const int t1 = min(max(uni(*const_space(P->cu + P->N)), t0), P->T);
   const bool loose = tok < P->T && (tok < t0 || tok >= t1);
-  SharedRec a = {0, -1}, b = {0, 0};
-  if (tok >= t0 && tok < t1) a = S->recs[(int64_t)hb * P->T + tok];
-  const bool live = a.parts >= 0, two = live && (a.at & kSharedHas);
-  if (two) b = S->recs[(int64_t)(P->H_KV * hblk + hb) * P->T + tok];
-  const int na = live ? max(a.parts, 1) : 0, nb = two ? max(b.parts, 1) : 0, n = na + nb;
+  // (loaded with the bounds, not behind them: a token of no sequence has no record, and
+  // none is used)
+  SharedRec a{}, b{};
+  if (tok < P->T) {
+    a = S->recs[(int64_t)hb * P->T + tok];
+    b = S->recs[(int64_t)(P->H_KV * hblk + hb) * P->T + tok];
+  }
+  const bool live = tok >= t0 && tok < t1 && a.parts >= 0, has = live && (a.at & kSharedHas);
+  auto parts = [&](int x) { return min(max(x, 0), P->waves); };  // (whatever cu holds, the loop ends)
+  const int na = live ? max(parts(a.parts), 1) : 0, nc = has ? parts(a.full) : 0;
+  const int nb = has && (a.at & kSharedRest) ? max(parts(b.parts), 1) : 0, n = nc + nb + na;
   const float c2 = P->c2;
   float M = kNegInf, L = 0.f;
   f32x4_t o[4];
@@ -137,20 +80,22 @@ __global__ __launch_bounds__(256) void paged_shared_join_kernel(const PagedShare
       for (int g = 0; g < 4; ++g) x[k][g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       int j = j0 + k;
       if (j >= n) continue;
-      const bool second = j >= nb;  // the shared rows' parts first
-      if (second) j -= nb;
-      const SharedRec r = second ? a : b;
+      // the shared rows' chunks, their rest, the token's own rows
+      const int which = j < nc ? 0 : j < nc + nb ? 1 : 2;
+      const SharedRec& r = which == 1 ? b : a;
+      j -= which == 0 ? 0 : which == 1 ? nc : nc + nb;
       const float *src, *src_ml;
       int step;
-      if (r.parts == 0) {
-        const int64_t row = ((int64_t)!second * P->T + tok) * P->H + h;
+      if (which != 0 && r.parts == 0) {
+        const int64_t row = ((int64_t)(which == 1) * P->T + tok) * P->H + h;
         src = S->whole + row * D + 32 * d + 4 * hl;
         src_ml = S->whole_ml + 2 * row;
         step = 8;
       } else {
-        const int run = min((r.at & 0xffff) + j, P->waves - 1), at = (r.at >> 16) & 0x7f;
+        const int at = which == 0 ? a.at0 & 0x7f : (r.at >> 16) & 0x7f;
+        const int run = which == 0 ? a.run0 + j * a.stride : (r.at & 0xffff) + j;
         const int wv = ((at >> 5) * hw + hin) & 3;
-        const int64_t slot = (2 * (int64_t)run + (j == 0 ? 1 : 0)) * 4 + wv;
+        const int64_t slot = (2 * (int64_t)min(max(run, 0), P->waves - 1) + (which == 0 || j == 0 ? 1 : 0)) * 4 + wv;
         src = P->part + slot * 32 * D + d * 1024 + 4 * ((at & 31) + 32 * hl);
         src_ml = P->ml + 2 * (slot * 32 + (at & 31));
         step = 256;
@@ -249,9 +194,12 @@ hipError_t launch_paged_shared(const PagedSharedParams& S, int rpl, hipStream_t 
 #undef FNA2_SHARED_HW
 #undef FNA2_SHARED_OF
   if (!k) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(paged_shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, S);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  hipError_t e = hipSuccess;
+  if (!S.small) {
+    hipLaunchKernelGGL(paged_shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, S);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   hipLaunchKernelGGL(k, dim3((uint32_t)P.waves), dim3(256), 0, s, S);
   e = hipGetLastError();
   if (e != hipSuccess) return e;

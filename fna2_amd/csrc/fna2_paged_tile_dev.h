@@ -42,6 +42,7 @@ __device__ __forceinline__ void tile_body() {
   constexpr int BN = C::BN;
   __shared__ __attribute__((aligned(1024))) uint8_t stage0[C::STAGE];
   __shared__ __attribute__((aligned(1024))) uint8_t stage1[C::STAGE];
+  __shared__ typename std::conditional<SHARED, SharedSmallPlan, int>::type small;  // (SHARED) the plan
   __shared__ volatile int odd_flag;  // a V tile holds infinities or NaN (see fna2_paged_dev.h)
   const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
   const int l32 = lane & 31, hl = lane >> 5;
@@ -50,30 +51,62 @@ __device__ __forceinline__ void tile_body() {
   const int TB = 128 / hw;
   const int hblk = cdiv(P->group, hw);  // blocks of heads of a KV head
 
-  const int run = run_of(blockIdx.x, gridDim.x);
+  int run = run_of(blockIdx.x, gridDim.x);
+  bool full = false;  // (SHARED) a chunk of a tile of shared rows, the run's all
   int64_t left, per;  // units of this run still to do, and of a run
   int b, hb, qt, s0;
   PagedSeq e;
   SharedSeq v{};  // (SHARED) the rest of the sequence's record
+  SharedPlanRef plan{};
   auto cut = [&](int seq, int head, int tile, int parts) {
     if (threadIdx.x == 0) P->cuts[run] = PagedCut{seq, head, tile, parts};
   };
   if constexpr (SHARED) {
     SArg S = sargs();
-    const int64_t total = S->V > 0 ? uni64(S->ends[S->V - 1]) : 0;
-    per = run_units(P, total, P->min_steps);
-    const int64_t u = (int64_t)run * per;
-    left = min(total - u, per);
-    if (left <= 0) return;
-    int64_t rem;
-    b = shared_seek(S, lane, u, rem);
-    v = shared_seq_uniform(S, b);
-    e = v.s;
-    const int64_t hu = TilePlan::head_units(P, e);
-    hb = uni((int)div64(rem, hu));
-    int64_t r = rem - hb * hu;
-    qt = uni(TilePlan::find(P, e, r));
-    s0 = uni((int)r);
+    plan = SharedPlanRef{S->meta, S->groups, S->group_ends, S->seqs, S->ends};
+    if (S->small) {
+      plan = SharedPlanRef{&small.meta, small.groups, small.group_ends, small.seqs, small.ends};
+      if (wv == 0) shared_plan_small(S, small, lane);
+      __syncthreads();
+    }
+    per = uni64(plan.meta->per);
+    const int nfull = (int)uni64(plan.meta->full);
+    const int64_t units = uni64(plan.meta->units);
+    // Every XCD has its share of the full runs, first, and of the others.
+    const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
+    const int lo = nfull * x / 8, mine = nfull * (x + 1) / 8 - lo;
+    full = j < mine;
+    if (full) {
+      run = lo + j;
+      int64_t at;
+      const SharedGroup& g = plan.groups[shared_seek(plan.group_ends, S->G, lane, run, at)];
+      e = PagedSeq{uni(g.s.q0), uni(g.s.lq), uni(g.s.lk), uni(g.s.off)};
+      v.table = uni(g.table);
+      const int tiles = uni(g.tiles);
+      const int c = (int)at / (tiles * TilePlan::blocks(P)), rest = (int)at - c * (tiles * TilePlan::blocks(P));
+      b = 0;
+      hb = uni(rest / tiles);
+      qt = uni(rest - hb * tiles);
+      left = per - S->start;
+      s0 = uni((int)(c * left));
+    } else {
+      run = nfull + x * (int)(gridDim.x >> 3) - lo + (j - mine);
+      const int64_t u = (int64_t)(run - nfull) * per;
+      left = min(units - u, per);
+      if (left <= 0) return;
+      int64_t rem;
+      b = shared_seek(plan.ends, S->V, lane, u, rem);
+      v = shared_seq_uniform(plan.seqs, b);
+      e = v.s;
+      const int64_t hu = SharedUnits::head_units(S, e);
+      hb = uni((int)div64(rem, hu));
+      int64_t r = rem - hb * hu;
+      qt = uni(SharedUnits::find(S, e, r));
+      // (a run that ends in a tile's start leaves the tile to the next one)
+      s0 = uni((int)max(r - S->start, (int64_t)0));
+      left -= max(S->start - r, (int64_t)0);
+      if (left <= 0) return;
+    }
   } else {
     auto units = [&](const PagedSeq& s) { return TilePlan::units(P, s); };
     SeqWork<decltype(units)> work(P, lane, units);
@@ -373,7 +406,7 @@ __device__ __forceinline__ void tile_body() {
 
     P = kargs();
     const float l_tot = wave_pair_sum(l_i);
-    const bool whole = s0 == 0 && s1 == steps;
+    const bool whole = s0 == 0 && s1 == steps && !full;
     if (whole && (!SHARED || v.kind == kSharedAlone)) {
       if (live) {
         const float inv = 1.f / (l_tot + 1e-6f);
@@ -407,7 +440,7 @@ __device__ __forceinline__ void tile_body() {
       }
     } else if (live) {
       // As the registers lie: [slot][wave][d][4][lane] of 16 bytes.
-      const int64_t slot = (2 * (int64_t)run + (s0 == 0 ? 1 : 0)) * 4 + wv;
+      const int64_t slot = (2 * (int64_t)run + (s0 == 0 || full ? 1 : 0)) * 4 + wv;
       float* arow = P->part + slot * 32 * D + 4 * lane;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
@@ -420,17 +453,28 @@ __device__ __forceinline__ void tile_body() {
     }
 
     if constexpr (SHARED) {
+      if (full) return;
       // The run in which a tile begins says where its parts lie.
       if (s0 == 0 && wv % hw == 0 && live && hl == 0) {
         SArg S = sargs();
         const int rest = steps - s1;
-        SharedRec rec;
-        rec.at = run | (tok - qt * TB) << 16 | (v.kind == kSharedOwn ? kSharedHas : 0);
+        SharedRec rec{};
+        rec.at = run | (tok - qt * TB) << 16;
         rec.parts = rest > 0 ? 1 + (int)div64(rest + per - 1, per) : v.kind == kSharedAlone ? -1 : 0;
+        if (v.kind == kSharedOwn) {
+          const SharedGroup g = plan.groups[v.group];
+          const int t = e.q0 + tok - g.s.q0;
+          rec.at |= kSharedHas | (g.full * (per - S->start) * 32 < g.s.lk ? kSharedRest : 0);
+          rec.run0 = (int)g.run0 + hb * g.tiles + t / TB;
+          rec.stride = g.tiles * TilePlan::blocks(P);
+          rec.full = (int)g.full;
+          rec.at0 = t % TB;
+        }
         S->recs[((int64_t)(v.kind == kSharedPrefix) * (P->H_KV * hblk) + hb) * P->T + e.q0 + tok] = rec;
       }
     }
     left -= s1 - s0;
+    if constexpr (SHARED) left -= sargs()->start;  // of the next tile
     if (SHARED && left <= 0) return;
     if (left <= 0) {
       const int rest = steps - s1;
@@ -444,7 +488,7 @@ __device__ __forceinline__ void tile_body() {
         hb = 0;
         if constexpr (SHARED) {
           SArg S = sargs();
-          do v = shared_seq_uniform(S, ++b); while (v.s.lq == 0 && b + 1 < S->V);
+          do v = shared_seq_uniform(plan.seqs, ++b); while (v.s.lq == 0 && b + 1 < S->V);
           e = v.s;
         } else {
           do e = paged_seq_uniform(P, ++b); while (e.lq == 0 && b + 1 < P->N);
