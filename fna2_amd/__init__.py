@@ -7,7 +7,10 @@ constructor and forward signatures.  Around the path: ``rope.rope_varlen``
 (varlen rotary embedding, optionally with the QK RMSNorm) and
 ``decode.flash_naylis_decode`` (one-token decode against a KV cache), and
 for serving from a paged cache ``paged.flash_naylis_paged`` (chunks of new
-tokens), ``paged.paged_append`` and ``paged.paged_evict``.
+tokens), ``paged.flash_naylis_shared`` (the same for sequences that share
+their first rows), ``paged.paged_append`` and ``paged.paged_evict``, and its
+books on the GPU, ``paged.DevicePageTable``.  ``rope.rotary_embed`` rotates in other
+layouts, over part of the head, and scaled.
 ``ops`` registers the path as the custom operators ``fna2::fwd`` /
 ``fna2::bwd`` (fake and autograd registrations), which ``flash_naylis_attn``
 calls, so that ``torch.compile`` traces it.
@@ -21,6 +24,7 @@ from .flash_naylis_attn import (  # noqa: F401
     flash_naylis_attn,
 )
 from .paged import (  # noqa: F401
+    DevicePageTable,
     PagedKVCache,
     PageTable,
     flash_naylis_paged,
@@ -35,6 +39,6 @@ from .rope import rope_varlen, rotary_embed, rotary_frequencies  # noqa: F401
 from . import ops  # noqa: F401,E402  (registers the fna2::fwd / fna2::bwd custom ops)
 
 __all__ = ["BLOCK_M", "BLOCK_N", "BLOCK_R", "FlashNaylisAttnFunc", "flash_naylis_attn",
-           "flash_naylis_decode", "flash_naylis_paged", "flash_naylis_shared", "PagedKVCache",
+           "flash_naylis_decode", "flash_naylis_paged", "flash_naylis_shared", "DevicePageTable", "PagedKVCache",
            "PageTable", "paged_append", "paged_evict", "paged_extend", "paged_groups", "paged_trim",
            "rope_varlen", "rotary_embed", "rotary_frequencies"]

@@ -18,7 +18,10 @@ The module keeps the reference's constructor and ``forward`` signatures
   place: no per-step copy of the cache);
 * with a ``PagedKVCache`` as ``past_kv`` a call serves the new tokens of many
   sequences, prompts in pieces and single tokens together, on the paged kernels
-  (``paged_append``, ``flash_naylis_paged``), always with the graph bias;
+  (``paged_append``, ``flash_naylis_paged``, or ``flash_naylis_shared`` where a
+  ``DevicePageTable``'s sequences share pages), always with the graph bias;
+* ``rotate_by`` has a layer rotate part of the head, neighbouring pairs, or with frequencies
+  scaled for long contexts (``rotary_embed``);
 * the other paths the reference sends elsewhere keep going elsewhere:
   ``soft_cap`` and modules built with ``use_fna2=False`` use PyTorch's SDPA
   with a materialised bias, or the explicit softmax when a ``soft_cap`` or
@@ -49,8 +52,9 @@ from .flash_naylis_attn import BLOCK_R, flash_naylis_attn, rank_supported
 from .flash_naylis_attn import FlashNaylisAttnFunc as _FNA2Func
 from .flash_naylis_attn import _plain_eager as _fna2_plain_eager
 from .decode import decode_supported, flash_naylis_decode
-from .paged import PagedKVCache, PageTable, flash_naylis_paged, paged_append  # noqa: F401
-from .rope import rope_varlen
+from .paged import (DevicePageTable, PagedKVCache, PageTable, flash_naylis_paged,  # noqa: F401
+                    flash_naylis_shared, paged_append)
+from .rope import rope_varlen, rotary_embed, rotary_frequencies
 
 
 def _detect_fna2() -> bool:
@@ -155,12 +159,27 @@ class RMSNorm(nn.Module):
 
 class RotaryPositionalEmbedding(nn.Module):
     """Rotary embedding on the last dimension (two halves rotated), with the
-    optional YaRN frequency stretch of attention_fna2.py:129-142."""
+    optional YaRN frequency stretch of attention_fna2.py:129-142.
+
+    Beyond the reference's, ``extended``: the first ``rotary_dim`` features only, neighbouring
+    ones paired (``interleaved``), or frequencies scaled for contexts ``factor`` times
+    ``original_max_len`` (``scaling``: see ``rotary_frequencies``).  These go through
+    ``rotary_embed`` on the GPU, in fp32 with one rounding."""
 
     def __init__(self, dim: int, max_seq_len: int = 2048, base: int = 10000,
                  use_yarn: bool = False, yarn_scale: float = 1.0,
-                 yarn_original_max_len: int = 1024):
+                 yarn_original_max_len: int = 1024, rotary_dim: Optional[int] = None,
+                 interleaved: bool = False, scaling: Optional[str] = None, factor: float = 1.0,
+                 original_max_len: int = 2048):
         super().__init__()
+        if rotary_dim is not None and not (0 < rotary_dim <= dim and rotary_dim % 2 == 0):
+            raise ValueError("rotary_dim must be even, positive and at most dim")
+        self.extended = ((rotary_dim is not None and rotary_dim != dim) or bool(interleaved)
+                         or scaling is not None)
+        if use_yarn and self.extended:
+            raise ValueError("use_yarn is of the whole head in halves: scaling='yarn' goes with "
+                             "rotary_dim and interleaved")
+        self.interleaved, self.factor = bool(interleaved), 1.0
         self.dim = dim
         self.max_seq_len = max_seq_len
         self.base = base
@@ -175,6 +194,9 @@ class RotaryPositionalEmbedding(nn.Module):
             start = max(dim // 2, int(dim * 0.25))
             ramp = 1 + (yarn_scale - 1) * (half - start) / (dim - start)
             inv_freq = inv_freq / torch.where(half < start, torch.ones_like(half), ramp)
+        if self.extended:
+            inv_freq, self.factor = rotary_frequencies(
+                dim if rotary_dim is None else rotary_dim, base, scaling, factor, original_max_len)
         self.register_buffer("inv_freq", inv_freq)
         self._cache_key = None
         self._cos = self._sin = None
@@ -207,8 +229,25 @@ class RotaryPositionalEmbedding(nn.Module):
     def rotate(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
         return x * cos + self._rotate_half(x) * sin
 
+    def _turn(self, x: torch.Tensor, position_offset: int) -> torch.Tensor:
+        """``rotary_embed``'s rotation of x [.., S, D] by the formula (``extended``)."""
+        pos = torch.arange(position_offset, position_offset + x.shape[-2], device=x.device)
+        ang = torch.outer(pos.double(), self.inv_freq.double().to(x.device))
+        cos, sin = (ang.cos() * self.factor).float(), (ang.sin() * self.factor).float()
+        rd = 2 * self.inv_freq.numel()
+        y, rest = x.float()[..., :rd], x[..., rd:]
+        if self.interleaved:
+            u, v = y[..., 0::2], y[..., 1::2]
+            y = torch.stack((u * cos - v * sin, v * cos + u * sin), -1).flatten(-2)
+        else:
+            u, v = y.chunk(2, -1)
+            y = torch.cat((u * cos - v * sin, v * cos + u * sin), -1)
+        return torch.cat((y.to(x.dtype), rest), -1)
+
     def forward(self, q: torch.Tensor, k: torch.Tensor,
                 position_offset: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+        if self.extended:
+            return self._turn(q, position_offset), self._turn(k, position_offset)
         s = q.shape[2]
         cos, sin = self._table(s + position_offset, q.device, q.dtype)
         cos = cos[position_offset:position_offset + s][None, None]
@@ -223,6 +262,9 @@ class RotaryPositionalEmbedding(nn.Module):
         (the HIP rotary kernel; GPU tensors only).  With norm weights the
         rows are RMS-normalised first, in the same launch.  grad_slab: where
         the backward writes dq, dk (GradSlab blocks 0 and 1)."""
+        if self.extended:
+            return rotary_embed(q, k, self.inv_freq, None, cu_seqlens, self.interleaved,
+                                self.factor, norm_q, norm_k, eps, grad_slab)
         return rope_varlen(q, k, cu_seqlens, self.inv_freq, norm_q, norm_k, eps, grad_slab)
 
 
@@ -505,6 +547,21 @@ class NaylisAttention(nn.Module):
         with torch.no_grad():
             self._pack_projection_weights()
 
+    def rotate_by(self, rotary_dim: Optional[int] = None, interleaved: bool = False,
+                  scaling: Optional[str] = None, factor: float = 1.0,
+                  original_max_len: int = 2048) -> "NaylisAttention":
+        """Another rotary embedding for this layer (in place; returns the layer): of the first
+        ``rotary_dim`` features, of neighbouring pairs, scaled for long contexts (see
+        ``RotaryPositionalEmbedding``, ``rotary_frequencies``)."""
+        if self.rope is None:
+            raise ValueError("rotate_by: this layer has no rotary embedding (use_rope=False)")
+        old = self.rope
+        self.rope = RotaryPositionalEmbedding(
+            self.head_dim, old.max_seq_len, old.base, rotary_dim=rotary_dim, interleaved=interleaved,
+            scaling=scaling, factor=factor, original_max_len=original_max_len
+        ).to(old.inv_freq.device)
+        return self
+
     # ── helpers ────────────────────────────────────────────────────────────
     def _attn_scale(self) -> float:
         if self.rope is not None and self.rope.use_yarn and self.rope.yarn_scale > 1.0:
@@ -763,7 +820,14 @@ class NaylisAttention(nn.Module):
         wq = wk = inv = None
         eps = 1e-6
         called = not self._plain_norm_rope()  # replaced or hooked modules: called as such
-        if self.use_qk_norm and q.dtype == cache.k.dtype and not called:
+        extended = _plain(self.rope, RotaryPositionalEmbedding) and self.rope is not None and \
+            self.rope.extended
+        if extended and not called:
+            # (the norm and the rotation in a launch of their own, ahead of the append's)
+            assert not self.use_qk_norm or self.q_norm.eps == self.k_norm.eps
+            norm = (self.q_norm, self.k_norm) if self.use_qk_norm else (None, None)
+            q, k = self._rotate_extended(q, k, t, cu_seqlens_q, *norm)
+        elif self.use_qk_norm and q.dtype == cache.k.dtype and not called:
             # with the rotation in the append's launch: in fp32, rounded once
             assert self.q_norm.eps == self.k_norm.eps
             wq, wk, eps = self.q_norm.weight, self.k_norm.weight, self.q_norm.eps
@@ -778,6 +842,8 @@ class NaylisAttention(nn.Module):
                 q, k = self.q_norm(q), self.k_norm(k)
             if not _plain(self.rope, RotaryPositionalEmbedding):
                 q, k = self._rotate_called(q, k, t, cu_seqlens_q)
+            elif extended:
+                q, k = self._rotate_extended(q, k, t, cu_seqlens_q)
             elif self.rope is not None:
                 cos, sin = self.rope._at(t.token_positions(x2.shape[0], cu), torch.float64
                                          if self.use_qk_norm and not called else q.dtype)
@@ -786,11 +852,25 @@ class NaylisAttention(nn.Module):
         q, k, v = (y.to(cache.k.dtype) for y in (q, k, v))
         q = paged_append(q, k, v, cache.k, cache.v, t.block_table, t.seqlens, cu, r_k, cache.r_k,
                          inv, None, wq, wk, eps, t.position_shift if inv is not None else None)
-        out = flash_naylis_paged(q, cache.k, cache.v, t.block_table, t.seqlens, cu, max_q, r_q,
-                                 cache.r_k, self.graph_scale, softmax_scale=self._attn_scale(),
-                                 key_weights=cache.key_weights)
+        bias = (r_q, cache.r_k, self.graph_scale)
+        if isinstance(t, DevicePageTable) and t.cu_groups is not None:
+            out = flash_naylis_shared(q, cache.k, cache.v, t.block_table, t.seqlens, cu, max_q,
+                                      t.cu_groups, t.shared_rows, *bias,
+                                      softmax_scale=self._attn_scale(), key_weights=cache.key_weights)
+        else:
+            out = flash_naylis_paged(q, cache.k, cache.v, t.block_table, t.seqlens, cu, max_q, *bias,
+                                     softmax_scale=self._attn_scale(), key_weights=cache.key_weights)
         y = self._finish(out.view(x2.shape[0], self.embed_dim), orig_dtype)
         return y.view(*lead, self.embed_dim), (cache if use_kv_cache else None)
+
+    def _rotate_extended(self, q, k, table, cu_seqlens_q, q_norm=None, k_norm=None):
+        """q [T, H, D], k [T, H_KV, D] of a step, normalised if modules are given and rotated
+        by ``rotary_embed``."""
+        pos = table.positions if cu_seqlens_q is None and isinstance(table, DevicePageTable) else \
+            table.token_positions(q.shape[0], cu_seqlens_q).to(torch.int32)
+        rope, weight = self.rope, lambda n: None if n is None else n.weight
+        return rotary_embed(q, k, rope.inv_freq, pos, None, rope.interleaved, rope.factor,
+                            weight(q_norm), weight(k_norm), 1e-6 if q_norm is None else q_norm.eps)
 
     def _rotate_called(self, q, k, table: PageTable, cu_seqlens_q):
         """q [T, H, D], k [T, H_KV, D] through a rope module that is not this
@@ -799,6 +879,9 @@ class NaylisAttention(nn.Module):
         if q.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a replaced or hooked rope takes positions from the host: its "
                                "paged steps cannot be captured into a graph")
+        if not isinstance(table, PageTable):
+            raise RuntimeError("a replaced or hooked rope takes positions from the host, which a "
+                               "DevicePageTable does not know: it needs a PageTable")
         cu = table._cu if cu_seqlens_q is None else cu_seqlens_q.tolist()
         qs, ks = [q[:cu[0]]], [k[:cu[0]]]
         for s, e, after in zip(cu, cu[1:], table.next_position):
@@ -828,7 +911,8 @@ class NaylisAttention(nn.Module):
         if (torch.is_grad_enabled() or not _fna2_plain_eager(q) or
                 torch.is_autocast_enabled(q.device.type) or
                 type(cache) is not StaticKVCache or n >= cache.capacity or
-                (cache.r_k is None) != (r_k is None) or not self._plain_norm_rope()):
+                (cache.r_k is None) != (r_k is None) or not self._plain_norm_rope() or
+                (self.rope is not None and self.rope.extended)):
             return None
         qn, kn, rope = self.q_norm, self.k_norm, self.rope
         wq, wk = None if qn is None else qn.weight, None if kn is None else kn.weight

@@ -28,12 +28,14 @@ calls added up.
 
 The reference's multi-token step against a cache runs PyTorch SDPA without
 the bias, or fails with it (FNA2/attention_fna2.py:412-429, :445-473).  All
-lengths and tables stay on the device: none of the three functions
+lengths and tables stay on the device: none of the functions
 synchronises (given device tensors), and each can be captured into a graph.  How
 they run (parts, buffers) goes by the table's width, not by the lengths, which the
 host does not know: a table not much wider than its sequences' pages serves them
 best.  ``PageTable`` keeps its books on the host, and each of its methods waits for
-the stream while it uploads them.  Forward only (no autograd).  There is no
+the stream while it uploads them; ``DevicePageTable`` keeps them on the device
+(``paged_extend``, ``paged_trim``, ``paged_groups``).  Where sequences share their first
+pages, ``flash_naylis_shared`` attends to those once for all.  Forward only (no autograd).  There is no
 fallback: without the HIP library, or off the GPU, the calls raise.
 """
 from __future__ import annotations
@@ -629,6 +631,16 @@ def paged_groups(block_table: torch.Tensor, page_size: int) -> Tuple[torch.Tenso
     return cu, rows
 
 
+def _token_positions(table, tokens: int, cu_seqlens_q: Optional[torch.Tensor]) -> torch.Tensor:
+    row = torch.arange(tokens, device=table.seqlens.device)
+    N = table.seqlens.shape[0]
+    if not N:
+        return row
+    cu = table.cu_seqlens_q if cu_seqlens_q is None else _ints(cu_seqlens_q, row.device)
+    b = torch.searchsorted(cu[1:], row.to(cu.dtype), right=True).clamp(max=N - 1)
+    return row - cu[b + 1] + table.seqlens[b] + table.position_shift[b]
+
+
 class PageTable:
     """Which pages hold the rows of which sequence: one for all the layers of
     a model, whose pools (``PagedKVCache``) all have its pages.
@@ -682,12 +694,7 @@ class PageTable:
         """[tokens] positions of a step's packed tokens, formed on the device from
         what this table keeps there, so that a captured step forms its own anew.
         (Tokens of no sequence: any number.)"""
-        row = torch.arange(tokens, device=self.seqlens.device)
-        if not self.rows:
-            return row
-        cu = self.cu_seqlens_q if cu_seqlens_q is None else _ints(cu_seqlens_q, row.device)
-        b = torch.searchsorted(cu[1:], row.to(cu.dtype), right=True).clamp(max=len(self.rows) - 1)
-        return row - cu[b + 1] + self.seqlens[b] + self.position_shift[b]
+        return _token_positions(self, tokens, cu_seqlens_q)
 
     def _upload(self, table: bool) -> None:
         shift = [p - r for r, p in zip(self.rows, self.next_position)]
@@ -749,8 +756,145 @@ class PageTable:
         self._upload(True)
 
 
+class DevicePageTable:
+    """A ``PageTable`` whose books lie on the device, for lengths that the host does not
+    know (drafted tokens accepted, sequences ended by their own tokens) and steps
+    captured whole into a graph: but for ``check`` nothing is read back, and nothing
+    waits for the stream but the upload of numbers that are given as such (counts in a
+    list, the places of ``release`` and ``share``).  Sequences may share their first pages.
+
+    ``extend`` takes in a step's tokens (``paged_extend``) and leaves ``cu_seqlens_q``,
+    ``slots``, ``sequences`` and ``positions`` of them, and ``status``, 0 where the pages
+    sufficed; with another status the step has no tokens (``check`` raises it, and waits
+    for it).  What ``PageTable`` keeps, ``block_table``, ``seqlens``, ``position_shift``,
+    ``cu_seqlens_q`` (written in place), ``total_q`` and ``max_seqlen_q`` (the host's bounds of the
+    step), is here too: a ``PagedKVCache`` takes either.
+
+    ``share`` lets a sequence begin with another's pages; ``cu_groups`` and
+    ``shared_rows`` then say which neighbouring sequences share how many rows, and a
+    layer attends to those once (``flash_naylis_shared``).  Rows of shared pages stay as
+    they are: no eviction while they are shared."""
+
+    def __init__(self, sequences: int, num_pages: int, page_size: int = 64,
+                 max_pages: Optional[int] = None, device="cuda"):
+        assert page_size > 0 and page_size % 16 == 0, "page_size must be a multiple of 16"
+        assert sequences >= 0 and num_pages >= 0
+        self.page_size, self.num_pages = int(page_size), int(num_pages)
+        self.width = int(num_pages if max_pages is None else max_pages)
+        zeros = lambda n: torch.zeros(n, dtype=torch.int32, device=device)
+        self.block_table = torch.full((sequences, self.width), -1, dtype=torch.int32, device=device)
+        self.seqlens, self.position_shift = zeros(sequences), zeros(sequences)
+        self.borrowed = zeros(sequences)  # first pages of a sequence that are another's
+        self.cu_seqlens_q = zeros(sequences + 1)
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+        self.status = zeros(1)
+        self.slots = self.sequences = self.positions = None
+        self.cu_groups = self.shared_rows = None
+        self.max_seqlen_q = self.total_q = 0
+        self._lent = {}  # lender -> its borrowers
+
+    def extend(self, counts, total_q: Optional[int] = None, max_seqlen_q: Optional[int] = None
+               ) -> PagedStep:
+        """counts[b] new tokens for sequence b: numbers, or a tensor on the device together with
+        ``total_q``, the tokens that the step has room for (and ``max_seqlen_q``, a hint of the
+        longest chunk)."""
+        if not torch.is_tensor(counts):
+            counts = [int(c) for c in counts]
+            total_q = sum(counts) if total_q is None else total_q
+            max_seqlen_q = max(counts, default=0) if max_seqlen_q is None else max_seqlen_q
+            counts = torch.tensor(counts, dtype=torch.int32, device=self.seqlens.device)
+        assert total_q is not None, "extend: counts on the device need total_q"
+        step = paged_extend(self.block_table, self.seqlens, counts, self.free_pages,
+                            self.free_count, self.page_size, total_q, self.position_shift)
+        torch._foreach_copy_([self.seqlens, self.free_count, self.cu_seqlens_q, self.status],
+                             [step.seqlens, step.free_count, step.cu_seqlens_q, step.status])
+        self.slots, self.sequences, self.positions = step.slots, step.sequences, step.positions
+        self.total_q = int(total_q)
+        self.max_seqlen_q = self.total_q if max_seqlen_q is None else int(max_seqlen_q)
+        return step
+
+    def check(self) -> None:
+        """Raises ValueError where the last ``extend`` did not take its tokens in (waits)."""
+        s = int(self.status)
+        if s:
+            raise ValueError("DevicePageTable full: " + (
+                f"{s} pages are missing" if s > 0 else "a sequence outgrows its table" if s == -1
+                else f"more than {self.total_q} tokens"))
+
+    def token_positions(self, tokens: int, cu_seqlens_q: Optional[torch.Tensor] = None
+                        ) -> torch.Tensor:
+        """As ``PageTable.token_positions``."""
+        return _token_positions(self, tokens, cu_seqlens_q)
+
+    def _trim(self, keep: torch.Tensor) -> None:
+        lens, count = paged_trim(self.block_table, self.seqlens, keep, self.free_pages,
+                                 self.free_count, self.page_size, self.borrowed)
+        self.seqlens.copy_(lens)
+        self.free_count.copy_(count)
+        torch.minimum(self.borrowed, (lens + self.page_size - 1) // self.page_size,
+                      out=self.borrowed)
+
+    def rollback(self, keep: torch.Tensor) -> None:
+        """The rows from ``keep[b]`` on (int32, on the device) were never there: drafted tokens
+        that were refused.  Their positions come again."""
+        self._trim(keep)
+
+    def truncate(self, budget: int) -> None:
+        """As ``PageTable.truncate``, after every layer's ``evict(budget)``."""
+        before = self.seqlens.clone()
+        self._trim(torch.full_like(self.seqlens, int(budget)))
+        self.position_shift += before - self.seqlens
+
+    def release(self, *done: int) -> None:
+        """Sequences that are done: their pages are free, and their places for others.  One
+        whose pages others have borrowed goes after them."""
+        for b in done:
+            left = self._lent.get(b, set()) - set(done)
+            if left:
+                raise ValueError(f"release: sequence {b}'s pages are shared by {sorted(left)}")
+        at = torch.tensor(done, dtype=torch.long, device=self.seqlens.device)
+        self._trim(torch.full_like(self.seqlens, 1 << 30).index_fill_(0, at, 0))
+        self.position_shift.index_fill_(0, at, 0)
+        for b in done:
+            self._lent.pop(b, None)
+            for borrowers in self._lent.values():
+                borrowers.discard(b)
+        self._regroup()
+
+    def share(self, lender: int, borrowers: Sequence[int], rows: int) -> int:
+        """Each of ``borrowers`` (places without rows) begins with the first ``rows`` rows of
+        sequence ``lender``, cut to whole pages; returns how many those are.  The lender keeps
+        its rows until its borrowers are released.  Sequences that share are attended to together
+        where their places are neighbours."""
+        borrowers = [int(b) for b in borrowers]
+        assert lender not in borrowers and len(set(borrowers)) == len(borrowers), \
+            "share: the lender and its borrowers are different sequences"
+        p = int(rows) // self.page_size
+        assert 0 <= p <= self.width, "share: more rows than a table has room for"
+        if not borrowers or not p:
+            return 0
+        at = torch.tensor(borrowers, dtype=torch.long, device=self.seqlens.device)
+        self.block_table[at, :p] = self.block_table[lender, :p].clone()
+        self.seqlens.index_fill_(0, at, p * self.page_size)
+        self.borrowed.index_fill_(0, at, p)
+        self.position_shift[at] = self.position_shift[lender].clone()
+        self._lent.setdefault(int(lender), set()).update(borrowers)
+        if self.cu_groups is None:
+            self.cu_groups = torch.zeros_like(self.cu_seqlens_q)
+            self.shared_rows = torch.zeros_like(self.seqlens)
+        self._regroup()
+        return p * self.page_size
+
+    def _regroup(self) -> None:
+        if self.cu_groups is not None:
+            cu, rows = paged_groups(self.block_table, self.page_size)
+            self.cu_groups.copy_(cu)
+            self.shared_rows.copy_(rows)
+
+
 class PagedKVCache:
-    """One layer's pools on the pages of a ``PageTable``: a ``past_kv`` of
+    """One layer's pools on the pages of a ``PageTable`` or ``DevicePageTable``: a ``past_kv`` of
     ``NaylisAttention`` that serves many sequences of differing lengths, prompts
     in pieces and single tokens in one call.
 
@@ -773,7 +917,7 @@ class PagedKVCache:
               rank: int = 0, dtype=torch.bfloat16, weigh: bool = False) -> "PagedKVCache":
         dev, ps = table.block_table.device, table.page_size
         mk = lambda h, f, dt: torch.zeros(table.num_pages, h, ps, f, dtype=dt, device=dev)
-        w = torch.zeros(len(table.rows), n_kv_heads, table.width * ps, device=dev) if weigh else None
+        w = torch.zeros(table.block_table.shape[0], n_kv_heads, table.width * ps, device=dev) if weigh else None
         return cls(table, mk(n_kv_heads, head_dim, dtype), mk(n_kv_heads, head_dim, dtype),
                    mk(graph_heads, rank, torch.bfloat16) if graph_heads > 0 else None, w)
 
