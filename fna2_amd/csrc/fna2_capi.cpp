@@ -1614,7 +1614,10 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
 // equal in key steps and 8 for each tile that they begin, which takes as long as those: its
 // page ids, first rows, queries, and the part that it leaves (us, 0, 4, 8, 12: the 16 x 128
 // 852, 420, 378, 380; 16 x 64, rank 32 561, 227, 190, 188; 64 tokens, as above 117, 118, 116, 114;
-// 4 over 2000 18.2 with 8, 19.8 with 4).
+// 4 over 2000 18.2 with 8, 19.8 with 4).  Rows are not shared where reading
+// them once saves fewer than 64 bytes for a token, head and feature's second part (us, never
+// shared, always, here: 3 groups of 16 x 25 tokens over 64 rows 29.8, 38.3, 29.8; 3 of 18 x 6 over 64
+// 29.8, 34.7, 30.0; 10 x 100 over 1024 39.0, 44.3, 38.9; 5 of 25 x 9 over 960 68.9, 43.9, 44.1).
 struct SharedPlan {
   int hw, waves, min_steps;
   size_t ml, meta, groups, group_ends, seqs, ends, recs, whole, whole_ml, bytes;
@@ -1789,6 +1792,7 @@ int fna2_paged_shared(const fna2_paged_shared_args* a, void* stream_ptr) {
   S.p.part = (float*)ws;
   S.p.ml = (float*)(ws + k.ml);
   S.start = 8;  // (see shared_plan)
+  S.worth = 32.f;
   S.small = a->groups <= fna2::kSharedSmall && a->attn.c.batch <= fna2::kSharedSmall;
   S.G = a->groups;
   S.V = a->groups + a->attn.c.batch;

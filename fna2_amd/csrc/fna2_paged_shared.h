@@ -67,6 +67,7 @@ struct SharedSmallPlan {
 struct PagedSharedParams {
   PagedParams p;
   int start;  // what starting and ending a tile costs, in steps
+  float worth;
   int G, V;  // groups; virtual sequences: the rests of the groups' rows, then the N sequences'
   const int* cu_groups;
   const int* shared_rows;
@@ -151,6 +152,16 @@ __device__ __forceinline__ int64_t shared_per(SArg S, int64_t A, int64_t B) {
   return max((int64_t)ceilf(x), (int64_t)(S->p.min_steps + S->start));
 }
 
+// How many of `rows` rows, that n sequences with tokens in all share, are worth it.  Sharing saves
+// reading their K, V and R_k n - 1 times and costs every token and head a second part, written
+// and read in fp32, which is worth it from `worth` elements for each of it on.
+__device__ __forceinline__ int shared_worth(SArg S, int rows, int n, int tokens) {
+  KArg P = &S->p;
+  rows = n > 1 && rows > 0 ? rows & ~31 : 0;
+  const float saved = (float)(n - 1) * (float)rows * (float)(2 * P->H_KV * P->D + P->H_G * P->R);
+  return saved >= S->worth * (float)tokens * (float)(P->H * P->D) ? rows : 0;
+}
+
 // Sum of x over the threads before this one, and over all (total), in one workgroup.
 template <int NT>
 __device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t* sums, int64_t& total) {
@@ -201,13 +212,15 @@ __device__ __forceinline__ void shared_plan(SArg S, const SharedPlanRef R, int64
       first = min(first, __shfl_xor(first, k));
       n += __shfl_xor(n, k);
     }
-    int rows = min(least, uni(S->shared_rows[g]));
-    rows = n > 1 && rows > 0 ? rows & ~31 : 0;
     SharedGroup x{};
-    if (rows > 0) {
+    int rows = 0;
+    if (n > 1) {
       x.s.q0 = seqs[G + c0].s.q0;
       const PagedSeq last = seqs[G + c1 - 1].s;
       x.s.lq = max(last.q0 + last.lq - x.s.q0, 0);
+      rows = shared_worth(S, min(least, uni(S->shared_rows[g])), n, x.s.lq);
+    }
+    if (rows > 0) {
       x.s.lk = x.s.off = rows;
       x.table = first;
       x.tiles = cdiv(x.s.lq, TilePlan::tokens(P));
@@ -222,6 +235,7 @@ __device__ __forceinline__ void shared_plan(SArg S, const SharedPlanRef R, int64
         seqs[G + b] = y;
       }
     }
+    if (rows <= 0) x = SharedGroup{};
     if (lane == 0) groups[g] = x;
   }
   __threadfence_block();
@@ -329,11 +343,12 @@ __device__ __forceinline__ void shared_plan_small(SArg S, SharedSmallPlan& R, in
     todo &= todo - 1;
     const uint64_t m = (uint64_t)lane64((int64_t)members, g);
     const bool in = (m >> lane) & 1;
-    const int n = min(wave_min(in ? s.off : 0x7fffffff), __builtin_amdgcn_readlane(said, g)) & ~31;
-    if (n <= 0) continue;
     const int b0 = __builtin_amdgcn_readlane(c0, g), b1 = __builtin_amdgcn_readlane(c1, g) - 1;
     const int t0 = __builtin_amdgcn_readlane(s.q0, b0);
     const int t1 = __builtin_amdgcn_readlane(s.q0, b1) + __builtin_amdgcn_readlane(s.lq, b1);
+    const int least = min(wave_min(in ? s.off : 0x7fffffff), __builtin_amdgcn_readlane(said, g));
+    const int n = shared_worth(S, least, __builtin_popcountll(m), max(t1 - t0, 0));
+    if (n <= 0) continue;
     if (lane == g) rows = n, q0 = t0, lq = max(t1 - t0, 0), first = __builtin_ctzll(m);
     if (in) row0 = n, group = g;
   }
@@ -370,6 +385,110 @@ __device__ __forceinline__ void shared_plan_small(SArg S, SharedSmallPlan& R, in
     R.ends[G + lane] = rests + own_end;
   }
   if (lane == 0) R.meta = SharedMeta{per, runs, rests + own};
+}
+
+// Sums of K values over the threads up to and including this one, and over all, of NW waves.
+template <int K>
+__device__ __forceinline__ void plan_scans(int64_t (&x)[K], int64_t (&total)[K], int64_t (*sums)[16], int nw) {
+  const int lane = threadIdx.x & 63, wv = uni(threadIdx.x >> 6);
+#pragma unroll
+  for (int k = 0; k < K; ++k) x[k] = lane_scan64(x[k]);
+  __syncthreads();  // (the last scan's sums have been read)
+  if (lane == 63) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) sums[k][wv] = x[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) total[k] = 0;
+  for (int w = 0; w < nw; ++w) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t v = sums[k][w];
+      if (w < wv) x[k] += v;
+      total[k] += v;
+    }
+  }
+}
+
+// The same by one workgroup for at most 1024 sequences and 1024 groups: thread i has sequence i
+// and group i in registers.
+constexpr int kSharedMid = 1024;
+struct SharedMidPlan {
+  int cu[kSharedMid + 1], least[kSharedMid], first[kSharedMid], n[kSharedMid], rows[kSharedMid];
+  int q0[kSharedMid], lq[kSharedMid];
+  int64_t sums[3][16];
+};
+__device__ __forceinline__ void shared_plan_mid(SArg S, const SharedPlanRef R, SharedMidPlan& L) {
+  KArg P = &S->p;
+  const int tid = threadIdx.x, nw = blockDim.x >> 6, N = P->N, G = S->G;
+  PagedSeq s{0, 0, 0, 0};
+  int c0 = N, said = 0;
+  if (tid < N) s = paged_seq(P, tid);
+  if (tid <= G) c0 = min(max(S->cu_groups[tid], 0), N);
+  if (tid < G) said = S->shared_rows[tid];
+  if (tid <= G) L.cu[tid] = c0;
+  if (tid == 0 && G >= (int)blockDim.x) L.cu[G] = min(max(S->cu_groups[G], 0), N);
+  L.least[tid] = L.first[tid] = 0x7fffffff, L.n[tid] = 0;
+  L.q0[tid] = s.q0, L.lq[tid] = s.lq;
+  __syncthreads();
+  int g = -1;
+  if (s.lq > 0 && G > 0 && L.cu[0] <= tid && tid < L.cu[G]) {
+    int lo = 0, hi = G;  // cu[lo] <= tid < cu[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (L.cu[mid] <= tid) lo = mid;
+      else hi = mid;
+    }
+    g = lo;
+    atomicMin(&L.least[g], s.off);
+    atomicMin(&L.first[g], tid);
+    atomicAdd(&L.n[g], 1);
+  }
+  __syncthreads();
+  int rows = 0, q0 = 0, lq = 0, first = 0;
+  if (tid < G && L.n[tid] > 1) {
+    const int b0 = L.cu[tid], b1 = max(L.cu[tid + 1] - 1, b0);
+    q0 = L.q0[b0];
+    lq = max(L.q0[b1] + L.lq[b1] - q0, 0);
+    first = L.first[tid];
+    rows = shared_worth(S, min(L.least[tid], said), L.n[tid], lq);
+  }
+  L.rows[tid] = rows;
+  __syncthreads();
+  const int row0 = g >= 0 ? L.rows[g] : 0;
+  if (row0 > 0) s.lk = max(s.lk - row0, 0), s.off -= row0;
+  const int64_t blocks = TilePlan::blocks(P), start = S->start;
+  const int tiles1 = rows > 0 ? cdiv(lq, TilePlan::tokens(P)) : 0, n = rows / 32;
+  const int64_t tiles = tiles1 * blocks, mine = tid < N ? SharedUnits::units(S, s) : 0;
+  int64_t sum[3], total[3], own, own_end;
+  {
+    int64_t x[3] = {mine, tiles * n, tiles * start};
+    plan_scans<3>(x, total, L.sums, nw);
+    own = total[0], own_end = x[0];
+  }
+  int64_t per = shared_per(S, own + total[2], total[1]), full, end[2];
+  while (true) {
+    full = div64(n, per - start);
+    const int64_t left = n - full * (per - start);
+    int64_t x[2] = {full * tiles, left > 0 ? (left + start) * tiles : 0}, t[2];
+    plan_scans<2>(x, t, L.sums, nw);
+    end[0] = x[0], end[1] = x[1], sum[0] = t[0], sum[1] = t[1];
+    if (sum[0] + div64(sum[1] + own + per - 1, per) <= P->waves) break;
+    per += 1 + per / 32;
+  }
+  if (tid < G) {
+    R.groups[tid] = SharedGroup{PagedSeq{q0, lq, rows, rows}, end[0] - full * tiles, end[0], first, tiles1, full};
+    R.group_ends[tid] = end[0];
+    const int at = (int)(full * (per - start) * 32), lk = rows - at;
+    R.seqs[tid] = SharedSeq{PagedSeq{q0, lk > 0 ? lq : 0, lk, lk}, at, first, kSharedPrefix, tid};
+    R.ends[tid] = end[1];
+  }
+  if (tid < N) {
+    R.seqs[G + tid] = SharedSeq{s, row0, tid, row0 > 0 ? kSharedOwn : kSharedAlone, g};
+    R.ends[G + tid] = sum[1] + own_end;
+  }
+  if (tid == 0) *R.meta = SharedMeta{per, sum[0], sum[1] + own};
 }
 
 // Kernel launches (fna2_paged_shared.hip): the plan, the tiles, the join.

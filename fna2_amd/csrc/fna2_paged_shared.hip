@@ -14,7 +14,8 @@
 // The plan forms the units, key steps of tiles of 128 (token, head) columns, of the
 // groups' shared rows with all the group's tokens and of the sequences' own rows, and cuts
 // them into equal runs: every workgroup for itself where 64 sequences and 64 groups at
-// most fit its LDS, else in a launch of its own.  The tile kernel
+// most fit its LDS, else in a launch of its own, in one workgroup's registers up to 1024 (5 groups of
+// 22 sequences: the call 48 us with the general form, 39 so).  The tile kernel
 // (fna2_paged_tile_dev.h) takes a run a workgroup.  A tile that runs cut, or
 // that is one of two for its tokens, leaves unnormalised parts; the join, another
 // launch, adds a token's parts up in a fixed order.
@@ -34,15 +35,25 @@ __global__ __launch_bounds__(kPlanThreads) void paged_shared_plan_kernel(const P
   shared_plan<kPlanThreads>(S, SharedPlanRef{S->meta, S->groups, S->group_ends, S->seqs, S->ends}, sums);
 }
 
-// The join: a workgroup takes 32 tokens, a query head and 32 features; its
-// waves every fourth group of four parts each.  Column = lane % 32, as in a
+__global__ __launch_bounds__(kSharedMid) void paged_shared_plan_mid_kernel(const PagedSharedParams) {
+  SArg S = sargs();
+  __shared__ SharedMidPlan mid;
+  shared_plan_mid(S, SharedPlanRef{S->meta, S->groups, S->group_ends, S->seqs, S->ends}, mid);
+}
+
+// The join: a workgroup takes 32 tokens, a query head and 32 features; its NW
+// waves every NW-th group of four parts each.  Column = lane % 32, as in a
 // tile, so that the parts of tokens that are neighbours in a tile are read as they lie.
-template <int D, bool F16>
-__global__ __launch_bounds__(256) void paged_shared_join_kernel(const PagedSharedParams) {
+// Four waves where there are few workgroups, so that many parts are in flight (the whole call,
+// one wave against four: 32 sequences of 5 tokens over 3001 shared rows 41.0 us, 34.5; 4 of 1
+// over 2000 23.7, 18.8), one where the workgroups alone fill the chip (10 of 100 tokens over 1024
+// rows 38.9, 42.3; 24 of 195 over 131 43.9, 48.3).
+template <int D, bool F16, int NW>
+__global__ __launch_bounds__(64 * NW) void paged_shared_join_kernel(const PagedSharedParams) {
   SArg S = sargs();
   KArg P = &S->p;
-  __shared__ f32x4_t part[4][4][64];
-  __shared__ float stat[4][2][32];
+  __shared__ f32x4_t part[NW][4][64];
+  __shared__ float stat[NW][2][32];
   const int lane = threadIdx.x & 63, own = uni(threadIdx.x >> 6);
   const int l32 = lane & 31, hl = lane >> 5;
   const int h = uni(blockIdx.y / (D / 32)), d = uni(blockIdx.y % (D / 32));
@@ -70,7 +81,7 @@ __global__ __launch_bounds__(256) void paged_shared_join_kernel(const PagedShare
 #pragma unroll
   for (int g = 0; g < 4; ++g) o[g] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   constexpr int U = 4;  // parts in flight
-  for (int j0 = U * own; __builtin_amdgcn_ballot_w64(j0 < n) != 0; j0 += 4 * U) {
+  for (int j0 = U * own; __builtin_amdgcn_ballot_w64(j0 < n) != 0; j0 += NW * U) {
     f32x4_t x[U][4];
     f32x2 ml[U];
 #pragma unroll
@@ -127,7 +138,7 @@ __global__ __launch_bounds__(256) void paged_shared_join_kernel(const PagedShare
   __syncthreads();
   if (own != 0 || !(live || loose)) return;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) {
+  for (int w = 1; w < NW; ++w) {
     const float mw = stat[w][0][l32], m = fmaxf(M, mw);
     const float ref = m == kNegInf ? 0.f : m;
     const float wa = weight2((M - ref) * c2), wb = weight2((mw - ref) * c2);
@@ -196,7 +207,11 @@ hipError_t launch_paged_shared(const PagedSharedParams& S, int rpl, hipStream_t 
   if (!k) return hipErrorInvalidValue;
   hipError_t e = hipSuccess;
   if (!S.small) {
-    hipLaunchKernelGGL(paged_shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, S);
+    const int most = std::max(P.N, S.G);
+    if (most <= kSharedMid)
+      hipLaunchKernelGGL(paged_shared_plan_mid_kernel, dim3(1), dim3((most + 63) / 64 * 64), 0, s, S);
+    else
+      hipLaunchKernelGGL(paged_shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, S);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -204,10 +219,12 @@ hipError_t launch_paged_shared(const PagedSharedParams& S, int rpl, hipStream_t 
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   const dim3 grid((uint32_t)((P.T + 31) / 32), (uint32_t)(P.H * (P.D / 32)));
-  void (*m)(const PagedSharedParams) =
-      P.D == 64 ? (P.f16 ? paged_shared_join_kernel<64, true> : paged_shared_join_kernel<64, false>)
-                : (P.f16 ? paged_shared_join_kernel<128, true> : paged_shared_join_kernel<128, false>);
-  hipLaunchKernelGGL(m, grid, dim3(256), 0, s, S);
+  const bool one = (int64_t)grid.x * grid.y >= 1024;  // (4 a CU)
+#define FNA2_JOIN(D, F16) (one ? paged_shared_join_kernel<D, F16, 1> : paged_shared_join_kernel<D, F16, 4>)
+  void (*m)(const PagedSharedParams) = P.D == 64 ? (P.f16 ? FNA2_JOIN(64, true) : FNA2_JOIN(64, false))
+                                                 : (P.f16 ? FNA2_JOIN(128, true) : FNA2_JOIN(128, false));
+#undef FNA2_JOIN
+  hipLaunchKernelGGL(m, grid, dim3(one ? 64 : 256), 0, s, S);
   return hipGetLastError();
 }
 

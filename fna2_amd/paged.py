@@ -214,7 +214,8 @@ def flash_naylis_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     ``shared_rows[g]`` rows of each lie in the same pages: their rows of
     ``block_table`` begin alike (``paged_groups`` finds such groups).  Of these
     rows, those are shared that lie before every chunk of the group, in whole steps of
-    32, if two of its sequences have tokens; ``shared_rows`` may be larger or 0.
+    32, if two of its sequences have tokens and reading the rows once saves more than the
+    tokens' second part costs; ``shared_rows`` may be larger or 0.
     """
     assert cu_groups is not None and shared_rows is not None, \
         "flash_naylis_shared: cu_groups and shared_rows expected"

@@ -423,7 +423,8 @@ int fna2_paged_attn(const fna2_paged_attn_args* args, void* hip_stream);
  * in two groups; the others share nothing); the first shared_rows[g] rows of each
  * of them lie in the same pages, which their rows of the block table all name.
  * Of these rows, those are shared that lie before every chunk of the group, in whole
- * steps of 32, where two of its sequences have tokens. */
+ * steps of 32, where two of its sequences have tokens and where sharing them saves
+ * more reading than a second part of each token's sum costs. */
 typedef struct fna2_paged_shared_args {
   fna2_paged_attn_args attn;    /* scores unused                                 */
   int32_t groups;               /* G >= 0                                       */

@@ -152,6 +152,13 @@ CASES = {
              [(2, 240, 240), (2, 144, 144)], dict(dtype=torch.float16)),
     "many_tokens": (([70, 64, 31], [390, 384, 351], 4, 1, 4, 64, 32, 64), [(3, 320, 320)], {}),
     "many_tokens_d128": (([129, 100], [390, 361], 2, 2, 2, 128, 64, 64), [(2, 256, 256)], {}),
+    # enough shared rows to be worth it for many tokens
+    "many_tokens_long": (([70, 64, 31], [1670, 1664, 1631], 4, 1, 4, 64, 32, 64),
+                         [(3, 1600, 1600)], {}),
+    "many_tokens_long_d128": (([150, 3, 100], [1500, 1353, 1450], 2, 2, 2, 128, 64, 64),
+                              [(3, 1344, 1344)], {}),
+    "many_sequences_long": (([2] * 70, [270 + i % 23 for i in range(70)], 2, 1, 2, 64, 8, 16),
+                            [(30, 256, 256), (40, 240, 250)], {}),
     "loose_tokens": (([1, 1], [150, 150], 4, 2, 4, 64, 16, 16), [(2, 128, 128)],
                      dict(head=37, tail=40)),
     "rows_of_heads": (([1, 2], [150, 150], 4, 2, 4, 64, 16, 16), [(2, 128, 128)],
@@ -174,6 +181,23 @@ def make(name, **kw):
 def test_against_the_oracle(name, causal):
     print(name, causal, flush=True)
     check_attend(make(name), causal=causal)
+
+
+LONG = [n for n, (_, groups, _) in CASES.items()
+        if len(groups) < 3 and any(pages and said for _, pages, said in groups) and "long" not in n]
+
+
+@gpu
+@pytest.mark.parametrize("name", LONG)
+def test_long_shared_rows_against_the_oracle(name):
+    """The same with 3840 shared rows more, which are worth sharing for any of
+    these tokens; whole pages and key steps, so that what lies behind stays."""
+    print(name, flush=True)
+    (lq, lk, *rest), groups, more = CASES[name]
+    shared = range(more.get("apart", 0), more.get("apart", 0) + sum(g[0] for g in groups))
+    lk = [n + 3840 * (b in shared) for b, n in enumerate(lk)]
+    groups = [(n, pages + 3840, said + 3840 * (said > 0)) for n, pages, said in groups]
+    check_attend(SharedCase(lq, lk, *rest, groups=groups, device="cuda", **more))
 
 
 @gpu
