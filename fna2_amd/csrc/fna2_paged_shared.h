@@ -181,7 +181,8 @@ __device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t* sums, int64_t& 
 }
 
 // The plan, made by one workgroup of NT threads.  A wave per group: the rows that it
-// shares.  Then all threads: the units of all tiles, what a run takes of them, the
+// shares.  Then all threads: what is left of each sequence (of one group at most, whatever
+// cu_groups holds), the units of all tiles, what a run takes of them, the
 // groups' full chunks, and the units that are left, added up.  (R: in LDS or in memory.)
 template <int NT>
 __device__ __forceinline__ void shared_plan(SArg S, const SharedPlanRef R, int64_t* sums) {
@@ -224,19 +225,29 @@ __device__ __forceinline__ void shared_plan(SArg S, const SharedPlanRef R, int64
       x.s.lk = x.s.off = rows;
       x.table = first;
       x.tiles = cdiv(x.s.lq, TilePlan::tokens(P));
-      for (int b = c0 + lane; b < c1; b += 64) {
-        SharedSeq y = seqs[G + b];
-        if (y.s.lq <= 0) continue;
-        y.s.lk = max(y.s.lk - rows, 0);
-        y.s.off -= rows;
-        y.row0 = rows;
-        y.kind = kSharedOwn;
-        y.group = g;
-        seqs[G + b] = y;
-      }
     }
     if (rows <= 0) x = SharedGroup{};
     if (lane == 0) groups[g] = x;
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (int b = tid; b < N && G > 0; b += NT) {
+    SharedSeq y = seqs[G + b];
+    if (y.s.lq <= 0 || S->cu_groups[0] > b || S->cu_groups[G] <= b) continue;
+    int lo = 0, hi = G;  // cu_groups[lo] <= b < cu_groups[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (S->cu_groups[mid] <= b) lo = mid;
+      else hi = mid;
+    }
+    const int rows = groups[lo].s.lk;
+    if (rows <= 0) continue;
+    y.s.lk = max(y.s.lk - rows, 0);
+    y.s.off -= rows;
+    y.row0 = rows;
+    y.kind = kSharedOwn;
+    y.group = lo;
+    seqs[G + b] = y;
   }
   __threadfence_block();
   __syncthreads();

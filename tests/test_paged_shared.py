@@ -167,6 +167,11 @@ CASES = {
                     [(2, 64, 64)] * 80, {}),
     "many_sequences": (([1] * 130, [70 + i % 23 for i in range(130)], 2, 1, 2, 64, 8, 16),
                        [(130, 64, 64)], {}),
+    # (more than a workgroup has threads)
+    "more_sequences": (([1] * 1100, [134 + i % 23 for i in range(1100)], 2, 1, 2, 64, 8, 16),
+                       [(3, 128, 128), (1050, 128, 112), (40, 96, 96)], dict(apart=5)),
+    "more_groups": (([1] * 1080, [70 + i % 23 for i in range(1080)], 2, 1, 2, 64, 8, 16),
+                    [(1, 0, 64)] * 1000 + [(2, 64, 64)] * 40, {}),
 }
 
 
