@@ -760,9 +760,9 @@ class PageTable:
 class DevicePageTable:
     """A ``PageTable`` whose books lie on the device, for lengths that the host does not
     know (drafted tokens accepted, sequences ended by their own tokens) and steps
-    captured whole into a graph: but for ``check`` nothing is read back, and nothing
-    waits for the stream but the upload of numbers that are given as such (counts in a
-    list, the places of ``release`` and ``share``).  Sequences may share their first pages.
+    captured whole into a graph: but for ``check`` and ``share`` nothing is read back, and nothing
+    else waits for the stream but the upload of numbers that are given as such (counts in a
+    list, the places of ``release``).  Sequences may share their first pages.
 
     ``extend`` takes in a step's tokens (``paged_extend``) and leaves ``cu_seqlens_q``,
     ``slots``, ``sequences`` and ``positions`` of them, and ``status``, 0 where the pages
@@ -773,8 +773,9 @@ class DevicePageTable:
 
     ``share`` lets a sequence begin with another's pages; ``cu_groups`` and
     ``shared_rows`` then say which neighbouring sequences share how many rows, and a
-    layer attends to those once (``flash_naylis_shared``).  Rows of shared pages stay as
-    they are: no eviction while they are shared."""
+    layer attends to those once (``flash_naylis_shared``).  While rows are shared they stay as
+    they are, the lender's and the borrowers': ``rollback`` keeps them, ``truncate`` and
+    ``PagedKVCache.evict`` raise ValueError."""
 
     def __init__(self, sequences: int, num_pages: int, page_size: int = 64,
                  max_pages: Optional[int] = None, device="cuda"):
@@ -786,6 +787,7 @@ class DevicePageTable:
         self.block_table = torch.full((sequences, self.width), -1, dtype=torch.int32, device=device)
         self.seqlens, self.position_shift = zeros(sequences), zeros(sequences)
         self.borrowed = zeros(sequences)  # first pages of a sequence that are another's
+        self.held = zeros(sequences)      # first rows of a sequence that it shares
         self.cu_seqlens_q = zeros(sequences + 1)
         self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
@@ -837,19 +839,30 @@ class DevicePageTable:
                       out=self.borrowed)
 
     def rollback(self, keep: torch.Tensor) -> None:
-        """The rows from ``keep[b]`` on (int32, on the device) were never there: drafted tokens
-        that were refused.  Their positions come again."""
-        self._trim(keep)
+        """The rows from ``keep[b]`` on (int32, on the device) were never there, but for those
+        that b shares: drafted tokens that were refused.  Their positions come again."""
+        self._trim(torch.maximum(_ints(keep, self.held.device), self.held))
 
     def truncate(self, budget: int) -> None:
         """As ``PageTable.truncate``, after every layer's ``evict(budget)``."""
+        self._unshared("truncate")
         before = self.seqlens.clone()
         self._trim(torch.full_like(self.seqlens, int(budget)))
         self.position_shift += before - self.seqlens
 
+    def _unshared(self, what: str) -> None:
+        if any(self._lent.values()):
+            raise ValueError(f"{what}: sequences share rows")
+
+    def _place(self, what: str, b: int) -> int:
+        if not 0 <= int(b) < self.seqlens.shape[0]:
+            raise ValueError(f"{what}: there is no sequence {b}")
+        return int(b)
+
     def release(self, *done: int) -> None:
         """Sequences that are done: their pages are free, and their places for others.  One
         whose pages others have borrowed goes after them."""
+        done = [self._place("release", b) for b in done]
         for b in done:
             left = self._lent.get(b, set()) - set(done)
             if left:
@@ -857,30 +870,41 @@ class DevicePageTable:
         at = torch.tensor(done, dtype=torch.long, device=self.seqlens.device)
         self._trim(torch.full_like(self.seqlens, 1 << 30).index_fill_(0, at, 0))
         self.position_shift.index_fill_(0, at, 0)
+        self.held.index_fill_(0, at, 0)
         for b in done:
             self._lent.pop(b, None)
-            for borrowers in self._lent.values():
+            for lender, borrowers in self._lent.items():
                 borrowers.discard(b)
+                if not borrowers:
+                    self.held[lender] = self.borrowed[lender] * self.page_size
+        self._lent = {lender: left for lender, left in self._lent.items() if left}
         self._regroup()
 
     def share(self, lender: int, borrowers: Sequence[int], rows: int) -> int:
         """Each of ``borrowers`` (places without rows) begins with the first ``rows`` rows of
-        sequence ``lender``, cut to whole pages; returns how many those are.  The lender keeps
-        its rows until its borrowers are released.  Sequences that share are attended to together
-        where their places are neighbours."""
-        borrowers = [int(b) for b in borrowers]
+        sequence ``lender``, cut to whole pages; returns how many those are.  ValueError (the
+        lengths are read back for it) where the lender has fewer or a borrower has some.  The
+        lender keeps its rows until its borrowers are released.  Sequences that share are attended
+        to together where their places are neighbours."""
+        lender, *borrowers = (self._place("share", b) for b in (lender, *borrowers))
         assert lender not in borrowers and len(set(borrowers)) == len(borrowers), \
             "share: the lender and its borrowers are different sequences"
         p = int(rows) // self.page_size
         assert 0 <= p <= self.width, "share: more rows than a table has room for"
         if not borrowers or not p:
             return 0
+        lens = self.seqlens.tolist()
+        if p * self.page_size > lens[lender] or any(lens[b] > 0 for b in borrowers):
+            raise ValueError(f"share: sequence {lender} has {lens[lender]} rows and its borrowers "
+                             f"{[lens[b] for b in borrowers]}, of {rows} to share")
         at = torch.tensor(borrowers, dtype=torch.long, device=self.seqlens.device)
         self.block_table[at, :p] = self.block_table[lender, :p].clone()
         self.seqlens.index_fill_(0, at, p * self.page_size)
         self.borrowed.index_fill_(0, at, p)
+        self.held.index_fill_(0, at, p * self.page_size)
+        self.held[lender] = self.held[lender].clamp(min=p * self.page_size)
         self.position_shift[at] = self.position_shift[lender].clone()
-        self._lent.setdefault(int(lender), set()).update(borrowers)
+        self._lent.setdefault(lender, set()).update(borrowers)
         if self.cu_groups is None:
             self.cu_groups = torch.zeros_like(self.cu_seqlens_q)
             self.shared_rows = torch.zeros_like(self.seqlens)
@@ -929,6 +953,8 @@ class PagedKVCache:
         every layer has done so, ``PageTable.truncate(budget)``."""
         assert self.key_weights is not None, "evict: this cache does not weigh its rows"
         t = self.table
+        if isinstance(t, DevicePageTable):
+            t._unshared("evict")
         kept, _, w = paged_evict(self.k, self.v, t.block_table, t.seqlens, self.key_weights,
                                  budget, recent, first, self.r_k, heads)
         self.key_weights.copy_(w)

@@ -66,7 +66,15 @@ def test_table_refusals():
     with pytest.raises(AssertionError):
         t.share(0, [1], 16 * 9)
     assert t.share(0, [1], 15) == 0 and t.cu_groups is None
+    for call in (lambda: t.share(0, [-3], 16), lambda: t.share(-1, [0], 16), lambda: t.release(3),
+                 lambda: t.share(0, [1], 16)):  # (which has no rows)
+        with pytest.raises(ValueError):
+            call()
     t._lent[0] = {1}
+    with pytest.raises(ValueError, match="share rows"):
+        t.truncate(8)
+    with pytest.raises(ValueError, match="share rows"):
+        PagedKVCache.empty(t, 1, 64, weigh=True).evict(8)
     with pytest.raises(ValueError, match="shared by"):
         t.release(0)
     with pytest.raises(RuntimeError, match="GPU"):
@@ -141,7 +149,9 @@ def test_shared_pages_go_back_once(gpu):
     t.extend([1, 20, 1, 1])
     assert t.positions.tolist() == [70, *range(64, 84), 0, 64] and t.free_count.item() == 11
     t.rollback(torch.tensor([71, 40, 1, 100], dtype=torch.int32, device=gpu))
-    assert t.borrowed.tolist() == [0, 3, 0, 4] and t.free_count.item() == 13
+    # (shared rows stay, or the next token's row would lie on a page that is another's too)
+    assert t.borrowed.tolist() == [0, 4, 0, 4] and t.free_count.item() == 13
+    assert t.seqlens.tolist() == [71, 64, 1, 65]
     with pytest.raises(ValueError, match=r"shared by \[1, 3\]"):
         t.release(0)
     t.release(1)
@@ -151,6 +161,34 @@ def test_shared_pages_go_back_once(gpu):
     t.release(2)
     assert t.free_count.item() == 20 and sorted(t.free_pages.tolist()) == list(range(20))
     assert (t.block_table == -1).all()
+
+
+@gpu_test
+def test_shared_rows_stay(gpu):
+    t = DevicePageTable(4, 20, page_size=16, device=gpu)
+    t.extend([40, 0, 5, 0])
+    for lender, borrowers, rows in ((0, [2], 16), (0, [1], 48), (3, [1], 16)):
+        with pytest.raises(ValueError, match="rows"):
+            t.share(lender, borrowers, rows)
+    assert t.share(0, [1], 40) == 32
+    t.extend([0, 20, 0, 0])
+    assert t.share(1, [3], 48) == 48  # two pages of the first's, one of the second's
+    assert t.cu_groups.tolist() == [0, 2, 3, 4, 4] and t.held.tolist() == [32, 48, 0, 48]
+    t.rollback(torch.zeros(4, dtype=torch.int32, device=gpu))
+    assert t.seqlens.tolist() == [32, 48, 0, 48] and t.free_count.item() == 17
+    for b in (0, 1):
+        with pytest.raises(ValueError, match="shared by"):
+            t.release(b)
+    t.release(3)
+    assert t.held.tolist() == [32, 32, 0, 0]
+    t.rollback(torch.zeros(4, dtype=torch.int32, device=gpu))
+    assert t.seqlens.tolist() == [32, 32, 0, 0] and t.free_count.item() == 18
+    t.release(1)
+    assert t.held.tolist() == [0] * 4
+    t.truncate(16)
+    assert t.seqlens.tolist() == [16, 0, 0, 0] and t.position_shift.tolist() == [16, 0, 0, 0]
+    t.release(0)
+    assert sorted(t.free_pages.tolist()) == list(range(20)) and t.free_count.item() == 20
 
 
 # ── GPU: a layer on it ───────────────────────────────────────────────────────
