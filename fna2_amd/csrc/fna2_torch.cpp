@@ -20,7 +20,9 @@
 //
 // The library's functions come as addresses (bind), so that the binding
 // always calls the library that _capi.py loaded.
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <cstring>
@@ -702,6 +704,23 @@ std::optional<std::tuple<Tensor, Tensor, OptTensor, OptTensor>> rotary_bwd(
   return std::make_tuple(dq, dk, dn[0], dn[1]);
 }
 
+// A backward pass recorded into a graph sums a leaf's gradients on the stream that the leaf's
+// accumulator was made on.  One that an eager graph keeps alive from the default stream, which
+// cannot be recorded, ends the process there: refused while there is still a call to raise from.
+void recordable(const std::vector<OptTensor>& leaves) {
+  if (!at::GradMode::is_enabled() ||
+      c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None)
+    return;
+  for (const OptTensor& t : leaves) {
+    if (!t.has_value() || !t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto sum = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = sum ? sum->stream() : std::nullopt;
+    TORCH_CHECK(!stream || stream->id() != 0,
+                "rotary_embed: a graph is being captured while an eager autograd graph of the same "
+                "leaf, made on the default stream, is alive: let go of that graph's outputs first");
+  }
+}
+
 // rotary_embed with gradients: an autograd node in native code, which takes 20 us of
 // host time a pass where one in Python takes 80.
 OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
@@ -733,9 +752,19 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
                               ctx->saved_data["scale"].toDouble(), given(s[5]), given(s[6]),
                               ctx->saved_data["eps"].toDouble(), std::nullopt, std::nullopt);
     TORCH_CHECK(d.has_value(), "rotary_embed: gradients of another shape, type or device");
-    auto some = [](const OptTensor& t) { return t.has_value() ? *t : Tensor(); };
-    return {std::get<0>(*d), std::get<1>(*d), Tensor(), Tensor(), Tensor(), some(std::get<2>(*d)),
-            some(std::get<3>(*d)), Tensor(), Tensor(), Tensor()};
+    torch::autograd::variable_list out = {std::get<0>(*d), std::get<1>(*d)};
+    for (const OptTensor& t : {std::get<2>(*d), std::get<3>(*d)})
+      if (t.has_value()) out.push_back(*t);
+    if (at::GradMode::is_enabled()) {  // (differentiated again, it raises)
+      const auto once = std::make_shared<torch::autograd::DelayedError>(
+          "rotary_embed is differentiable once", (int64_t)out.size());
+      for (Tensor& t : out) t.set_requires_grad(true);
+      out = (*once)(std::move(out));
+    }
+    size_t at = 2;
+    auto next = [&](const OptTensor& t) { return t.has_value() ? out[at++] : Tensor(); };
+    const Tensor dnq = next(std::get<2>(*d)), dnk = next(std::get<3>(*d));
+    return {out[0], out[1], Tensor(), Tensor(), Tensor(), dnq, dnk, Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -749,6 +778,7 @@ Rows rotary_embed(const Tensor& q, const Tensor& k, const Tensor& inv, const Opt
   auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
   if (!at::GradMode::is_enabled() || !(wants(q) || wants(k) || wants(opt(nq)) || wants(opt(nk))))
     return rotary_launch(a, q, k);
+  recordable({q, k, nq, nk});
   // (what would be refused has to be, by the caller's checks, before the node is made)
   a.r.q_out = view(q, true);
   a.r.k_out = view(k, true);
@@ -1135,6 +1165,7 @@ PYBIND11_MODULE(_torch_binding, m) {
   m.def("decode_rows", &decode_rows, Free());
   m.def("rope_fwd", &rope_fwd, Free());
   m.def("rope_bwd", &rope_bwd, Free());
+  m.def("recordable", &recordable);
   m.def("rotary_fwd", &rotary_fwd, Free());
   m.def("rotary_bwd", &rotary_bwd, Free());
   m.def("rotary_embed", &rotary_embed, Free());

@@ -26,6 +26,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _capi
 
@@ -332,6 +333,7 @@ class RotaryFunc(torch.autograd.Function):
                                 norm_k, eps)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         q, k, inv, pos, cu, wq, wk = ctx.saved_tensors
         if not ctx.norm:  # the inverse rotation reads no inputs: any same-shaped tensors do
@@ -361,8 +363,9 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
 
     A token's position is ``positions[t]`` (int32), or its place in its sequence by
     ``cu_seqlens`` (tokens of no sequence are left as they are): one of the two.  The
-    chain is evaluated in fp32, the angle in fp64, and rounded once.  Differentiable in
-    q, k and the norm weights.  ``rotary_frequencies`` makes ``inv_freq`` and ``scale``."""
+    chain is evaluated in fp32, the angle in fp64, and rounded once.  Differentiable, once, in
+    q, k and the norm weights; into a graph only without an eager autograd graph of the same
+    leaves (RuntimeError).  ``rotary_frequencies`` makes ``inv_freq`` and ``scale``."""
     args = (q, k, inv_freq, positions, cu_seqlens, norm_q, norm_k)
     nat = _capi.native_or_none() if q.is_cuda and grad_slab is None else None
     if nat is not None:
@@ -371,6 +374,9 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
             return done
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (q, k, norm_q, norm_k)):
+        nat = _capi.native_or_none() if q.is_cuda else None
+        if nat is not None:
+            nat.recordable([q, k, norm_q, norm_k])
         return RotaryFunc.apply(*args, (bool(interleaved), float(scale), float(eps)), grad_slab)
     return rotary_embed_raw(q, k, inv_freq, positions, cu_seqlens, interleaved, scale, norm_q,
                             norm_k, eps)

@@ -352,6 +352,54 @@ def test_gradients_of_expanded_and_unused_outputs():
     within("dq", q.grad, dx, HALF[c.dtype] * dx.abs() + 8e-6 * mag)
 
 
+class _Slab:  # (as a GradSlab without room: the Python node's path)
+    def block(self, i, layout):
+        return None
+
+
+@gpu
+@pytest.mark.parametrize("slab", [None, _Slab()])
+def test_second_derivatives_are_refused(slab):
+    c = Case(12, 4, 2, 64, 32, True, torch.float32)
+    q = c.q.clone().requires_grad_()
+    y, z = rotary_embed(q, c.k, c.inv, **c.args(), grad_slab=slab)
+    (g,) = torch.autograd.grad((y.square().sum() + z.sum()), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), q, retain_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("slab", [None, _Slab()])
+def test_captured_training(slab):
+    c = Case(70, 4, 2, 64, 32, True, torch.bfloat16)
+    args = c.args()
+    leaf = args["norm_q"] = args["norm_q"].detach().clone().requires_grad_()
+
+    def step():
+        y, z = rotary_embed(c.q, c.k, c.inv, **args, grad_slab=slab)
+        (g,) = torch.autograd.grad((y, z), leaf, (c.dyq, c.dyk))
+        return y, g
+
+    eager = rotary_embed(c.q, c.k, c.inv, **args, grad_slab=slab)  # an eager graph that lives
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="is alive"), torch.cuda.graph(graph):
+        rotary_embed(c.q, c.k, c.inv, **args, grad_slab=slab)
+    del eager, graph
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(3):
+        c.pos += 11
+        c.q.mul_(1.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
 # ── CPU ──────────────────────────────────────────────────────────────────────
 
 def _args(**over):
