@@ -1609,8 +1609,11 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
 
 // The same for groups that share rows: the tile kernel, whatever the chunks' length,
 // since the shared rows have the tokens of a whole group, with up to 4 heads a tile, since
-// the own rows may have one token (us, 1, 2, 4 heads of 4: 64 tokens over 16384 shared and up
-// to 1000 own rows, rank 32 179, 127, 103; 16 x 128 over 8192, rank 64 345, 361, 350).  Runs are
+// the own rows may have one token, but 2 where sequences have 32 tokens on average, which read
+// fewer queries and leave fewer parts a step (us, 1, 2, 4 heads of 4: 64 tokens over 16384 shared
+// and up to 1000 own rows, rank 32 179, 121, 106; 16 x 32 over 4096 83, 72, 74; 16 x 64 over 8192
+// 214, 206, 211; 8 x 100 over 2048 and 1000 own, rank 64 97, 95, 100; 16 x up to 128 over 8192,
+// rank 64 351, 352, 365; 8 x up to 189 over 5771, 3 heads of 64 68, 70, 74).  Runs are
 // equal in key steps and 8 for each tile that they begin, which takes as long as those: its
 // page ids, first rows, queries, and the part that it leaves (us, 0, 4, 8, 12: the 16 x 128
 // 852, 420, 378, 380; 16 x 64, rank 32 561, 227, 190, 188; 64 tokens, as above 117, 118, 116, 114;
@@ -1626,7 +1629,7 @@ SharedPlan shared_plan(const fna2_paged_shared_args& a) {
   const fna2_paged_cache& c = a.attn.c;
   SharedPlan k{};
   const int group = c.heads / c.heads_kv, rpl = fna2::padded_rank32(c.heads_graph, c.rank);
-  k.hw = group >= 3 ? 4 : group;
+  k.hw = c.total_q >= 32 * (int64_t)c.batch ? std::min(group, 2) : group >= 3 ? 4 : group;
   k.min_steps = 4;
   const int64_t blocks = (int64_t)c.heads_kv * ((group + k.hw - 1) / k.hw);
   const int64_t steps = std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);

@@ -159,6 +159,9 @@ CASES = {
                               [(3, 1344, 1344)], {}),
     "many_sequences_long": (([2] * 70, [270 + i % 23 for i in range(70)], 2, 1, 2, 64, 8, 16),
                             [(30, 256, 256), (40, 240, 250)], {}),
+    "few_tokens_each": (([3] * 40, [300 + i % 7 for i in range(40)], 8, 2, 8, 64, 32, 16),
+                        [(40, 256, 256)], {}),
+    "heads_3_many": (([150, 60], [480, 390], 6, 2, 6, 128, 32, 64), [(2, 320, 320)], {}),
     "loose_tokens": (([1, 1], [150, 150], 4, 2, 4, 64, 16, 16), [(2, 128, 128)],
                      dict(head=37, tail=40)),
     "rows_of_heads": (([1, 2], [150, 150], 4, 2, 4, 64, 16, 16), [(2, 128, 128)],
