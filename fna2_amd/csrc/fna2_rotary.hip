@@ -17,6 +17,9 @@
 // neighbours; LPR = D / (2 EPL) lanes a row.  Halves that do not begin on a chunk
 // (rd / 2 not a multiple of EPL) have their pairs in different lanes: those go
 // through LDS.  A wave forms the token's cos and sin once, a lane a pair.
+//
+// 16384 tokens of 32 + 8 heads of 128 in bf16, no norm, 65 us: 5.2 TB/s; of 16 + 16 with the norm
+// 61 forward (4.4 TB/s), 91 backward (4.4), 5 for dw; 64 tokens of 32 + 8 5.6, one launch's latency.
 #include <algorithm>
 
 #include "fna2_rope_dev.h"
