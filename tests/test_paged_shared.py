@@ -161,6 +161,7 @@ CASES = {
                             [(30, 256, 256), (40, 240, 250)], {}),
     "few_tokens_each": (([3] * 40, [300 + i % 7 for i in range(40)], 8, 2, 8, 64, 32, 16),
                         [(40, 256, 256)], {}),
+    "heads_5": (([1, 6], [300, 305], 10, 2, 7, 64, 16, 16), [(2, 288, 288)], {}),
     "heads_3_many": (([150, 60], [480, 390], 6, 2, 6, 128, 32, 64), [(2, 320, 320)], {}),
     "loose_tokens": (([1, 1], [150, 150], 4, 2, 4, 64, 16, 16), [(2, 128, 128)],
                      dict(head=37, tail=40)),
@@ -334,6 +335,21 @@ def test_two_captured_graphs_share_nothing():
         ga.replay(), gb.replay()
         torch.cuda.synchronize()
         assert torch.equal(oa, want[0]) and torch.equal(ob, want[1])
+
+
+@gpu
+def test_pools_past_32_bits():
+    """The same pages at the end of pools of more than 2^31 elements."""
+    c = make("two_groups")
+    want = c.attend()
+    n, P = c.k.shape[0], 2 ** 31 // c.k[0].numel() + 1
+    for name in ("k", "v", "rk"):
+        old = getattr(c, name)
+        big = torch.empty((P + n, *old.shape[1:]), dtype=old.dtype, device="cuda")
+        big[P:] = old
+        setattr(c, name, big)
+    c.table = torch.where(c.table >= 0, c.table + P, c.table)
+    assert c.k.numel() > 2 ** 31 and torch.equal(c.attend(), want)
 
 
 @gpu

@@ -324,6 +324,27 @@ def test_norm_weights_of_another_type(wdtype):
 
 
 @gpu
+def test_rows_past_32_bits():
+    """The last tokens of a call of more than 2^31 elements, forward and backward, as by themselves."""
+    c = Case(48, 8, 2, 512, 96, True, torch.bfloat16)
+    T = 2 ** 31 // (8 * 512) + 100
+
+    def long(t):
+        y = torch.zeros(T, *t.shape[1:], dtype=t.dtype, device="cuda")
+        y[-48:] = t
+        return y
+
+    want = (*rope.rotary_embed_raw(c.q, c.k, c.inv, **c.args()),
+            *rope.rotary_embed_bwd(c.dyq, c.dyk, c.q, c.k, c.inv, **c.args())[:2])
+    c.q, c.k, c.dyq, c.dyk, c.pos = (long(t) for t in (c.q, c.k, c.dyq, c.dyk, c.pos))
+    assert c.q.numel() > 2 ** 31
+    for a, b in zip(rope.rotary_embed_raw(c.q, c.k, c.inv, **c.args()), want[:2]):
+        assert torch.equal(a[-48:], b)
+    for a, b in zip(rope.rotary_embed_bwd(c.dyq, c.dyk, c.q, c.k, c.inv, **c.args()), want[2:]):
+        assert torch.equal(a[-48:], b)
+
+
+@gpu
 def test_captured():
     c = Case(70, 4, 2, 128, 64, True, torch.bfloat16)
     c.run()
