@@ -853,7 +853,7 @@ class NaylisAttention(nn.Module):
         q = paged_append(q, k, v, cache.k, cache.v, t.block_table, t.seqlens, cu, r_k, cache.r_k,
                          inv, None, wq, wk, eps, t.position_shift if inv is not None else None)
         bias = (r_q, cache.r_k, self.graph_scale)
-        if isinstance(t, DevicePageTable) and t.cu_groups is not None:
+        if isinstance(t, DevicePageTable) and t.shares:
             out = flash_naylis_shared(q, cache.k, cache.v, t.block_table, t.seqlens, cu, max_q,
                                       t.cu_groups, t.shared_rows, *bias,
                                       softmax_scale=self._attn_scale(), key_weights=cache.key_weights)

@@ -850,6 +850,12 @@ class DevicePageTable:
         self._trim(torch.full_like(self.seqlens, int(budget)))
         self.position_shift += before - self.seqlens
 
+    @property
+    def shares(self) -> bool:
+        """Whether sequences share rows now: a layer then goes by ``cu_groups`` (a few us more
+        for a small step that shares none).  A captured step stays right either way."""
+        return self.cu_groups is not None and any(self._lent.values())
+
     def _unshared(self, what: str) -> None:
         if any(self._lent.values()):
             raise ValueError(f"{what}: sequences share rows")

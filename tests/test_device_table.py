@@ -170,7 +170,7 @@ def test_shared_rows_stay(gpu):
     for lender, borrowers, rows in ((0, [2], 16), (0, [1], 48), (3, [1], 16)):
         with pytest.raises(ValueError, match="rows"):
             t.share(lender, borrowers, rows)
-    assert t.share(0, [1], 40) == 32
+    assert not t.shares and t.share(0, [1], 40) == 32 and t.shares
     t.extend([0, 20, 0, 0])
     assert t.share(1, [3], 48) == 48  # two pages of the first's, one of the second's
     assert t.cu_groups.tolist() == [0, 2, 3, 4, 4] and t.held.tolist() == [32, 48, 0, 48]
@@ -184,7 +184,7 @@ def test_shared_rows_stay(gpu):
     t.rollback(torch.zeros(4, dtype=torch.int32, device=gpu))
     assert t.seqlens.tolist() == [32, 32, 0, 0] and t.free_count.item() == 18
     t.release(1)
-    assert t.held.tolist() == [0] * 4
+    assert t.held.tolist() == [0] * 4 and not t.shares
     t.truncate(16)
     assert t.seqlens.tolist() == [16, 0, 0, 0] and t.position_shift.tolist() == [16, 0, 0, 0]
     t.release(0)
@@ -405,6 +405,40 @@ def test_a_step_captured_whole(gpu, kw):
             assert torch.equal(graphed.table.seqlens, eager.table.seqlens)
         eager.table.check()
         graphed.table.check()
+
+
+@gpu_test
+def test_a_captured_step_outlives_its_sharing(gpu):
+    """Captured while rows are shared and replayed after the last borrower's release, and the
+    other way round."""
+    m = layer(gpu)
+    with torch.no_grad():
+        for shared in (True, False):
+            s = Served(m, gpu)
+            if not shared:
+                s.table.release(1, 2, 3)
+                s.table.extend([0, 20, 20, 20])
+                m(torch.randn(60, 512, device=gpu).bfloat16(), past_kv=s.cache)
+            x = torch.randn(3, 512, device=gpu).bfloat16()
+            step = lambda: m(x, past_kv=s.cache)[0]
+            s.table.extend([0, 1, 1, 1])
+            assert s.table.shares == shared
+            step()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                y = step()
+            for i in range(3):
+                if i == 1 and shared:
+                    s.table.release(1, 2, 3)
+                elif i == 1:
+                    s.table.release(1, 2, 3)
+                    assert s.table.share(0, [1, 2, 3], 96) == 96
+                s.table.extend([0, 1, 1, 1])
+                x.normal_()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert rel_norm(y, step()) <= TOL
 
 
 @gpu_test
