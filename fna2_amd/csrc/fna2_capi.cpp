@@ -1614,11 +1614,12 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
 // and up to 1000 own rows, rank 32 179, 121, 106; 16 x 32 over 4096 83, 72, 74; 16 x 64 over 8192
 // 214, 206, 211; 8 x 100 over 2048 and 1000 own, rank 64 97, 95, 100; 16 x up to 128 over 8192,
 // rank 64 351, 352, 365; 8 x up to 189 over 5771, 3 heads of 64 68, 70, 74).  Runs are
-// equal in key steps and 8 for each tile that they begin, which takes as long as those: its
-// page ids, first rows, queries, and the part that it leaves (us, 0, 4, 8, 12: the 16 x 128
-// 852, 420, 378, 380; 16 x 64, rank 32 561, 227, 190, 188; 64 tokens, as above 117, 118, 116, 114;
-// 4 over 2000 18.2 with 8, 19.8 with 4).  Rows are not shared where reading
-// them once saves fewer than 64 bytes for a token, head and feature's second part (us, never
+// equal in key steps and 8 for each tile that they go on to, which takes as long as those: its
+// page ids, first rows, queries, and the part that it leaves (us, 4, 6, 8, 10: 16 x up to 128 over 8192 391,
+// 335, 334, 336; 9 x up to 193 over 12689 237, 218, 210, 204; 4 groups of 32 x 1 over 2821, 32 heads of 64
+// 62, 58, 60, 65), and of 6 steps at least (us, 4, 6, 8, 12: 4 x 1 over 2000 20.2, 17.6, 18.1, 20.2;
+// 2 groups of 2 x 1 over 500 18.2, 19.8, 21.3, 23.4; 8 groups of 4 x 3 over 400 25.5, 25.7, 25.5, 30.7).
+// Rows are not shared where reading them once saves fewer than 64 bytes for a token, head and feature's second part (us, never
 // shared, always, here: 3 groups of 16 x 25 tokens over 64 rows 29.8, 38.3, 29.8; 3 of 18 x 6 over 64
 // 29.8, 34.7, 30.0; 10 x 100 over 1024 39.0, 44.3, 38.9; 5 of 25 x 9 over 960 68.9, 43.9, 44.1).
 struct SharedPlan {
@@ -1630,12 +1631,12 @@ SharedPlan shared_plan(const fna2_paged_shared_args& a) {
   SharedPlan k{};
   const int group = c.heads / c.heads_kv, rpl = fna2::padded_rank32(c.heads_graph, c.rank);
   k.hw = c.total_q >= 32 * (int64_t)c.batch ? std::min(group, 2) : group >= 3 ? 4 : group;
-  k.min_steps = 4;
+  k.min_steps = 6;
   const int64_t blocks = (int64_t)c.heads_kv * ((group + k.hw - 1) / k.hw);
   const int64_t steps = std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);
   const int64_t tiles = (2 * ((int64_t)c.total_q / (128 / k.hw)) + c.batch + a.groups) * blocks;
   k.waves = (int)std::min(256. * fna2::paged_tile_per_cu(c.head_dim, rpl, k.hw),
-                          std::max(std::ceil((double)tiles * steps / k.min_steps), 1.));
+                          std::max(std::ceil((double)tiles * (steps + fna2::kSharedStart) / k.min_steps), 1.));
   k.waves = (int)cdiv64(k.waves, 8) * 8;  // (whole turns of the XCDs)
   const size_t virt = (size_t)c.batch + (size_t)a.groups, rows = 2 * (size_t)c.total_q * (size_t)c.heads;
   size_t at = 0;
@@ -1794,7 +1795,7 @@ int fna2_paged_shared(const fna2_paged_shared_args* a, void* stream_ptr) {
   S.p.hw = k.hw;
   S.p.part = (float*)ws;
   S.p.ml = (float*)(ws + k.ml);
-  S.start = 8;  // (see shared_plan)
+  S.start = fna2::kSharedStart;
   S.worth = 32.f;
   S.small = a->groups <= fna2::kSharedSmall && a->attn.c.batch <= fna2::kSharedSmall;
   S.G = a->groups;

@@ -64,6 +64,8 @@ struct SharedSmallPlan {
   int64_t ends[2 * kSharedSmall];
 };
 
+constexpr int kSharedStart = 8;  // PagedSharedParams::start
+
 struct PagedSharedParams {
   PagedParams p;
   int start;  // what starting and ending a tile costs, in steps
@@ -140,16 +142,12 @@ __device__ __forceinline__ int shared_seek(const int64_t* ends, int n, int lane,
   return lo + min(l, n - 1);
 }
 
-// The units of a run, to begin with: as few as the runs that there are can do.  A unit
-// is a step or a tile's start's share; rows in chunks of per - start steps cost per each,
-// so that with A units besides and B steps in chunks, W runs:
-//     per W = A + B per / (per - start).
-// (What does not fit then takes a little more.)
+// The units of a run, to begin with: as few as the runs that there are can do of A units and B
+// steps in chunks.  A unit is a step or a tile's start's share.  A run starts somewhere, in a
+// chunk or inside a tile, and pays for it once; tiles that it goes on to are counted, so that a run takes
+// as long as a chunk of as many steps.  (What does not fit then takes a little more.)
 __device__ __forceinline__ int64_t shared_per(SArg S, int64_t A, int64_t B) {
-  const float W = (float)S->p.waves, st = (float)S->start, a = (float)A;
-  const float p = a + (float)B + st * W;
-  const float x = (p + sqrtf(fmaxf(p * p - 4.f * W * a * st, 0.f))) / (2.f * W);
-  return max((int64_t)ceilf(x), (int64_t)(S->p.min_steps + S->start));
+  return max(div64(A + B + S->p.waves - 1, S->p.waves), (int64_t)S->p.min_steps);
 }
 
 // How many of `rows` rows, that n sequences with tokens in all share, are worth it.  Sharing saves
@@ -272,7 +270,7 @@ __device__ __forceinline__ void shared_plan(SArg S, const SharedPlanRef R, int64
     for (int g0 = 0; g0 < G; g0 += NT) {
       const int g = g0 + tid;
       const int64_t n = g < G ? groups[g].s.lk / 32 : 0, tiles = g < G ? groups[g].tiles * blocks : 0;
-      const int64_t full = div64(n, per - start), left = n - full * (per - start);
+      const int64_t full = div64(n, per), left = n - full * per;
       plan_scan<NT>(full * tiles, sums, sum);
       runs += sum;
       plan_scan<NT>(left > 0 ? (left + start) * tiles : 0, sums, sum);
@@ -286,7 +284,7 @@ __device__ __forceinline__ void shared_plan(SArg S, const SharedPlanRef R, int64
     const int g = g0 + tid;
     SharedGroup x{};
     if (g < G) x = groups[g];
-    x.full = div64(x.s.lk / 32, per - start);
+    x.full = div64(x.s.lk / 32, per);
     const int64_t mine = x.full * x.tiles * blocks;
     x.run0 = runs + plan_scan<NT>(mine, sums, sum);
     x.end = x.run0 + mine;
@@ -294,7 +292,7 @@ __device__ __forceinline__ void shared_plan(SArg S, const SharedPlanRef R, int64
     if (g >= G) continue;
     groups[g] = x;
     R.group_ends[g] = x.end;
-    SharedSeq y{x.s, (int)(x.full * (per - start) * 32), x.table, kSharedPrefix, g};
+    SharedSeq y{x.s, (int)(x.full * per * 32), x.table, kSharedPrefix, g};
     y.s.lk = y.s.off = x.s.lk - y.row0;
     if (y.s.lk <= 0) y.s.lq = 0;
     seqs[g] = y;
@@ -374,8 +372,8 @@ __device__ __forceinline__ void shared_plan_small(SArg S, SharedSmallPlan& R, in
   per = any ? shared_per(S, own + lane64(lane_scan64(tiles * start), 63), lane64(lane_scan64(tiles * n), 63))
             : shared_per(S, own, 0);
   while (any) {
-    full = div64(n, per - start);
-    const int64_t left = n - full * (per - start);
+    full = div64(n, per);
+    const int64_t left = n - full * per;
     run_end = lane_scan64(full * tiles);
     runs = lane64(run_end, 63);
     rest = left > 0 ? (left + start) * tiles : 0;
@@ -387,7 +385,7 @@ __device__ __forceinline__ void shared_plan_small(SArg S, SharedSmallPlan& R, in
   if (lane < G) {
     R.groups[lane] = SharedGroup{PagedSeq{q0, lq, rows, rows}, run_end - full * tiles, run_end, first, tiles1, full};
     R.group_ends[lane] = run_end;
-    const int at = (int)(full * (per - start) * 32), lk = rows - at;
+    const int at = (int)(full * per * 32), lk = rows - at;
     R.seqs[lane] = SharedSeq{PagedSeq{q0, lk > 0 ? lq : 0, lk, lk}, at, first, kSharedPrefix, lane};
     R.ends[lane] = rest_end;
   }
@@ -480,8 +478,8 @@ __device__ __forceinline__ void shared_plan_mid(SArg S, const SharedPlanRef R, S
   }
   int64_t per = shared_per(S, own + total[2], total[1]), full, end[2];
   while (true) {
-    full = div64(n, per - start);
-    const int64_t left = n - full * (per - start);
+    full = div64(n, per);
+    const int64_t left = n - full * per;
     int64_t x[2] = {full * tiles, left > 0 ? (left + start) * tiles : 0}, t[2];
     plan_scans<2>(x, t, L.sums, nw);
     end[0] = x[0], end[1] = x[1], sum[0] = t[0], sum[1] = t[1];
@@ -491,7 +489,7 @@ __device__ __forceinline__ void shared_plan_mid(SArg S, const SharedPlanRef R, S
   if (tid < G) {
     R.groups[tid] = SharedGroup{PagedSeq{q0, lq, rows, rows}, end[0] - full * tiles, end[0], first, tiles1, full};
     R.group_ends[tid] = end[0];
-    const int at = (int)(full * (per - start) * 32), lk = rows - at;
+    const int at = (int)(full * per * 32), lk = rows - at;
     R.seqs[tid] = SharedSeq{PagedSeq{q0, lk > 0 ? lq : 0, lk, lk}, at, first, kSharedPrefix, tid};
     R.ends[tid] = end[1];
   }

@@ -87,7 +87,7 @@ __device__ __forceinline__ void tile_body() {
       b = 0;
       hb = uni(rest / tiles);
       qt = uni(rest - hb * tiles);
-      left = per - S->start;
+      left = per;
       s0 = uni((int)(c * left));
     } else {
       run = nfull + x * (int)(gridDim.x >> 3) - lo + (j - mine);
@@ -464,7 +464,7 @@ __device__ __forceinline__ void tile_body() {
         if (v.kind == kSharedOwn) {
           const SharedGroup g = plan.groups[v.group];
           const int t = e.q0 + tok - g.s.q0;
-          rec.at |= kSharedHas | (g.full * (per - S->start) * 32 < g.s.lk ? kSharedRest : 0);
+          rec.at |= kSharedHas | (g.full * per * 32 < g.s.lk ? kSharedRest : 0);
           rec.run0 = (int)g.run0 + hb * g.tiles + t / TB;
           rec.stride = g.tiles * TilePlan::blocks(P);
           rec.full = (int)g.full;
