@@ -1348,7 +1348,7 @@ fna2::RotaryParams rotary_params(const fna2_rotary_args* a) {
 
 size_t rotary_ws(const fna2_rotary_args* a) {
   if (!(a->r.norm_q || a->r.norm_k) || rope_empty(&a->r)) return 0;
-  return align_up(sizeof(float) * 2u * (size_t)fna2::rotary_bwd_blocks(a->r.total_tokens) *
+  return align_up(sizeof(float) * 2u * (size_t)fna2::rotary_bwd_blocks(rope_params(&a->r)) *
                   (size_t)a->r.head_dim);
 }
 

@@ -118,7 +118,7 @@ struct RotaryParams {
   const int* pos;  // [T], or null: the packed sequences'
   int share;       // waves of a token (set by the launch)
 };
-int rotary_bwd_blocks(int T);
+int rotary_bwd_blocks(const RopeParams& R);
 hipError_t launch_rotary(const RotaryParams& P, hipStream_t s);
 hipError_t launch_rotary_norm_bwd(const RotaryParams& P, hipStream_t s);
 

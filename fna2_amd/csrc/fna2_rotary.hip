@@ -304,7 +304,8 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
   const int wv = uni(threadIdx.x >> 6);
   rot_weights(P, wsh);
   RotLane<DT, MODE> L(P, shared[wv]);
-  RotTokens tokens(P, blockIdx.x * kRotWaves + wv);
+  const int unit = blockIdx.x * kRotWaves + wv, step = L.rpw * P.share, first = unit % P.share * L.rpw;
+  RotTokens tokens(P, unit / P.share);
   const float inv_d = 1.f / (float)R.D, sign = -(float)R.sign;
   float dw[2][N];
 #pragma unroll
@@ -376,8 +377,8 @@ __global__ __launch_bounds__(64 * kRotWaves, MODE == kRotAny ? 2 : 4) void rotar
         y2.store(out + L.o2 * ES);
       }
     };
-    for (int r = 0; r < R.Hq; r += L.rpw) rows(std::integral_constant<int, 0>{}, r);
-    for (int r = 0; r < R.Hk; r += L.rpw) rows(std::integral_constant<int, 1>{}, r);
+    for (int r = first; r < R.Hq; r += step) rows(std::integral_constant<int, 0>{}, r);
+    for (int r = first; r < R.Hk; r += step) rows(std::integral_constant<int, 1>{}, r);
   }
 
   // dw: lanes that share features, then the waves.
@@ -470,12 +471,20 @@ int rot_tokens(const RotaryParams& P) {
   return P.r.T <= 4096 ? 1 : P.r.T <= 12288 ? 2 : 4;
 }
 int rot_bwd_tokens(int T) { return T <= 1024 ? 1 : T <= 12288 ? 2 : 4; }
+// Few tokens with four passes of rows and more: the waves of a workgroup share each (us, one wave a
+// token and four: 64 tokens x 64 rows of 128 17.3, 12.3; 256 20.0, 13.0; 500 21.2, 17.1; 1000 x 32 17.6, 19.9;
+// 500 x 16 rows of 64, two passes, 13.8, 15.4).
+int rot_bwd_share(const RopeParams& R) {
+  const int rpw = 64 * (R.dtype == kRopeF32 ? 8 : 16) / R.D;
+  return R.T <= 512 && cdiv(R.Hq, rpw) + cdiv(R.Hk, rpw) >= 4 ? kRotWaves : 1;
+}
 
 }  // namespace
 
-int rotary_bwd_blocks(int T) {
-  const int tpw = rot_bwd_tokens(T);
-  return (int)(((int64_t)T + kRotWaves * tpw - 1) / (kRotWaves * tpw));
+int rotary_bwd_blocks(const RopeParams& R) {
+  const int T = R.T;
+  const int64_t waves = ((int64_t)T + rot_bwd_tokens(T) - 1) / rot_bwd_tokens(T) * rot_bwd_share(R);
+  return (int)((waves + kRotWaves - 1) / kRotWaves);
 }
 
 hipError_t launch_rotary(const RotaryParams& args, hipStream_t s) {
@@ -500,7 +509,8 @@ hipError_t launch_rotary_norm_bwd(const RotaryParams& args, hipStream_t s) {
   RotaryParams P = args;
   if (P.r.T <= 0 || P.r.Hq + P.r.Hk <= 0) return hipSuccess;
   P.r.tpw = rot_bwd_tokens(P.r.T);
-  const int nb = rotary_bwd_blocks(P.r.T);
+  P.share = rot_bwd_share(P.r);
+  const int nb = rotary_bwd_blocks(P.r);
   const dim3 grid((uint32_t)nb);
   switch (P.r.dtype) {
     case kRopeBF16: launch_bwd<kRopeBF16>(P, rot_mode(P), grid, s); break;

@@ -213,6 +213,15 @@ def test_token_counts(T):
 
 
 @gpu
+@pytest.mark.parametrize("cu", [None, [3, 100, 100, 505]])
+@pytest.mark.parametrize("heads", [(8, 8), (19, 1), (1, 13)])
+@pytest.mark.parametrize("T", [511, 512, 513])
+def test_token_counts_of_shared_tokens(T, heads, cu):
+    """Where the waves of a workgroup share a token's rows in the backward, and no longer do."""
+    check_backward(Case(T, *heads, 256, 64, True, torch.bfloat16, far=5000, cu=cu))
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_far_and_negative_positions(dtype):
     c = Case(64, 2, 1, 64, 64, False, dtype, norm=(False, False), far=2 ** 31 - 1)
