@@ -768,8 +768,10 @@ class DevicePageTable:
     ``slots``, ``sequences`` and ``positions`` of them, and ``status``, 0 where the pages
     sufficed; with another status the step has no tokens (``check`` raises it, and waits
     for it).  What ``PageTable`` keeps, ``block_table``, ``seqlens``, ``position_shift``,
-    ``cu_seqlens_q`` (written in place), ``total_q`` and ``max_seqlen_q`` (the host's bounds of the
-    step), is here too: a ``PagedKVCache`` takes either.
+    ``cu_seqlens_q``, ``total_q`` and ``max_seqlen_q`` (the host's bounds of the
+    step), is here too: a ``PagedKVCache`` takes either.  All on the device is written in place,
+    what is a token's in the same memory for steps of as many tokens, so that a captured graph
+    reads the step at hand.
 
     ``share`` lets a sequence begin with another's pages; ``cu_groups`` and
     ``shared_rows`` then say which neighbouring sequences share how many rows, and a
@@ -793,6 +795,7 @@ class DevicePageTable:
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
         self.status = zeros(1)
         self.slots = self.sequences = self.positions = None
+        self._tokens = {}  # buffers of slots, sequences, positions, by the power of two they hold
         self.cu_groups = self.shared_rows = None
         self.max_seqlen_q = self.total_q = 0
         self._lent = {}  # lender -> its borrowers
@@ -810,12 +813,26 @@ class DevicePageTable:
         assert total_q is not None, "extend: counts on the device need total_q"
         step = paged_extend(self.block_table, self.seqlens, counts, self.free_pages,
                             self.free_count, self.page_size, total_q, self.position_shift)
-        torch._foreach_copy_([self.seqlens, self.free_count, self.cu_seqlens_q, self.status],
-                             [step.seqlens, step.free_count, step.cu_seqlens_q, step.status])
-        self.slots, self.sequences, self.positions = step.slots, step.sequences, step.positions
         self.total_q = int(total_q)
+        self.slots, self.sequences, self.positions = self._of_tokens(self.total_q)
+        torch._foreach_copy_(
+            [self.seqlens, self.free_count, self.cu_seqlens_q, self.status, self.sequences,
+             self.positions],
+            [step.seqlens, step.free_count, step.cu_seqlens_q, step.status, step.sequences,
+             step.positions])
+        self.slots.copy_(step.slots)
         self.max_seqlen_q = self.total_q if max_seqlen_q is None else int(max_seqlen_q)
         return step
+
+    def _of_tokens(self, n: int) -> Tuple[torch.Tensor, ...]:
+        """(slots, sequences, positions) of a step of n tokens.  Kept for good: graphs captured
+        with steps of n tokens read and write them."""
+        size = max(n - 1, 0).bit_length()
+        if size not in self._tokens:
+            with torch.inference_mode(False):  # (or they could not be written outside it)
+                new = lambda dt: torch.empty(1 << size, dtype=dt, device=self.seqlens.device)
+                self._tokens[size] = new(torch.int64), new(torch.int32), new(torch.int32)
+        return tuple(t[:n] for t in self._tokens[size])
 
     def check(self) -> None:
         """Raises ValueError where the last ``extend`` did not take its tokens in (waits)."""

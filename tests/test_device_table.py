@@ -11,7 +11,8 @@ import pytest
 import torch
 
 from fna2_amd.attention_fna2 import NaylisAttention, RotaryPositionalEmbedding
-from fna2_amd.paged import DevicePageTable, PagedKVCache, PageTable
+from fna2_amd import paged
+from fna2_amd.paged import DevicePageTable, PagedKVCache, PagedStep, PageTable
 from tests.helpers import rel_norm
 
 gpu_test = pytest.mark.gpu
@@ -472,3 +473,89 @@ def test_weights_of_shared_rows(gpu):
             s.run()
             got.append(s.cache.key_weights)
         assert (got[0] - got[1]).abs().max() <= 2e-2 and got[0].sum() > 0
+
+
+def plain_extend(table, seqlens, counts, free_pages, free_count, page_size, total_q, shift=None):
+    """paged_extend's step in plain Python (pages apart), on the CPU."""
+    c, lens, T = counts.tolist(), seqlens.tolist(), total_q
+    pos = [n + i for n, k in zip(lens, c) for i in range(k)]
+    of = [b for b, k in enumerate(c) for _ in range(k)]
+    ints = lambda x, n: torch.tensor(x + [-1] * (n - len(x)), dtype=torch.int32)
+    cu = [sum(c[:b]) for b in range(len(c) + 1)]
+    return PagedStep(ints(cu, len(cu)), ints([n + k for n, k in zip(lens, c)], len(c)),
+                     free_count.clone(), ints(pos, T).long(), ints(of, T), ints(pos, T),
+                     torch.zeros(1, dtype=torch.int32))
+
+
+def test_a_steps_numbers_stay_where_they_are(monkeypatch):
+    """What a captured layer reads of a step lies where it lay in the step that was captured,
+    whatever steps came between."""
+    monkeypatch.setattr(paged, "paged_extend", plain_extend)
+    t = DevicePageTable(3, 8, page_size=16, device="cpu")
+    with torch.inference_mode():
+        t.extend([1, 1, 1])
+    seen = {n: getattr(t, n) for n in ("slots", "sequences", "positions", "seqlens",
+                                       "cu_seqlens_q", "status", "block_table", "position_shift")}
+    for counts in ([40, 0, 3], [0, 0, 0], [1, 0, 0], [0, 1, 1], [2, 1, 1]):
+        t.extend(counts)
+        n = sum(counts)
+        assert t.total_q == n and t.positions.shape == t.slots.shape == t.sequences.shape == (n,)
+    t.extend([0, 2, 1])
+    for n, x in seen.items():
+        y = getattr(t, n)
+        assert x.data_ptr() == y.data_ptr() and torch.equal(x, y)
+    assert seen["positions"].tolist() == [3, 4, 6] and seen["sequences"].tolist() == [1, 1, 2]
+
+
+@gpu_test
+@pytest.mark.parametrize("kw", EXTENDED)
+@pytest.mark.parametrize("inside", [False, True])
+def test_a_captured_layer_in_another_layout_follows_the_table(gpu, kw, inside):
+    """Captured with its extend outside the graph (or inside it), and replayed after steps of
+    other sizes: the rows that it appends, and their angles, are the step's at hand."""
+    m = layer(gpu, **kw)
+    with torch.no_grad():
+        eager, graphed = Served(m, gpu), Served(m, gpu)
+        counts = torch.tensor([0, 1, 1, 1], dtype=torch.int32, device=gpu)
+        x = torch.randn(3, 512, device=gpu).bfloat16()
+
+        def take(s):
+            s.table.extend(counts, total_q=3, max_seqlen_q=1)
+
+        def step(s):
+            return m(x, past_kv=s.cache)[0]
+
+        for s in (eager, graphed):
+            take(s)
+            step(s)
+        torch.cuda.synchronize()
+        take(eager)
+        graph = torch.cuda.CUDAGraph()
+        if inside:
+            with torch.cuda.graph(graph):
+                take(graphed)
+                y = step(graphed)
+        else:
+            take(graphed)
+            with torch.cuda.graph(graph):
+                y = step(graphed)
+        for i in range(5):
+            if i > 0:
+                take(eager)
+                if not inside:
+                    take(graphed)
+            x.normal_()
+            graph.replay()
+            want = step(eager)
+            torch.cuda.synchronize()
+            assert torch.equal(y, want)
+            used = graphed.table.block_table.flatten().unique()[1:].long()
+            assert torch.equal(graphed.cache.k[used], eager.cache.k[used])
+            other = torch.randn(40 + 7 * i, 512, device=gpu).bfloat16()
+            for s in (eager, graphed):  # (a step of another size between the replays)
+                s.table.extend([0, 9 + i, 30 + 6 * i, 1])
+                m(other, past_kv=s.cache)
+            junk = [torch.full((n,), 1 << 20, dtype=torch.int32, device=gpu) for n in (3, 4, 8) * 20]
+            del junk
+        eager.table.check()
+        graphed.table.check()
