@@ -1623,6 +1623,7 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
 // shared, always, here: 3 groups of 16 x 25 tokens over 64 rows 29.8, 38.3, 29.8; 3 of 18 x 6 over 64
 // 29.8, 34.7, 30.0; 10 x 100 over 1024 39.0, 44.3, 38.9; 5 of 25 x 9 over 960 68.9, 43.9, 44.1).
 struct SharedPlan {
+  bool two;
   int hw, waves, min_steps;
   size_t ml, meta, groups, group_ends, seqs, ends, recs, whole, whole_ml, bytes;
 };
@@ -1630,12 +1631,13 @@ SharedPlan shared_plan(const fna2_paged_shared_args& a) {
   const fna2_paged_cache& c = a.attn.c;
   SharedPlan k{};
   const int group = c.heads / c.heads_kv, rpl = fna2::padded_rank32(c.heads_graph, c.rank);
+  k.two = !paged_plan(c).tile;
   k.hw = c.total_q >= 32 * (int64_t)c.batch ? std::min(group, 2) : group >= 3 ? 4 : group;
   k.min_steps = 6;
   const int64_t blocks = (int64_t)c.heads_kv * ((group + k.hw - 1) / k.hw);
   const int64_t steps = std::max<int64_t>(cdiv64(cached_rows(c), 32), 1);
   const int64_t tiles = (2 * ((int64_t)c.total_q / (128 / k.hw)) + c.batch + a.groups) * blocks;
-  k.waves = (int)std::min(256. * fna2::paged_tile_per_cu(c.head_dim, rpl, k.hw),
+  k.waves = (int)std::min(256. * fna2::paged_tile_per_cu(c.head_dim, rpl, k.hw, k.two),
                           std::max(std::ceil((double)tiles * (steps + fna2::kSharedStart) / k.min_steps), 1.));
   k.waves = (int)cdiv64(k.waves, 8) * 8;  // (whole turns of the XCDs)
   const size_t virt = (size_t)c.batch + (size_t)a.groups, rows = 2 * (size_t)c.total_q * (size_t)c.heads;
@@ -1798,6 +1800,7 @@ int fna2_paged_shared(const fna2_paged_shared_args* a, void* stream_ptr) {
   S.start = fna2::kSharedStart;
   S.worth = 32.f;
   S.small = a->groups <= fna2::kSharedSmall && a->attn.c.batch <= fna2::kSharedSmall;
+  S.two = k.two;
   S.G = a->groups;
   S.V = a->groups + a->attn.c.batch;
   S.cu_groups = a->cu_groups;

@@ -261,7 +261,7 @@ struct TilePlan {
 };
 
 // Kernel launches (fna2_paged_attn.hip, fna2_paged_tile.hip, fna2_paged_rows.hip).
-int paged_tile_per_cu(int D, int rpl, int hw);  // resident workgroups of the tile kernel
+int paged_tile_per_cu(int D, int rpl, int hw, bool two = false);  // resident workgroups of the tile kernel
 size_t paged_tile_slot(int D);                  // bytes of a split tile's part
 hipError_t launch_paged_tile(const PagedParams& P, int rpl, hipStream_t s);
 int paged_rank_chunks(int rch);      // as decode_rank_chunks

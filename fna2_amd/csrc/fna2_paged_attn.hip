@@ -320,12 +320,6 @@ __device__ __forceinline__ void packed_body() {
       const float m_use = (m_new == kNegInf) ? 0.f : m_new;
       const float nm = -m_use * c2;
       float ls = 0.f;
-      // P in two parts (as the decode kernel): the first cut to the element
-      // type, the second what that cut off, so that the result does not
-      // depend on where a tile is split.  A part of a visible key is never
-      // zero (an infinite V stays infinite), a hidden key's both are.  The second
-      // part's lowest bit, which sees to that, is 2^-24 in fp16 (p's scale: the
-      // largest is 1), which is then each key's error at most; in bf16 nothing.
       bf16x8 pb[2], pe[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -336,17 +330,7 @@ __device__ __forceinline__ void packed_body() {
           const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v0], c2, nm));
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v0 + 1], c2, nm));
           ls += p0 + p1;
-          if constexpr (F16) {
-            pk[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-            ek[i] = pack_e<true>(p0 - elt_lo<true>(pk[i]), p1 - elt_hi<true>(pk[i]));
-          } else {
-            const uint32_t u0 = __builtin_bit_cast(uint32_t, p0);
-            const uint32_t u1 = __builtin_bit_cast(uint32_t, p1);
-            pk[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // their upper halves
-            ek[i] = pack_bf16(p0 - __builtin_bit_cast(float, u0 & 0xffff0000u),
-                              p1 - __builtin_bit_cast(float, u1 & 0xffff0000u));
-          }
-          ek[i] |= (p0 > 0.f ? 1u : 0u) | (p1 > 0.f ? 0x10000u : 0u);
+          split_p<F16>(p0, p1, pk, ek, i);
         }
         pb[half] = as_bf16x8(pk);
         pe[half] = as_bf16x8(ek);

@@ -30,6 +30,28 @@ __device__ __forceinline__ float weight2(float x) {
   return fmaxf(__builtin_amdgcn_exp2f(x), 1.17549435e-38f);
 }
 
+// P in two parts (as the decode kernel): the first cut to the element
+// type, the second what that cut off, so that the result does not
+// depend on where a tile is split.  No part of a visible key is
+// zero (an infinite V stays infinite; in fp16 from a p of 2^-24 on, below which the first is),
+// both of a hidden key's are.  The second
+// part's lowest bit, which sees to that, is 2^-24 in fp16 (p's scale: the
+// largest is 1), which is then each key's error at most; in bf16 nothing.
+template <bool F16>
+__device__ __forceinline__ void split_p(float p0, float p1, u32x4& first, u32x4& second, int i) {
+  if constexpr (F16) {
+    first[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+    second[i] = pack_e<true>(p0 - elt_lo<true>(first[i]), p1 - elt_hi<true>(first[i]));
+  } else {
+    const uint32_t u0 = __builtin_bit_cast(uint32_t, p0);
+    const uint32_t u1 = __builtin_bit_cast(uint32_t, p1);
+    first[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // their upper halves
+    second[i] = pack_bf16(p0 - __builtin_bit_cast(float, u0 & 0xffff0000u),
+                          p1 - __builtin_bit_cast(float, u1 & 0xffff0000u));
+  }
+  second[i] |= (p0 > 0.f ? 1u : 0u) | (p1 > 0.f ? 0x10000u : 0u);
+}
+
 // Hidden V rows.  In a step whose rows some columns see and others do not, a
 // hidden row's probability is 0, and 0 times an infinity or a NaN in it (a later
 // token's V) is NaN.  So such a step looks through its V tile first

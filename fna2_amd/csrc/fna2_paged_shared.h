@@ -74,6 +74,7 @@ struct PagedSharedParams {
   const int* cu_groups;
   const int* shared_rows;
   int small;  // every workgroup makes the plan in its LDS
+  int two;    // P in two parts (set where fna2_paged_attn's packed kernel would run)
   SharedMeta* meta;  // ... else as in SharedPlanRef
   SharedGroup* groups;
   int64_t* group_ends;

@@ -16,7 +16,10 @@
 // them into equal runs: every workgroup for itself where 64 sequences and 64 groups at
 // most fit its LDS, else in a launch of its own, in one workgroup's registers up to 1024 (5 groups of
 // 22 sequences: the call 48 us with the general form, 39 so).  The tile kernel
-// (fna2_paged_tile_dev.h) takes a run a workgroup.  A tile that runs cut, or
+// (fna2_paged_tile_dev.h) takes a run a workgroup, with P in two parts for chunks that
+// fna2_paged_attn's packed kernel would take, which has it so: a layer that begins to share is
+// then as precise as before (P in one part: 1.4 times the error of the output's rounding alone; two
+// cost 64 tokens over 16384 shared rows 104 us for 99, 4 over 2000 18.3 for 17.4).  A tile that runs cut, or
 // that is one of two for its tokens, leaves unnormalised parts; the join, another
 // launch, adds a token's parts up in a fixed order.
 //
@@ -175,6 +178,14 @@ __global__ __launch_bounds__(64 * NW) void paged_shared_join_kernel(const PagedS
   __global__ __launch_bounds__(256, tile_occ(D, RPL, HW)) void                                    \
       paged_shared_d##D##_r##RPL##_h##HW##_f16(const PagedSharedParams) {                         \
     tile_body<D, RPL, HW, true, true>();                                                          \
+  }                                                                                               \
+  __global__ __launch_bounds__(256, tile_occ(D, RPL, HW, true)) void                              \
+      paged_shared_d##D##_r##RPL##_h##HW##_p2(const PagedSharedParams) {                          \
+    tile_body<D, RPL, HW, false, true, true>();                                                   \
+  }                                                                                               \
+  __global__ __launch_bounds__(256, tile_occ(D, RPL, HW, true)) void                              \
+      paged_shared_d##D##_r##RPL##_h##HW##_p2_f16(const PagedSharedParams) {                      \
+    tile_body<D, RPL, HW, true, true, true>();                                                    \
   }
 FNA2_SHARED(64, 0, 1)
 FNA2_SHARED(64, 32, 1)
@@ -198,7 +209,8 @@ hipError_t launch_paged_shared(const PagedSharedParams& S, int rpl, hipStream_t 
   const PagedParams& P = S.p;
   void (*k)(const PagedSharedParams) = nullptr;
 #define FNA2_SHARED_OF(D, RPL, HW) \
-  (P.f16 ? paged_shared_d##D##_r##RPL##_h##HW##_f16 : paged_shared_d##D##_r##RPL##_h##HW)
+  (S.two ? (P.f16 ? paged_shared_d##D##_r##RPL##_h##HW##_p2_f16 : paged_shared_d##D##_r##RPL##_h##HW##_p2) \
+         : (P.f16 ? paged_shared_d##D##_r##RPL##_h##HW##_f16 : paged_shared_d##D##_r##RPL##_h##HW))
 #define FNA2_SHARED_HW(D, RPL)                             \
   (P.hw == 1   ? FNA2_SHARED_OF(D, RPL, 1)                 \
    : P.hw == 2 ? FNA2_SHARED_OF(D, RPL, 2)                 \

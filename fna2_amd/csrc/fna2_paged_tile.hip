@@ -157,7 +157,7 @@ FNA2_TILE(128, 64, 4)
 
 }  // namespace
 
-int paged_tile_per_cu(int D, int rpl, int hw) { return tile_occ(D, rpl, hw); }
+int paged_tile_per_cu(int D, int rpl, int hw, bool two) { return tile_occ(D, rpl, hw, two); }
 
 size_t paged_tile_slot(int D) { return (size_t)128 * D * 4; }
 

@@ -34,8 +34,8 @@ __device__ __forceinline__ int run_of(int wg, int n) {
 
 // SHARED: the sequences are those of a plan (PagedSharedParams), in which a
 // sequence may begin behind rows that its group shares; a tile leaves its
-// output for the join of the two.
-template <int D, int RPL, int HW, bool F16, bool SHARED>
+// output for the join of the two.  TWO: P in two parts, as the packed kernel has it.
+template <int D, int RPL, int HW, bool F16, bool SHARED, bool TWO = false>
 __device__ __forceinline__ void tile_body() {
   KArg P = kargs();
   using C = TileCfg<D, RPL, HW>;
@@ -353,8 +353,8 @@ __device__ __forceinline__ void tile_body() {
       }
       const float nm = -((m_i == kNegInf) ? 0.f : m_i) * c2;
       float ls = 0.f;
-      bf16x8 pb[BN / 16];
-      u32x4 pk[BN / 16];
+      bf16x8 pb[BN / 16], pe[BN / 16];
+      u32x4 pk[BN / 16], ek[BN / 16];  // (ek, pe: TWO)
       auto exps = [&](int q, int i0, int i1) {
 #pragma unroll
         for (int i = i0; i < i1; ++i) {
@@ -362,9 +362,16 @@ __device__ __forceinline__ void tile_body() {
           const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[q >> 1][v0], c2, nm));
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[q >> 1][v0 + 1], c2, nm));
           ls += p0 + p1;
-          pk[q][i] = pack_e<F16>(p0, p1);
+          if constexpr (TWO) {
+            split_p<F16>(p0, p1, pk[q], ek[q], i);
+          } else {
+            pk[q][i] = pack_e<F16>(p0, p1);
+          }
         }
-        if (i1 == 4) pb[q] = as_bf16x8(pk[q]);
+        if (i1 == 4) {
+          pb[q] = as_bf16x8(pk[q]);
+          if constexpr (TWO) pe[q] = as_bf16x8(ek[q]);
+        }
       };
       constexpr int NS = BN / 16, N = NS * (D / 32), PPM = 4 / (D / 32);
       exps(0, 0, 4);
@@ -377,6 +384,7 @@ __device__ __forceinline__ void tile_body() {
       for (int i = 0; i < N; ++i) {
         const int s = i / (D / 32), d = i % (D / 32);
         oacc[d] = mfma_e<F16>(vr[i % C::A2], pb[s], oacc[d]);
+        if constexpr (TWO) oacc[d] = mfma_e<F16>(vr[i % C::A2], pe[s], oacc[d]);
         if (i + C::A2 < N)
           vr[i % C::A2] = tr_operand<BN>(vl, tl, 16 * ((i + C::A2) / (D / 32)), 32 * ((i + C::A2) % (D / 32)));
         __builtin_amdgcn_sched_barrier(0);
@@ -504,7 +512,11 @@ __device__ __forceinline__ void tile_body() {
 // (1024-token piece, rank 64, in turn: 346 us, two 351).  Two for the others: the third
 // costs spilled registers (mixed step, 4 heads of rank 32: 146 us, two 133; d =
 // 64, rank 16, 509-token pieces with their weights: 103, 97).  A third ring
-// stage in the room that leaves: 136 and 99.
-constexpr int tile_occ(int D, int RPL, int HW) { return D == 128 && (RPL == 0 || HW == 1) ? 3 : 2; }
+// stage in the room that leaves: 136 and 99.  Two for P in two parts with ranks too,
+// where a third spills 19 to 106 registers (32 sequences of a token over 8192 shared and 512 own
+// rows, 16 heads, rank 32 85 us, two 74; rank 64 103, 83).
+constexpr int tile_occ(int D, int RPL, int HW, bool TWO = false) {
+  return D == 128 && (RPL == 0 || (HW == 1 && !TWO)) ? 3 : 2;
+}
 
 }  // namespace fna2

@@ -364,3 +364,50 @@ def test_strided_inputs():
     c.rq = odd[:, :, 4:]
     c.cg, c.rows = c.cg.long(), c.rows.cpu()
     assert torch.equal(c.attend(), want)
+
+
+# Chunks that flash_naylis_paged serves with P in two parts (one column tile holds them)
+SHORT = ["decode", "two_groups", "beside_others", "without_tokens", "heads_3", "heads_8", "no_ranks",
+         "fp16", "few_tokens_each", "many_sequences_long", "more_sequences", "loose_tokens"]
+
+
+def rounding(c, ref):
+    """Root mean square of what the output's own rounding leaves."""
+    own = torch.from_numpy(ref).to(c.dtype).double().numpy() - ref
+    return np.sqrt((own ** 2).mean())
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("name", SHORT)
+def test_short_chunks_are_as_precise_as_without_groups(name, causal):
+    """P in two parts is off by 2^-16 of each p (bf16) or less, the scores by some 1e-5: against
+    the output's rounding, which is off by 2^-9 / sqrt(3) = 1.1e-3 (bf16) or 1.4e-4 (fp16) of the
+    value on average, both add less than 1% to the root of the mean square (1.1 allowed).  P in
+    one part is off by as much again as the output: 1.4 times."""
+    print(name, causal, flush=True)
+    c = make(name)
+    ref = c.oracle(causal=causal)[0]
+    err = np.sqrt(((c.attend(is_causal=causal).double().cpu().numpy() - ref) ** 2).mean())
+    assert err <= 1.1 * rounding(c, ref)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("score", [-12, 12])
+@pytest.mark.parametrize("row", [5, 113])
+def test_an_infinite_row_stays_infinite(row, score, dtype):
+    """A first row, which is shared, or an own one, that weighs e^-12 (fp16 holds 2^-24 = e^-16.6)
+    of the others, or that most of the weight is on, where p is 1 and its second part nothing: as
+    without groups."""
+    c = SharedCase([1] * 3, [150, 137, 170], 4, 2, 0, 64, 0, 16, groups=[(3, 112, 112)], dtype=dtype,
+                   device="cuda")
+    c.q[:] = c.q[:1, :1]
+    for b in (range(1) if row < 112 else range(3)):
+        page, off = c.slot(b, row)
+        c.k[page, :, off] = score * 8 * c.q[0, 0] / c.q[0, 0].float().square().sum()
+        c.v[page, 1, off, 3] = float("inf")
+    for out in (c.attend(), paged.flash_naylis_paged(c.q, c.k, c.v, c.table, c.lens, c.cu, 1)):
+        assert torch.isposinf(out[:, 2:, 3]).all()
+        out[:, 2:, 3] = 0
+        assert torch.isfinite(out).all()
