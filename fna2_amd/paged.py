@@ -41,6 +41,7 @@ fallback: without the HIP library, or off the GPU, the calls raise.
 from __future__ import annotations
 
 import ctypes
+import weakref
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -857,8 +858,13 @@ class DevicePageTable:
 
     def rollback(self, keep: torch.Tensor) -> None:
         """The rows from ``keep[b]`` on (int32, on the device) were never there, but for those
-        that b shares: drafted tokens that were refused.  Their positions come again."""
+        that b shares: drafted tokens that were refused.  Their positions come again, and in
+        caches that weigh their rows the next tokens' weights there start at 0.  What the
+        refused tokens added to the weights of rows that stay is not taken back."""
         self._trim(torch.maximum(_ints(keep, self.held.device), self.held))
+        for cache in _CACHES.get(self, ()):
+            if cache.table is self:
+                cache._forget_behind(self.seqlens)
 
     def truncate(self, budget: int) -> None:
         """As ``PageTable.truncate``, after every layer's ``evict(budget)``."""
@@ -941,6 +947,9 @@ class DevicePageTable:
             self.shared_rows.copy_(rows)
 
 
+_CACHES = weakref.WeakKeyDictionary()  # DevicePageTable -> the caches on it, while they live
+
+
 class PagedKVCache:
     """One layer's pools on the pages of a ``PageTable`` or ``DevicePageTable``: a ``past_kv`` of
     ``NaylisAttention`` that serves many sequences of differing lengths, prompts
@@ -959,6 +968,15 @@ class PagedKVCache:
                                and r_k.shape[2] == k.shape[2]), \
             "r_k must be [pages, H_G, page_size, R]"
         self.table, self.k, self.v, self.r_k, self.key_weights = table, k, v, r_k, key_weights
+        self._join()
+
+    def _join(self) -> None:
+        if isinstance(self.table, DevicePageTable):
+            _CACHES.setdefault(self.table, weakref.WeakSet()).add(self)
+
+    def __setstate__(self, state) -> None:  # (a copy, with a table of its own or the same)
+        self.__dict__.update(state)
+        self._join()
 
     @classmethod
     def empty(cls, table: PageTable, n_kv_heads: int, head_dim: int, graph_heads: int = 0,
@@ -982,6 +1000,11 @@ class PagedKVCache:
                                  budget, recent, first, self.r_k, heads)
         self.key_weights.copy_(w)
         return kept
+
+    def _forget_behind(self, lens: torch.Tensor) -> None:
+        w = self.key_weights
+        if w is not None:
+            w.masked_fill_(torch.arange(w.shape[2], device=w.device) >= lens[:, None, None], 0.0)
 
     def forget(self, b: int) -> None:
         """Sequence b's place is for another: its weights start at 0 (after

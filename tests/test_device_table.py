@@ -559,3 +559,76 @@ def test_a_captured_layer_in_another_layout_follows_the_table(gpu, kw, inside):
             del junk
         eager.table.check()
         graphed.table.check()
+
+
+def test_rollback_reaches_the_caches_that_weigh(monkeypatch):
+    """Every cache on the table, copies with theirs, none that has gone; rows that stay keep what
+    they have."""
+    import copy
+    import pickle
+
+    def trim(table, lens, keep, free, count, ps, borrowed=None):
+        return torch.minimum(lens, keep), count.clone()
+
+    monkeypatch.setattr(paged, "paged_trim", trim)
+    t = DevicePageTable(2, 4, page_size=16, device="cpu")
+    caches = [PagedKVCache.empty(t, 2, 64, weigh=w) for w in (True, False, True)]
+    t.seqlens += torch.tensor([20, 9], dtype=torch.int32)
+    for c in caches[::2]:
+        c.key_weights += 1
+    other = copy.deepcopy(caches[0])
+    again = pickle.loads(pickle.dumps(caches[0]))
+    assert other.table is not t and again.table is not t
+    t.rollback(torch.tensor([17, 30], dtype=torch.int32))
+    for c in caches[::2]:
+        assert (c.key_weights[0, :, :17] == 1).all() and (c.key_weights[1, :, :9] == 1).all()
+        assert c.key_weights.sum() == 2 * (17 + 9)
+    for c in (other, again):
+        assert (c.key_weights == 1).all()
+        c.table.rollback(torch.tensor([0, 3], dtype=torch.int32))
+        assert c.key_weights.sum() == 2 * 3
+    assert caches[0].key_weights.sum() == 2 * (17 + 9)
+    del caches[1:]
+    assert len(paged._CACHES[t]) == 1
+
+
+@gpu_test
+@pytest.mark.parametrize("captured", [False, True])
+def test_rows_that_were_rolled_back_weigh_nothing(gpu, captured):
+    """Refused tokens' rows start again from no weight, as in a cache that never saw them."""
+    m = layer(gpu)
+    x = torch.randn(29, 512, device=gpu).bfloat16()
+    accepted, drafted, after = (torch.randn(n, 512, device=gpu).bfloat16() for n in (1, 6, 5))
+    with torch.no_grad():
+        caches = []
+        for drafts in (True, False):
+            t = DevicePageTable(2, 20, page_size=16, max_pages=5, device=gpu)
+            c = cache(m, t, weigh=True)
+            t.extend([20, 9])
+            m(x, past_kv=c)
+            if drafts:  # four tokens of the first sequence, three of the second: one stays
+                t.extend([4, 3])
+                m(torch.cat((accepted, drafted)), past_kv=c)
+                keep = torch.tensor([21, 9], dtype=torch.int32, device=gpu)
+                if captured:
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        t.rollback(keep)
+                    for _ in range(3):
+                        graph.replay()
+                else:
+                    t.rollback(keep)
+                assert t.seqlens.tolist() == [21, 9]
+                assert (c.key_weights[0, :, 21:] == 0).all() and (c.key_weights[1, :, 9:] == 0).all()
+                assert (c.key_weights[0, :, :21] > 0).all() and (c.key_weights[1, :, :9] > 0).all()
+            else:
+                t.extend([1, 0])
+                m(accepted, past_kv=c)
+            t.extend([2, 3])
+            m(after, past_kv=c)
+            caches.append(c)
+    a, b = (c.key_weights for c in caches)
+    # (the same queries over rows that round to neighbours; sums over a KV head's four heads)
+    assert (a[0, :, 21:] - b[0, :, 21:]).abs().max() <= 4 * 2.0 ** -6
+    assert (a[1, :, 9:] - b[1, :, 9:]).abs().max() <= 4 * 2.0 ** -6
+    assert (a[0, :, 21:23] > 0).all() and (a[1, :, 9:12] > 0).all()
