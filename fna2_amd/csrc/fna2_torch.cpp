@@ -775,6 +775,9 @@ Rows rotary_embed(const Tensor& q, const Tensor& k, const Tensor& inv, const Opt
   Tensor w[3];
   const c10::OptionalDeviceGuard guard(at::device_of(q));
   if (!rotary_args(a, q, k, inv, pos, cu, nq, nk, Rotary{inter, scale, eps}, w)) return std::nullopt;
+  // (forward-mode tangents: the caller's node, which refuses them)
+  for (const Tensor* t : {&q, &k, &inv, &opt(nq), &opt(nk)})
+    if (t->defined() && t->_fw_grad(0).defined()) return std::nullopt;
   auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
   if (!at::GradMode::is_enabled() || !(wants(q) || wants(k) || wants(opt(nq)) || wants(opt(nk))))
     return rotary_launch(a, q, k);

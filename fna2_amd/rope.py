@@ -363,8 +363,8 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
 
     A token's position is ``positions[t]`` (int32), or its place in its sequence by
     ``cu_seqlens`` (tokens of no sequence are left as they are): one of the two.  The
-    chain is evaluated in fp32, the angle in fp64, and rounded once.  Differentiable, once, in
-    q, k and the norm weights; into a graph only without an eager autograd graph of the same
+    chain is evaluated in fp32, the angle in fp64, and rounded once.  Differentiable, once and in
+    reverse, in q, k and the norm weights; into a graph only without an eager autograd graph of the same
     leaves (RuntimeError).  ``rotary_frequencies`` makes ``inv_freq`` and ``scale``."""
     args = (q, k, inv_freq, positions, cu_seqlens, norm_q, norm_k)
     nat = _capi.native_or_none() if q.is_cuda and grad_slab is None else None
@@ -377,6 +377,5 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor,
         nat = _capi.native_or_none() if q.is_cuda else None
         if nat is not None:
             nat.recordable([q, k, norm_q, norm_k])
-        return RotaryFunc.apply(*args, (bool(interleaved), float(scale), float(eps)), grad_slab)
-    return rotary_embed_raw(q, k, inv_freq, positions, cu_seqlens, interleaved, scale, norm_q,
-                            norm_k, eps)
+    # (without a gradient to come, too: the node refuses forward-mode tangents)
+    return RotaryFunc.apply(*args, (bool(interleaved), float(scale), float(eps)), grad_slab)

@@ -557,3 +557,22 @@ def test_frequencies():
                 dict(rotary_dim=8, scaling="linear", factor=0.5)):
         with pytest.raises(ValueError):
             rotary_frequencies(**bad)
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("what", ["q", "k", "norm_q", "norm_k", "inv_freq"])
+def test_tangents_are_refused(what, native, monkeypatch):
+    """Forward-mode differentiation raises, as rope_varlen's does: no output without its tangent."""
+    import torch.autograd.forward_ad as fw
+    c = Case(9, 2, 1, 64, 32, True, torch.float32)
+    args = dict(c.args(), q=c.q.contiguous(), k=c.k.contiguous(), inv_freq=c.inv)
+    if not native:
+        monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+    with fw.dual_level():
+        args[what] = fw.make_dual(args[what], torch.ones_like(args[what]))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, NotImplementedError)):
+                rotary_embed(**args)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            rotary_embed(**args, grad_slab=_Slab())
