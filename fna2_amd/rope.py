@@ -130,8 +130,9 @@ def rope_varlen_bwd(dq_out, dk_out, q, k, cu_seqlens, inv_freq, sign=1, norm_q=N
     if dk is None:
         dk = torch.empty_like(k, memory_format=torch.contiguous_format)
     b.dq_out, b.dk_out, b.dq, b.dk = _view(dq_out), _view(dk_out), _view(dq), _view(dk)
-    dwq = None if wq is None else torch.empty_like(wq)
-    dwk = None if wk is None else torch.empty_like(wk)
+    # (without rows nothing is written)
+    dwq = None if wq is None else torch.empty_like(wq) if q.numel() else torch.zeros_like(wq)
+    dwk = None if wk is None else torch.empty_like(wk) if k.numel() else torch.zeros_like(wk)
     b.dnorm_q = None if dwq is None else dwq.data_ptr()
     b.dnorm_k = None if dwk is None else dwk.data_ptr()
     lib = _capi.lib()

@@ -275,3 +275,17 @@ def test_norm_rope_forward_backward(gpu, dtype, which):
     for a, b in zip(grads, grads2):
         assert torch.equal(a, b)
 
+
+
+@pytest.mark.gpu
+def test_no_tokens_give_zero_weight_gradients(gpu):
+    from fna2_amd.rope import rope_varlen
+    w = [torch.ones(64, device=gpu, requires_grad=True) for _ in range(2)]
+    q, k = torch.zeros(0, 4, 64, device=gpu), torch.zeros(0, 2, 64, device=gpu)
+    cu = torch.zeros(1, dtype=torch.int32, device=gpu)
+    for _ in range(4):  # (memory that the allocator hands out again)
+        full = [torch.full((64,), float("nan"), device=gpu) for _ in range(64)]
+        del full
+        y = rope_varlen(q, k, cu, torch.ones(32, device=gpu), *w)
+        for g in torch.autograd.grad(y, w, [torch.zeros_like(t) for t in y]):
+            assert (g == 0).all()
