@@ -164,7 +164,9 @@ class RotaryPositionalEmbedding(nn.Module):
     Beyond the reference's, ``extended``: the first ``rotary_dim`` features only, neighbouring
     ones paired (``interleaved``), or frequencies scaled for contexts ``factor`` times
     ``original_max_len`` (``scaling``: see ``rotary_frequencies``).  These go through
-    ``rotary_embed`` on the GPU, in fp32 with one rounding."""
+    ``rotary_embed`` on the GPU, in fp32 with one rounding.  Their ``inv_freq`` is of these
+    arguments alone: it stays in 32 bits when the module is cast (8 bits would be 13 radians off
+    at position 30,000), and checkpoints neither hold nor change it."""
 
     def __init__(self, dim: int, max_seq_len: int = 2048, base: int = 10000,
                  use_yarn: bool = False, yarn_scale: float = 1.0,
@@ -194,12 +196,29 @@ class RotaryPositionalEmbedding(nn.Module):
             start = max(dim // 2, int(dim * 0.25))
             ramp = 1 + (yarn_scale - 1) * (half - start) / (dim - start)
             inv_freq = inv_freq / torch.where(half < start, torch.ones_like(half), ramp)
+        self._scaled = (dim if rotary_dim is None else rotary_dim, base, scaling, factor,
+                        original_max_len)
         if self.extended:
-            inv_freq, self.factor = rotary_frequencies(
-                dim if rotary_dim is None else rotary_dim, base, scaling, factor, original_max_len)
-        self.register_buffer("inv_freq", inv_freq)
+            inv_freq, self.factor = rotary_frequencies(*self._scaled)
+        self.register_buffer("inv_freq", inv_freq, persistent=not self.extended)
         self._cache_key = None
         self._cos = self._sin = None
+
+    def _apply(self, fn, recurse=True):
+        inv = self.inv_freq
+        super()._apply(fn, recurse)
+        if self.extended:  # (where it went, with the values and the type that it had)
+            dev = self.inv_freq.device
+            self.inv_freq = rotary_frequencies(*self._scaled, device=dev)[0] if inv.is_meta else \
+                inv.to(dev)
+        return self
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                              unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys,
+                                      unexpected_keys, error_msgs)
+        if self.extended and prefix + "inv_freq" in unexpected_keys:
+            unexpected_keys.remove(prefix + "inv_freq")
 
     def _table(self, n: int, device, dtype):
         """cos / sin rows of positions 0 .. n-1 (at least): the table is

@@ -7,6 +7,8 @@ values and may round six things between to other neighbours (the rotated q and k
 parts' join, the attention's output and the layer's), each by at most 2^-8 of the value:
 6 * 2^-8 of the output's norm.
 """
+import math
+
 import pytest
 import torch
 
@@ -632,3 +634,68 @@ def test_rows_that_were_rolled_back_weigh_nothing(gpu, captured):
     assert (a[0, :, 21:] - b[0, :, 21:]).abs().max() <= 4 * 2.0 ** -6
     assert (a[1, :, 9:] - b[1, :, 9:]).abs().max() <= 4 * 2.0 ** -6
     assert (a[0, :, 21:23] > 0).all() and (a[1, :, 9:12] > 0).all()
+
+
+def far_angles(rope, pos):
+    return pos * rope.inv_freq.double().cpu()
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(),
+                                  lambda m: m.to(torch.bfloat16).float(), lambda m: m.cpu()])
+@pytest.mark.parametrize("scaling", ["linear", "yarn"])
+def test_scaled_frequencies_stay_in_32_bits(cast, scaling):
+    """Whatever the layer is cast to, before or after rotate_by, the angles of far positions are
+    those of the formula, rounded to fp32 once: off by 2^-24 of the angle."""
+    factor, length, rd = 8.0, 4096, 64
+    i = torch.arange(rd // 2, dtype=torch.float64)
+    inv = 10000.0 ** (-2 * i / rd)
+    if scaling == "linear":
+        want = inv / factor
+    else:  # by the turns over the original length: more than 32 kept, fewer than 1 divided
+        pair = lambda turns: rd * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(10000.0))
+        low, high = math.floor(pair(32.0)), math.ceil(pair(1.0))
+        ramp = ((i - low) / (high - low)).clamp(0, 1)
+        want = inv * (1 - ramp) + inv / factor * ramp
+    how = dict(rotary_dim=rd, scaling=scaling, factor=factor, original_max_len=length)
+    make = lambda: NaylisAttention(256, 2, rel_rank=8)
+    for m in (cast(make().rotate_by(**how)), cast(make()).rotate_by(**how)):
+        assert m.rope.inv_freq.dtype == torch.float32
+        for pos in (1000, 30000, 10 ** 6):
+            assert ((far_angles(m.rope, pos) - pos * want).abs() <= 2.0 ** -24 * pos * want + 1e-12).all()
+        assert m.q_proj.weight.dtype == cast(make()).q_proj.weight.dtype
+
+
+def test_a_checkpoint_does_not_change_the_frequencies():
+    """inv_freq is of the layer's arguments: a plain layer's, or one's of another width, that a
+    checkpoint holds, is left; the other parameters load."""
+    make = lambda **how: NaylisAttention(256, 2, rel_rank=8).rotate_by(**how) if how else \
+        NaylisAttention(256, 2, rel_rank=8)
+    how = dict(rotary_dim=64, interleaved=True, scaling="yarn", factor=8.0, original_max_len=4096)
+    plain, other = make(), make(rotary_dim=32)
+    assert "rope.inv_freq" in plain.state_dict() and "rope.inv_freq" not in other.state_dict()
+    older = dict(other.state_dict())
+    older["rope.inv_freq"] = other.rope.inv_freq.clone()
+    for saved in (plain.state_dict(), other.state_dict(), older):
+        for assign in (False, True):
+            m = make(**how)
+            want = m.rope.inv_freq.clone()
+            assert m.load_state_dict(saved, assign=assign) == ([], [])
+            assert torch.equal(m.rope.inv_freq, want) and m.rope.factor > 1
+            assert torch.equal(m.q_proj.weight, saved["q_proj.weight"])
+    with pytest.raises(RuntimeError, match="q_nothing"):
+        m.load_state_dict({**plain.state_dict(), "q_nothing": torch.ones(1)})
+    with pytest.raises(RuntimeError, match="rope.nothing"):
+        m.load_state_dict({**plain.state_dict(), "rope.nothing": torch.ones(1)})
+    with torch.device("meta"):
+        m = make(**how)
+    assert m.rope.inv_freq.is_meta
+    m.to_empty(device="cpu")
+    assert torch.equal(m.rope.inv_freq, want) and m.rope.inv_freq.dtype == torch.float32
+    m.to_empty(device="cpu")
+    assert torch.equal(m.rope.inv_freq, want)
+
+
+def test_a_plain_layers_frequencies_go_with_it():
+    m = NaylisAttention(256, 2, rel_rank=8)
+    assert m.bfloat16().rope.inv_freq.dtype == torch.bfloat16
+    assert m.load_state_dict(NaylisAttention(256, 2, rel_rank=8).state_dict()) == ([], [])
