@@ -571,10 +571,14 @@ class NaylisAttention(nn.Module):
                   original_max_len: int = 2048) -> "NaylisAttention":
         """Another rotary embedding for this layer (in place; returns the layer): of the first
         ``rotary_dim`` features, of neighbouring pairs, scaled for long contexts (see
-        ``RotaryPositionalEmbedding``, ``rotary_frequencies``)."""
+        ``RotaryPositionalEmbedding``, ``rotary_frequencies``).  Not for one built with
+        ``use_yarn``."""
         if self.rope is None:
             raise ValueError("rotate_by: this layer has no rotary embedding (use_rope=False)")
         old = self.rope
+        if old.use_yarn:
+            raise ValueError("rotate_by: this layer was built with use_yarn, which scales its scores "
+                             "as well: build it without, and use scaling='yarn'")
         self.rope = RotaryPositionalEmbedding(
             self.head_dim, old.max_seq_len, old.base, rotary_dim=rotary_dim, interleaved=interleaved,
             scaling=scaling, factor=factor, original_max_len=original_max_len

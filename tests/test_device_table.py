@@ -699,3 +699,14 @@ def test_a_plain_layers_frequencies_go_with_it():
     m = NaylisAttention(256, 2, rel_rank=8)
     assert m.bfloat16().rope.inv_freq.dtype == torch.bfloat16
     assert m.load_state_dict(NaylisAttention(256, 2, rel_rank=8).state_dict()) == ([], [])
+
+
+def test_rotate_by_does_not_take_a_yarn_stretch_away():
+    """A layer built with use_yarn scales its scores by yarn_scale too, which another rotation
+    would drop unseen."""
+    m = NaylisAttention(256, 2, rel_rank=8, use_yarn=True, yarn_scale=4.0)
+    scale, rope = m._attn_scale(), m.rope
+    for how in (dict(rotary_dim=64), dict(scaling="yarn", factor=4.0), dict()):
+        with pytest.raises(ValueError, match="use_yarn"):
+            m.rotate_by(**how)
+    assert m.rope is rope and m._attn_scale() == scale
