@@ -939,13 +939,23 @@ std::optional<std::tuple<Tensor, OptTensor>> paged_attn(
     sa.shared_rows = shared.data_ptr<int32_t>();
     if (L.check_paged_shared(&sa) != FNA2_OK) return std::nullopt;
   }
-  const size_t need =
-      groups.defined() ? L.paged_shared_workspace_bytes(&sa) : L.paged_attn_workspace_bytes(&a);
-  const Tensor ws = bytes_on(need, q);
-  a.workspace = sa.attn.workspace = ws.data_ptr();
-  a.workspace_bytes = sa.attn.workspace_bytes = need;
+  bool shares = groups.defined();
+  Tensor ws;
+  auto workspace = [&] {
+    const size_t need = shares ? L.paged_shared_workspace_bytes(&sa) : L.paged_attn_workspace_bytes(&a);
+    ws = bytes_on(need, q);
+    a.workspace = sa.attn.workspace = ws.data_ptr();
+    a.workspace_bytes = sa.attn.workspace_bytes = need;
+  };
+  try {
+    workspace();
+  } catch (const c10::OutOfMemoryError&) {
+    if (!shares) throw;
+    shares = false;  // (no room for the shared rows' parts: each sequence by itself)
+    workspace();
+  }
   void* const stream = stream_of(dev);
-  if (!launched(groups.defined() ? L.paged_shared(&sa, stream) : L.paged_attn(&a, stream), what))
+  if (!launched(shares ? L.paged_shared(&sa, stream) : L.paged_attn(&a, stream), what))
     return std::nullopt;
   if (w.defined()) {
     // (checked above: what is left to fail is a launch)

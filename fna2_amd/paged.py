@@ -216,7 +216,8 @@ def flash_naylis_shared(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     ``block_table`` begin alike (``paged_groups`` finds such groups).  Of these
     rows, those are shared that lie before every chunk of the group, in whole steps of
     32, if two of its sequences have tokens and reading the rows once saves more than the
-    tokens' second part costs; ``shared_rows`` may be larger or 0.
+    tokens' second part costs; ``shared_rows`` may be larger or 0.  The parts take 8 bytes a
+    token, head and feature; without that memory the call is ``flash_naylis_paged``'s.
     """
     assert cu_groups is not None and shared_rows is not None, \
         "flash_naylis_shared: cu_groups and shared_rows expected"
@@ -316,7 +317,15 @@ def _attention(what, q, k_pages, v_pages, block_table, seqlens_k, cu_seqlens_q, 
     if T > 0:
         args, at = (a, a) if sa is None else (sa, sa.attn)
         nbytes = size(ctypes.byref(args))
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        try:
+            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        except torch.OutOfMemoryError:
+            if sa is None:
+                raise
+            # (no room for the shared rows' parts: each sequence by itself)
+            call, args, at = lib.fna2_paged_attn, a, a
+            nbytes = lib.fna2_paged_attn_workspace_bytes(ctypes.byref(a))
+            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
         at.workspace, at.workspace_bytes = ws.data_ptr(), nbytes
         with torch.cuda.device(dev):
             _capi.raise_for(call(ctypes.byref(args), _stream(dev)), what)

@@ -11,6 +11,7 @@ fp32 scores; LSE 1e-4, weights 2e-4 relatively.  A token's parts are joined in
 fp32, a few 2^-24 of the sums.
 """
 import ctypes
+import gc
 import subprocess
 
 import numpy as np
@@ -411,3 +412,53 @@ def test_an_infinite_row_stays_infinite(row, score, dtype):
         assert torch.isposinf(out[:, 2:, 3]).all()
         out[:, 2:, 3] = 0
         assert torch.isfinite(out).all()
+
+
+def limited(c):
+    """The call with memory for flash_naylis_paged, but not for the shared rows' parts."""
+    plain = lambda: paged.flash_naylis_paged(c.q, c.k, c.v, c.table, c.lens, c.cu, c.max_q, r_q=c.rq,
+                                             rk_pages=c.rk, graph_scale=c.gs, return_lse=True)
+    want = [t.cpu() for t in plain()]
+    total = torch.cuda.get_device_properties(0).total_memory
+    limit = lambda nbytes: torch.cuda.set_per_process_memory_fraction(nbytes / total)
+    peaks, held = [], []
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    try:
+        # what other tests left between their tensors is taken first
+        limit(torch.cuda.memory_reserved())
+        size = 1 << 32
+        while size >= 1 << 21:
+            try:
+                held.append(torch.empty(size, dtype=torch.uint8, device="cuda"))
+            except torch.OutOfMemoryError:
+                size >>= 1
+        limit(total)
+        for call in (plain, lambda: c.attend(return_lse=True)):
+            torch.cuda.reset_peak_memory_stats()
+            call()
+            torch.cuda.synchronize()
+            peaks.append(torch.cuda.max_memory_reserved())
+            torch.cuda.empty_cache()
+        assert peaks[1] > peaks[0] + (8 << 20)
+        limit(sum(peaks) / 2)
+        return [t.cpu() for t in c.attend(return_lse=True)], want
+    finally:
+        limit(total)
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_without_the_memory_each_sequence_by_itself(native, monkeypatch):
+    """The shared rows' parts take 8 bytes a token, head and feature; without them the call is
+    flash_naylis_paged's."""
+    if not native:
+        monkeypatch.setattr(_capi, "native_or_none", lambda: None)
+    c = SharedCase([60] * 64, [140 + i % 9 for i in range(64)], 16, 4, 16, 128, 32, 16,
+                   groups=[(64, 64, 64)], device="cuda")
+    got, want = limited(c)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    monkeypatch.undo()
+    c.max_q = 1 << 20  # (and with no limit, again)
+    assert (c.attend().cpu().float() - want[0].float()).abs().max() < 0.05
