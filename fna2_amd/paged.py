@@ -825,12 +825,12 @@ class DevicePageTable:
                             self.free_count, self.page_size, total_q, self.position_shift)
         self.total_q = int(total_q)
         self.slots, self.sequences, self.positions = self._of_tokens(self.total_q)
+        words = lambda t: t.view(torch.int32)  # (of one type: one launch)
         torch._foreach_copy_(
             [self.seqlens, self.free_count, self.cu_seqlens_q, self.status, self.sequences,
-             self.positions],
+             self.positions, words(self.slots)],
             [step.seqlens, step.free_count, step.cu_seqlens_q, step.status, step.sequences,
-             step.positions])
-        self.slots.copy_(step.slots)
+             step.positions, words(step.slots)])
         self.max_seqlen_q = self.total_q if max_seqlen_q is None else int(max_seqlen_q)
         return step
 
