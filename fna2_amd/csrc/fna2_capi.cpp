@@ -1615,7 +1615,7 @@ PagedPlan paged_plan(const fna2_paged_cache& c) {
 // 214, 206, 211; 8 x 100 over 2048 and 1000 own, rank 64 97, 95, 100; 16 x up to 128 over 8192,
 // rank 64 351, 352, 365; 8 x up to 189 over 5771, 3 heads of 64 68, 70, 74).  Runs are
 // equal in key steps and 8 for each tile that they go on to, which takes as long as those: its
-// page ids, first rows, queries, and the part that it leaves (us, 4, 6, 8, 10: 16 x up to 128 over 8192 391,
+// page ids, first rows, queries, and the part that it leaves (these figures with P in one part; us, 4, 6, 8, 10: 16 x up to 128 over 8192 391,
 // 335, 334, 336; 9 x up to 193 over 12689 237, 218, 210, 204; 4 groups of 32 x 1 over 2821, 32 heads of 64
 // 62, 58, 60, 65), and of 6 steps at least (us, 4, 6, 8, 12: 4 x 1 over 2000 20.2, 17.6, 18.1, 20.2;
 // 2 groups of 2 x 1 over 500 18.2, 19.8, 21.3, 23.4; 8 groups of 4 x 3 over 400 25.5, 25.7, 25.5, 30.7).

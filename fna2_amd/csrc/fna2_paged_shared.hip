@@ -24,10 +24,10 @@
 // launch, adds a token's parts up in a fixed order.
 //
 // Bound by memory where the sequences' own rows are many: 64 tokens over 16384 shared and up
-// to 1000 own rows, 32 heads over 8 of 128, rank 32 95 + 8 us (tiles + join; 406 MB at 4.3 TB/s, the
+// to 1000 own rows, 32 heads over 8 of 128, rank 32 96 + 8 us (tiles + join; 406 MB at 4.2 TB/s, the
 // least that it can read being 395); by the matrix cores where chunks are long: 16 x up to 128 tokens
 // over 8192, rank 64 333 to 352, up to 0.87 10^15 operations a second, 24 of them the join's; by chains of dependent loads (plan, page
-// ids, rows, parts, join) where there is little: 4 tokens over 2000 rows 12 + 6.
+// ids, rows, parts, join) where there is little: 4 tokens over 2000 rows 13 + 6.
 #include <algorithm>
 
 #include "fna2_paged_tile_dev.h"

@@ -20,6 +20,9 @@
 //
 // 16384 tokens of 32 + 8 heads of 128 in bf16, no norm, 65 us: 5.2 TB/s; of 16 + 16 with the norm
 // 61 forward (4.4 TB/s), 91 backward (4.4), 5 for dw; 64 tokens of 32 + 8 5.6, one launch's latency.
+// Halves that begin off a chunk (24 features; 32 of them, which do not, beside it): 16384 tokens of 16 + 16
+// heads of 128 in bf16 59 us (43), with the norm 78 (45), backward and dw 116 (92), where the waves are two
+// a SIMD and LDS takes the exchange; 5003 of 8 + 4 of 64 in fp32 9.8 (7.9), 11.0 (9.2), 20 (19).
 #include <algorithm>
 
 #include "fna2_rope_dev.h"

@@ -721,8 +721,8 @@ void recordable(const std::vector<OptTensor>& leaves) {
   }
 }
 
-// rotary_embed with gradients: an autograd node in native code, which takes 20 us of
-// host time a pass where one in Python takes 80.
+// rotary_embed with gradients: an autograd node in native code: forward and backward
+// with norms take 78 us of host time, through Python 191 (the forward alone 8 and 26).
 OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 struct RotaryNode : torch::autograd::Function<RotaryNode> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,

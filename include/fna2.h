@@ -435,7 +435,8 @@ typedef struct fna2_paged_shared_args {
 /* Host-only validation; no GPU call. */
 int fna2_check_paged_shared(const fna2_paged_shared_args* args);
 size_t fna2_paged_shared_workspace_bytes(const fna2_paged_shared_args* args);
-/* Three launches: a plan, the tiles, the join of their parts. */
+/* Two launches, the tiles and the join of their parts; beyond 64 sequences or groups a
+ * plan before them. */
 int fna2_paged_shared(const fna2_paged_shared_args* args, void* hip_stream);
 
 /* The cached rows' attention weights of a fna2_paged_attn call:
